@@ -343,10 +343,10 @@ def _own(s):
             calls.append((lib.sg_cross_attention_grad, ins + (desc(s["out"], **at_q), desc(s["lse"]), desc(s["gout"], **at_q), desc(s["gq"], **at_q),
                                                               desc(s["gk"], **at_k), desc(s["gv"], **at_k))))
     else:
-        lr, b1, b2, eps, decay, _, _ = _adamw_constants()
+        lr, b1, b2, eps, decay, c1, c2 = _adamw_constants()
         sizes = _sizes(s)
         starts, _ = _starts(sizes)
-        hyper = abi.sg_adamw_hyper(lr, b1, b2, eps, decay, SEED)
+        hyper, noise = abi.sg_adam_hyper(lr, b1, b2, c1, c2, eps, decay), C.c_uint32(SEED)
 
         def table(name, per, dtype=None):
             """One descriptor for each tensor; `per` of its elements share one of this buffer's."""
@@ -359,11 +359,11 @@ def _own(s):
 
         if s["bits"] == 8:
             states = (table("m", 4, abi.UINT), table("v", 4, abi.UINT), table("m_scale", 256), table("v_scale", 256))
-            calls.append((lib.sg_adamw_update, (len(sizes), table("value", 1), table("grad", 1)) + states + (desc(s["step_t"]), C.byref(hyper))))
+            calls.append((lib.sg_adamw_update, (len(sizes), table("value", 1), table("grad", 1)) + states + (desc(s["step_t"]), C.byref(hyper), noise)))
             calls.append((lib.sg_adamw_state_read, (len(sizes),) + states + (table("m_out", 1), table("v_out", 1))))
         else:
             calls.append((lib.sg_adamw_update, (len(sizes), table("value", 1), table("grad", 1), table("m", 1), table("v", 1), None, None,
-                                                desc(s["step_t"]), C.byref(hyper))))
+                                                desc(s["step_t"]), C.byref(hyper), noise)))
         kept.append(hyper)
     names = {"embedding": ("out", "gtable"), "logprobs": ("logprob", "entropy", "top_ids", "top_logprobs", "glogits"), "cross": ("out", "gq", "gk", "gv")}
     if s["op"] == "adamw":
