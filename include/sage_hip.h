@@ -209,6 +209,24 @@ int sg_unslice(sg_ctx *ctx, int axis, int64_t start, const sg_tensor *x, const s
 /* Concat::compute (core.rs:892-934). */
 int sg_concat(sg_ctx *ctx, int axis, const sg_tensor *in, int n_in, const sg_tensor *out);
 
+/* ---- embedding lookup and its gradient ------------------------------------------------------- */
+
+/* The four groups below (embedding, token log probabilities, cross attention, AdamW) have no kernel of their own in
+ * the reference; each names what it stands beside.  They check every argument before anything is launched, and in
+ * front of ctx itself, so a call with ctx = NULL gives the same status for a wrong argument and SG_ERR_ARG for a right
+ * one.  Inputs may have any strides on the axes that are not named unit-stride, 0 among them; outputs must not overlap
+ * inputs or each other unless it is said; an optional tensor may be NULL. */
+
+/* out[.., :] = scale * table[ids[..], :]: the lookup of Embedding::pass (layers.rs:406-463) without the expanded index
+ * tensor, and the scaling a decoder applies to it.  table [V, E] (unit stride on E), ids of rank 1..7, SG_UINT or SG_INT
+ * read as unsigned, out: ids' extents and E, dense.  An id of V or more (-1 among them) is no token: its row is zero. */
+int sg_embedding(sg_ctx *ctx, const sg_tensor *table, const sg_tensor *ids, float scale, const sg_tensor *out);
+/* The adjoint: gtable[v, :] = scale * sum of gout[i, :] over the tokens i with id v, zeros for a row without tokens (what
+ * Gather::grad builds from a scatter, core.rs:651-653).  The tokens are sorted by id and each row's are summed in an order
+ * that depends on the ids alone: the same inputs give the same bits.  gout: ids' extents and E, unit stride on E; gtable
+ * [V, E] dense, rewritten as a whole.  Its workspace comes from the context allocator (SG_ERR_OOM). */
+int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_tensor *ids, float scale, const sg_tensor *gtable);
+
 /* ---- GEMM: ops/gemm.rs + ops/kernels/matmul_direct.opencl ------------------------------------ */
 
 typedef enum sg_act { SG_ACT_NONE = 0, SG_ACT_RELU = 1, SG_ACT_GELU_ERF = 2 } sg_act;
@@ -322,6 +340,31 @@ typedef struct sg_adam_hyper {
 int sg_adam_update(sg_ctx *ctx, int n_tensors, const sg_tensor *values, const sg_tensor *grads,
                    const sg_tensor *m, const sg_tensor *v, const sg_tensor *step, const sg_adam_hyper *h);
 
+/* One AdamW step (Adam, optim.rs:98-177, with the weight decay applied to the value instead of the gradient) over n_tensors
+ * parameters in place, many tensors a launch:
+ *   m' = beta1 m + one_minus_beta1 g;  v' = beta2 v + one_minus_beta2 (g g);
+ *   value' = value - lr ((m' / (1 - beta1^t)) / (sqrt(v' / (1 - beta2^t)) + eps) + weight_decay value)
+ * step: one fp32 element on the device holding t >= 1 (read, not advanced, as in sg_adam_update).  values, grads: dense
+ * fp32, equal sizes per tensor.  States in 32 bits (m_scale and v_scale NULL): m, v dense fp32 of the values' sizes.
+ * States in 8 bits (both scale arrays given): m[i], v[i] dense SG_UINT of ceil(n/4) words, byte j of word w standing for
+ * element 4w+j, and m_scale[i], v_scale[i] dense fp32 of ceil(n/256).  A block of 256 elements shares the power of two
+ * 2^(e-127) that its scale holds, e = max(33, exponent field of the block's largest magnitude with its mantissa rounded up
+ * to 3 bits).  A byte of v holds 5 exponent and 3 mantissa bits, 0 standing for zero, else the number with the bits
+ * (byte + 8e + 7 - 255) << 20; a byte of m a sign (bit 7) and 4 + 3 bits, 127 in the place of 255.  All zeros are zero states.
+ * A new state is cut to a byte after 16 bits of noise are added below the bits that are kept (so it is rounded up or down
+ * with the chance that keeps its mean; a step moves v by less than half a code), and a v that is not zero does not become
+ * zero.  The noise of element i is a hash of i + seed + t, low half for m, high half for v: h = i 0x9E3779B9 + seed +
+ * t 0xAC502949; h = (h ^ h >> 16) 0x82D3099F; h = (h ^ h >> 15) 0x2ACAE79F; h ^= h >> 16.  A value or gradient that is
+ * not finite makes its value and state not finite (an 8-bit state: its whole block, NaN).  Two tensors of a call must not
+ * share memory. */
+int sg_adamw_update(sg_ctx *ctx, int n_tensors, const sg_tensor *values, const sg_tensor *grads, const sg_tensor *m,
+                    const sg_tensor *v, const sg_tensor *m_scale, const sg_tensor *v_scale, const sg_tensor *step,
+                    const sg_adam_hyper *h, uint32_t seed);
+/* The numbers 8-bit states stand for, m_out[i] and v_out[i] dense fp32 (their sizes are the tensors' sizes), for
+ * checkpoints and inspection. */
+int sg_adamw_state_read(sg_ctx *ctx, int n_tensors, const sg_tensor *m, const sg_tensor *v, const sg_tensor *m_scale,
+                        const sg_tensor *v_scale, const sg_tensor *m_out, const sg_tensor *v_out);
+
 /* ---- fused row operators: compositions of ops/nn.rs ------------------------------------------ */
 
 /* softmax over the last axis (nn.rs:42-56) of (x + addend): one pass instead of reduce(max),
@@ -337,6 +380,25 @@ int sg_softmax_cross_entropy(sg_ctx *ctx, const sg_tensor *logits, const sg_tens
 int sg_layer_norm_lastaxis(sg_ctx *ctx, const sg_tensor *x, const sg_tensor *gamma,
                            const sg_tensor *beta, float eps, const sg_tensor *out);
 
+/* Log probabilities of given tokens under z = scale * logits (scale > 0: one over a temperature), with
+ * lse = log sum_j e^(z_j): logprob = z_token - lse, entropy = lse - sum_j p_j z_j, and the k largest logits' indexes with
+ * their log probabilities, largest first, equal ones by index.  Beside sg_softmax_cross_entropy, whose loss is -logprob.
+ * logits [.., C], unit stride on C; tokens, logprob, entropy, lse: the leading extents (a rank-1 logits: one element),
+ * tokens SG_UINT or SG_INT read as unsigned with any strides, outputs dense; top_ids SG_UINT and top_logprobs: the leading
+ * extents and k, dense, both or neither, k = 1..64 and at most C.  Any output but lse may be NULL; logprob needs tokens.
+ * A token of C or more (-100 among them) is no token: its logprob is 0.  A logit of -inf has p = 0.  A row of nothing but
+ * -inf has lse = -inf, entropy 0 and every log probability -inf.  A NaN or +inf logit makes the row's lse, entropy and log
+ * probabilities NaN (the logprob of a row without a token stays 0); a NaN ranks below every number. */
+int sg_token_logprobs(sg_ctx *ctx, const sg_tensor *logits, const sg_tensor *tokens, float scale, const sg_tensor *logprob,
+                      const sg_tensor *entropy, const sg_tensor *lse, const sg_tensor *top_ids, const sg_tensor *top_logprobs);
+/* glogits_j = scale (g_logprob (delta_{j,token} - p_j) - g_entropy p_j (log p_j + entropy)) from the lse and entropy of the
+ * forward call.  g_logprob (needs tokens) and g_entropy (needs entropy): the leading extents, any strides, one of them at
+ * least; glogits: logits' extents, dense, and may be the very memory of dense logits.  A row without a token takes nothing
+ * from g_logprob; a logit of -inf has gradient 0, as has every logit of a row of nothing but -inf. */
+int sg_token_logprobs_grad(sg_ctx *ctx, const sg_tensor *logits, const sg_tensor *tokens, float scale, const sg_tensor *lse,
+                           const sg_tensor *entropy, const sg_tensor *g_logprob, const sg_tensor *g_entropy,
+                           const sg_tensor *glogits);
+
 /* ---- fused attention: the operator chain of MultiHeadAttention::pass (bert.rs:262-271) --------- */
 
 /* out = softmax_lastaxis(scale * (q . k^T) + addend) . v, i.e. matmul_batched (gemm.rs:53-104), the
@@ -350,6 +412,27 @@ int sg_layer_norm_lastaxis(sg_ctx *ctx, const sg_tensor *x, const sg_tensor *gam
  * as in the reference (reduce.rs:282), so a fully masked row gives the reference's 0/0. */
 int sg_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v,
                  const sg_tensor *addend, float scale, const sg_tensor *out);
+
+/* ---- cross attention: queries of one sequence over the states of another --------------------- */
+
+/* out = softmax(scale * (q . k^T)) . v over the visible keys, the shape of MultiHeadAttention::pass (bert.rs:262-271) with
+ * keys and values of an encoder: q, out [N, H, Lq, D]; k, v [N, G, Lk, D], G a divisor of H, query head h reading key head
+ * h / (H/G); unit stride on D, any strides elsewhere (separate_heads views, merged-heads outputs); D = 32 or 64.
+ * mask: NULL or fp32 [N, Lk], unit stride on Lk, any batch stride: key j of sequence b is visible unless mask[b, j] is 0.
+ * What a hidden key's k and v hold is not used, NaN or not.  A query without a visible key gives zeros and lse = -inf.
+ * The softmax shift is the row's largest visible score.  lse: NULL or dense [N, H, Lq], log of the row's sum, for the
+ * gradient.  A call with few query rows splits the keys over workgroups and joins the parts through a workspace of the
+ * context allocator (SG_ERR_OOM). */
+int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask,
+                       float scale, const sg_tensor *out, const sg_tensor *lse);
+/* Its gradient: with P = e^(scale q.k - lse), dP = gout . v^T and dS = P (dP - rowsum(gout out)):
+ * gq = scale dS . k, gk = scale dS^T . q, gv = P^T . gout, gk and gv summed over the query heads that share a key head;
+ * hidden keys and queries without a visible key get zeros.  out, lse: of the forward call; gout, gq as q, gk and gv as k
+ * (unit stride on D, any strides that keep elements apart).  Sums are in a fixed order: the same inputs give the same bits.
+ * Workspace from the context allocator (SG_ERR_OOM). */
+int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask,
+                            float scale, const sg_tensor *out, const sg_tensor *lse, const sg_tensor *gout,
+                            const sg_tensor *gq, const sg_tensor *gk, const sg_tensor *gv);
 
 /* ---- replay of a recorded launch sequence --------------------------------------------------- */
 

@@ -214,6 +214,11 @@ extern "C" {
     pub fn sg_unslice(ctx: *mut sg_ctx, axis: c_int, start: i64, x: *const sg_tensor, out: *const sg_tensor) -> c_int;
     pub fn sg_concat(ctx: *mut sg_ctx, axis: c_int, inputs: *const sg_tensor, n_in: c_int, out: *const sg_tensor) -> c_int;
 
+    // ---- embedding lookup and its gradient
+    pub fn sg_embedding(ctx: *mut sg_ctx, table: *const sg_tensor, ids: *const sg_tensor, scale: f32, out: *const sg_tensor) -> c_int;
+    pub fn sg_embedding_grad(ctx: *mut sg_ctx, gout: *const sg_tensor, ids: *const sg_tensor, scale: f32,
+                             gtable: *const sg_tensor) -> c_int;
+
     // ---- GEMM
     pub fn sg_gemm(ctx: *mut sg_ctx, transpose_a: c_int, transpose_b: c_int, a: *const sg_tensor, b: *const sg_tensor,
                    c: *const sg_tensor, epi: *const sg_gemm_epilogue) -> c_int;
@@ -242,6 +247,12 @@ extern "C" {
     // ---- optimizer step
     pub fn sg_adam_update(ctx: *mut sg_ctx, n_tensors: c_int, values: *const sg_tensor, grads: *const sg_tensor,
                           m: *const sg_tensor, v: *const sg_tensor, step: *const sg_tensor, h: *const sg_adam_hyper) -> c_int;
+    pub fn sg_adamw_update(ctx: *mut sg_ctx, n_tensors: c_int, values: *const sg_tensor, grads: *const sg_tensor,
+                           m: *const sg_tensor, v: *const sg_tensor, m_scale: *const sg_tensor, v_scale: *const sg_tensor,
+                           step: *const sg_tensor, h: *const sg_adam_hyper, seed: u32) -> c_int;
+    pub fn sg_adamw_state_read(ctx: *mut sg_ctx, n_tensors: c_int, m: *const sg_tensor, v: *const sg_tensor,
+                               m_scale: *const sg_tensor, v_scale: *const sg_tensor, m_out: *const sg_tensor,
+                               v_out: *const sg_tensor) -> c_int;
 
     // ---- fused row operators, attention
     pub fn sg_softmax_lastaxis(ctx: *mut sg_ctx, x: *const sg_tensor, addend: *const sg_tensor, out: *const sg_tensor) -> c_int;
@@ -249,8 +260,20 @@ extern "C" {
                                     loss: *const sg_tensor) -> c_int;
     pub fn sg_layer_norm_lastaxis(ctx: *mut sg_ctx, x: *const sg_tensor, gamma: *const sg_tensor, beta: *const sg_tensor,
                                   eps: f32, out: *const sg_tensor) -> c_int;
+    pub fn sg_token_logprobs(ctx: *mut sg_ctx, logits: *const sg_tensor, tokens: *const sg_tensor, scale: f32,
+                             logprob: *const sg_tensor, entropy: *const sg_tensor, lse: *const sg_tensor,
+                             top_ids: *const sg_tensor, top_logprobs: *const sg_tensor) -> c_int;
+    pub fn sg_token_logprobs_grad(ctx: *mut sg_ctx, logits: *const sg_tensor, tokens: *const sg_tensor, scale: f32,
+                                  lse: *const sg_tensor, entropy: *const sg_tensor, g_logprob: *const sg_tensor,
+                                  g_entropy: *const sg_tensor, glogits: *const sg_tensor) -> c_int;
     pub fn sg_attention(ctx: *mut sg_ctx, q: *const sg_tensor, k: *const sg_tensor, v: *const sg_tensor,
                         addend: *const sg_tensor, scale: f32, out: *const sg_tensor) -> c_int;
+    pub fn sg_cross_attention(ctx: *mut sg_ctx, q: *const sg_tensor, k: *const sg_tensor, v: *const sg_tensor,
+                              mask: *const sg_tensor, scale: f32, out: *const sg_tensor, lse: *const sg_tensor) -> c_int;
+    pub fn sg_cross_attention_grad(ctx: *mut sg_ctx, q: *const sg_tensor, k: *const sg_tensor, v: *const sg_tensor,
+                                   mask: *const sg_tensor, scale: f32, out: *const sg_tensor, lse: *const sg_tensor,
+                                   gout: *const sg_tensor, gq: *const sg_tensor, gk: *const sg_tensor,
+                                   gv: *const sg_tensor) -> c_int;
 
     // ---- replay of a recorded launch sequence
     pub fn sg_graph_begin(ctx: *mut sg_ctx) -> c_int;

@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "libsage_hip.so")
 MAX_RANK = 8
 MAX_MAP_INPUTS = 16
 MAX_EXPR = 128
+MAX_TOP = 64  # alternatives of sg_token_logprobs
 REFERENCE_CAPACITY_BYTES = 1000 * 1024 * 1024
 GEMM_NOALLOC_SCRATCH_BYTES = 32 << 20
 
@@ -106,6 +107,14 @@ PROTOTYPES = {
     "sg_rand_uniform": (C.c_int, [_CTX, C.c_uint32, C.c_uint32, _TP]),
     "sg_rand_normal": (C.c_int, [_CTX, C.c_uint32, C.c_uint32, _TP]),
     "sg_adam_update": (C.c_int, [_CTX, C.c_int, _TP, _TP, _TP, _TP, _TP, C.POINTER(sg_adam_hyper)]),
+    "sg_adamw_update": (C.c_int, [_CTX, C.c_int, _TP, _TP, _TP, _TP, _TP, _TP, _TP, C.POINTER(sg_adam_hyper), C.c_uint32]),
+    "sg_adamw_state_read": (C.c_int, [_CTX, C.c_int, _TP, _TP, _TP, _TP, _TP, _TP]),
+    "sg_embedding": (C.c_int, [_CTX, _TP, _TP, C.c_float, _TP]),
+    "sg_embedding_grad": (C.c_int, [_CTX, _TP, _TP, C.c_float, _TP]),
+    "sg_token_logprobs": (C.c_int, [_CTX, _TP, _TP, C.c_float, _TP, _TP, _TP, _TP, _TP]),
+    "sg_token_logprobs_grad": (C.c_int, [_CTX, _TP, _TP, C.c_float, _TP, _TP, _TP, _TP, _TP]),
+    "sg_cross_attention": (C.c_int, [_CTX, _TP, _TP, _TP, _TP, C.c_float, _TP, _TP]),
+    "sg_cross_attention_grad": (C.c_int, [_CTX, _TP, _TP, _TP, _TP, C.c_float, _TP, _TP, _TP, _TP, _TP, _TP]),
     "sg_attention": (C.c_int, [_CTX, _TP, _TP, _TP, _TP, C.c_float, _TP]),
 }
 

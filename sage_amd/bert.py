@@ -9,6 +9,7 @@ the configured eps, an optional segment table, classifier on token 0.
 """
 import numpy as np
 
+from . import nn
 from .layers import Dense, Dropout, Embedding, Gelu, Layer, LayerNorm, Relu, Sequential, Softmax
 from .tensor import FLOAT, UINT, Tensor
 from .var import Var, into_var
@@ -75,6 +76,41 @@ class MultiHeadAttention(Layer):
         av = self.merge_heads(att.matmul_batched(v))
         y = self.dense.pass_(av)
         return self.norm.pass_(y + x)
+
+
+class CrossAttention(Layer):
+    """MultiHeadAttention (bert.rs:206-314) whose keys and values come from an encoder's states: x [N, Lq, E], states
+    [N, Lk, E'], mask [N, Lk] (1 = visible, 0 = padding) or None.  `num_kv_heads` below `num_heads` shares each key head
+    among several query heads.  The reference has no decoder; projections, residual and norm are its own."""
+
+    def __init__(self, embed_dim, num_heads, layer_norm_eps=1e-5, states_dim=None, num_kv_heads=None, reference_exact=True):
+        self.num_heads, self.num_kv_heads = num_heads, num_heads if num_kv_heads is None else num_kv_heads
+        self.head_dim = embed_dim // num_heads
+        states_dim = embed_dim if states_dim is None else states_dim
+        self.query_proj = Dense(embed_dim, embed_dim)
+        self.key_proj = Dense(states_dim, self.num_kv_heads * self.head_dim)
+        self.value_proj = Dense(states_dim, self.num_kv_heads * self.head_dim)
+        self.dense = Dense(embed_dim, embed_dim)
+        self.norm = LayerNorm(2, layer_norm_eps, embed_dim, reference_exact)
+
+    def params(self):
+        return (self.query_proj.params() + self.key_proj.params() + self.value_proj.params() + self.dense.params() + self.norm.params())
+
+    def keys_values(self, states):
+        """The states' keys and values as [N, G, Lk, D]: a program that decodes token by token makes them once."""
+        split = lambda f: f.view([f.extent(0), f.extent(1), self.num_kv_heads, self.head_dim]).transpose(2, 1)  # noqa: E731
+        return split(self.key_proj.pass_(states)), split(self.value_proj.pass_(states))
+
+    def attend(self, x, k, v, mask=None):
+        n, l = x.extent(0), x.extent(1)
+        q = self.query_proj.pass_(x).view([n, l, self.num_heads, self.head_dim]).transpose(2, 1)
+        av = nn.cross_attention(q, k, v, mask).transpose(2, 1).view([n, l, self.num_heads * self.head_dim])
+        return self.norm.pass_(self.dense.pass_(av) + x)
+
+    def pass_(self, x, states, mask=None):
+        x, states = into_var(x), into_var(states)
+        k, v = self.keys_values(states)
+        return self.attend(x, k, v, mask)
 
 
 class BertLayer(Layer):

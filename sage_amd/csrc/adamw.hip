@@ -1,0 +1,363 @@
+// One AdamW step over many parameters, in place, with states in 32 or in 8 bits, for gfx950.
+//   m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g g
+//   value' = value - lr ((m' / (1 - beta1^t)) / (sqrt(v' / (1 - beta2^t)) + eps) + decay value)
+// Bound by memory: 28 bytes an element with states in 32 bits, 16 with states in 8.
+//
+// 8-bit states.  256 elements share a power of two, so scaling is an addition to exponent fields and exact, and a byte is
+// the top of a number's fp32 pattern: no division, no table.  v is never negative and gets the sign's bit for a fifth
+// exponent bit: it is a square, and 32 octaves of v are the 16 octaves of g that the 4 exponent bits of m cover.
+// Bytes keep 3 mantissa bits (steps of 6 to 12 %), while a step moves v by 1 - beta2 = 0.1 %: rounded to nearest it would
+// stay where it is for good.  So 16 bits of noise, a hash of element, step and seed, are added below the kept bits before
+// the rest is cut off, which rounds up or down with the chances that keep the mean.
+// The moments are formed without contraction (this file is compiled with -ffp-contract=off): which byte a moment becomes
+// hangs on its last bit.
+#include "rows.h"
+
+#include <cmath>
+
+namespace {
+
+constexpr int MAX_TENSORS = 56;       // table entries per launch: the arguments stay below 4 KB
+constexpr uint32_t CHUNK = 4096;      // elements per workgroup: 4 wavefronts x 4 blocks of 256
+constexpr uint32_t BLOCK = 256;       // elements that share a scale: 4 for each lane of a wavefront
+constexpr int MIN_EXPONENT = 33;      // the smallest number of a block, 31 octaves below its largest, stays normal
+constexpr uint32_t V_TOP = 255, M_TOP = 127;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct Entry {
+    float *value;
+    const float *grad;
+    void *m, *v;
+    float *m_scale, *v_scale;
+    uint32_t n, first_chunk;
+    uint32_t vec;  // all pointers of 4 elements 16-byte aligned
+};
+
+struct StepArgs {
+    Entry t[MAX_TENSORS];
+    int count;
+    const float *step;
+    float lr, beta1, beta2, c1, c2, eps, decay, ln1, ln2;
+    uint32_t seed;
+};
+
+struct ReadArgs {
+    Entry t[MAX_TENSORS];  // value: m_out, grad: v_out
+    int count;
+};
+
+// The entry a workgroup belongs to: the last one that starts at or before it.
+__device__ __forceinline__ int find_entry(const Entry *t, int count, uint32_t chunk) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t[mid].first_chunk <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+struct Correction {
+    float first, second;  // 1 / (1 - beta1^t), 1 / (1 - beta2^t)
+};
+
+// 1 - beta^t as -expm1(t ln beta): for small t the difference would lose what it is made of
+__device__ __forceinline__ Correction correction(const StepArgs &a) {
+    const float t = *a.step;
+    return {-1.0f / expm1f(t * a.ln1), -1.0f / expm1f(t * a.ln2)};
+}
+
+__device__ __forceinline__ void step_element(float &value, float g, float &m, float &v, const StepArgs &a, const Correction &c) {
+    m = m * a.beta1 + g * a.c1;
+    v = v * a.beta2 + g * g * a.c2;
+    value = value - a.lr * (m * c.first / (sqrtf(v * c.second) + a.eps) + a.decay * value);
+}
+
+__global__ void __launch_bounds__(256) adamw_kernel(const StepArgs a) {
+    const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
+    const Correction c = correction(a);
+    const uint32_t base = (blockIdx.x - t.first_chunk) * CHUNK;
+    float *mp = (float *)t.m, *vp = (float *)t.v;
+#pragma unroll
+    for (uint32_t k = 0; k < CHUNK / 1024; ++k) {
+        const uint32_t i = base + k * 1024 + threadIdx.x * 4;
+        if (i >= t.n) return;
+        if (t.vec && i + 4 <= t.n) {
+            f32x4 x = *reinterpret_cast<const f32x4 *>(t.value + i), m = *reinterpret_cast<const f32x4 *>(mp + i), v = *reinterpret_cast<const f32x4 *>(vp + i);
+            const f32x4 g = *reinterpret_cast<const f32x4 *>(t.grad + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float xj = x[j], mj = m[j], vj = v[j];
+                step_element(xj, g[j], mj, vj, a, c);
+                x[j] = xj;
+                m[j] = mj;
+                v[j] = vj;
+            }
+            *reinterpret_cast<f32x4 *>(t.value + i) = x;
+            *reinterpret_cast<f32x4 *>(mp + i) = m;
+            *reinterpret_cast<f32x4 *>(vp + i) = v;
+        } else {
+            for (uint32_t j = i; j < i + 4 && j < t.n; ++j) {
+                float x = t.value[j], m = mp[j], v = vp[j];
+                step_element(x, t.grad[j], m, v, a, c);
+                t.value[j] = x;
+                mp[j] = m;
+                vp[j] = v;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t noise(uint32_t i, uint32_t salt) {
+    uint32_t h = i * 0x9E3779B9u + salt;
+    h = (h ^ (h >> 16)) * 0x82D3099Fu;
+    h = (h ^ (h >> 15)) * 0x2ACAE79Fu;
+    return h ^ (h >> 16);
+}
+
+// e: exponent field of the block's scale; 255 marks a block that holds NaN
+__device__ __forceinline__ float decode(uint32_t low, uint32_t e, uint32_t top) {
+    if (e == 255) return __builtin_nanf("");
+    return low ? __uint_as_float((low + e * 8 + 7 - top) << 20) : 0.0f;
+}
+__device__ __forceinline__ float decode_m(uint32_t byte, uint32_t e) {
+    const float x = decode(byte & 127u, e, M_TOP);
+    return byte & 128u ? -x : x;
+}
+
+__device__ __forceinline__ uint32_t encode(uint32_t bits, uint32_t noise16, uint32_t e, int top) {
+    const int c = (int)((bits + (noise16 << 4)) >> 20) - (int)(e * 8 + 7) + top;
+    return (uint32_t)(c < 0 ? 0 : c > top ? top : c);
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t y = (uint32_t)__shfl_xor((int)x, o, 64);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+
+// exponent field of a block's scale from the largest of its patterns without signs
+__device__ __forceinline__ uint32_t scale_exponent(uint32_t largest) {
+    const uint32_t e = (largest + 0xFFFFFu) >> 23;
+    return e < MIN_EXPONENT ? MIN_EXPONENT : e > 255u ? 255u : e;
+}
+
+// A wavefront takes a block of 256 elements, a lane 4 of them and one word of either state.
+__global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
+    const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
+    const Correction c = correction(a);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t salt = a.seed + (uint32_t)*a.step * 0xAC502949u;
+    uint32_t *mp = (uint32_t *)t.m, *vp = (uint32_t *)t.v;
+#pragma unroll
+    for (uint32_t k = 0; k < CHUNK / (4 * BLOCK); ++k) {
+        const uint32_t block = (blockIdx.x - t.first_chunk) * (CHUNK / BLOCK) + k * 4 + wave;
+        if (block * BLOCK >= t.n) return;  // the whole wavefront
+        const uint32_t i = block * BLOCK + lane * 4;
+        const uint32_t left = i < t.n ? (t.n - i < 4 ? t.n - i : 4) : 0;
+        float x[4] = {}, g[4] = {}, m[4], v[4];
+        uint32_t mw = 0, vw = 0;
+        if (left == 4 && t.vec) {
+            const f32x4 x4 = *reinterpret_cast<const f32x4 *>(t.value + i), g4 = *reinterpret_cast<const f32x4 *>(t.grad + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { x[j] = x4[j]; g[j] = g4[j]; }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (j < left) { x[j] = t.value[i + j]; g[j] = t.grad[i + j]; }
+        }
+        if (left) { mw = mp[i / 4]; vw = vp[i / 4]; }
+        const uint32_t me = __float_as_uint(t.m_scale[block]) >> 23 & 255u, ve = __float_as_uint(t.v_scale[block]) >> 23 & 255u;
+        uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            m[j] = decode_m(mw >> (8 * j) & 255u, me);
+            v[j] = decode(vw >> (8 * j) & 255u, ve, V_TOP);
+            step_element(x[j], g[j], m[j], v[j], a, c);
+            if (j < left) {
+                const uint32_t mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+                mtop = mtop > mb ? mtop : mb;
+                vtop = vtop > vb ? vtop : vb;
+            }
+        }
+        const uint32_t me2 = scale_exponent(wave_max(mtop)), ve2 = scale_exponent(wave_max(vtop));
+        mw = vw = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (j >= left) continue;
+            const uint32_t h = noise(i + j, salt);
+            const uint32_t mb = __float_as_uint(m[j]), vb = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+            uint32_t mc = encode(mb & 0x7FFFFFFFu, h & 0xFFFFu, me2, (int)M_TOP);
+            if (mc && (mb >> 31)) mc |= 128u;
+            uint32_t vc = encode(vb, h >> 16, ve2, (int)V_TOP);
+            if (vb && !vc) vc = 1;
+            mw |= mc << (8 * j);
+            vw |= vc << (8 * j);
+        }
+        if (left == 4 && t.vec) *reinterpret_cast<f32x4 *>(t.value + i) = f32x4{x[0], x[1], x[2], x[3]};
+        else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (j < left) t.value[i + j] = x[j];
+        }
+        if (left) { mp[i / 4] = mw; vp[i / 4] = vw; }
+        if (lane == 0) {
+            t.m_scale[block] = __uint_as_float(me2 == 255 ? 0x7FC00000u : me2 << 23);
+            t.v_scale[block] = __uint_as_float(ve2 == 255 ? 0x7FC00000u : ve2 << 23);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) adamw_state_read_kernel(const ReadArgs a) {
+    const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
+    const uint32_t base = (blockIdx.x - t.first_chunk) * CHUNK;
+    const uint32_t *mp = (const uint32_t *)t.m, *vp = (const uint32_t *)t.v;
+    float *mo = t.value, *vo = const_cast<float *>(t.grad);
+#pragma unroll
+    for (uint32_t k = 0; k < CHUNK / 1024; ++k) {
+        const uint32_t i = base + k * 1024 + threadIdx.x * 4;
+        if (i >= t.n) return;
+        const uint32_t mw = mp[i / 4], vw = vp[i / 4];
+        const uint32_t me = __float_as_uint(t.m_scale[i / BLOCK]) >> 23 & 255u, ve = __float_as_uint(t.v_scale[i / BLOCK]) >> 23 & 255u;
+        f32x4 m, v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m[j] = decode_m(mw >> (8 * j) & 255u, me);
+            v[j] = decode(vw >> (8 * j) & 255u, ve, V_TOP);
+        }
+        if (t.vec && i + 4 <= t.n) {
+            *reinterpret_cast<f32x4 *>(mo + i) = m;
+            *reinterpret_cast<f32x4 *>(vo + i) = v;
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (i + j < t.n) { mo[i + j] = m[j]; vo[i + j] = v[j]; }
+        }
+    }
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p) % 16 == 0; }
+float *f32_ptr(const sg_tensor *t) { return (float *)t->base + t->offset; }
+
+int check_dense(sg_ctx *ctx, const sg_tensor *t, int dtype, int64_t n, const char *who) {
+    const int rc = sg_validate_tensor(ctx, t, who);
+    if (rc != SG_OK) return rc;
+    if (t->dtype != dtype) return sg_fail(ctx, SG_ERR_DTYPE, "%s: %s expected", who, dtype == SG_FLOAT ? "fp32" : "uint");
+    if (!sg_is_dense(t)) return sg_fail(ctx, SG_ERR_SHAPE, "%s: must be dense row-major", who);
+    if (n && sg_numel(t) != n) return sg_fail(ctx, SG_ERR_SHAPE, "%s: %lld elements, expected %lld", who, (long long)sg_numel(t), (long long)n);
+    return SG_OK;
+}
+
+int check_state8(sg_ctx *ctx, const sg_tensor *m, const sg_tensor *v, const sg_tensor *ms, const sg_tensor *vs, int64_t n) {
+    int rc;
+    if ((rc = check_dense(ctx, m, SG_UINT, (n + 3) / 4, "AdamW first moment")) != SG_OK) return rc;
+    if ((rc = check_dense(ctx, v, SG_UINT, (n + 3) / 4, "AdamW second moment")) != SG_OK) return rc;
+    if ((rc = check_dense(ctx, ms, SG_FLOAT, (n + BLOCK - 1) / BLOCK, "AdamW first moment's scale")) != SG_OK) return rc;
+    return check_dense(ctx, vs, SG_FLOAT, (n + BLOCK - 1) / BLOCK, "AdamW second moment's scale");
+}
+
+// Fills one launch's table from tensor `first` on; returns the index behind the last one taken, the workgroups in *chunks.
+template <class Fill>
+int fill_table(Entry *table, int *count, uint32_t *chunks, int first, int n_tensors, const sg_tensor *sizes, Fill fill) {
+    uint64_t at = 0;
+    int i = first;
+    for (*count = 0; i < n_tensors && *count < MAX_TENSORS; ++i) {
+        const int64_t n = sg_numel(&sizes[i]);
+        const uint64_t need = (uint64_t)(n + CHUNK - 1) / CHUNK;
+        if (at + need >= (1ull << 31)) break;  // the rest in a launch of its own
+        Entry &e = table[(*count)++];
+        fill(e, i);
+        e.n = (uint32_t)n;
+        e.first_chunk = (uint32_t)at;
+        at += need;
+    }
+    *chunks = (uint32_t)at;
+    return i;
+}
+
+}  // namespace
+
+extern "C" int sg_adamw_update(sg_ctx *ctx, int n_tensors, const sg_tensor *values, const sg_tensor *grads, const sg_tensor *m, const sg_tensor *v,
+                               const sg_tensor *m_scale, const sg_tensor *v_scale, const sg_tensor *step, const sg_adam_hyper *h, uint32_t seed) {
+    if (n_tensors < 0) return sg_fail(ctx, SG_ERR_ARG, "sg_adamw_update: %d tensors", n_tensors);
+    if (n_tensors && (!values || !grads || !m || !v)) return sg_fail(ctx, SG_ERR_ARG, "sg_adamw_update: null tensor array");
+    if (!h || !m_scale != !v_scale) return sg_fail(ctx, SG_ERR_ARG, "sg_adamw_update: %s", h ? "one scale array without the other" : "null scalars");
+    if (!(h->beta1 >= 0.0f && h->beta1 < 1.0f && h->beta2 >= 0.0f && h->beta2 < 1.0f)) return sg_fail(ctx, SG_ERR_ARG, "sg_adamw_update: betas must be in [0, 1)");
+    int rc;
+    if ((rc = check_dense(ctx, step, SG_FLOAT, 1, "sg_adamw_update step")) != SG_OK) return rc;
+    const bool eight = m_scale != nullptr;
+    // everything is checked before the first launch: a failed call changes nothing
+    for (int i = 0; i < n_tensors; ++i) {
+        if ((rc = check_dense(ctx, &values[i], SG_FLOAT, 0, "sg_adamw_update value")) != SG_OK) return rc;
+        const int64_t n = sg_numel(&values[i]);
+        if ((rc = check_dense(ctx, &grads[i], SG_FLOAT, n, "sg_adamw_update grad")) != SG_OK) return rc;
+        if (eight) {
+            if ((rc = check_state8(ctx, &m[i], &v[i], &m_scale[i], &v_scale[i], n)) != SG_OK) return rc;
+        } else {
+            if ((rc = check_dense(ctx, &m[i], SG_FLOAT, n, "sg_adamw_update first moment")) != SG_OK) return rc;
+            if ((rc = check_dense(ctx, &v[i], SG_FLOAT, n, "sg_adamw_update second moment")) != SG_OK) return rc;
+        }
+    }
+    if (!ctx) return SG_ERR_ARG;
+    sg_device_guard guard(ctx);
+    for (int first = 0; first < n_tensors;) {
+        StepArgs a{};
+        a.step = f32_ptr(step);
+        a.lr = h->lr; a.beta1 = h->beta1; a.beta2 = h->beta2; a.c1 = h->one_minus_beta1; a.c2 = h->one_minus_beta2;
+        a.eps = h->eps; a.decay = h->weight_decay;
+        a.ln1 = (float)std::log((double)h->beta1);
+        a.ln2 = (float)std::log((double)h->beta2);
+        a.seed = seed;
+        uint32_t chunks = 0;
+        first = fill_table(a.t, &a.count, &chunks, first, n_tensors, values, [&](Entry &e, int i) {
+            e.value = f32_ptr(&values[i]);
+            e.grad = f32_ptr(&grads[i]);
+            e.m = f32_ptr(&m[i]);
+            e.v = f32_ptr(&v[i]);
+            e.vec = aligned16(e.value) && aligned16(e.grad) && (eight || (aligned16(e.m) && aligned16(e.v)));
+            if (eight) {
+                e.m_scale = f32_ptr(&m_scale[i]);
+                e.v_scale = f32_ptr(&v_scale[i]);
+            }
+        });
+        if (eight) hipLaunchKernelGGL(adamw8_kernel, dim3(chunks), dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL(adamw_kernel, dim3(chunks), dim3(256), 0, ctx->stream, a);
+        SG_CHECK_LAUNCH(ctx, "adamw");
+    }
+    return SG_OK;
+}
+
+extern "C" int sg_adamw_state_read(sg_ctx *ctx, int n_tensors, const sg_tensor *m, const sg_tensor *v, const sg_tensor *m_scale, const sg_tensor *v_scale,
+                                   const sg_tensor *m_out, const sg_tensor *v_out) {
+    if (n_tensors < 0) return sg_fail(ctx, SG_ERR_ARG, "sg_adamw_state_read: %d tensors", n_tensors);
+    if (n_tensors && (!m || !v || !m_scale || !v_scale || !m_out || !v_out)) return sg_fail(ctx, SG_ERR_ARG, "sg_adamw_state_read: null tensor array");
+    int rc;
+    for (int i = 0; i < n_tensors; ++i) {
+        if ((rc = check_dense(ctx, &m_out[i], SG_FLOAT, 0, "sg_adamw_state_read m_out")) != SG_OK) return rc;
+        const int64_t n = sg_numel(&m_out[i]);
+        if ((rc = check_dense(ctx, &v_out[i], SG_FLOAT, n, "sg_adamw_state_read v_out")) != SG_OK) return rc;
+        if ((rc = check_state8(ctx, &m[i], &v[i], &m_scale[i], &v_scale[i], n)) != SG_OK) return rc;
+    }
+    if (!ctx) return SG_ERR_ARG;
+    sg_device_guard guard(ctx);
+    for (int first = 0; first < n_tensors;) {
+        ReadArgs a{};
+        uint32_t chunks = 0;
+        first = fill_table(a.t, &a.count, &chunks, first, n_tensors, m_out, [&](Entry &e, int i) {
+            e.value = f32_ptr(&m_out[i]);
+            e.grad = f32_ptr(&v_out[i]);
+            e.m = f32_ptr(&m[i]);
+            e.v = f32_ptr(&v[i]);
+            e.m_scale = f32_ptr(&m_scale[i]);
+            e.v_scale = f32_ptr(&v_scale[i]);
+            e.vec = aligned16(e.value) && aligned16(e.grad);
+        });
+        hipLaunchKernelGGL(adamw_state_read_kernel, dim3(chunks), dim3(256), 0, ctx->stream, a);
+        SG_CHECK_LAUNCH(ctx, "adamw_state_read");
+    }
+    return SG_OK;
+}

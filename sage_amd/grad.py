@@ -22,6 +22,7 @@ import math
 
 from . import nn
 from . import var as V
+from .shape import Shape
 from .tensor import FLOAT
 from .var import Var, scalar
 
@@ -213,7 +214,29 @@ def op_grad(v, gy):
         return _through_composition(v, gy, nn.layer_norm_composed(x[0], [x[0].rank - 1], x[1], x[2], a["eps"]))
     if op == "matmul_nd":
         return _through_composition(v, gy, V.matmul_batched_composed(x[0], x[1]))
+    # ---- operators of language models: one kernel for the gradient
+    if op == "embedding":
+        return [Var(Shape(x[0].extents), FLOAT, "embedding_grad", [gy, x[1]], dict(a)), None]
+    if op == "embedding_grad":  # linear: its adjoint is the lookup
+        return [nn.embedding(gy, x[1], a["scale"]), None]
+    if op == "token_logprob":
+        return [nn.token_logprobs_grad(x[0], x[1], x[2], g_logprob=gy), None, None]
+    if op == "token_entropy":
+        return [nn.token_logprobs_grad(x[0], x[1], g_entropy=gy), None]
+    if op == "cross_attention":
+        gq = Var(Shape(x[0].extents), FLOAT, "cross_attention_grad", [*x, v, gy], dict(a))
+        return [gq, V.part(gq, "gk", x[1].extents), V.part(gq, "gv", x[2].extents), None][:len(x)]
     raise ValueError(f"no gradient rule for operator {op}")
+
+
+def _accumulate(new, old):
+    """new + old (var.rs:80-90); where one is the gradient of a row's log probability and the other that of the same row's
+    entropy, both come out of one pass over the logits."""
+    if (new.op == old.op == "token_logprobs_grad" and new.inputs[:2] == old.inputs[:2]
+            and new.attrs["logprob"] != old.attrs["logprob"] and new.attrs["entropy"] != old.attrs["entropy"]):
+        lp, en = (new, old) if new.attrs["logprob"] else (old, new)
+        return nn.token_logprobs_grad(*lp.inputs[:3], g_logprob=lp.inputs[3], g_entropy=en.inputs[2])
+    return new + old
 
 
 def grad(y, xs, seed=None, allow_unreached=False):
@@ -244,7 +267,7 @@ def grad(y, xs, seed=None, allow_unreached=False):
                 counter += 1
                 grads[id(xi)] = gx
             else:
-                grads[id(xi)] = gx + grads[id(xi)]
+                grads[id(xi)] = _accumulate(gx, grads[id(xi)])
     out = []
     for x in xs:
         if id(x) not in grads:

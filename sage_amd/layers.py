@@ -98,10 +98,12 @@ class Conv2d(Layer):
 
 
 class Embedding(Layer):
-    """layers.rs:406-463: ids -> view [B*L,1] -> expand [B*L,E] (stride 0) -> gather(weight, ., 0)."""
+    """layers.rs:406-463: ids -> view [B*L,1] -> expand [B*L,E] (stride 0) -> gather(weight, ., 0).  With a `scale` (a
+    decoder's sqrt(embedding_dim), say; 1.0 for none) the lookup is nn.embedding: ids of any rank, ids outside the table
+    stand for no token, and the gradient adds each row's tokens in a fixed order."""
 
-    def __init__(self, num_embeddings, embedding_dim):
-        self.num_embeddings, self.embedding_dim = num_embeddings, embedding_dim
+    def __init__(self, num_embeddings, embedding_dim, scale=None):
+        self.num_embeddings, self.embedding_dim, self.scale = num_embeddings, embedding_dim, scale
         self.weight = Var.empty([num_embeddings, embedding_dim]).name("embedding.weight")
 
     def params(self):
@@ -114,6 +116,8 @@ class Embedding(Layer):
     def pass_(self, idx):
         idx = into_var(idx)
         e = self.embedding_dim
+        if self.scale is not None:
+            return nn.embedding(self.weight, idx, self.scale).name("embedding")
         if idx.rank > 1:
             b, l = idx.extent(0), idx.extent(1)
             i = idx.view([b * l, 1]).expand([b * l, e])

@@ -5,10 +5,14 @@ single graph nodes that the backend runs as one fused row kernel; in every other
 with `var.set_fusion(False)` — they are the reference's compositions of maps and reductions, op for
 op.  Both forms are compared against each other and against the CPU oracle by the parity tests.
 """
+from collections import namedtuple
+
+import numpy as np
+
 from . import abi
 from .shape import Shape, norm_axes
 from .tensor import FLOAT, UINT, INT
-from .var import Var, fusion_enabled, gt, into_var
+from .var import Var, fusion_enabled, gt, into_var, part
 
 
 def relu(x):
@@ -91,3 +95,84 @@ def accuracy(logits, labels):
     hit = logits.argmax(1, True)
     from .var import eq
     return eq(hit, labels).sum(0, False).float() / float(logits.extents[0])
+
+
+# ----------------------------------------------------------------------------- operators of language models
+# These have one kernel each and no composition: they run the same with fusion on and off.
+def embedding(table, ids, scale=1.0):
+    """scale * table[ids]: [V, E] and ids of rank 1..7 (uint or int) -> ids' extents and E.  An id outside 0..V-1 (-1, say)
+    is no token: its row is zero and it adds nothing to the gradient.  Embedding::pass (layers.rs:406-463) gathers
+    through an expanded index tensor and its gradient scatters with additions in any order; here the gradient sorts the
+    tokens and adds each row's in a fixed order."""
+    table, ids = into_var(table), into_var(ids)
+    if table.dtype != FLOAT or ids.dtype not in (UINT, INT):
+        raise abi.DTypeError(abi.ERR_DTYPE, "embedding: a float table and uint or int ids expected")
+    if table.rank != 2 or ids.rank >= abi.MAX_RANK:
+        raise abi.ShapeError(abi.ERR_SHAPE, "embedding: a [V, E] table and ids of rank 1..7 expected")
+    return Var(Shape(list(ids.extents) + [table.extents[1]]), FLOAT, "embedding", [table, ids], {"scale": float(np.float32(scale))})
+
+
+TokenLogprobs = namedtuple("TokenLogprobs", "logprob entropy lse top_ids top_logprobs")
+
+
+def token_logprobs(logits, tokens=None, top=0, scale=1.0):
+    """Log probabilities under softmax(scale * logits) over the last axis: of `tokens` (uint or int, the leading extents),
+    the entropy, the log of the sum of exponentials and, with top > 0, the `top` most likely indexes with their log
+    probabilities, largest first and equal ones by index.  A token outside the vocabulary (-100, say) is no token: its
+    log probability is 0 and has no gradient.  logprob and entropy have gradients; the rest is for reading.
+    -logprob is softmax_cross_entropy (nn.rs:70-82)."""
+    logits = into_var(logits)
+    if logits.dtype != FLOAT:
+        raise abi.DTypeError(abi.ERR_DTYPE, "token_logprobs: float logits expected")
+    lead = list(logits.extents[:-1]) or [1]
+    ins = [logits]
+    if tokens is not None:
+        tokens = into_var(tokens)
+        if tokens.dtype not in (UINT, INT):
+            raise abi.DTypeError(abi.ERR_DTYPE, "token_logprobs: uint or int tokens expected")
+        if list(tokens.extents) != lead:
+            raise abi.ShapeError(abi.ERR_SHAPE, f"token_logprobs: tokens {tokens.extents} for logits {logits.extents}")
+        ins.append(tokens)
+    scale = float(np.float32(scale))
+    if not 0.0 < scale < float("inf"):
+        raise abi.SageError(abi.ERR_ARG, "token_logprobs: scale must be positive and finite")
+    if not 0 <= top <= min(abi.MAX_TOP, logits.extents[-1]):
+        raise abi.ShapeError(abi.ERR_SHAPE, f"token_logprobs: {top} alternatives of {logits.extents[-1]} (at most {abi.MAX_TOP})")
+    lse = Var(Shape(lead), FLOAT, "token_lse", ins, {"scale": scale, "top": int(top)})
+    tail = list(logits.extents[:-1]) + [top]
+    return TokenLogprobs(
+        Var(Shape(lead), FLOAT, "token_logprob", [logits, lse, tokens]) if tokens is not None else None,
+        Var(Shape(lead), FLOAT, "token_entropy", [logits, lse]),
+        lse,
+        part(lse, "top_ids", tail, UINT) if top else None,
+        part(lse, "top_logprobs", tail, FLOAT) if top else None)
+
+
+def token_logprobs_grad(logits, lse, tokens=None, g_logprob=None, g_entropy=None):
+    """The gradient of token_logprobs: the logits', from those of its log probabilities and entropies."""
+    ins = [logits, lse] + [v for v in (tokens, g_logprob, g_entropy) if v is not None]
+    return Var(Shape(logits.extents), FLOAT, "token_logprobs_grad", ins, {"logprob": g_logprob is not None, "entropy": g_entropy is not None})
+
+
+def cross_attention(q, k, v, mask=None, scale=None):
+    """softmax(scale * q . k^T) . v over the keys that `mask` ([N, Lk], 0 = hidden) leaves visible: q [N, H, Lq, D], k and v
+    [N, G, Lk, D] with G dividing H (query head h reads key head h / (H/G)), D = 32 or 64, scale 1/sqrt(D) by default.
+    A query without a visible key gives zeros; what hidden keys hold is not used.  MultiHeadAttention::pass
+    (bert.rs:262-271) with the keys and values of another sequence, and a gradient of its own."""
+    q, k, v = into_var(q), into_var(k), into_var(v)
+    ins = [q, k, v]
+    if mask is not None:
+        ins.append(into_var(mask))
+    if any(x.dtype != FLOAT for x in ins):
+        raise abi.DTypeError(abi.ERR_DTYPE, "cross_attention: float operands expected")
+    if q.rank != 4 or k.rank != 4 or v.extents != k.extents:
+        raise abi.ShapeError(abi.ERR_SHAPE, "cross_attention: q [N, H, Lq, D], k and v [N, G, Lk, D] expected")
+    n, h, _, d = q.extents
+    if k.extents[0] != n or k.extents[3] != d or h % k.extents[1] != 0:
+        raise abi.ShapeError(abi.ERR_SHAPE, f"cross_attention: q {q.extents} does not go with k {k.extents}")
+    if d not in (32, 64):
+        raise abi.ShapeError(abi.ERR_SHAPE, f"cross_attention: head size {d} (32 and 64 are built)")
+    if mask is not None and list(ins[3].extents) != [n, k.extents[2]]:
+        raise abi.ShapeError(abi.ERR_SHAPE, f"cross_attention: mask {ins[3].extents}, expected {[n, k.extents[2]]}")
+    scale = 1.0 / np.sqrt(d) if scale is None else scale
+    return Var(Shape(q.extents), FLOAT, "cross_attention", ins, {"scale": float(np.float32(scale))})

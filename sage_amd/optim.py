@@ -30,6 +30,11 @@ def _one_minus(x):
     return float(np.float32(1.0) - np.float32(x))
 
 
+def _dense(t, ctx):
+    """t, copied unless it is dense."""
+    return t if t.is_dense() else Var.new(t).copy().eval(ctx)
+
+
 def _value(grad, ctx):
     if grad.value is None:
         evaluate(ctx, [grad])
@@ -213,3 +218,98 @@ class Adam(Optimizer):
         prog.calls += tail.calls
         prog.keep = tail
         return prog
+
+
+class AdamW(Optimizer):
+    """Adam (optim.rs:98-178) with the weight decay applied to the value instead of the gradient, all parameters in one
+    sg_adamw_update:
+        m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+        value -= lr ((m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay value)
+    with both moments zero in front of the first update and t = 1 in it.  state_bits=8 keeps each moment in a byte (blocks of 256
+    elements share a power of two, rounding up or down by a hash of element, step and `seed`): 2 bytes a parameter
+    instead of 8.  Parameters and gradients are fp32."""
+
+    def __init__(self, lr, beta1=0.9, beta2=0.999, eps=1e-08, weight_decay=0.01, state_bits=32, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits is 8 or 32")
+        self.lr, self.beta1, self.beta2, self.eps = float(lr), float(beta1), float(beta2), float(eps)
+        self.weight_decay, self.state_bits, self.seed = float(weight_decay), int(state_bits), int(seed) & 0xFFFFFFFF
+        self.t = None
+        self.states = {}  # parameter -> its state tensors: (m, v) or (m, v, m_scale, v_scale)
+
+    def init(self, ctx):
+        import numpy as np
+        self.states.clear()
+        self.t = Tensor.from_numpy(ctx, np.ones(1, np.float32))
+
+    def _state(self, param, ctx):
+        import numpy as np
+        if param not in self.states:
+            n = param.size()
+            if self.state_bits == 32:
+                zeros = [np.zeros(n, np.float32)] * 2
+            else:
+                zeros = [np.zeros((n + 3) // 4, np.uint32)] * 2 + [np.zeros((n + 255) // 256, np.float32)] * 2
+            self.states[param] = tuple(Tensor.from_numpy(ctx, z) for z in zeros)
+        return self.states[param]
+
+    def _call(self, grads, grad_tensors, ctx):
+        """The arguments of sg_adamw_update behind the context, and what has to live as long as they are used."""
+        from . import abi
+        cols = [[] for _ in range(2 + (2 if self.state_bits == 32 else 4))]
+        for param, g in zip(grads, grad_tensors):
+            if not param.is_data():
+                raise TypeError("param is not data tensor")
+            if g.extents != param.extents:
+                raise abi.ShapeError(abi.ERR_SHAPE, f"AdamW: gradient {g.extents} for a parameter {param.extents}")
+            if not param.value.is_dense():
+                param.set(_dense(param.value, ctx))
+            for col, x in zip(cols, (param.value, g) + self._state(param, ctx)):
+                col.append(x)
+        n = len(grads)
+        arrays = [(abi.sg_tensor * max(n, 1))(*[x.c() for x in col]) for col in cols]
+        hyper = abi.sg_adam_hyper(self.lr, self.beta1, self.beta2, _one_minus(self.beta1), _one_minus(self.beta2), self.eps, self.weight_decay)
+        scales = arrays[4:] or [None, None]
+        args = (C.c_int(n), *arrays[:4], *scales, C.byref(self.t.c()), C.byref(hyper), C.c_uint32(self.seed))
+        return args, [cols, arrays, hyper, self.t]
+
+    def update(self, grads, ctx):
+        if self.t is None:
+            self.init(ctx)
+        args, _ = self._call(grads, [_dense(_value(g, ctx), ctx) for g in grads.values()], ctx)
+        ctx.launches += 1
+        ctx.check(ctx._lib.sg_adamw_update(ctx.handle, *args))
+        params_changed()
+        t = (Var.new(self.t) + 1.0).eval(ctx)
+        ctx.check(ctx._lib.sg_memcpy_d2d(ctx.handle, C.c_void_p(self.t.buf.ptr), C.c_void_p(t.buf.ptr), 4))
+
+    def compile(self, grads, ctx):
+        """As Optimizer.compile: building the program performs one update; the state, t among it, is shared with `update`."""
+        from .var import Program
+        if self.t is None:
+            self.init(ctx)
+        values = [_value(g, ctx) for g in grads.values()]
+        strided = [Var.new(t).copy() for t in values if not t.is_dense()]
+        prog = Program(ctx, strided)  # their copies, made again on every run
+        copies = iter(prog.outputs)
+        args, keep = self._call(grads, [t if t.is_dense() else next(copies) for t in values], ctx)
+        lib = ctx._lib
+        ctx.check(lib.sg_adamw_update(ctx.handle, *args))
+        prog.calls.append((lib.sg_adamw_update, args, keep))
+        tail = _compile(ctx, [(Var.new(self.t) + 1.0, self.t)])
+        prog.calls += tail.calls
+        prog.keep = tail
+        prog.changes_params = True
+        params_changed()
+        return prog
+
+    def state(self, param, ctx):
+        """(m, v) of a parameter as fp32 tensors, whatever the bits they are held in."""
+        from . import abi
+        s = self.states[param]
+        if self.state_bits == 32:
+            return s
+        out = tuple(Tensor.uninit(ctx, param.extents) for _ in range(2))
+        arrays = [(abi.sg_tensor * 1)(x.c()) for x in s + out]
+        ctx.check(ctx._lib.sg_adamw_state_read(ctx.handle, 1, *arrays))
+        return out

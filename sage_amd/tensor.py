@@ -93,6 +93,7 @@ class Tensor:
         self.buf = buf
         self.dtype = dtype
         self.shape = shape
+        self.parts = None  # further outputs of the operator that made this tensor, by name
 
     # ---- construction / readback (Tensor::new + to_device, tensor.rs:280-309; Buffer::read)
     @staticmethod

@@ -637,6 +637,12 @@ def batch_norm_2d(x, gamma, beta, mean_, var_, eps):
     return into_var(gamma) * xc + beta
 
 
+# ----------------------------------------------------------------------------- operators with several outputs
+def part(v, name, extents, dtype=FLOAT):
+    """One of the outputs that v's operator has beside its own tensor (`Tensor.parts`)."""
+    return Var(Shape(list(extents)), dtype, "part", [v], {"name": name})
+
+
 # ----------------------------------------------------------------------------- evaluation
 def _lit_bits(value, dtype):
     np_t = {FLOAT: np.float32, INT: np.int32, UINT: np.uint32}[dtype]
@@ -1178,7 +1184,10 @@ class _Evaluator:
 
     def run_copy(self, x):
         """UnaryMap::Copy as Var::organize (var.rs:506-512)."""
-        return self.run_map([(abi.EXPR_UNARY, abi.U["copy"], 0, 0), (abi.EXPR_INPUT, 0, 0, 0)], [x], x.extents, x.dtype)
+        y = self.run_map([(abi.EXPR_UNARY, abi.U["copy"], 0, 0), (abi.EXPR_INPUT, 0, 0, 0)], [x], x.extents, x.dtype)
+        if self.record is not None:
+            self.keepalive.append(y)  # a recorded program writes it on every replay, so nobody else may be given its memory
+        return y
 
     def _ev_map(self, v):
         if _FUSION["on"]:
@@ -1187,6 +1196,8 @@ class _Evaluator:
                 return t
             if v.op == "unary" and v.attrs["name"] == "copy":
                 t = self.try_permuted_matmul(v)
+                if t is None:
+                    t = self.try_merged_heads(v)
                 if t is not None:
                     return t
         mb = _MapBuilder()
@@ -1728,6 +1739,15 @@ class _Evaluator:
             return m, res
         return None, None
 
+    def try_merged_heads(self, v):
+        """copy(permute(x)) where cross attention or its gradient left x in the permuted layout already."""
+        p = v.inputs[0]
+        if p.op != "permute" or self.done(p) or p.inputs[0].op not in ("cross_attention", "cross_attention_grad", "part"):
+            return None
+        x = self.get(p.inputs[0])
+        x = x.with_shape(x.shape.permute(p.attrs["axes"]))
+        return x if x.is_dense() else None
+
     def try_permuted_matmul(self, v):
         """copy(permute(G)) with the last axis kept in place: let G write the permuted layout."""
         p = v.inputs[0]
@@ -1789,3 +1809,89 @@ class _Evaluator:
         xc, gc, bc, yc = x.c(), g.c(), b.c(), y.c()
         self.call(self.lib.sg_layer_norm_lastaxis, C.byref(xc), C.byref(gc), C.byref(bc), C.c_float(v.attrs["eps"]), C.byref(yc))
         return y
+
+    # ---- operators of language models
+    def unit_stride(self, x):
+        """x, copied unless its last axis has unit stride."""
+        return x if x.strides[-1] == 1 or x.extents[-1] == 1 else self.run_copy(x)
+
+    def _ev_part(self, v):
+        return self.get(v.inputs[0]).parts[v.attrs["name"]]
+
+    def _ev_embedding(self, v):
+        table, ids = self.unit_stride(self.get(v.inputs[0])), self.get(v.inputs[1])
+        y = self.out(v.extents, FLOAT)
+        tc, ic, yc = table.c(), ids.c(), y.c()
+        self.call(self.lib.sg_embedding, C.byref(tc), C.byref(ic), C.c_float(v.attrs["scale"]), C.byref(yc))
+        return y
+
+    def _ev_embedding_grad(self, v):
+        g, ids = self.unit_stride(self.get(v.inputs[0])), self.get(v.inputs[1])
+        y = self.out(v.extents, FLOAT)
+        gc, ic, yc = g.c(), ids.c(), y.c()
+        self.call(self.lib.sg_embedding_grad, C.byref(gc), C.byref(ic), C.c_float(v.attrs["scale"]), C.byref(yc))
+        return y
+
+    def _ev_token_lse(self, v):
+        x = self.unit_stride(self.get(v.inputs[0]))
+        tokens = self.get(v.inputs[1]) if len(v.inputs) > 1 else None
+        top, lead = v.attrs["top"], list(v.inputs[0].extents[:-1])
+        lse = self.out(v.extents, FLOAT)
+        lse.parts = {"entropy": self.out(v.extents, FLOAT)}
+        if tokens is not None:
+            lse.parts["logprob"] = self.out(v.extents, FLOAT)
+        if top:
+            lse.parts["top_ids"], lse.parts["top_logprobs"] = self.out(lead + [top], UINT), self.out(lead + [top], FLOAT)
+
+        def ref(t):
+            return C.byref(t.c()) if t is not None else None
+        get = lse.parts.get
+        self.call(self.lib.sg_token_logprobs, ref(x), ref(tokens), C.c_float(v.attrs["scale"]), ref(get("logprob")), ref(get("entropy")), ref(lse),
+                  ref(get("top_ids")), ref(get("top_logprobs")))
+        return lse
+
+    def _ev_token_logprob(self, v):
+        return self.get(v.inputs[1]).parts["logprob"]
+
+    def _ev_token_entropy(self, v):
+        return self.get(v.inputs[1]).parts["entropy"]
+
+    def _ev_token_logprobs_grad(self, v):
+        x, lse = self.unit_stride(self.get(v.inputs[0])), self.get(v.inputs[1])
+        rest = [self.get(i) for i in v.inputs[2:]]
+        tokens, gl = (rest[0], rest[1]) if v.attrs["logprob"] else (None, None)
+        ge = rest[-1] if v.attrs["entropy"] else None
+        y = self.out(v.extents, FLOAT)
+
+        def ref(t):
+            return C.byref(t.c()) if t is not None else None
+        self.call(self.lib.sg_token_logprobs_grad, ref(x), ref(tokens), C.c_float(v.inputs[1].attrs["scale"]), ref(lse), ref(lse.parts["entropy"]),
+                  ref(gl), ref(ge), ref(y))
+        return y
+
+    def heads_out(self, extents):
+        """A [N, H, L, D] tensor with the heads of a position side by side in memory: merge_heads (bert.rs:293-302) finds
+        the layout it asks for."""
+        n, h, l, d = extents
+        return self.out([n, l, h, d], FLOAT).with_shape(Shape(extents, [l * h * d, d, h * d, 1]))
+
+    def _cross_inputs(self, inputs):
+        xs = [self.unit_stride(self.get(i)) for i in inputs]
+        return [C.byref(x.c()) for x in xs] + [None] * (4 - len(xs))
+
+    def _ev_cross_attention(self, v):
+        ins = self._cross_inputs(v.inputs)
+        y = self.heads_out(v.extents)
+        y.parts = {"lse": self.out(v.extents[:3], FLOAT)}
+        self.call(self.lib.sg_cross_attention, *ins, C.c_float(v.attrs["scale"]), C.byref(y.c()), C.byref(y.parts["lse"].c()))
+        return y
+
+    def _ev_cross_attention_grad(self, v):
+        out_node, gy = v.inputs[-2:]
+        ins = self._cross_inputs(v.inputs[:-2])
+        o, g = self.get(out_node), self.unit_stride(self.get(gy))
+        gq = self.heads_out(v.extents)
+        gq.parts = {"gk": self.heads_out(v.inputs[1].extents), "gv": self.heads_out(v.inputs[1].extents)}
+        self.call(self.lib.sg_cross_attention_grad, *ins, C.c_float(v.attrs["scale"]), C.byref(o.c()), C.byref(o.parts["lse"].c()), C.byref(g.c()),
+                  C.byref(gq.c()), C.byref(gq.parts["gk"].c()), C.byref(gq.parts["gv"].c()))
+        return gq

@@ -1,0 +1,681 @@
+"""The language-model operators on the GPU, through the C ABI and the front end, against the plain 64-bit implementations
+of tests/lm_reference.py with the tolerances derived there."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import sage_amd as S
+from sage_amd import abi, bert, nn, optim
+from sage_amd import var as V
+from sage_amd.grad import grad, grad_param
+from sage_amd.layers import Dense, Embedding, Layer
+from sage_amd.shape import Shape, default_strides
+from sage_amd.tensor import FLOAT, INT, UINT, Tensor
+from sage_amd.var import Program, Var
+from tests import lm_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = S.Context()
+    yield c
+    c.close()
+
+
+def say(*a):
+    print("[case]", *a, flush=True)
+
+
+def dev(ctx, a):
+    return Tensor.from_numpy(ctx, a)
+
+
+def strided(ctx, a, pad=3, order=None, offset=0):
+    """`a` on the device with its axes in memory order `order` (the last axis stays last) and `pad` further elements behind
+    each innermost row, `offset` elements into its buffer; what lies between the elements is NaN."""
+    a = np.asarray(a)
+    order = list(range(a.ndim)) if order is None else order
+    ext = [a.shape[i] for i in order]
+    ext[-1] += pad
+    st = default_strides(ext)
+    host = np.full(int(np.prod(ext)) + offset, np.nan if a.dtype == np.float32 else 7, a.dtype)
+    strides = [0] * a.ndim
+    for i, ax in enumerate(order):
+        strides[ax] = st[i]
+    view = np.lib.stride_tricks.as_strided(host[offset:], a.shape, [s * 4 for s in strides])
+    view[...] = a
+    t = dev(ctx, host)
+    return Tensor(t.buf, t.dtype, Shape(list(a.shape), strides, offset))
+
+
+def ref(t):
+    """The argument for a tensor, which lives as long as the argument does."""
+    if t is None:
+        return None
+    c = t.c()
+    c.keep = t
+    return C.byref(c)
+
+
+def near(got, want, tol, what):
+    got, want, tol = np.asarray(got, np.float64), np.asarray(want, np.float64), np.broadcast_to(np.asarray(tol, np.float64), np.shape(want))
+    assert got.shape == want.shape, f"{what}: {got.shape} for {want.shape}"
+    assert np.array_equal(np.isnan(got), np.isnan(want)), f"{what}: NaN in other places"
+    inf = np.isinf(want)
+    assert np.array_equal(np.isinf(got), inf) and np.array_equal(got[inf], want[inf]), f"{what}: infinities differ"
+    ok = np.isfinite(want)
+    if ok.any():
+        off = np.abs(got[ok] - want[ok]) - tol[ok]
+        assert off.max() <= 0, f"{what}: {np.abs(got[ok] - want[ok])[off.argmax()]:.3g} off, {tol[ok][off.argmax()]:.3g} allowed"
+
+
+def same_bits(a, b):
+    return np.array_equal(np.ascontiguousarray(a).view(np.uint32), np.ascontiguousarray(b).view(np.uint32))
+
+
+# ----------------------------------------------------------------------------- embedding
+def zipf_ids(rng, n, v):
+    return np.minimum(np.exp(rng.random(n) * np.log(v + 1)).astype(np.int64) - 1, v - 1)
+
+
+@pytest.mark.parametrize("n,v,e", [(1, 1, 1), (1, 5, 768), (7, 3, 64), (64, 1000, 33), (257, 10, 260), (300, 70000, 4), (4096, 500, 96), (5, 100, 2050)])
+def test_embedding_and_gradient(ctx, n, v, e):
+    say("embedding", n, v, e)
+    rng = np.random.default_rng(n + v + e)
+    table, g = R.f32(rng.standard_normal((v, e))), R.f32(rng.standard_normal((n, e)))
+    ids = zipf_ids(rng, n, v).astype(np.int32)
+    ids[rng.random(n) < 0.1] = -1
+    ids[rng.random(n) < 0.05] = v
+    t, i = dev(ctx, table), dev(ctx, ids)
+    y = nn.embedding(Var.new(t), Var.new(i), 1.7).eval(ctx).numpy()
+    assert same_bits(y, R.embedding(table, ids, 1.7))
+    out = dev(ctx, np.full((v, e), np.nan, np.float32))
+    gd = dev(ctx, g)
+    want, tol = R.embedding_grad(g, ids, v, 1.7)
+    first = None
+    for _ in range(3):
+        ctx.check(ctx._lib.sg_embedding_grad(ctx.handle, ref(gd), ref(i), C.c_float(1.7), ref(out)))
+        got = out.numpy()
+        near(got, want, tol, "gtable")
+        assert first is None or same_bits(got, first)  # the same bits every time
+        first = got
+
+
+@pytest.mark.parametrize("n,distinct", [(2048, 1), (5000, 1), (20000, 3), (8193, 2), (70000, 5), (16384, 16384)])
+def test_embedding_gradient_of_long_runs_and_many_tokens(ctx, n, distinct):
+    """All tokens on a few rows of a large table, and every token on a row of its own."""
+    say("runs", n, distinct)
+    rng = np.random.default_rng(n)
+    v, e = 300000, 20
+    ids = (rng.integers(0, distinct, n) * (v // distinct)).astype(np.uint32)
+    if distinct == n:
+        ids = rng.permutation(v)[:n].astype(np.uint32)
+    g = R.f32(rng.standard_normal((n, e)))
+    out = Tensor.uninit(ctx, [v, e])
+    ctx.check(ctx._lib.sg_embedding_grad(ctx.handle, ref(dev(ctx, g)), ref(dev(ctx, ids)), C.c_float(0.5), ref(out)))
+    want, tol = R.embedding_grad(g, ids, v, 0.5)
+    near(out.numpy(), want, tol, "gtable")
+
+
+def test_embedding_strided_operands(ctx):
+    """Ids of a wider batch (its last position dropped), a broadcast batch, a table and a gradient with padded or permuted rows."""
+    rng = np.random.default_rng(3)
+    table = R.f32(rng.standard_normal((50, 36)))
+    ids = rng.integers(0, 50, (4, 9)).astype(np.uint32)
+    whole = dev(ctx, ids)
+    cut = Tensor(whole.buf, UINT, Shape([4, 8], [9, 1], 1))
+    for tab in (dev(ctx, table), strided(ctx, table, pad=5, offset=1), strided(ctx, table, pad=4)):
+        out = Tensor.uninit(ctx, [4, 8, 36])
+        ctx.check(ctx._lib.sg_embedding(ctx.handle, ref(tab), ref(cut), C.c_float(0.25), ref(out)))
+        assert same_bits(out.numpy(), R.embedding(table, ids[:, 1:], 0.25))
+    g = R.f32(rng.standard_normal((4, 8, 36)))
+    want, tol = R.embedding_grad(g, ids[:, 1:], 50, 0.25)
+    for gd in (dev(ctx, g), strided(ctx, g, pad=1), strided(ctx, g, pad=4, order=[1, 0, 2]), strided(ctx, g, pad=0, order=[1, 0, 2], offset=2)):
+        out = Tensor.uninit(ctx, [50, 36])
+        ctx.check(ctx._lib.sg_embedding_grad(ctx.handle, ref(gd), ref(cut), C.c_float(0.25), ref(out)))
+        near(out.numpy(), want, tol, "gtable")
+    one = dev(ctx, g[0, 0])  # a gradient broadcast over all tokens
+    out = Tensor.uninit(ctx, [50, 36])
+    ctx.check(ctx._lib.sg_embedding_grad(ctx.handle, ref(Tensor(one.buf, FLOAT, Shape([4, 8, 36], [0, 0, 1], 0))), ref(cut), C.c_float(1.0), ref(out)))
+    want, tol = R.embedding_grad(np.broadcast_to(g[0, 0], g.shape), ids[:, 1:], 50, 1.0)
+    near(out.numpy(), want, tol, "broadcast gradient")
+    row = Tensor(whole.buf, UINT, Shape([6, 9], [0, 1], 9))  # one sequence six times
+    out = Tensor.uninit(ctx, [6, 9, 36])
+    ctx.check(ctx._lib.sg_embedding(ctx.handle, ref(dev(ctx, table)), ref(row), C.c_float(1.0), ref(out)))
+    assert same_bits(out.numpy(), R.embedding(table, np.broadcast_to(ids[1], (6, 9)), 1.0))
+
+
+def test_embedding_of_unknown_tokens_only(ctx):
+    ids = dev(ctx, np.full((3, 4), -1, np.int32))
+    table = dev(ctx, np.full((5, 8), np.nan, np.float32))
+    assert not nn.embedding(Var.new(table), Var.new(ids)).eval(ctx).numpy().any()
+    g = Var.new(dev(ctx, np.full((3, 4, 8), np.nan, np.float32)))
+    t = Var.new(table)
+    assert not grad(nn.embedding(t, Var.new(ids)), [t], seed=g)[0].eval(ctx).numpy().any()
+
+
+# ----------------------------------------------------------------------------- log probabilities
+def run_logprobs(ctx, x, tokens, scale, top=0, shape=None):
+    """x: a Tensor or an array [.., C]."""
+    x = x if isinstance(x, Tensor) else dev(ctx, x)
+    lead = list(x.extents[:-1]) or [1]
+    outs = {k: Tensor.from_numpy(ctx, np.full(lead, np.nan, np.float32)) for k in ("logprob", "entropy", "lse")}
+    ids = tops = None
+    if top:
+        ids, tops = Tensor.uninit(ctx, list(x.extents[:-1]) + [top], UINT), Tensor.uninit(ctx, list(x.extents[:-1]) + [top])
+    tok = tokens if tokens is None or isinstance(tokens, Tensor) else dev(ctx, tokens)
+    ctx.check(ctx._lib.sg_token_logprobs(ctx.handle, ref(x), ref(tok), C.c_float(scale), ref(outs["logprob"]) if tok is not None else None, ref(outs["entropy"]),
+                                         ref(outs["lse"]), ref(ids), ref(tops)))
+    r = {k: v.numpy() for k, v in outs.items()}
+    if top:
+        r["top_ids"], r["top_logprobs"] = ids.numpy(), tops.numpy()
+    r["dev"] = (x, tok, outs)
+    return r
+
+
+def check_logprobs(ctx, x, tokens, scale, top):
+    want = R.logprobs(x, tokens, scale, top)
+    got = run_logprobs(ctx, x, tokens, scale, top)
+    t_lp, t_h = R.logprobs_tol(x, scale)
+    far = np.abs(np.where(np.isfinite(x), x, 0)).max(1) * scale
+    near(got["lse"], want["lse"], t_lp + 2 * R.U * far, "lse")
+    near(got["entropy"], want["entropy"], t_h, "entropy")
+    near(got["logprob"], want["logprob"], t_lp + 2 * R.U * np.abs(np.where(np.isfinite(want["logprob"]), want["logprob"], 0)), "logprob")
+    if top:
+        assert np.array_equal(got["top_ids"], want["top_ids"])
+        near(got["top_logprobs"], want["top_logprobs"], t_lp[:, None] + 2 * R.U * np.abs(np.where(np.isfinite(want["top_logprobs"]), want["top_logprobs"], 0)), "top")
+    return want, got
+
+
+@pytest.mark.parametrize("rows,c,top", [(1, 1, 1), (1, 2, 2), (3, 63, 5), (2, 64, 64), (5, 257, 20), (1, 30522, 5), (4, 50257, 32), (37, 4099, 64), (300, 1000, 1), (2, 131071, 64)])
+@pytest.mark.parametrize("scale", [1.0, 1.7])
+def test_token_logprobs(ctx, rows, c, top, scale):
+    say("logprobs", rows, c, top, scale)
+    rng = np.random.default_rng(rows * c + top)
+    x = R.f32(rng.standard_normal((rows, c)) * 3 + rng.standard_normal(c))
+    tokens = rng.integers(0, c, rows).astype(np.int32)
+    tokens[rng.random(rows) < 0.2] = -100
+    check_logprobs(ctx, x, tokens, scale, top)
+
+
+@pytest.mark.parametrize("c", [40, 1000, 20000])
+def test_token_logprobs_of_masked_vocabularies_and_ties(ctx, c):
+    """Rows with -inf, with nothing else, with one token left, with equal logits (all, and rising blocks), far from 0, in
+    rising and in falling order."""
+    say("masked", c)
+    rng = np.random.default_rng(c)
+    x = R.f32(rng.standard_normal((9, c)))
+    x[0, rng.random(c) < 0.9] = -np.inf
+    x[1] = -np.inf
+    x[2] = -np.inf
+    x[2, c - 3] = 4.0
+    x[3] = 0.5
+    x[4] = np.arange(c) // 7
+    x[5] = np.sort(x[5])
+    x[6] = np.sort(x[6])[::-1]
+    x[7] = x[7] * 50 + 1000
+    x[8] = np.where(np.arange(c) % 2, 0.0, -0.0)
+    tokens = np.array([0, 5, c - 3, c - 1, 3, 0, 0, 2, c], np.int32)
+    want, got = check_logprobs(ctx, x, tokens, 1.0, 32)
+    assert got["entropy"][1] == 0 and np.isneginf(got["lse"][1])
+    gl, ge = R.f32(rng.standard_normal(9)), R.f32(rng.standard_normal(9))
+    xd, tok, outs = got["dev"]
+    out = Tensor.uninit(ctx, [9, c])
+    ctx.check(ctx._lib.sg_token_logprobs_grad(ctx.handle, ref(xd), ref(tok), C.c_float(1.0), ref(outs["lse"]), ref(outs["entropy"]), ref(dev(ctx, gl)), ref(dev(ctx, ge)), ref(out)))
+    near(out.numpy(), R.logprobs_grad(want, 1.0, gl, ge), R.logprobs_grad_tol(want, x, 1.0, gl, ge), "glogits")
+
+
+@pytest.mark.parametrize("c", [50, 5000, 70001])
+def test_token_logprobs_of_nan_and_infinity(ctx, c):
+    rng = np.random.default_rng(c)
+    x = R.f32(rng.standard_normal((4, c)))
+    x[0, c // 2] = np.nan
+    x[1, 3] = np.inf
+    x[2] = np.nan
+    r = run_logprobs(ctx, x, np.array([0, 0, -1, 0], np.int32), 1.0, 8)
+    for row in range(3):
+        assert np.isnan(r["lse"][row]) and np.isnan(r["entropy"][row]) and np.isnan(r["top_logprobs"][row]).all()
+    assert np.isnan(r["logprob"][:2]).all() and r["logprob"][2] == 0
+    assert np.array_equal(r["top_ids"][0], np.argsort(-np.where(np.isnan(x[0]), -np.inf, x[0]), kind="stable")[:8])
+    assert r["top_ids"][1, 0] == 3 and np.array_equal(r["top_ids"][2], np.arange(8))
+    assert np.isfinite(r["lse"][3])
+
+
+@pytest.mark.parametrize("rows,c", [(1, 1), (3, 64), (5, 257), (2, 30522), (129, 1023)])
+def test_token_logprobs_gradient(ctx, rows, c):
+    say("logprobs grad", rows, c)
+    rng = np.random.default_rng(rows + c)
+    x = R.f32(rng.standard_normal((rows, c)) * 2)
+    tokens = rng.integers(0, c, rows).astype(np.int32)
+    tokens[::3] = -100
+    gl, ge = R.f32(rng.standard_normal(rows)), R.f32(rng.standard_normal(rows))
+    want, got = check_logprobs(ctx, x, tokens, 0.8, 0)
+    xd, tok, outs = got["dev"]
+    for a, b in ((gl, ge), (gl, None), (None, ge)):
+        out = Tensor.uninit(ctx, [rows, c])
+        ctx.check(ctx._lib.sg_token_logprobs_grad(ctx.handle, ref(xd), ref(tok) if a is not None else None, C.c_float(0.8), ref(outs["lse"]),
+                                                  ref(outs["entropy"]) if b is not None else None, ref(dev(ctx, a)) if a is not None else None,
+                                                  ref(dev(ctx, b)) if b is not None else None, ref(out)))
+        near(out.numpy(), R.logprobs_grad(want, 0.8, a, b), R.logprobs_grad_tol(want, x, 0.8, a, b), "glogits")
+    # in place, with a gradient broadcast over the rows
+    one = dev(ctx, gl[:1])
+    ctx.check(ctx._lib.sg_token_logprobs_grad(ctx.handle, ref(xd), ref(tok), C.c_float(0.8), ref(outs["lse"]), None, ref(Tensor(one.buf, FLOAT, Shape([rows], [0], 0))), None, ref(xd)))
+    all_same = np.full(rows, gl[0])
+    near(xd.numpy(), R.logprobs_grad(want, 0.8, all_same), R.logprobs_grad_tol(want, x, 0.8, all_same), "in place")
+
+
+def test_token_logprobs_strided_operands(ctx):
+    """[2, 3, C] logits with padded rows at every alignment and permuted leading axes; strided tokens; a rank-1 call."""
+    rng = np.random.default_rng(9)
+    for c in (100, 1027):
+        x = R.f32(rng.standard_normal((2, 3, c)))
+        tokens = rng.integers(0, c, (2, 3)).astype(np.int32)
+        want = R.logprobs(x.reshape(6, c), tokens.reshape(6), 1.0, 7)
+        t_lp, t_h = R.logprobs_tol(x.reshape(6, c), 1.0)
+        tok = strided(ctx, tokens, pad=2, order=[0, 1])
+        for pad, order, offset in ((0, [0, 1, 2], 1), (1, [0, 1, 2], 0), (2, [1, 0, 2], 3), (4, [1, 0, 2], 0)):
+            got = run_logprobs(ctx, strided(ctx, x, pad, order, offset), tok, 1.0, 7)
+            near(got["logprob"].reshape(6), want["logprob"], t_lp, "logprob")
+            near(got["entropy"].reshape(6), want["entropy"], t_h, "entropy")
+            assert np.array_equal(got["top_ids"].reshape(6, 7), want["top_ids"])
+    got = run_logprobs(ctx, x[0, 0].copy(), tokens[0, :1].copy(), 1.0, 7)
+    near(got["logprob"], want["logprob"][:1], t_lp[:1], "rank 1")
+    assert np.array_equal(got["top_ids"], want["top_ids"][0])
+
+
+# ----------------------------------------------------------------------------- cross attention
+def cross_case(rng, n, h, g, lq, lk, d):
+    q, k, v, go = (R.f32(rng.standard_normal(s)) for s in ((n, h, lq, d), (n, g, lk, d), (n, g, lk, d), (n, h, lq, d)))
+    return q, k, v, go
+
+
+def run_cross(ctx, q, k, v, mask, scale, go=None, out=None):
+    n, h, lq, d = q.extents
+    out = Tensor.from_numpy(ctx, np.full(q.extents, np.nan, np.float32)) if out is None else out
+    lse = Tensor.uninit(ctx, [n, h, lq])
+    ctx.check(ctx._lib.sg_cross_attention(ctx.handle, ref(q), ref(k), ref(v), ref(mask), C.c_float(scale), ref(out), ref(lse)))
+    r = {"out": out, "lse": lse}
+    if go is not None:
+        nan = lambda e: Tensor.from_numpy(ctx, np.full(e, np.nan, np.float32))  # noqa: E731
+        r.update(gq=nan(q.extents), gk=nan(k.extents), gv=nan(k.extents))
+        ctx.check(ctx._lib.sg_cross_attention_grad(ctx.handle, ref(q), ref(k), ref(v), ref(mask), C.c_float(scale), ref(out), ref(lse), ref(go), ref(r["gq"]),
+                                                   ref(r["gk"]), ref(r["gv"])))
+    return {key: t.numpy() for key, t in r.items()}
+
+
+def check_cross(ctx, q, k, v, mask, scale, go, tensors=None):
+    t = tensors or [dev(ctx, a) for a in (q, k, v, go)]
+    got = run_cross(ctx, *t[:3], None if mask is None else dev(ctx, mask), scale, t[3])
+    clean = lambda a: a if mask is None else np.where((np.asarray(mask) != 0)[:, None, :, None], a, np.float32(0))  # noqa: E731
+    kc, vc = clean(k), clean(v)
+    out, lse, _ = R.cross(q, kc, vc, mask, scale)
+    t_out, t_lse = R.cross_tol(q, kc, vc, mask, scale)
+    near(got["out"], out, t_out, "out")
+    near(got["lse"], lse, t_lse, "lse")
+    for name, want, tol in zip(("gq", "gk", "gv"), R.cross_grad(q, kc, vc, mask, scale, go), R.cross_grad_tol(q, kc, vc, mask, scale, go)):
+        near(got[name], want, tol, name)
+    return got
+
+
+CROSS = [(1, 1, 1, 1, 1, 32), (1, 1, 1, 1, 1, 64), (2, 3, 3, 5, 7, 64), (1, 2, 1, 33, 65, 32), (3, 4, 2, 1, 200, 64), (2, 12, 12, 1, 513, 64), (2, 8, 2, 31, 130, 32),
+         (1, 4, 1, 129, 64, 64), (2, 2, 2, 128, 128, 64), (1, 1, 1, 300, 33, 32), (1, 6, 3, 2, 1000, 32), (1, 1, 1, 3, 3000, 64), (9, 12, 4, 4, 96, 64)]
+
+
+@pytest.mark.parametrize("n,h,g,lq,lk,d", CROSS)
+def test_cross_attention_and_gradient(ctx, n, h, g, lq, lk, d):
+    say("cross", n, h, g, lq, lk, d)
+    rng = np.random.default_rng(n + h + lq + lk)
+    q, k, v, go = cross_case(rng, n, h, g, lq, lk, d)
+    check_cross(ctx, q, k, v, None, 1 / np.sqrt(d), go)
+
+
+@pytest.mark.parametrize("n,h,g,lq,lk,d", [(4, 4, 2, 9, 150, 64), (4, 2, 2, 1, 700, 32), (5, 6, 2, 70, 257, 32), (4, 3, 1, 130, 128, 64), (3, 1, 1, 2, 64, 64)])
+def test_cross_attention_masks(ctx, n, h, g, lq, lk, d):
+    """Lengths, holes, a single visible key, an empty row; hidden keys hold NaN and infinities."""
+    say("masks", n, h, g, lq, lk, d)
+    rng = np.random.default_rng(lk)
+    q, k, v, go = cross_case(rng, n, h, g, lq, lk, d)
+    mask = np.zeros((n, lk), np.float32)
+    mask[0, :lk // 2 + 1] = 1.0
+    mask[1] = np.where(rng.random(lk) < 0.4, -2.5, 0.0)  # anything but 0 is visible
+    if n > 3:
+        mask[3, lk - 1] = 1e-30
+    hidden = np.broadcast_to((mask == 0)[:, None, :, None], k.shape)
+    k[hidden], v[hidden] = np.nan, np.inf
+    got = check_cross(ctx, q, k, v, mask, 0.2, go)
+    assert not got["out"][2].any() and np.isneginf(got["lse"][2]).all() and not got["gq"][2].any() and not got["gk"][2].any() and not got["gv"][2].any()
+    again = run_cross(ctx, *[dev(ctx, a) for a in (q, k, v)], dev(ctx, mask), 0.2, dev(ctx, go))
+    assert all(same_bits(got[x], again[x]) for x in got)
+
+
+def test_cross_attention_large_scores_do_not_overflow(ctx):
+    rng = np.random.default_rng(5)
+    q, k, v, go = cross_case(rng, 1, 2, 2, 40, 300, 64)
+    check_cross(ctx, q * 30, k, v, None, 1.0, go)
+    check_cross(ctx, q, k - 100 * q[:, :, :1], v, None, 1.0, go)  # all scores far below 0
+    check_cross(ctx, q, k, v, None, -0.5, go)
+
+
+@pytest.mark.parametrize("d", [32, 64])
+def test_cross_attention_layouts(ctx, d):
+    """Heads side by side, padded and unaligned rows, broadcast keys, gradients and masks, outputs in the merged layout."""
+    rng = np.random.default_rng(d)
+    n, h, g, lq, lk = 2, 4, 2, 37, 70
+    q, k, v, go = cross_case(rng, n, h, g, lq, lk, d)
+    for pad, order, offset in ((0, [0, 2, 1, 3], 0), (1, [0, 2, 1, 3], 0), (4, [0, 1, 2, 3], 4), (3, [2, 0, 1, 3], 1)):
+        check_cross(ctx, q, k, v, None, 0.3, go, [strided(ctx, a, pad, order, offset) for a in (q, k, v, go)])
+    kb = np.broadcast_to(k[:1, :1], k.shape)
+    t = dev(ctx, k[0, 0])
+    shared = Tensor(t.buf, FLOAT, Shape([n, g, lk, d], [0, 0, d, 1], 0))
+    gt = dev(ctx, go[0, 0, 0])
+    check_cross(ctx, q, kb, kb, None, 0.3, np.broadcast_to(go[0, 0, 0], go.shape), [dev(ctx, q), shared, shared, Tensor(gt.buf, FLOAT, Shape([n, h, lq, d], [0, 0, 0, 1], 0))])
+    # one mask for the whole batch; outputs with heads side by side leave what lies between rows alone
+    mask = dev(ctx, np.where(rng.random(lk) < 0.5, 1.0, 0.0).astype(np.float32))
+    m = Tensor(mask.buf, FLOAT, Shape([n, lk], [0, 1], 0))
+    wide = dev(ctx, np.full((n, lq, h, d + 4), 7.0, np.float32))
+    view = Tensor(wide.buf, FLOAT, Shape([n, h, lq, d], [lq * h * (d + 4), d + 4, h * (d + 4), 1], 0))
+    got = run_cross(ctx, dev(ctx, q), dev(ctx, k), dev(ctx, v), m, 0.3, out=view)["out"]
+    mm = np.broadcast_to(mask.numpy(), (n, lk))
+    near(got, R.cross(q, k, v, mm, 0.3)[0], R.cross_tol(q, k, v, mm, 0.3)[0], "merged out")
+    assert (wide.numpy()[..., d:] == 7.0).all()
+
+
+# ----------------------------------------------------------------------------- AdamW
+SIZES = [1, 3, 255, 256, 257, 1000, 4096, 4097, 10000]
+
+
+def adamw_arrays(ctx, xs):
+    arr = (abi.sg_tensor * len(xs))(*[x.c() for x in xs])
+    arr.keep = xs
+    return arr
+
+
+HYPER = (1e-2, 0.9, 0.999, 1e-8, 0.1)
+
+
+def hyper():
+    lr, b1, b2, eps, wd = HYPER
+    return abi.sg_adam_hyper(lr, b1, b2, float(np.float32(1) - np.float32(b1)), float(np.float32(1) - np.float32(b2)), eps, wd)
+
+
+def test_adamw_32_bit_states(ctx):
+    """150 tensors (three launches), some unaligned: the moments bit for bit, three steps."""
+    say("adamw 32")
+    rng = np.random.default_rng(0)
+    sizes = (SIZES * 17)[:150]
+    value, m, v = ([R.f32(rng.standard_normal(n)) for n in sizes] for _ in range(3))
+    v = [np.abs(x) for x in v]
+    up = lambda xs: [strided(ctx, x, 0, None, i % 3) for i, x in enumerate(xs)]  # noqa: E731
+    dv, dm, ds = up(value), up(m), up(v)
+    for t in (1, 2, 3):
+        g = [R.f32(rng.standard_normal(n)) for n in sizes]
+        dg = up(g)
+        h = hyper()
+        ctx.check(ctx._lib.sg_adamw_update(ctx.handle, len(sizes), *[adamw_arrays(ctx, x) for x in (dv, dg, dm, ds)], None, None, ref(dev(ctx, R.f32([t]))), C.byref(h), 0))
+        for i in range(len(sizes)):
+            m[i], v[i] = R.adamw_moments(m[i], v[i], g[i], 0.9, 0.999)
+            assert same_bits(dm[i].numpy(), m[i]) and same_bits(ds[i].numpy(), v[i]), (t, i)
+            want, tol = R.adamw_value(value[i], m[i], v[i], t, *HYPER)
+            value[i] = dv[i].numpy()
+            near(value[i], want, tol, f"value {i}")
+
+
+@pytest.mark.parametrize("far", [0, 1])
+def test_adamw_8_bit_states(ctx, far):
+    """Bytes and scales exactly as defined, over 20 steps from zero states; far: gradients over many octaves, blocks of zeros."""
+    say("adamw 8", far)
+    rng = np.random.default_rng(1)
+    sizes = SIZES * 8  # 72 tensors: two launches
+    value = [R.f32(rng.standard_normal(n)) for n in sizes]
+    codes = [[np.zeros(n, np.uint8) for n in sizes] for _ in range(2)]
+    scales = [[np.zeros(-(-n // 256), np.float32) for n in sizes] for _ in range(2)]
+    dv = [strided(ctx, x, 0, None, i % 3) for i, x in enumerate(value)]
+    dm, ds = ([dev(ctx, R.pack(c)) for c in cs] for cs in codes)
+    dms, dss = ([dev(ctx, s) for s in sc] for sc in scales)
+    for t in range(1, 21):
+        g = [R.f32(rng.standard_normal(n) * (np.exp(12 * rng.standard_normal(n)) if far else 1.0)) for n in sizes]
+        if far:
+            g[4][:256] = 0.0
+            g[5][::2] = 0.0
+        h = hyper()
+        ctx.check(ctx._lib.sg_adamw_update(ctx.handle, len(sizes), *[adamw_arrays(ctx, x) for x in (dv, [dev(ctx, x) for x in g], dm, ds, dms, dss)],
+                                           ref(dev(ctx, R.f32([t]))), C.byref(h), 77))
+        for i, n in enumerate(sizes):
+            m, v = R.adamw_moments(R.decode(codes[0][i], scales[0][i], True), R.decode(codes[1][i], scales[1][i], False), g[i], 0.9, 0.999)
+            want, tol = R.adamw_value(value[i], m, v, t, *HYPER)
+            value[i] = dv[i].numpy()
+            near(value[i], want, tol, f"value {i} step {t}")
+            nm, nv = R.noise(n, t, 77)
+            codes[0][i], scales[0][i] = R.encode(m, True, nm)
+            codes[1][i], scales[1][i] = R.encode(v, False, nv)
+            if t in (1, 2, 7, 20):
+                assert np.array_equal(dm[i].numpy(), R.pack(codes[0][i])) and np.array_equal(ds[i].numpy(), R.pack(codes[1][i])), (t, i)
+                assert same_bits(dms[i].numpy(), scales[0][i]) and same_bits(dss[i].numpy(), scales[1][i]), (t, i)
+    outs = [[Tensor.uninit(ctx, [n]) for n in sizes] for _ in range(2)]
+    ctx.check(ctx._lib.sg_adamw_state_read(ctx.handle, len(sizes), *[adamw_arrays(ctx, x) for x in (dm, ds, dms, dss, *outs)]))
+    for i in range(len(sizes)):
+        assert same_bits(outs[0][i].numpy(), R.decode(codes[0][i], scales[0][i], True)) and same_bits(outs[1][i].numpy(), R.decode(codes[1][i], scales[1][i], False))
+
+
+def test_adamw_not_finite_gradient_spoils_its_own_only(ctx):
+    n = 600
+    g = np.ones(n, np.float32)
+    g[300], g[10] = np.inf, np.nan
+    for bits in (32, 8):
+        p = Var.new(dev(ctx, np.ones(n, np.float32)))
+        opt = optim.AdamW(1e-2, state_bits=bits)
+        opt.update({p: Var.new(dev(ctx, g))}, ctx)
+        m, v = (x.numpy() for x in opt.state(p, ctx))
+        bad = ~np.isfinite(p.value.numpy())
+        assert bad[10] and bad[300] and bad.sum() == 2
+        spoilt = ~np.isfinite(m)
+        assert spoilt.sum() == (2 if bits == 32 else 512) and not spoilt[512:].any() and np.isnan(v[10])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_optimizer_eager_compiled_and_captured(ctx, bits):
+    """update(), a compiled program and its replayed graph take the same steps, bit for bit."""
+    rng = np.random.default_rng(2)
+    shapes = [(33, 7), (256,), (1,), (64, 65)]
+    start = [R.f32(rng.standard_normal(s)) for s in shapes]
+    steps = [[R.f32(rng.standard_normal(s)) for s in shapes] for _ in range(6)]
+
+    def fresh():
+        params = [Var.new(dev(ctx, a.copy())) for a in start]
+        grads = [Var.new(dev(ctx, a)) for a in steps[0]]
+        return params, grads, optim.AdamW(1e-2, state_bits=bits, seed=5)
+
+    p1, g1, o1 = fresh()
+    for s in steps:
+        for gv, a in zip(g1, s):
+            gv.value.copy_from_numpy(a)
+        o1.update(dict(zip(p1, g1)), ctx)
+    p2, g2, o2 = fresh()
+    prog = o2.compile(dict(zip(p2, g2)), ctx)  # the first step
+    for i, s in enumerate(steps[1:]):
+        for gv, a in zip(g2, s):
+            gv.value.copy_from_numpy(a)
+        if i == 2:
+            prog.capture()
+        prog.run()
+        ctx.sync()
+    for a, b in zip(p1, p2):
+        assert same_bits(a.value.numpy(), b.value.numpy())
+        for x, y in zip(o1.state(a, ctx), o2.state(b, ctx)):
+            assert same_bits(x.numpy(), y.numpy())
+    prog.release_graph()
+
+
+def test_adamw_takes_strided_gradients_and_a_broadcast_one(ctx):
+    rng = np.random.default_rng(4)
+    a, g = R.f32(rng.standard_normal((6, 10))), R.f32(rng.standard_normal((10, 6)))
+    p, q = Var.new(dev(ctx, a)), Var.new(dev(ctx, a))
+    gt = dev(ctx, g)
+    turned = Var.new(Tensor(gt.buf, FLOAT, Shape([6, 10], [1, 6], 0)))
+    o1, o2 = optim.AdamW(1e-2), optim.AdamW(1e-2)
+    for _ in range(2):
+        o1.update({p: turned}, ctx)
+        o2.update({q: Var.new(dev(ctx, g.T.copy()))}, ctx)
+    assert same_bits(p.value.numpy(), q.value.numpy())
+    r = Var.new(dev(ctx, a))
+    prog = optim.AdamW(1e-2).compile({r: turned}, ctx)
+    prog.run()
+    assert same_bits(p.value.numpy(), r.value.numpy())
+    with pytest.raises(abi.ShapeError):
+        o1.update({p: Var.new(gt)}, ctx)
+
+
+# ----------------------------------------------------------------------------- together
+class Reader(Layer):
+    """Tokens that attend to an encoder's states and predict the next token: the operators as a training step uses them."""
+
+    def __init__(self, vocab, dim, heads, kv_heads, state_bits):
+        self.embedding = Embedding(vocab, dim, scale=np.sqrt(dim))
+        self.cross = bert.CrossAttention(dim, heads, num_kv_heads=kv_heads)
+        self.head = Dense(dim, vocab)
+        self.opt = optim.AdamW(1e-3, state_bits=state_bits)
+
+    def params(self):
+        return self.embedding.params() + self.cross.params() + self.head.params()
+
+    def pass_(self, ids, states, mask):
+        return self.head.pass_(self.cross.pass_(self.embedding.pass_(ids), states, mask))
+
+
+def reader_in_64_bits(arrays, ids, states, mask, targets, heads, kv):
+    """The same step with torch's float64 autograd: the loss and the gradients of every parameter."""
+    import torch
+    ps = [torch.tensor(np.asarray(a, np.float64), requires_grad=True) for a in arrays]
+    emb, wq, bq, wk, bk, wv, bv, wo, bo, ga, be, wh, bh = ps
+    n, l = ids.shape
+    e = emb.shape[1]
+    d = e // heads
+    known = torch.tensor(ids >= 0)
+    x = emb[torch.tensor(np.where(ids >= 0, ids, 0)).long()] * float(np.float32(np.sqrt(e))) * known[..., None]
+    st = torch.tensor(states.astype(np.float64))
+    q = (x @ wq + bq).view(n, l, heads, d).transpose(1, 2)
+    k = (st @ wk + bk).view(n, -1, kv, d).transpose(1, 2).repeat_interleave(heads // kv, 1)
+    v = (st @ wv + bv).view(n, -1, kv, d).transpose(1, 2).repeat_interleave(heads // kv, 1)
+    s = (q @ k.transpose(2, 3)) / np.sqrt(d)
+    s = s.masked_fill(torch.tensor(mask == 0)[:, None, None, :], -1e300)
+    a = (torch.softmax(s, 3) @ v).transpose(1, 2).reshape(n, l, e) * torch.tensor((mask != 0).any(1)).double()[:, None, None]
+    y = a @ wo + bo + x
+    mu, var = y.mean(2, keepdim=True), (y ** 2).mean(2, keepdim=True) - y.mean(2, keepdim=True) ** 2
+    z = ((y - mu) / (var + 1e-5).sqrt() * ga + be) @ wh + bh
+    lp = torch.log_softmax(z, 2)
+    ok = torch.tensor(targets >= 0)
+    chosen = torch.where(ok, lp.gather(2, torch.tensor(np.where(targets >= 0, targets, 0)).long()[..., None])[..., 0], torch.zeros((), dtype=torch.float64))
+    h = -(lp.exp() * lp).sum(2)
+    loss = (-chosen - 0.01 * h).sum()
+    loss.backward()
+    return float(loss.detach()), [p.grad.numpy() for p in ps]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_training_step_of_all_operators(ctx, bits):
+    """Embedding, cross attention, log probabilities and AdamW as one program: gradients against float64 autograd, then the
+    compiled and captured step with eager work between the replays against the eager one."""
+    rng = np.random.default_rng(7)
+    vocab, dim, heads, kv, n, l, lk = 211, 128, 4, 2, 3, 9, 21
+    model = Reader(vocab, dim, heads, kv, bits)
+    arrays = [R.f32(rng.standard_normal(p.extents) * (1.0 if i == 0 else 0.1)) for i, p in enumerate(model.params())]
+    ids = rng.integers(0, vocab, (n, l)).astype(np.int32)
+    ids[0, -3:] = -1
+    targets = rng.integers(0, vocab, (n, l)).astype(np.int32)
+    targets[0, -3:] = -100
+    mask = np.ones((n, lk), np.float32)
+    mask[1, 10:], mask[2] = 0.0, 0.0
+    states = R.f32(rng.standard_normal((n, lk, dim)))
+
+    def build():
+        for p, a in zip(model.params(), arrays):
+            p.set(dev(ctx, a))
+        model.opt = optim.AdamW(1e-3, state_bits=bits)
+        r = nn.token_logprobs(model.pass_(Var.new(dev(ctx, ids)), Var.new(dev(ctx, states)), Var.new(dev(ctx, mask))), Var.new(dev(ctx, targets)), top=3)
+        loss = (-r.logprob - r.entropy * 0.01).sum([0, 1], False)
+        return r, loss, grad_param(loss, model)
+
+    r, loss, grads = build()
+    want_loss, want = reader_in_64_bits(arrays, ids, states, mask, targets, heads, kv)
+    prog = Program(ctx, [loss, r.top_ids] + list(grads.values())).bind()
+    # products of length 128 to 211 and sums of at most 27 rows behind one another: 1e-4 of the largest element, as for models
+    assert abs(float(loss.value.numpy()[0]) - want_loss) < 1e-4 * abs(want_loss)
+    for i, (g, w, p) in enumerate(zip(grads.values(), want, model.params())):
+        # a constant added to every key moves no probability, so the key bias's gradient is a sum that cancels to 0: its
+        # terms are the key weight's without the factors of unit size that the states are, and so is what rounding leaves
+        size = np.abs(want[i - 1] if p is model.cross.key_proj.bias else w).max()
+        near(g.value.numpy(), w.reshape(g.extents), 1e-4 * size + 1e-12, p.label)
+    assert r.top_ids.value.extents == [n, l, 3]
+    step = model.opt.compile(grads, ctx)
+    for _ in range(3):
+        prog.run()
+        step.run()
+    eager = [p.value.numpy() for p in model.params()]
+    r, loss, grads = build()
+    prog = Program(ctx, [loss] + list(grads.values())).bind()
+    step = model.opt.compile(grads, ctx)
+    prog.capture()
+    step.capture()
+    for _ in range(3):
+        prog.run()
+        nn.softmax(Var.new(dev(ctx, states)), [2]).eval(ctx)  # other work of the program in between
+        ctx.sync()
+        step.run()
+    # the sums of the composed parts (LayerNorm's gradient among them) are the same launches, so the bits are too
+    for a, p in zip(eager, model.params()):
+        assert same_bits(a, p.value.numpy()), p.label
+    prog.release_graph()
+    step.release_graph()
+
+
+def test_two_captured_programs_and_an_eager_call_keep_their_workspaces_apart(ctx):
+    """Two graphs of the calls that use workspaces, replayed in turn with eager calls of other sizes between them."""
+    rng = np.random.default_rng(8)
+
+    def program(n, v, seed):
+        rr = np.random.default_rng(seed)
+        ids, g = zipf_ids(rr, n, v).astype(np.uint32), R.f32(rr.standard_normal((n, 40)))
+        q, k, vv, _ = cross_case(rr, 1, 2, 2, 1, 900 + n, 64)
+        x = R.f32(rr.standard_normal((2, 40000)))
+        table = Var.empty([v, 40])
+        seedv = Var.new(dev(ctx, g))
+        ge = Var(Shape([v, 40]), FLOAT, "embedding_grad", [seedv, Var.new(dev(ctx, ids))], {"scale": 1.0})
+        at = nn.cross_attention(*[Var.new(dev(ctx, a)) for a in (q, k, vv)])
+        lp = nn.token_logprobs(Var.new(dev(ctx, x)), top=9)
+        prog = Program(ctx, [ge, at, lp.top_ids, lp.entropy])
+        return prog, [o.numpy() for o in prog.outputs], (table,)
+
+    p1, w1, _ = program(700, 90, 1)
+    p2, w2, _ = program(9000, 1000, 2)
+    p1.capture()
+    p2.capture()
+    for _ in range(3):
+        for p, w in ((p1, w1), (p2, w2)):
+            p.run()
+            nn.cross_attention(*[Var.new(dev(ctx, R.f32(rng.standard_normal((1, 3, s, 32))))) for s in (1, 2000, 2000)]).eval(ctx)
+            ctx.sync()
+            for o, a in zip(p.outputs, w):
+                assert same_bits(o.numpy(), a)
+    p1.release_graph()
+    p2.release_graph()
+
+
+def test_serving_steps_reuse_the_states_keys(ctx):
+    """Token by token against the whole sequence at once: each query attends on its own."""
+    rng = np.random.default_rng(11)
+    layer = bert.CrossAttention(128, 2, num_kv_heads=1)
+    for p in layer.params():
+        p.set(dev(ctx, R.f32(rng.standard_normal(p.extents) * 0.1)))
+    x, states = R.f32(rng.standard_normal((2, 4, 128))), R.f32(rng.standard_normal((2, 300, 128)))
+    mask = np.ones((2, 300), np.float32)
+    mask[1, 200:] = 0.0
+    m = Var.new(dev(ctx, mask))
+    whole = layer.pass_(Var.new(dev(ctx, x)), Var.new(dev(ctx, states)), m).eval(ctx).numpy()
+    k, v = (Var.new(t.eval(ctx)) for t in layer.keys_values(Var.new(dev(ctx, states))))
+    for i in range(4):
+        one = layer.attend(Var.new(dev(ctx, x[:, i:i + 1])), k, v, m).eval(ctx).numpy()
+        # two different splits of the same sums behind products of length 128: 1e-4 of the layer's unit variance
+        near(one[:, 0], whole[:, i], 1e-4, "token")
