@@ -1,135 +1,595 @@
-// Cross attention of queries to the states of another sequence, forward and backward, for gfx950.
+// Cross attention of queries to the states of another sequence, forward and backward, fp32 on the CDNA4 matrix cores.
+//   forward:  S = c Q K^T over the visible keys, P = e^(S - lse), O = P V, lse = log sum e^S
+//   backward: dP = dO V^T, delta = rowsum(dO O), dS = P (dP - delta), dQ = c dS K, dK = c dS^T Q, dV = P^T dO
+// The query heads that share a key head are rows below one another: a (batch, key head) pair has R = H/G * Lq rows, row r
+// being query r % Lq of head r / Lq of its group, and any number of sharing heads fills the 32-row tiles alike.
+//
+// Tiles.  A wavefront owns 32 rows (forward, dQ) or 32 keys (dK, dV) and walks the other side in blocks through LDS with
+// v_mfma_f32_32x32x2_f32.  What it owns is always the column of the accumulators, lane % 32: score blocks come out as
+// S^T (keys x rows) in the forward and dQ kernels and as S (rows x keys) in the dK/dV kernel, with register 4g + s of a
+// lane holding index 8g + 4 (lane / 32) + s of the other side, and that is the assignment the next product wants of its
+// right operand: P and dS go from accumulators to operands without LDS and without moves between lanes.  Row statistics
+// (maximum, sum, lse, delta) are a lane's own in the forward and dQ kernels; hidden keys are a lane's own in the dK/dV
+// kernel, where columns do not mix: they are left in and written as zeros.
 #include "rows.h"
 
 namespace {
 
-struct CrossP {
-    const float *q, *k, *v, *mask, *out, *gout;
-    float *lse;  // also read, by the gradient
-    float *o, *gq, *gk, *gv;
-    int N, H, G, Lq, Lk;
-    // strides over batch, head and position of: q, k, v, out, gout, gq, gk, gv
-    int64_t q_b, q_h, q_l, k_b, k_h, k_l, v_b, v_h, v_l, o_b, o_h, o_l, go_b, go_h, go_l, gq_b, gq_h, gq_l, gk_b, gk_h, gk_l, gv_b, gv_h, gv_l;
-    int64_t mask_b;
-    float scale;
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+struct Rows {  // [N, heads, length, D] operand
+    const float *p;
+    int64_t b, h, l;  // element strides
 };
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-    return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
+struct CrossP {
+    Rows q, k, v, o, go, gq, gk, gv;  // o: written by the forward call, read by the gradient
+    const float *mask;
+    float *lse, *delta;
+    float *part_o, *part_ml;  // of split sums: [split][row][D], [split][row][2]
+    float *part_k, *part_v;   // [split][key][D]
+    int N, H, G, Lq, Lk, R;   // R = H / G * Lq: rows of a (batch, key head) pair
+    int64_t mask_b;
+    float scale;
+    uint32_t tiles, pairs, splits;
+    sg_fastdiv d_lq, d_tiles, d_pairs, d_g;
+};
+
+__device__ __forceinline__ uint32_t fdiv(uint32_t n, sg_fastdiv d) { return (__umulhi(n, d.magic) + n) >> d.shift; }
+
+// Workgroup ids go round-robin over the 8 XCDs; consecutive work (tiles of one pair, which share keys or rows) goes to one.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t total) {
+    const uint32_t per = total / 8, rest = total % 8, x = id % 8;
+    return x * per + (x < rest ? x : rest) + id / 8;
 }
 
-// A wavefront per query row, 64 keys at a time: a key per lane for the scores, a head index per lane for the sums.
+struct Work {
+    uint32_t split, pair, tile;
+    int b, g;
+};
+__device__ __forceinline__ Work find_work(const CrossP &p) {
+    Work w;
+    const uint32_t id = xcd_order(blockIdx.x, p.tiles * p.pairs * p.splits);
+    const uint32_t rest = fdiv(id, p.d_tiles);
+    w.tile = id - rest * p.tiles;
+    w.split = fdiv(rest, p.d_pairs);
+    w.pair = rest - w.split * p.pairs;
+    w.b = (int)fdiv(w.pair, p.d_g);
+    w.g = (int)w.pair - w.b * p.G;
+    return w;
+}
+
+// Element offset of row r of a pair.
+__device__ __forceinline__ int64_t row_at(const CrossP &p, const Rows &x, const Work &w, uint32_t r) {
+    const uint32_t hh = fdiv(r, p.d_lq);
+    return w.b * x.b + (int64_t)(w.g * (p.H / p.G) + (int)hh) * x.h + (int64_t)(r - hh * p.Lq) * x.l;
+}
+
+__device__ __forceinline__ f32x4 load4(const float *p, bool vec) {
+    f32x4 v;
+    if (vec) v = *reinterpret_cast<const f32x4 *>(p);
+    else { v.x = p[0]; v.y = p[1]; v.z = p[2]; v.w = p[3]; }
+    return v;
+}
+__device__ __forceinline__ void store4(float *p, f32x4 v, bool vec) {
+    if (vec) *reinterpret_cast<f32x4 *>(p) = v;
+    else { p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w; }
+}
+
+// One behind the last visible key of a sequence: a padded batch costs what its lengths cost.
+__device__ __forceinline__ int visible_end(const CrossP &p, int b, int *lds) {
+    if (!p.mask) return p.Lk;
+    const float *m = p.mask + b * p.mask_b;
+    int end = 0;
+    for (int j = threadIdx.x; j < p.Lk; j += 256)
+        if (m[j] != 0.0f) end = j + 1;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) end = max(end, __shfl_xor(end, o, 64));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = end;
+    __syncthreads();
+    end = max(max(lds[0], lds[1]), max(lds[2], lds[3]));
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(end);
+}
+
+// Blocks [first, last) of the `blocks` that this split takes.
+__device__ __forceinline__ void split_range(uint32_t blocks, uint32_t split, uint32_t splits, uint32_t *first, uint32_t *last) {
+    const uint32_t per = blocks / splits, rest = blocks % splits;
+    *first = split * per + (split < rest ? split : rest);
+    *last = *first + per + (split < rest ? 1u : 0u);
+}
+
+// Rows of D floats from memory to registers to LDS, KB rows a block, 256 threads.  Piece i of a thread: row (tid + 256 i) / ROWV.
+template <int D, int KB>
+struct Stage {
+    static constexpr int LD = D + 4;  // LDS row stride (floats): 8 consecutive rows cover all banks
+    static constexpr int ROWV = D / 4, N = KB * ROWV / 256;
+    f32x4 x[N];
+    __device__ static int row(int i) { return ((int)threadIdx.x + i * 256) / ROWV; }
+    __device__ static int col() { return ((int)threadIdx.x % ROWV) * 4; }
+    __device__ void deposit(float *lds) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4 *>(&lds[row(i) * LD + col()]) = x[i];
+    }
+    // rows of hidden keys become zeros: 0 * NaN is NaN
+    __device__ void hide(const uint64_t *seen) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!(seen[row(i) / 64] >> (row(i) % 64) & 1)) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+};
+
+// Which keys of a block are visible: requested with the block, turned into bits (the same in every wavefront) and an
+// addend of the scores when it is deposited.
+template <int KB>
+struct Visible {
+    float x[KB / 64];
+    __device__ void request(const float *mask, int j0, int Lk) {
+#pragma unroll
+        for (int i = 0; i < KB / 64; ++i) {
+            const int j = j0 + i * 64 + ((int)threadIdx.x & 63);
+            x[i] = j < Lk ? (mask ? mask[j] : 1.0f) : 0.0f;
+        }
+    }
+    template <class S>
+    __device__ void hide(S &k, S &v) const {
+        uint64_t seen[KB / 64];
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < KB / 64; ++i) {
+            seen[i] = __builtin_amdgcn_ballot_w64(x[i] != 0.0f);
+            all = all && seen[i] == ~0ull;
+        }
+        if (all) return;
+        k.hide(seen);
+        v.hide(seen);
+    }
+    __device__ void deposit(float *lds_m) const {
+#pragma unroll
+        for (int i = 0; i < KB / 64; ++i)
+            if (threadIdx.x < 64) lds_m[i * 64 + threadIdx.x] = x[i] != 0.0f ? 0.0f : -__builtin_inff();
+    }
+};
+
+// A wavefront's own 32 columns as the right operand: register [g][s] of lane (c, h) = x[c][8g + 4h + s].
 template <int D>
-__global__ void __launch_bounds__(64) cross_forward_kernel(const CrossP p) {
-    const int lane = threadIdx.x;
-    const unsigned id = blockIdx.x;
-    const int l = id % p.Lq, h = id / p.Lq % p.H, b = id / p.Lq / p.H, g = h / (p.H / p.G);
-    const float *q = p.q + b * p.q_b + h * p.q_h + l * p.q_l, *K = p.k + b * p.k_b + g * p.k_h, *V = p.v + b * p.v_b + g * p.v_h;
+struct Own {
+    float x[D / 8][4];
+    __device__ void take(const float *lds, int c, int h) {  // row c of an LDS tile
+#pragma unroll
+        for (int g = 0; g < D / 8; ++g) {
+            const f32x4 t = *reinterpret_cast<const f32x4 *>(&lds[c * (D + 4) + 8 * g + 4 * h]);
+            x[g][0] = t.x; x[g][1] = t.y; x[g][2] = t.z; x[g][3] = t.w;
+        }
+    }
+};
+
+__device__ __forceinline__ floatx16 zero16() {
+    floatx16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    return z;
+}
+
+// 32 rows of an LDS tile times a wavefront's own columns, contracted over the head dimension.
+template <int D>
+__device__ __forceinline__ floatx16 scores(const float *tile, const Own<D> &own, int c, int h) {
+    floatx16 acc = zero16();
+#pragma unroll
+    for (int g = 0; g < D / 8; ++g) {
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(&tile[c * (D + 4) + 8 * g + 4 * h]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], own.x[g][s], acc, 0, 0, 0);
+    }
+    return acc;
+}
+
+// acc[j] += tile^T . w over the tile's 32 rows.  Row m of output block j stands for head index ND m + j, so that what a
+// lane feeds to the ND blocks for one row is adjacent in LDS.
+template <int D>
+__device__ __forceinline__ void accumulate(const float *tile, const floatx16 &w, floatx16 *acc, int c, int h) {
+    constexpr int ND = D / 32;
+    typedef float vecND __attribute__((ext_vector_type(ND)));
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        vecND a[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a[s] = *reinterpret_cast<const vecND *>(&tile[(8 * g + 4 * h + s) * (D + 4) + ND * c]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < ND; ++j) acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s][j], w[4 * g + s], acc[j], 0, 0, 0);
+    }
+}
+
+// What accumulate() left of column c: consecutive head indices ND (8g + 4h) .. + 4 ND, times f.
+template <int D>
+__device__ __forceinline__ void write_column(float *row, const floatx16 *acc, float f, int h, bool vec) {
+    constexpr int ND = D / 32;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        float t[4 * ND];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < ND; ++j) t[ND * s + j] = acc[j][4 * g + s] * f;
+#pragma unroll
+        for (int c = 0; c < ND; ++c) store4(row + ND * (8 * g + 4 * h) + 4 * c, f32x4{t[4 * c], t[4 * c + 1], t[4 * c + 2], t[4 * c + 3]}, vec);
+    }
+}
+
+// The 32 RW rows of a workgroup's tile, through the LDS of the key blocks, to the wavefronts that own them.
+template <int D, int RW, int KB>
+__device__ __forceinline__ void take_rows(const CrossP &p, const Rows &x, const Work &w, bool vec, float *lds_a, float *lds_b, int own_row, int h, Own<D> &own) {
+    constexpr int ROWV = D / 4, LD = D + 4;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 32 * RW * ROWV / 256; ++i) {
+        const int f = threadIdx.x + i * 256, row = f / ROWV, c = (f % ROWV) * 4;
+        const uint32_t r = min(w.tile * (32 * RW) + row, (uint32_t)p.R - 1);  // a row past the end repeats the last one; it is not written
+        *reinterpret_cast<f32x4 *>(&(row < KB ? lds_a : lds_b)[(row % KB) * LD + c]) = load4(x.p + row_at(p, x, w, r) + c, vec);
+    }
+    __syncthreads();
+    own.take(&(own_row < KB ? lds_a : lds_b)[(own_row - own_row % 32) % KB * LD], own_row % 32, h);
+}
+
+// ---- forward.  RW wavefronts take the workgroup's 32 RW rows, the 4 / RW times as many share each block's keys and are
+// merged through LDS at the end.
+template <int D, int RW, bool VEC>
+__global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
+    constexpr int KW = 4 / RW, KB = RW == 1 ? 128 : 64, NKB = KB / KW / 32, LD = D + 4, ND = D / 32;
+    __shared__ __attribute__((aligned(16))) float lds_k[KB * LD], lds_v[KB * LD], lds_m[KB];
+    const Work w = find_work(p);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
+    const int own_row = (wave % RW) * 32 + c, kw = wave / RW * (KB / KW);
+    const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
+    const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
+    const int end = visible_end(p, w.b, reinterpret_cast<int *>(lds_m));
     const float inf = __builtin_inff();
-    float m = -inf, s = 0.0f, acc = 0.0f;
-    for (int j0 = 0; j0 < p.Lk; j0 += 64) {
-        const int j = j0 + lane;
-        const bool seen = j < p.Lk && (!p.mask || p.mask[b * p.mask_b + j] != 0.0f);
-        float x = -inf;
-        if (seen) {
-            x = 0.0f;
-            for (int d = 0; d < D; ++d) x += q[d] * K[j * p.k_l + d];
-            x *= p.scale;
-        }
-        const float mn = fmaxf(m, wave_max(x));
-        if (mn == -inf) continue;
-        const float c = expf(m - mn), e = expf(x - mn);
-        s = s * c + wave_sum(e);
-        acc *= c;
-        m = mn;
-        for (int r = 0; r < 64; ++r) {
-            const float er = __shfl(e, r, 64);
-            if (__shfl((int)seen, r, 64) && lane < D) acc += er * V[(j0 + r) * p.v_l + lane];
-        }
-    }
-    if (lane < D) p.o[b * p.o_b + h * p.o_h + l * p.o_l + lane] = s > 0.0f ? acc / s : s == s ? 0.0f : s;
-    if (p.lse && lane == 0) p.lse[id] = s == 0.0f ? -inf : m + logf(s);
-}
 
-template <int D>
-__global__ void __launch_bounds__(64) cross_gq_kernel(const CrossP p) {
-    const int lane = threadIdx.x;
-    const unsigned id = blockIdx.x;
-    const int l = id % p.Lq, h = id / p.Lq % p.H, b = id / p.Lq / p.H, g = h / (p.H / p.G);
-    const float *q = p.q + b * p.q_b + h * p.q_h + l * p.q_l, *K = p.k + b * p.k_b + g * p.k_h, *V = p.v + b * p.v_b + g * p.v_h;
-    const float *go = p.gout + b * p.go_b + h * p.go_h + l * p.go_l, *o = p.out + b * p.o_b + h * p.o_h + l * p.o_l;
-    const float lse = p.lse[id];
-    const float delta = wave_sum(lane < D ? go[lane] * o[lane] : 0.0f);
-    float acc = 0.0f;
-    for (int j0 = 0; j0 < p.Lk; j0 += 64) {
-        const int j = j0 + lane;
-        const bool seen = j < p.Lk && (!p.mask || p.mask[b * p.mask_b + j] != 0.0f);
-        float ds = 0.0f;
-        if (seen) {
-            float x = 0.0f, dp = 0.0f;
-            for (int d = 0; d < D; ++d) {
-                x += q[d] * K[j * p.k_l + d];
-                dp += go[d] * V[j * p.v_l + d];
-            }
-            ds = expf(x * p.scale - lse) * (dp - delta) * p.scale;
-        }
-        for (int r = 0; r < 64; ++r) {
-            const float dr = __shfl(ds, r, 64);
-            if (__shfl((int)seen, r, 64) && lane < D) acc += dr * K[(j0 + r) * p.k_l + lane];
-        }
-    }
-    if (lane < D) p.gq[b * p.gq_b + h * p.gq_h + l * p.gq_l + lane] = acc;
-}
+    Own<D> q;
+    take_rows<D, RW, KB>(p, p.q, w, VEC, lds_k, lds_v, own_row, h, q);
+    floatx16 acc[ND];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) acc[j] = zero16();
+    float m_run = -inf, l_run = 0.0f;
+    const float c2 = p.scale * LOG2E;
 
-template <int D>
-__global__ void __launch_bounds__(64) cross_gkv_kernel(const CrossP p) {
-    const int lane = threadIdx.x;
-    const unsigned id = blockIdx.x;
-    const int j = id % p.Lk, g = id / p.Lk % p.G, b = id / p.Lk / p.G, group = p.H / p.G;
-    const float *k = p.k + b * p.k_b + g * p.k_h + j * p.k_l, *v = p.v + b * p.v_b + g * p.v_h + j * p.v_l;
-    float ak = 0.0f, av = 0.0f;
-    if (!p.mask || p.mask[b * p.mask_b + j] != 0.0f) {
-        for (int hh = 0; hh < group; ++hh) {
-            const int h = g * group + hh;
-            const float *Q = p.q + b * p.q_b + h * p.q_h, *GO = p.gout + b * p.go_b + h * p.go_h, *O = p.out + b * p.o_b + h * p.o_h;
-            for (int l0 = 0; l0 < p.Lq; l0 += 64) {
-                const int l = l0 + lane;
-                float pr = 0.0f, ds = 0.0f;
-                if (l < p.Lq) {
-                    float x = 0.0f, dp = 0.0f, delta = 0.0f;
-                    for (int d = 0; d < D; ++d) {
-                        x += Q[l * p.q_l + d] * k[d];
-                        dp += GO[l * p.go_l + d] * v[d];
-                        delta += GO[l * p.go_l + d] * O[l * p.o_l + d];
-                    }
-                    pr = expf(x * p.scale - p.lse[((int64_t)b * p.H + h) * p.Lq + l]);
-                    ds = pr * (dp - delta) * p.scale;
-                }
-                for (int r = 0; r < 64 && l0 + r < p.Lq; ++r) {
-                    const float er = __shfl(pr, r, 64), dr = __shfl(ds, r, 64);
-                    if (lane < D) {
-                        av += er * GO[(l0 + r) * p.go_l + lane];
-                        ak += dr * Q[(l0 + r) * p.q_l + lane];
-                    }
+    Stage<D, KB> ks, vs;
+    Visible<KB> seen;
+    auto request = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < ks.N; ++i) {
+            const int64_t j = min(j0 + ks.row(i), p.Lk - 1);
+            ks.x[i] = load4(K + j * p.k.l + ks.col(), VEC);
+            vs.x[i] = load4(V + j * p.v.l + vs.col(), VEC);
+        }
+        seen.request(mask, j0, p.Lk);
+    };
+    uint32_t first, last;
+    split_range((end + KB - 1) / KB, w.split, p.splits, &first, &last);
+    if (first < last) request(first * KB);
+    for (uint32_t blk = first; blk < last; ++blk) {
+        seen.hide(ks, vs);
+        __syncthreads();
+        ks.deposit(lds_k);
+        vs.deposit(lds_v);
+        seen.deposit(lds_m);
+        __syncthreads();
+        if (blk + 1 < last) request((blk + 1) * KB);
+        floatx16 s[NKB];
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) s[b] = scores<D>(&lds_k[(kw + b * 32) * LD], q, c, h);
+        float top = -inf;
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 mk = *reinterpret_cast<const f32x4 *>(&lds_m[kw + b * 32 + 8 * g + 4 * h]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[b][4 * g + i] = __builtin_fmaf(s[b][4 * g + i], c2, mk[i]);
+                    top = fmaxf(top, s[b][4 * g + i]);
                 }
             }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float m_new = fmaxf(m_run, top);
+        const float shift = m_new == -inf ? 0.0f : m_new;  // nothing visible so far: every exponential below is 0
+        if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
+            const float f = __builtin_amdgcn_exp2f(m_run - shift);
+            l_run *= f;
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[j][r] *= f;
+        }
+        m_run = m_new;
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - shift);
+                l_run += s[b][r];
+            }
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) accumulate<D>(&lds_v[(kw + b * 32) * LD], s[b], acc, c, h);
+    }
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (KW > 1) {
+        constexpr int SLOT = 16 * ND + 2;  // floats of a lane
+        static_assert((KW - 1) * RW * 64 * SLOT <= KB * LD, "the merge fits in the keys' LDS");
+        __syncthreads();
+        if (wave >= RW) {
+            float *to = &lds_k[((wave - RW) * 64 + lane) * SLOT];
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) to[16 * j + r] = acc[j][r];
+            to[16 * ND] = m_run;
+            to[16 * ND + 1] = l_run;
+        }
+        __syncthreads();
+        if (wave >= RW) return;
+#pragma unroll
+        for (int o = 1; o < KW; ++o) {
+            const float *from = &lds_k[((o - 1) * RW * 64 + wave * 64 + lane) * SLOT];
+            const float mo = from[16 * ND], m = fmaxf(m_run, mo), shift = m == -inf ? 0.0f : m;
+            const float fa = __builtin_amdgcn_exp2f(m_run - shift), fb = __builtin_amdgcn_exp2f(mo - shift);
+            l_run = l_run * fa + from[16 * ND + 1] * fb;
+            m_run = m;
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[j][r] = acc[j][r] * fa + from[16 * j + r] * fb;
         }
     }
-    if (lane < D) {
-        p.gk[b * p.gk_b + g * p.gk_h + j * p.gk_l + lane] = ak;
-        p.gv[b * p.gv_b + g * p.gv_h + j * p.gv_l + lane] = av;
+    const uint32_t r = w.tile * (32 * RW) + own_row;
+    if (r >= (uint32_t)p.R) return;
+    const int64_t row = (int64_t)w.pair * p.R + r;
+    if (p.splits > 1) {
+        const int64_t at = (int64_t)w.split * p.pairs * p.R + row;
+        write_column<D>(p.part_o + at * D, acc, 1.0f, h, true);
+        if (h == 0) { p.part_ml[2 * at] = m_run; p.part_ml[2 * at + 1] = l_run; }
+        return;
+    }
+    write_column<D>(const_cast<float *>(p.o.p) + row_at(p, p.o, w, r), acc, l_run == 0.0f ? 0.0f : 1.0f / l_run, h, VEC);
+    if (p.lse && h == 0) p.lse[row] = l_run == 0.0f ? -inf : (m_run + __builtin_amdgcn_logf(l_run)) * LN2;
+}
+
+// Joins the splits of a row: D / 4 lanes a row.
+template <int D>
+__global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p, int vec) {
+    constexpr int LPR = D / 4;
+    const uint32_t total = p.pairs * p.R, row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
+    if (row >= total) return;
+    const float inf = __builtin_inff();
+    float m = -inf, l = 0.0f;
+    for (uint32_t i = 0; i < p.splits; ++i) m = fmaxf(m, p.part_ml[2 * ((int64_t)i * total + row)]);
+    const float shift = m == -inf ? 0.0f : m;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i = 0; i < p.splits; ++i) {
+        const int64_t at = (int64_t)i * total + row;
+        const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - shift);
+        l += p.part_ml[2 * at + 1] * f;
+        acc += *reinterpret_cast<const f32x4 *>(p.part_o + at * D + col) * f;
+    }
+    Work w;
+    w.pair = row / p.R;
+    w.b = (int)fdiv(w.pair, p.d_g);
+    w.g = (int)w.pair - w.b * p.G;
+    store4(const_cast<float *>(p.o.p) + row_at(p, p.o, w, row - w.pair * p.R) + col, acc * (l == 0.0f ? 0.0f : 1.0f / l), vec);
+    if (p.lse && col == 0) p.lse[row] = l == 0.0f ? -inf : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ---- gradient of the queries (and delta, for the other kernel)
+template <int D, int RW, bool VEC>
+__global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
+    constexpr int KW = 4 / RW, KB = RW == 1 ? 128 : 64, NKB = KB / KW / 32, LD = D + 4, ND = D / 32;
+    __shared__ __attribute__((aligned(16))) float lds_k[KB * LD], lds_v[KB * LD], lds_m[KB];
+    const Work w = find_work(p);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
+    const int own_row = (wave % RW) * 32 + c, kw = wave / RW * (KB / KW);
+    const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
+    const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
+    const int end = visible_end(p, w.b, reinterpret_cast<int *>(lds_m));
+    const uint32_t r = w.tile * (32 * RW) + own_row;
+    const int64_t row = (int64_t)w.pair * p.R + min(r, (uint32_t)p.R - 1);
+
+    Own<D> q, go;
+    float delta = 0.0f;
+    take_rows<D, RW, KB>(p, p.o, w, VEC, lds_k, lds_v, own_row, h, q);
+    take_rows<D, RW, KB>(p, p.go, w, VEC, lds_k, lds_v, own_row, h, go);
+#pragma unroll
+    for (int g = 0; g < D / 8; ++g)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) delta += q.x[g][s] * go.x[g][s];
+    delta += __shfl_xor(delta, 32, 64);
+    if (w.split == 0 && wave < RW && h == 0 && r < (uint32_t)p.R) p.delta[row] = delta;
+    take_rows<D, RW, KB>(p, p.q, w, VEC, lds_k, lds_v, own_row, h, q);
+    const float lse2 = p.lse[row] * LOG2E, c2 = p.scale * LOG2E;
+    floatx16 acc[ND];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) acc[j] = zero16();
+
+    Stage<D, KB> ks, vs;
+    Visible<KB> seen;
+    auto request = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < ks.N; ++i) {
+            const int64_t j = min(j0 + ks.row(i), p.Lk - 1);
+            ks.x[i] = load4(K + j * p.k.l + ks.col(), VEC);
+            vs.x[i] = load4(V + j * p.v.l + vs.col(), VEC);
+        }
+        seen.request(mask, j0, p.Lk);
+    };
+    uint32_t first, last;
+    split_range((end + KB - 1) / KB, w.split, p.splits, &first, &last);
+    if (first < last) request(first * KB);
+    for (uint32_t blk = first; blk < last; ++blk) {
+        seen.hide(ks, vs);
+        __syncthreads();
+        ks.deposit(lds_k);
+        vs.deposit(lds_v);
+        seen.deposit(lds_m);
+        __syncthreads();
+        if (blk + 1 < last) request((blk + 1) * KB);
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+            const int at = kw + b * 32;
+            floatx16 s = scores<D>(&lds_k[at * LD], q, c, h);
+            const floatx16 dp = scores<D>(&lds_v[at * LD], go, c, h);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 mk = *reinterpret_cast<const f32x4 *>(&lds_m[at + 8 * g + 4 * h]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c2, mk[i]) - lse2);
+                    s[4 * g + i] = e * (dp[4 * g + i] - delta);
+                }
+            }
+            accumulate<D>(&lds_k[at * LD], s, acc, c, h);
+        }
+    }
+    if (KW > 1) {
+        constexpr int SLOT = 16 * ND + 2;
+        static_assert((KW - 1) * RW * 64 * SLOT <= KB * LD, "the merge fits in the keys' LDS");
+        __syncthreads();
+        if (wave >= RW) {
+            float *to = &lds_k[((wave - RW) * 64 + lane) * SLOT];
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[16 * j + i] = acc[j][i];
+        }
+        __syncthreads();
+        if (wave >= RW) return;
+#pragma unroll
+        for (int o = 1; o < KW; ++o) {
+            const float *from = &lds_k[((o - 1) * RW * 64 + wave * 64 + lane) * SLOT];
+#pragma unroll
+            for (int j = 0; j < ND; ++j)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[j][i] += from[16 * j + i];
+        }
+    }
+    if (r >= (uint32_t)p.R) return;
+    if (p.splits > 1) write_column<D>(p.part_o + ((int64_t)w.split * p.pairs * p.R + row) * D, acc, p.scale, h, true);
+    else write_column<D>(const_cast<float *>(p.gq.p) + row_at(p, p.gq, w, r), acc, p.scale, h, VEC);
+}
+
+// ---- gradients of keys and values: a wavefront owns 32 keys and walks all rows of the pair.
+template <int D, bool VEC>
+__global__ void __launch_bounds__(256) cross_gkv_kernel(const CrossP p) {
+    constexpr int RB = 64, LD = D + 4, ND = D / 32, ROWV = D / 4;
+    __shared__ __attribute__((aligned(16))) float lds_q[RB * LD], lds_go[RB * LD], lds_lse[RB], lds_delta[RB];
+    const Work w = find_work(p);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
+    const int j = (int)w.tile * 128 + wave * 32 + c;
+    const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
+    const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
+    const bool seen = j < p.Lk && (!mask || mask[j] != 0.0f);
+    const float inf = __builtin_inff();
+
+    Own<D> k, v;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {  // two wavefronts' keys at a time go through the rows' LDS
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RB * ROWV / 256; ++i) {
+            const int f = tid + i * 256, row = f / ROWV, col = (f % ROWV) * 4;
+            const int64_t jj = min((int)w.tile * 128 + half * 64 + row, p.Lk - 1);
+            *reinterpret_cast<f32x4 *>(&lds_q[row * LD + col]) = load4(K + jj * p.k.l + col, VEC);
+            *reinterpret_cast<f32x4 *>(&lds_go[row * LD + col]) = load4(V + jj * p.v.l + col, VEC);
+        }
+        __syncthreads();
+        if (wave / 2 == half) {
+            k.take(&lds_q[(wave & 1) * 32 * LD], c, h);
+            v.take(&lds_go[(wave & 1) * 32 * LD], c, h);
+        }
+    }
+    const bool any = __syncthreads_or(seen);
+    floatx16 gk[ND], gv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) gk[d] = gv[d] = zero16();
+    const float c2 = p.scale * LOG2E;
+
+    Stage<D, RB> qs, gs;
+    float lreg = 0.0f, dreg = 0.0f;
+    auto request = [&](uint32_t r0) {
+#pragma unroll
+        for (int i = 0; i < qs.N; ++i) {
+            const uint32_t r = min(r0 + qs.row(i), (uint32_t)p.R - 1);
+            qs.x[i] = load4(p.q.p + row_at(p, p.q, w, r) + qs.col(), VEC);
+            gs.x[i] = load4(p.go.p + row_at(p, p.go, w, r) + gs.col(), VEC);
+        }
+        if (tid < RB) {
+            const uint32_t r = r0 + tid;
+            lreg = r < (uint32_t)p.R ? p.lse[(int64_t)w.pair * p.R + r] * LOG2E : inf;  // a row past the end: every exponential is 0
+            dreg = r < (uint32_t)p.R ? p.delta[(int64_t)w.pair * p.R + r] : 0.0f;
+        }
+    };
+    uint32_t first, last;
+    split_range((p.R + RB - 1) / RB, w.split, p.splits, &first, &last);
+    if (!any) last = first;
+    if (first < last) request(first * RB);
+    for (uint32_t blk = first; blk < last; ++blk) {
+        __syncthreads();
+        qs.deposit(lds_q);
+        gs.deposit(lds_go);
+        if (tid < RB) { lds_lse[tid] = lreg; lds_delta[tid] = dreg; }
+        __syncthreads();
+        if (blk + 1 < last) request((blk + 1) * RB);
+#pragma unroll
+        for (int b = 0; b < RB / 32; ++b) {
+            floatx16 s = scores<D>(&lds_q[b * 32 * LD], k, c, h);
+            floatx16 dp = scores<D>(&lds_go[b * 32 * LD], v, c, h);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 ls = *reinterpret_cast<const f32x4 *>(&lds_lse[b * 32 + 8 * g + 4 * h]);
+                const f32x4 dl = *reinterpret_cast<const f32x4 *>(&lds_delta[b * 32 + 8 * g + 4 * h]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c2, -ls[i]));
+                    s[4 * g + i] = e;
+                    dp[4 * g + i] = e * (dp[4 * g + i] - dl[i]);
+                }
+            }
+            accumulate<D>(&lds_go[b * 32 * LD], s, gv, c, h);
+            accumulate<D>(&lds_q[b * 32 * LD], dp, gk, c, h);
+        }
+    }
+    if (j >= p.Lk) return;
+    if (!seen) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) gk[d] = gv[d] = zero16();
+    }
+    if (p.splits > 1) {
+        const int64_t at = (((int64_t)w.split * p.pairs + w.pair) * p.Lk + j) * D;
+        write_column<D>(p.part_k + at, gk, p.scale, h, true);
+        write_column<D>(p.part_v + at, gv, 1.0f, h, true);
+    } else {
+        write_column<D>(const_cast<float *>(p.gk.p) + w.b * p.gk.b + w.g * p.gk.h + (int64_t)j * p.gk.l, gk, p.scale, h, VEC);
+        write_column<D>(const_cast<float *>(p.gv.p) + w.b * p.gv.b + w.g * p.gv.h + (int64_t)j * p.gv.l, gv, 1.0f, h, VEC);
     }
 }
 
-int check_operand(sg_ctx *ctx, const sg_tensor *t, int64_t n, int64_t heads, int64_t len, int64_t D, const char *who, const float **ptr, int64_t *sb,
-                  int64_t *sh, int64_t *sl) {
+// out[row] = sum of the splits' rows, in order: D / 4 lanes a row.  Rows of a pair are `heads` x `length`.
+template <int D>
+__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, Rows out, uint32_t total, uint32_t splits, uint32_t heads, uint32_t length, int vec) {
+    constexpr int LPR = D / 4;
+    const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
+    if (row >= total) return;
+    f32x4 acc = *reinterpret_cast<const f32x4 *>(part + (int64_t)row * D + col);
+    for (uint32_t i = 1; i < splits; ++i) acc += *reinterpret_cast<const f32x4 *>(part + ((int64_t)i * total + row) * D + col);
+    const uint32_t bh = row / length;
+    store4(const_cast<float *>(out.p) + bh / heads * out.b + bh % heads * out.h + (int64_t)(row - bh * length) * out.l + col, acc, vec);
+}
+
+int check_operand(sg_ctx *ctx, const sg_tensor *t, int64_t n, int64_t heads, int64_t len, int64_t D, const char *who, Rows *r) {
     const int rc = sg_check_f32(ctx, t, who);
     if (rc != SG_OK) return rc;
     if (t->rank != 4) return sg_fail(ctx, SG_ERR_SHAPE, "%s: rank %d, expected [batch, heads, length, head size]", who, t->rank);
@@ -137,10 +597,7 @@ int check_operand(sg_ctx *ctx, const sg_tensor *t, int64_t n, int64_t heads, int
         return sg_fail(ctx, SG_ERR_SHAPE, "%s: [%lld, %lld, %lld, %lld], expected [%lld, %lld, %lld, %lld]", who, (long long)t->extents[0], (long long)t->extents[1],
                        (long long)t->extents[2], (long long)t->extents[3], (long long)n, (long long)heads, (long long)len, (long long)D);
     if (t->strides[3] != 1) return sg_fail(ctx, SG_ERR_SHAPE, "%s: the head dimension must have unit stride", who);
-    *ptr = (const float *)t->base + t->offset;
-    *sb = t->strides[0];
-    *sh = t->strides[1];
-    *sl = t->strides[2];
+    *r = {(const float *)t->base + t->offset, t->strides[0], t->strides[1], t->strides[2]};
     return SG_OK;
 }
 
@@ -169,10 +626,10 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
     const int64_t N = q->extents[0], H = q->extents[1], Lq = q->extents[2], D = q->extents[3], G = k->extents[1], Lk = k->extents[2];
     if (D != 32 && D != 64) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: head size %lld (32 and 64 are built)", (long long)D);
     if (H % G != 0) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: %lld query heads over %lld key heads", (long long)H, (long long)G);
-    if ((rc = check_operand(ctx, q, N, H, Lq, D, "cross attention q", &p.q, &p.q_b, &p.q_h, &p.q_l)) != SG_OK) return rc;
-    if ((rc = check_operand(ctx, k, N, G, Lk, D, "cross attention k", &p.k, &p.k_b, &p.k_h, &p.k_l)) != SG_OK) return rc;
-    if ((rc = check_operand(ctx, v, N, G, Lk, D, "cross attention v", &p.v, &p.v_b, &p.v_h, &p.v_l)) != SG_OK) return rc;
-    if ((rc = check_operand(ctx, out, N, H, Lq, D, "cross attention out", &p.out, &p.o_b, &p.o_h, &p.o_l)) != SG_OK) return rc;
+    if ((rc = check_operand(ctx, q, N, H, Lq, D, "cross attention q", &p.q)) != SG_OK) return rc;
+    if ((rc = check_operand(ctx, k, N, G, Lk, D, "cross attention k", &p.k)) != SG_OK) return rc;
+    if ((rc = check_operand(ctx, v, N, G, Lk, D, "cross attention v", &p.v)) != SG_OK) return rc;
+    if ((rc = check_operand(ctx, out, N, H, Lq, D, "cross attention out", &p.o)) != SG_OK) return rc;
     if (out_written && (rc = check_apart(ctx, out, "cross attention out")) != SG_OK) return rc;
     if (mask) {
         if ((rc = sg_check_f32(ctx, mask, "cross attention mask")) != SG_OK) return rc;
@@ -188,24 +645,78 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
         p.lse = (float *)lse->base + lse->offset;
     }
     p.N = (int)N; p.H = (int)H; p.G = (int)G; p.Lq = (int)Lq; p.Lk = (int)Lk;
+    p.R = (int)(H / G * Lq);
+    p.pairs = (uint32_t)(N * G);
+    p.d_lq = sg_make_fastdiv((uint32_t)Lq);
+    p.d_g = sg_make_fastdiv((uint32_t)G);
+    p.d_pairs = sg_make_fastdiv(p.pairs);
+    return SG_OK;
+}
+
+bool vec_rows(const Rows &r) { return ((uintptr_t)r.p) % 16 == 0 && r.b % 4 == 0 && r.h % 4 == 0 && r.l % 4 == 0; }
+
+// Splits of a long axis of `blocks` blocks that bring `units` workgroups to two for each compute unit.
+uint32_t choose_splits(const sg_ctx *ctx, uint32_t units, uint32_t blocks) {
+    const uint32_t want = 2u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+    uint32_t s = units >= want ? 1 : (want + units - 1) / units;
+    if (s > blocks / 2) s = blocks / 2;
+    return s < 1 ? 1 : s > 64 ? 64 : s;
+}
+
+int row_waves(int R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
+
+int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
+    p.tiles = (uint32_t)tiles;
+    p.splits = splits;
+    if (tiles * p.pairs * splits >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: too many rows for one launch");
+    p.d_tiles = sg_make_fastdiv(p.tiles);
     return SG_OK;
 }
 
 }  // namespace
 
+#define SG_CROSS_LAUNCH(KERNEL, RW, VEC, GRID)                                                                          \
+    do {                                                                                                                \
+        if (D == 64 && VEC) hipLaunchKernelGGL((KERNEL<64, RW, true>), GRID, dim3(256), 0, ctx->stream, p);             \
+        else if (D == 64) hipLaunchKernelGGL((KERNEL<64, RW, false>), GRID, dim3(256), 0, ctx->stream, p);              \
+        else if (VEC) hipLaunchKernelGGL((KERNEL<32, RW, true>), GRID, dim3(256), 0, ctx->stream, p);                   \
+        else hipLaunchKernelGGL((KERNEL<32, RW, false>), GRID, dim3(256), 0, ctx->stream, p);                           \
+    } while (0)
+#define SG_CROSS_ROWS(KERNEL, RW, VEC, GRID)                                                                            \
+    do {                                                                                                                \
+        if (RW == 4) SG_CROSS_LAUNCH(KERNEL, 4, VEC, GRID);                                                             \
+        else if (RW == 2) SG_CROSS_LAUNCH(KERNEL, 2, VEC, GRID);                                                        \
+        else SG_CROSS_LAUNCH(KERNEL, 1, VEC, GRID);                                                                     \
+    } while (0)
+
 extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask, float scale,
                                   const sg_tensor *out, const sg_tensor *lse) {
     CrossP p{};
-    const int rc = check_call(ctx, q, k, v, mask, out, lse, true, p);
+    int rc = check_call(ctx, q, k, v, mask, out, lse, true, p);
     if (rc != SG_OK) return rc;
     if (!ctx) return SG_ERR_ARG;
-    p.o = const_cast<float *>(p.out);
     p.scale = scale;
     sg_device_guard guard(ctx);
-    const dim3 grid((unsigned)(p.N * p.H * p.Lq));
-    if (q->extents[3] == 64) hipLaunchKernelGGL((cross_forward_kernel<64>), grid, dim3(64), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((cross_forward_kernel<32>), grid, dim3(64), 0, ctx->stream, p);
+    const int64_t D = q->extents[3];
+    const int rw = row_waves(p.R), kb = rw == 1 ? 128 : 64;
+    const uint32_t tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), total = p.pairs * (uint32_t)p.R;
+    if ((rc = set_tiles(ctx, p, tiles, choose_splits(ctx, tiles * p.pairs, (uint32_t)((p.Lk + kb - 1) / kb)))) != SG_OK) return rc;
+    sg_workspace space(ctx);
+    if (p.splits > 1) {
+        if ((rc = space.take((uint64_t)p.splits * total * (D + 2) * 4)) != SG_OK) return rc;
+        p.part_o = (float *)space.p;
+        p.part_ml = p.part_o + (uint64_t)p.splits * total * D;
+    }
+    const bool vec_o = vec_rows(p.o), vec = vec_rows(p.q) && vec_rows(p.k) && vec_rows(p.v) && vec_o;
+    const dim3 grid(p.tiles * p.pairs * p.splits);
+    SG_CROSS_ROWS(cross_forward_kernel, rw, vec, grid);
     SG_CHECK_LAUNCH(ctx, "cross_attention");
+    if (p.splits > 1) {
+        const dim3 rows((unsigned)((total + 1024 / D - 1) / (1024 / D)));
+        if (D == 64) hipLaunchKernelGGL((cross_join_kernel<64>), rows, dim3(256), 0, ctx->stream, p, (int)vec_o);
+        else hipLaunchKernelGGL((cross_join_kernel<32>), rows, dim3(256), 0, ctx->stream, p, (int)vec_o);
+        SG_CHECK_LAUNCH(ctx, "cross_attention join");
+    }
     return SG_OK;
 }
 
@@ -217,28 +728,54 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     if (rc != SG_OK) return rc;
     if (!lse) return sg_fail(ctx, SG_ERR_ARG, "sg_cross_attention_grad: lse of the forward call expected");
     const int64_t N = p.N, D = q->extents[3];
-    const float *ptr;
-    if ((rc = check_operand(ctx, gout, N, p.H, p.Lq, D, "sg_cross_attention_grad gout", &p.gout, &p.go_b, &p.go_h, &p.go_l)) != SG_OK) return rc;
-    if ((rc = check_operand(ctx, gq, N, p.H, p.Lq, D, "sg_cross_attention_grad gq", &ptr, &p.gq_b, &p.gq_h, &p.gq_l)) != SG_OK) return rc;
-    p.gq = const_cast<float *>(ptr);
-    if ((rc = check_operand(ctx, gk, N, p.G, p.Lk, D, "sg_cross_attention_grad gk", &ptr, &p.gk_b, &p.gk_h, &p.gk_l)) != SG_OK) return rc;
-    p.gk = const_cast<float *>(ptr);
-    if ((rc = check_operand(ctx, gv, N, p.G, p.Lk, D, "sg_cross_attention_grad gv", &ptr, &p.gv_b, &p.gv_h, &p.gv_l)) != SG_OK) return rc;
-    p.gv = const_cast<float *>(ptr);
+    if ((rc = check_operand(ctx, gout, N, p.H, p.Lq, D, "sg_cross_attention_grad gout", &p.go)) != SG_OK) return rc;
+    if ((rc = check_operand(ctx, gq, N, p.H, p.Lq, D, "sg_cross_attention_grad gq", &p.gq)) != SG_OK) return rc;
+    if ((rc = check_operand(ctx, gk, N, p.G, p.Lk, D, "sg_cross_attention_grad gk", &p.gk)) != SG_OK) return rc;
+    if ((rc = check_operand(ctx, gv, N, p.G, p.Lk, D, "sg_cross_attention_grad gv", &p.gv)) != SG_OK) return rc;
     if ((rc = check_apart(ctx, gq, "sg_cross_attention_grad gq")) != SG_OK) return rc;
     if ((rc = check_apart(ctx, gk, "sg_cross_attention_grad gk")) != SG_OK) return rc;
     if ((rc = check_apart(ctx, gv, "sg_cross_attention_grad gv")) != SG_OK) return rc;
     if (!ctx) return SG_ERR_ARG;
     p.scale = scale;
     sg_device_guard guard(ctx);
-    const dim3 rows((unsigned)(p.N * p.H * p.Lq)), keys((unsigned)(p.N * p.G * p.Lk));
-    if (D == 64) {
-        hipLaunchKernelGGL((cross_gq_kernel<64>), rows, dim3(64), 0, ctx->stream, p);
-        hipLaunchKernelGGL((cross_gkv_kernel<64>), keys, dim3(64), 0, ctx->stream, p);
-    } else {
-        hipLaunchKernelGGL((cross_gq_kernel<32>), rows, dim3(64), 0, ctx->stream, p);
-        hipLaunchKernelGGL((cross_gkv_kernel<32>), keys, dim3(64), 0, ctx->stream, p);
+    const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
+    const int rw = row_waves(p.R), kb = rw == 1 ? 128 : 64;
+    const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 127) / 128);
+    const uint32_t row_splits = choose_splits(ctx, row_tiles * p.pairs, (uint32_t)((p.Lk + kb - 1) / kb));
+    const uint32_t key_splits = choose_splits(ctx, key_tiles * p.pairs, (uint32_t)((p.R + 63) / 64));
+    // delta, and the larger of the two kernels' split sums: they run one after the other
+    const uint64_t rows_part = row_splits > 1 ? row_splits * total * D : 0, keys_part = key_splits > 1 ? 2 * key_splits * keys * D : 0;
+    const uint64_t delta_floats = (total + 3) / 4 * 4;
+    sg_workspace space(ctx);
+    if ((rc = space.take((delta_floats + (rows_part > keys_part ? rows_part : keys_part)) * 4)) != SG_OK) return rc;
+    p.delta = (float *)space.p;
+    p.part_o = p.part_k = p.delta + delta_floats;
+    p.part_v = p.part_k + key_splits * keys * D;
+    const bool vec_gq = vec_rows(p.gq), vec_gk = vec_rows(p.gk), vec_gv = vec_rows(p.gv);
+    const bool vec = vec_rows(p.q) && vec_rows(p.k) && vec_rows(p.v) && vec_rows(p.o) && vec_rows(p.go) && vec_gq && vec_gk && vec_gv;
+    auto sum = [&](const float *part, const Rows &to, uint64_t n, uint32_t splits, int heads, int length, bool v4) {
+        const dim3 grid((unsigned)((n + 1024 / D - 1) / (1024 / D)));
+        if (D == 64) hipLaunchKernelGGL((cross_sum_kernel<64>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length, (int)v4);
+        else hipLaunchKernelGGL((cross_sum_kernel<32>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length, (int)v4);
+    };
+    if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
+    SG_CROSS_ROWS(cross_gq_kernel, rw, vec, dim3(p.tiles * p.pairs * p.splits));
+    SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
+    if (row_splits > 1) {
+        sum(p.part_o, p.gq, total, row_splits, p.H, p.Lq, vec_gq);
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries' sums");
     }
-    SG_CHECK_LAUNCH(ctx, "cross_attention_grad");
+    if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
+    const dim3 grid(p.tiles * p.pairs * p.splits);
+    if (D == 64 && vec) hipLaunchKernelGGL((cross_gkv_kernel<64, true>), grid, dim3(256), 0, ctx->stream, p);
+    else if (D == 64) hipLaunchKernelGGL((cross_gkv_kernel<64, false>), grid, dim3(256), 0, ctx->stream, p);
+    else if (vec) hipLaunchKernelGGL((cross_gkv_kernel<32, true>), grid, dim3(256), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((cross_gkv_kernel<32, false>), grid, dim3(256), 0, ctx->stream, p);
+    SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys and values");
+    if (key_splits > 1) {
+        sum(p.part_k, p.gk, keys, key_splits, p.G, p.Lk, vec_gk);
+        sum(p.part_v, p.gv, keys, key_splits, p.G, p.Lk, vec_gv);
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys' sums");
+    }
     return SG_OK;
 }
