@@ -43,37 +43,327 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbP p) {
     }
 }
 
-struct EmbGradP {
+// ---- gradient.  The tokens are sorted by id (stable, so a row's tokens stay in order), unknown ones behind the last row;
+// the sorted list is cut into chunks, each summed by wavefronts of its own; runs of one id that cross chunks leave partial
+// sums, which a last launch joins.  The order of every sum follows from the ids alone.
+//
+// Bound by memory: the gradient table is written once (rows without tokens are most of it) and gout read once.  The table
+// is cleared by the workgroups that ride in the sorting launches, which are otherwise a few workgroups on an idle chip;
+// rows with tokens are written a second time by the sums.
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+constexpr uint32_t MAX_DIGITS = 512;       // 9 bits a pass: two passes up to 262143 rows
+constexpr uint32_t TILE_ITEMS = 4;         // per thread, where tiles of 4096 tokens are sorted over several launches
+constexpr uint32_t TILE = SORT_THREADS * TILE_ITEMS;
+constexpr uint32_t SINGLE_ITEMS = 8;       // per thread, where one workgroup sorts everything in LDS in one launch:
+constexpr uint32_t SINGLE = SORT_THREADS * SINGLE_ITEMS;  // up to 8192 tokens
+constexpr uint32_t FILL = 8;               // 16-byte pieces a thread of a clearing workgroup writes
+
+struct SortP {
+    const uint32_t *ids;       // first pass: the ids themselves
+    const uint32_t *key_in, *pos_in;
+    uint32_t *key_out, *pos_out;
+    uint32_t *hist;            // [tile][digit]
+    sg_rows id_rows;
+    uint32_t n, V, tiles, shift, digits, from_ids;
+    uint32_t bits, passes;     // of the single-workgroup form
+    float *fill;               // what this launch clears
+    uint64_t fill_floats;
+    uint32_t fill_vec;
+};
+
+__device__ __forceinline__ void clear_part(const SortP &p, uint32_t block) {
+    const uint64_t base = (uint64_t)block * (SORT_THREADS * FILL * 4);
+#pragma unroll
+    for (uint32_t k = 0; k < FILL; ++k) {
+        const uint64_t i = base + ((uint64_t)k * SORT_THREADS + threadIdx.x) * 4;
+        if (i >= p.fill_floats) return;
+        if (p.fill_vec && i + 4 <= p.fill_floats) __builtin_nontemporal_store(f32x4{0.0f, 0.0f, 0.0f, 0.0f}, reinterpret_cast<f32x4 *>(p.fill + i));
+        else for (uint64_t j = i; j < i + 4 && j < p.fill_floats; ++j) p.fill[j] = 0.0f;
+    }
+}
+
+// Item k of a thread is token first + (wave * ITEMS + k) * 64 + lane: a wavefront's tokens are consecutive.
+__device__ __forceinline__ uint32_t item_index(uint32_t items, uint32_t k) { return ((threadIdx.x >> 6) * items + k) * 64 + (threadIdx.x & 63); }
+
+__device__ __forceinline__ uint32_t key_of(const SortP &p, uint32_t i) {
+    const uint32_t id = p.ids[sg_row_offset(p.id_rows, i)];
+    return id < p.V ? id : p.V;
+}
+
+// rank[k]: tokens of the same digit in front of item k in this tile.  counts: [wave][digit], zeroed, in LDS; left as the
+// exclusive sums over the wavefronts.  Items that are not there have digit `digits`, which nothing counts.
+template <uint32_t ITEMS>
+__device__ __forceinline__ void rank_items(const uint32_t *digit, uint32_t *rank, volatile uint32_t *counts, uint32_t digits) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (uint32_t k = 0; k < ITEMS; ++k) {
+        uint64_t same = __builtin_amdgcn_ballot_w64(digit[k] < digits);
+        for (uint32_t bit = 1; bit < digits; bit <<= 1) {
+            const uint64_t set = __builtin_amdgcn_ballot_w64((digit[k] & bit) != 0);
+            same &= digit[k] & bit ? set : ~set;
+        }
+        rank[k] = 0;
+        if (digit[k] < digits) {
+            volatile uint32_t *c = &counts[wave * digits + digit[k]];
+            const uint32_t before = *c;
+            __builtin_amdgcn_wave_barrier();  // every lane has read before the first of its digit writes
+            rank[k] = before + (uint32_t)__popcll(same & below);
+            if ((same & below) == 0) *c = before + (uint32_t)__popcll(same);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    if (threadIdx.x < digits) {
+        uint32_t sum = 0;
+        for (int w = 0; w < SORT_WAVES; ++w) {
+            const uint32_t x = counts[w * digits + threadIdx.x];
+            counts[w * digits + threadIdx.x] = sum;
+            sum += x;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < ITEMS; ++k)
+        if (digit[k] < digits) rank[k] += counts[wave * digits + digit[k]];
+}
+
+// Exclusive prefix sums of totals[0..digits) in LDS, in place.  scratch: one word per wavefront.
+__device__ __forceinline__ void prefix_digits(uint32_t *totals, uint32_t *scratch, uint32_t digits) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t x = threadIdx.x < digits ? totals[threadIdx.x] : 0;
+    uint32_t sum = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = (uint32_t)__shfl_up((int)sum, o, 64);
+        if ((int)lane >= o) sum += y;
+    }
+    if (lane == 63) scratch[wave] = sum;
+    __syncthreads();
+    for (uint32_t w = 0; w < wave; ++w) sum += scratch[w];
+    if (threadIdx.x < digits) totals[threadIdx.x] = sum - x;
+    __syncthreads();
+}
+
+// Up to 8192 tokens: workgroup 0 sorts them, all passes in LDS; the others clear the table.
+__global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const SortP p) {
+    __shared__ uint32_t keys[SINGLE], counts[SORT_WAVES * MAX_DIGITS], totals[MAX_DIGITS], scratch[SORT_WAVES];
+    __shared__ uint16_t places[SINGLE];
+    if (blockIdx.x > 0) {
+        clear_part(p, blockIdx.x - 1);
+        return;
+    }
+    uint32_t key[SINGLE_ITEMS], pos[SINGLE_ITEMS], digit[SINGLE_ITEMS], rank[SINGLE_ITEMS];
+    const uint32_t items = (p.n + SORT_THREADS - 1) / SORT_THREADS;  // per thread; the rest of the registers stay empty
+#pragma unroll
+    for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+        const uint32_t i = item_index(items, k);
+        pos[k] = i;
+        key[k] = k < items && i < p.n ? key_of(p, i) : 0;
+    }
+    for (uint32_t pass = 0; pass < p.passes; ++pass) {
+        const uint32_t shift = pass * p.bits, digits = 1u << p.bits;
+        for (uint32_t i = threadIdx.x; i < SORT_WAVES * digits; i += SORT_THREADS) counts[i] = 0;
+        if (threadIdx.x < digits) totals[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+            const bool there = k < items && item_index(items, k) < p.n;
+            digit[k] = there ? (key[k] >> shift) & (digits - 1) : digits;
+            if (there) atomicAdd(&totals[digit[k]], 1u);
+        }
+        rank_items<SINGLE_ITEMS>(digit, rank, counts, digits);
+        prefix_digits(totals, scratch, digits);
+#pragma unroll
+        for (uint32_t k = 0; k < SINGLE_ITEMS; ++k)
+            if (digit[k] < digits) {
+                const uint32_t to = totals[digit[k]] + rank[k];
+                keys[to] = key[k];
+                places[to] = (uint16_t)pos[k];
+            }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+            const uint32_t i = item_index(items, k);
+            if (k < items && i < p.n) { key[k] = keys[i]; pos[k] = places[i]; }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+        const uint32_t i = item_index(items, k);
+        if (k < items && i < p.n) { p.key_out[i] = key[k]; p.pos_out[i] = pos[k]; }
+    }
+}
+
+// More tokens: a launch counts every tile's digits, the next moves every token to its place of this pass.
+__global__ void __launch_bounds__(SORT_THREADS) embedding_count_kernel(const SortP p) {
+    __shared__ uint32_t count[MAX_DIGITS];
+    if (blockIdx.x >= p.tiles) {
+        clear_part(p, blockIdx.x - p.tiles);
+        return;
+    }
+    if (threadIdx.x < p.digits) count[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < TILE_ITEMS; ++k) {
+        const uint32_t i = blockIdx.x * TILE + k * SORT_THREADS + threadIdx.x;
+        if (i < p.n) atomicAdd(&count[((p.from_ids ? key_of(p, i) : p.key_in[i]) >> p.shift) & (p.digits - 1)], 1u);
+    }
+    __syncthreads();
+    if (threadIdx.x < p.digits) p.hist[blockIdx.x * p.digits + threadIdx.x] = count[threadIdx.x];
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) embedding_move_kernel(const SortP p) {
+    __shared__ uint32_t counts[SORT_WAVES * MAX_DIGITS], totals[MAX_DIGITS], before[MAX_DIGITS], scratch[SORT_WAVES];
+    if (blockIdx.x >= p.tiles) {
+        clear_part(p, blockIdx.x - p.tiles);
+        return;
+    }
+    const uint32_t tile = blockIdx.x;
+    uint32_t key[TILE_ITEMS], pos[TILE_ITEMS], digit[TILE_ITEMS], rank[TILE_ITEMS];
+#pragma unroll
+    for (uint32_t k = 0; k < TILE_ITEMS; ++k) {
+        const uint32_t i = tile * TILE + item_index(TILE_ITEMS, k);
+        key[k] = i < p.n ? (p.from_ids ? key_of(p, i) : p.key_in[i]) : 0;
+        pos[k] = i < p.n ? (p.from_ids ? i : p.pos_in[i]) : 0;
+        digit[k] = i < p.n ? (key[k] >> p.shift) & (p.digits - 1) : p.digits;
+    }
+    for (uint32_t i = threadIdx.x; i < SORT_WAVES * p.digits; i += SORT_THREADS) counts[i] = 0;
+    if (threadIdx.x < p.digits) totals[threadIdx.x] = before[threadIdx.x] = 0;
+    __syncthreads();
+    // the tiles' counts of one digit are shared out over 1024 / digits threads
+    {
+        const uint32_t d = threadIdx.x & (p.digits - 1), part = threadIdx.x / p.digits, parts = SORT_THREADS / p.digits;
+        uint32_t all = 0, front = 0;
+        for (uint32_t t = part; t < p.tiles; t += parts) {
+            const uint32_t x = p.hist[t * p.digits + d];
+            all += x;
+            if (t < tile) front += x;
+        }
+        atomicAdd(&totals[d], all);
+        atomicAdd(&before[d], front);
+    }
+    rank_items<TILE_ITEMS>(digit, rank, counts, p.digits);
+    prefix_digits(totals, scratch, p.digits);
+#pragma unroll
+    for (uint32_t k = 0; k < TILE_ITEMS; ++k)
+        if (digit[k] < p.digits) {
+            const uint32_t to = totals[digit[k]] + before[digit[k]] + rank[k];
+            p.key_out[to] = key[k];
+            p.pos_out[to] = pos[k];
+        }
+}
+
+struct SumP {
     const float *gout;
-    const uint32_t *ids;
-    float *gtable;
-    sg_rows id_rows, g_rows;
-    uint32_t n, E, V;
+    float *gtable, *part;  // part: [chunk][head, tail][E]
+    const uint32_t *key, *pos;
+    sg_rows g_rows;
+    uint32_t n, E, V, chunk, chunks, pieces;
     float scale;
 };
 
-// One workgroup per table row: it looks through the ids in order and adds the rows of its tokens.
-__global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbGradP p) {
-    __shared__ uint32_t found[256];
-    __shared__ uint32_t count;
-    const uint32_t v = blockIdx.x;
-    for (uint32_t c0 = 0; c0 < p.E; c0 += 256) {
-        const uint32_t c = c0 + threadIdx.x;
-        float acc = 0.0f;
-        for (uint32_t i0 = 0; i0 < p.n; i0 += 256) {
-            __syncthreads();
-            const uint32_t i = i0 + threadIdx.x;
-            found[threadIdx.x] = i < p.n && p.ids[sg_row_offset(p.id_rows, i)] == v;
-            if (threadIdx.x == 0) count = 0;
-            __syncthreads();
-            if (found[threadIdx.x]) count = 1;
-            __syncthreads();
-            if (count == 0) continue;
-            for (uint32_t j = 0; j < 256; ++j)
-                if (found[j] && c < p.E) acc += p.gout[sg_row_offset(p.g_rows, i0 + j) + c];
-        }
-        if (c < p.E) p.gtable[(int64_t)v * p.E + c] = acc * p.scale;
+// 4 columns of a lane: consecutive (VEC) or 64 apart.
+template <bool VEC>
+__device__ __forceinline__ f32x4 load_cols(const float *row, uint32_t c, uint32_t E) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (VEC) {
+        if (c < E) v = *reinterpret_cast<const f32x4 *>(row + c);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + 64 * j < E) v[j] = row[c + 64 * j];
     }
+    return v;
+}
+template <bool VEC>
+__device__ __forceinline__ void store_cols(float *row, uint32_t c, uint32_t E, f32x4 v) {
+    if (VEC) {
+        if (c < E) *reinterpret_cast<f32x4 *>(row + c) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + 64 * j < E) row[c + 64 * j] = v[j];
+    }
+}
+
+// A wavefront sums 256 columns of one chunk of sorted tokens; 8 rows are in flight at a time.
+template <bool VEC>
+__global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
+    const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (unit >= p.chunks * p.pieces) return;
+    const uint32_t chunk = unit / p.pieces, piece = unit - chunk * p.pieces;
+    const uint32_t c = piece * 256 + (VEC ? lane * 4 : lane);
+    const uint32_t first = chunk * p.chunk, last = min(first + p.chunk, p.n);
+    const uint32_t own = min(first + lane, p.n - 1);
+    const uint32_t key = p.key[own], pos = p.pos[own];
+    const uint32_t prev = first > 0 ? p.key[first - 1] : ~0u, next = last < p.n ? p.key[last] : ~0u;  // no key is ~0
+    bool from_before = prev == (uint32_t)__builtin_amdgcn_readfirstlane(key);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t b = first; b < last; b += 8) {
+        f32x4 x[8];
+        uint32_t id[9];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            const uint32_t at = min(b + k, last - 1) - first;
+            id[k] = (uint32_t)__builtin_amdgcn_readlane((int)key, (int)at);
+            if (b + k < last && id[k] < p.V)
+                x[k] = load_cols<VEC>(p.gout + sg_row_offset(p.g_rows, (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)at)), c, p.E);
+        }
+        id[8] = b + 8 < last ? (uint32_t)__builtin_amdgcn_readlane((int)key, (int)(b + 8 - first)) : next;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            if (b + k >= last || id[k] >= p.V) return;  // unknown tokens are the list's end
+            acc += x[k];
+            const bool end = b + k + 1 == last;
+            const uint32_t follow = end ? next : id[k + 1];
+            if (follow == id[k] && !end) continue;
+            if (from_before) store_cols<VEC>(p.part + (uint64_t)chunk * 2 * p.E, c, p.E, acc);
+            else if (follow == id[k]) store_cols<VEC>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E, acc);
+            else store_cols<VEC>(p.gtable + (uint64_t)id[k] * p.E, c, p.E, acc * p.scale);
+            acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            from_before = false;
+        }
+    }
+}
+
+// A workgroup for 256 columns of the run that begins in a chunk and goes on behind it: the partial sums of the chunks it
+// covers, shared out over the wavefronts in order and joined in order.
+template <bool VEC>
+__global__ void __launch_bounds__(256) embedding_join_kernel(const SumP p) {
+    __shared__ f32x4 sums[4][64];
+    const uint32_t chunk = blockIdx.x / p.pieces, piece = blockIdx.x - chunk * p.pieces;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t c = piece * 256 + (VEC ? lane * 4 : lane);
+    const uint32_t behind = (chunk + 1) * p.chunk;  // this kernel has a workgroup for every chunk but the last
+    const uint32_t id = p.key[behind];
+    if (id >= p.V || p.key[behind - 1] != id) return;                            // nothing goes on
+    if (chunk > 0 && p.key[chunk * p.chunk - 1] == id) return;                   // it began further in front
+    uint32_t lo = chunk + 1, hi = p.chunks - 1;  // the last chunk whose first token is of the run
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if (p.key[mid * p.chunk] == id) lo = mid;
+        else hi = mid - 1;
+    }
+    const uint32_t count = lo - chunk, from = chunk + 1 + count * wave / 4, to = chunk + 1 + count * (wave + 1) / 4;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (wave == 0) acc = load_cols<VEC>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E);
+    uint32_t i = from;
+    for (; i + 8 <= to; i += 8) {
+        f32x4 x[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) x[k] = load_cols<VEC>(p.part + (uint64_t)(i + k) * 2 * p.E, c, p.E);
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) acc += x[k];
+    }
+    for (; i < to; ++i) acc += load_cols<VEC>(p.part + (uint64_t)i * 2 * p.E, c, p.E);
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) acc += sums[w][lane];
+    store_cols<VEC>(p.gtable + (uint64_t)id * p.E, c, p.E, acc * p.scale);
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p) % 16 == 0; }
@@ -135,17 +425,100 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
     if (E > 1 && gout->strides[ids->rank] != 1) return sg_fail(ctx, SG_ERR_SHAPE, "sg_embedding_grad: gout must have unit stride on its last axis");
     if (!sg_is_dense(gtable)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_embedding_grad: gtable must be dense row-major");
     if (!ctx) return SG_ERR_ARG;
-    EmbGradP p{};
-    p.gout = (const float *)gout->base + gout->offset;
-    p.ids = (const uint32_t *)ids->base + ids->offset;
-    p.gtable = (float *)gtable->base + gtable->offset;
-    p.n = (uint32_t)sg_make_rows(ids, ids->rank, &p.id_rows);
-    (void)sg_make_rows(gout, ids->rank, &p.g_rows);
-    p.E = (uint32_t)E;
-    p.V = (uint32_t)gtable->extents[0];
-    p.scale = scale;
+    SortP s{};
+    s.ids = (const uint32_t *)ids->base + ids->offset;
+    s.n = (uint32_t)sg_make_rows(ids, ids->rank, &s.id_rows);
+    s.V = (uint32_t)gtable->extents[0];
+    float *table = (float *)gtable->base + gtable->offset;
+    const uint64_t table_floats = (uint64_t)s.V * E;
+    SumP m{};
+    m.gout = (const float *)gout->base + gout->offset;
+    (void)sg_make_rows(gout, ids->rank, &m.g_rows);
+    m.gtable = table;
+    m.n = s.n;
+    m.E = (uint32_t)E;
+    m.V = s.V;
+    m.scale = scale;
+    m.pieces = (m.E + 255) / 256;
+    // Chunks short enough that their wavefronts fill the chip (4096 tokens of 768: 768 wavefronts of 16 tokens), long enough
+    // that a run over all tokens leaves few partial sums.
+    m.chunk = s.n <= 16384 ? 16 : s.n <= 65536 ? 32 : 64;
+    m.chunks = (s.n + m.chunk - 1) / m.chunk;
+    if ((uint64_t)m.chunks * m.pieces >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_embedding_grad: too many elements for one launch");
+
+    uint32_t bits = 1;
+    while ((s.V >> bits) != 0) ++bits;  // keys are 0..V
+    s.passes = (bits + 8) / 9;
+    s.bits = (bits + s.passes - 1) / s.passes;
+    s.digits = 1u << s.bits;
+    const bool single = s.n <= SINGLE;
+    s.tiles = single ? 1 : (s.n + TILE - 1) / TILE;
+    // the sorted list, a second one to move between where there are several launches, the tiles' counts, the partial sums
+    const uint64_t list = (uint64_t)(s.n + 3) / 4 * 4, counts = single ? 0 : (uint64_t)s.tiles * s.digits;
+    const uint64_t words = list * (single ? 2 : 4) + (counts + 3) / 4 * 4 + (uint64_t)m.chunks * 2 * E;
     sg_device_guard guard(ctx);
-    hipLaunchKernelGGL(embedding_grad_kernel, dim3(p.V), dim3(256), 0, ctx->stream, p);
-    SG_CHECK_LAUNCH(ctx, "embedding_grad");
+    sg_workspace space(ctx);
+    if ((rc = space.take(words * 4)) != SG_OK) return rc;
+    uint32_t *key[2], *pos[2], *w = (uint32_t *)space.p;
+    key[0] = w;
+    pos[0] = w + list;
+    key[1] = single ? nullptr : w + 2 * list;
+    pos[1] = single ? nullptr : w + 3 * list;
+    w += list * (single ? 2 : 4);
+    s.hist = w;
+    m.part = (float *)(w + (counts + 3) / 4 * 4);
+
+    const uint64_t per_block = (uint64_t)SORT_THREADS * FILL * 4, fill_blocks = (table_floats + per_block - 1) / per_block;
+    s.fill_vec = aligned16(table);
+    if (single) {
+        s.key_out = key[0];
+        s.pos_out = pos[0];
+        s.fill = table;
+        s.fill_floats = table_floats;
+        hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)(1 + fill_blocks)), dim3(SORT_THREADS), 0, ctx->stream, s);
+        SG_CHECK_LAUNCH(ctx, "embedding_grad sort");
+        m.key = key[0];
+        m.pos = pos[0];
+    } else {
+        // every launch clears its share of the table
+        const uint32_t launches = 2 * s.passes;
+        const uint64_t share = (fill_blocks + launches - 1) / launches;
+        uint64_t cleared = 0;
+        auto take_share = [&]() {
+            const uint64_t at = cleared * per_block;
+            const uint64_t blocks = cleared + share <= fill_blocks ? share : fill_blocks - cleared;
+            s.fill = table + at;
+            s.fill_floats = blocks * per_block <= table_floats - at ? blocks * per_block : table_floats - at;
+            cleared += blocks;
+            return dim3((unsigned)(s.tiles + blocks));
+        };
+        for (uint32_t pass = 0; pass < s.passes; ++pass) {
+            s.from_ids = pass == 0;
+            s.shift = pass * s.bits;
+            s.key_in = key[(pass + 1) & 1];
+            s.pos_in = pos[(pass + 1) & 1];
+            s.key_out = key[pass & 1];
+            s.pos_out = pos[pass & 1];
+            const dim3 count_grid = take_share();
+            hipLaunchKernelGGL(embedding_count_kernel, count_grid, dim3(SORT_THREADS), 0, ctx->stream, s);
+            SG_CHECK_LAUNCH(ctx, "embedding_grad count");
+            const dim3 move_grid = take_share();
+            hipLaunchKernelGGL(embedding_move_kernel, move_grid, dim3(SORT_THREADS), 0, ctx->stream, s);
+            SG_CHECK_LAUNCH(ctx, "embedding_grad move");
+        }
+        m.key = s.key_out;
+        m.pos = s.pos_out;
+    }
+    bool vec = E % 4 == 0 && aligned16(m.gout) && aligned16(table);
+    for (int i = 0; i < m.g_rows.rank; ++i) vec = vec && m.g_rows.st[i] % 4 == 0;
+    const dim3 sum_grid((m.chunks * m.pieces + 3) / 4), join_grid((m.chunks - 1) * m.pieces);
+    if (vec) hipLaunchKernelGGL((embedding_sum_kernel<true>), sum_grid, dim3(256), 0, ctx->stream, m);
+    else hipLaunchKernelGGL((embedding_sum_kernel<false>), sum_grid, dim3(256), 0, ctx->stream, m);
+    SG_CHECK_LAUNCH(ctx, "embedding_grad sums");
+    if (m.chunks > 1) {
+        if (vec) hipLaunchKernelGGL((embedding_join_kernel<true>), join_grid, dim3(256), 0, ctx->stream, m);
+        else hipLaunchKernelGGL((embedding_join_kernel<false>), join_grid, dim3(256), 0, ctx->stream, m);
+        SG_CHECK_LAUNCH(ctx, "embedding_grad join");
+    }
     return SG_OK;
 }

@@ -679,3 +679,17 @@ def test_serving_steps_reuse_the_states_keys(ctx):
         one = layer.attend(Var.new(dev(ctx, x[:, i:i + 1])), k, v, m).eval(ctx).numpy()
         # two different splits of the same sums behind products of length 128: 1e-4 of the layer's unit variance
         near(one[:, 0], whole[:, i], 1e-4, "token")
+
+def test_out_of_memory_is_reported_and_harmless(ctx):
+    c = S.Context(capacity=1 << 20)
+    rng = np.random.default_rng(12)
+    ids, g, out = dev(c, rng.integers(0, 50, 3000).astype(np.uint32)), dev(c, R.f32(rng.standard_normal((3000, 64)))), dev(c, np.zeros((50, 64), np.float32))
+    hold = Tensor.uninit(c, [(c.mem_stats()["capacity"] - c.mem_stats()["used"]) // 4 - 16])
+    with pytest.raises(abi.OutOfMemory):
+        c.check(c._lib.sg_embedding_grad(c.handle, ref(g), ref(ids), C.c_float(1.0), ref(out)))
+    del hold
+    c.check(c._lib.sg_embedding_grad(c.handle, ref(g), ref(ids), C.c_float(1.0), ref(out)))
+    want, tol = R.embedding_grad(g.numpy(), ids.numpy(), 50, 1.0)
+    near(out.numpy(), want, tol, "gtable")
+    del ids, g, out
+    c.close()
