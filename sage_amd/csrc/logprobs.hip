@@ -1,20 +1,37 @@
 // Log probabilities of given tokens, entropy and top alternatives, and their gradient, for gfx950.
-// With z = scale * logits, m = max z, s = sum e^(z - m), t = sum e^(z - m) (z - m):
-//   lse = m + log s;  logprob = z_token - lse;  entropy = log s - t / s;  log p_j = (z_j - m) - log s.
-// Bound by memory: the logits are what is read.
+// With c = scale log2(e), m = max x, y_j = (x_j - m) c, s = sum 2^y_j, t = sum 2^y_j y_j over a row's logits x:
+//   lse = scale m + ln 2 log2 s;  log p_j = ln 2 (y_j - log2 s);  entropy = ln 2 (log2 s - t / s).
+// Bound by memory: the logits are read once (forward), read once and written once (gradient).
+//
+// Forward: a workgroup a row, or a row over several workgroups where rows are few, whose parts a second launch joins.  A
+// thread takes 16 logits a round and keeps (m, s, t) of its own; (m1, s1, t1) moved to a maximum m is
+// (m, f s1, f (t1 + s1 d)) with d = (m1 - m) c, f = 2^d.  The k largest come out of the same pass: k threads' maxima
+// are a bound that k logits reach, so after a round only logits above the k-th largest of the 256 threads' maxima are
+// collected (a later one equal to the bound has a higher index than k that reach it), a few hundred of a row.
 #include "rows.h"
+
+#include <type_traits>
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes at any element
+
 constexpr int TOP_MAX = 64;
+constexpr int THREADS = 256, VECS = 4, ROUND = THREADS * VECS * 4;  // logits a workgroup takes in a round
+constexpr int KEEP = 1024;                                          // candidates kept from round to round
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+typedef unsigned long long u64;
 
 struct LogpP {
     const float *logits;
     const uint32_t *tokens;
     float *logprob, *entropy, *lse, *top_logprobs;
     uint32_t *top_ids;
+    float *part_stats;    // of split rows: [row][split][3]
+    uint32_t *part_ids;   // [row][split][k], ~0 where a part has no k logits
     sg_rows rows, token_rows;
-    uint32_t R, C, k;
+    uint32_t R, C, k, splits;
     float scale;
 };
 
@@ -24,77 +41,314 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+__device__ __forceinline__ float number_of(uint32_t order) { return __uint_as_float((order & 0x80000000u) ? (order & 0x7FFFFFFFu) : ~order); }
+__device__ __forceinline__ u64 top_key(float x, uint32_t j) { return ((u64)order_bits(x) << 32) | (uint32_t)~j; }
+__device__ __forceinline__ uint32_t index_of(u64 key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ unsigned long long top_key(float x, uint32_t j) { return ((unsigned long long)order_bits(x) << 32) | (uint32_t)~j; }
+// 0 * -inf is NaN: a distance whose exponential is 0 anyway becomes a finite one; NaN stays
+__device__ __forceinline__ float finite(float y) { return y < -1e4f ? -1e4f : y; }
 
-__global__ void __launch_bounds__(256) logprobs_kernel(const LogpP p) {
-    __shared__ float red[256];
-    __shared__ unsigned long long best[256];
+struct Stats {
+    float m, s, t;  // m: NaN while no number has been seen
+    __device__ float shift() const { return m > -__builtin_inff() ? m : 0.0f; }
+    // to the larger maximum m_new (a number, or NaN if there is none still)
+    __device__ void move(float m_new, float c) {
+        const float to = m_new > -__builtin_inff() ? m_new : 0.0f;
+        const float d = s != 0.0f ? finite((m - to) * c) : 0.0f;  // nothing to move yet, whatever m is
+        const float f = __builtin_amdgcn_exp2f(d);
+        t = f * (t + s * d);
+        s = s * f;
+        m = m_new;
+    }
+    __device__ void join(float mo, float so, float to, float c) {
+        Stats o = {mo, so, to};
+        const float top = fmaxf(m, mo);
+        move(top, c);
+        o.move(top, c);
+        s += o.s;
+        t += o.t;
+    }
+};
+
+struct RowResult {
+    float shift, log2s, lse, entropy;
+    bool empty;  // nothing but -inf
+    __device__ RowResult(const Stats &a, float scale) {
+        const float inf = __builtin_inff();
+        shift = a.shift();
+        empty = a.m == -inf && a.s == 0.0f;
+        log2s = __builtin_amdgcn_logf(a.s);
+        lse = empty ? -inf : __builtin_fmaf(shift, scale, log2s * LN2);
+        entropy = empty ? 0.0f : (log2s - a.t / a.s) * LN2;
+    }
+    __device__ float logprob(float x, float c) const { return empty ? -__builtin_inff() : ((x - shift) * c - log2s) * LN2; }
+};
+
+// The row as 16-byte groups: group g holds logits 4g - lead .. 4g - lead + 3, those that exist.
+struct Groups {
+    const float *base;
+    uint32_t lead, C, count;
+    __device__ Groups(const float *x, uint32_t C_) : C(C_) {
+        lead = (uint32_t)(((uintptr_t)x & 15) / 4);
+        base = x - lead;
+        count = (lead + C + 3) / 4;
+    }
+    // NaN where there is no logit
+    __device__ f32x4 load(uint32_t g) const {
+        if (4 * g >= lead && 4 * g + 4 <= lead + C) return *reinterpret_cast<const f32x4 *>(base + 4 * g);
+        f32x4 v;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) v[j] = 4 * g + j >= lead && 4 * g + j < lead + C ? base[4 * g + j] : __builtin_nanf("");
+        return v;
+    }
+    __device__ bool whole(uint32_t g) const { return 4 * g >= lead && 4 * g + 4 <= lead + C; }
+    __device__ bool has(uint32_t g, uint32_t j) const { return 4 * g + j >= lead && 4 * g + j < lead + C; }
+    __device__ uint32_t index(uint32_t g, uint32_t j) const { return 4 * g + j - lead; }
+};
+
+__device__ __forceinline__ Stats block_join(Stats a, float c, float *lds) {  // lds: 12 floats
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) a.join(__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64), c);
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { lds[3 * wave] = a.m; lds[3 * wave + 1] = a.s; lds[3 * wave + 2] = a.t; }
+    __syncthreads();
+    a = {lds[0], lds[1], lds[2]};
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) a.join(lds[3 * w], lds[3 * w + 1], lds[3 * w + 2], c);
+    return a;
+}
+
+struct TopLds {
+    u64 keys[KEEP + ROUND];
+    u64 best[THREADS / 64];
+    __attribute__((aligned(16))) uint32_t maxima[THREADS];
+    uint32_t count, bound;
+};
+
+// The order of the k-th largest of the threads' maxima; 0 if fewer than k threads have seen a number.
+__device__ __forceinline__ uint32_t bound_of(TopLds &l, float thread_max, uint32_t k) {
+    const uint32_t mine = order_bits(thread_max);
+    __syncthreads();
+    l.maxima[threadIdx.x] = mine;
+    __syncthreads();
+    uint32_t rank = 0;
+    for (uint32_t i = 0; i < THREADS; i += 4) {
+        const uint4 o = *reinterpret_cast<const uint4 *>(&l.maxima[i]);
+        rank += (o.x > mine || (o.x == mine && i < threadIdx.x)) + (o.y > mine || (o.y == mine && i + 1 < threadIdx.x)) +
+                (o.z > mine || (o.z == mine && i + 2 < threadIdx.x)) + (o.w > mine || (o.w == mine && i + 3 < threadIdx.x));
+    }
+    if (rank == k - 1) l.bound = mine;
+    __syncthreads();
+    return l.bound;
+}
+
+__device__ __forceinline__ u64 block_max(u64 x, u64 *lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const u64 y = __shfl_xor(x, o, 64);
+        x = x > y ? x : y;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = lds[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) x = x > lds[w] ? x : lds[w];
+    return x;
+}
+
+// Leaves the candidates that reach `bound`, and if that leaves more than KEEP of them (long runs of equal logits, or large
+// ones all in one thread's places), exactly the k largest.
+__device__ __forceinline__ void tighten(TopLds &l, uint32_t bound, uint32_t k) {
+    __syncthreads();
+    const uint32_t n = l.count;
+    // a thread's share is read before any is written back
+    u64 mine[(KEEP + ROUND) / THREADS];
+#pragma unroll
+    for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i) {
+        const uint32_t at = i * THREADS + threadIdx.x;
+        mine[i] = at < n ? l.keys[at] : 0;
+        if ((uint32_t)(mine[i] >> 32) < bound) mine[i] = 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) l.count = 0;
+    __syncthreads();
+    uint32_t left = 0;
+#pragma unroll
+    for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i) left += mine[i] != 0;
+    const uint32_t at = left ? atomicAdd(&l.count, left) : 0;
+    __syncthreads();
+    if (l.count <= KEEP) {
+        uint32_t to = at;
+#pragma unroll
+        for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i)
+            if (mine[i]) l.keys[to++] = mine[i];
+        __syncthreads();
+        return;
+    }
+    u64 last = ~0ull;
+    for (uint32_t r = 0; r < k; ++r) {
+        u64 b = 0;
+#pragma unroll
+        for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i)
+            if (mine[i] < last && mine[i] > b) b = mine[i];
+        last = block_max(b, l.best);
+        if (threadIdx.x == 0) l.keys[r] = last;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) l.count = k;
+    __syncthreads();
+}
+
+// Place of a key among the n <= KEEP in LDS, largest first; keys are different.
+__device__ __forceinline__ uint32_t place_of(const u64 *keys, uint32_t n, u64 key) {
+    uint32_t r = 0;
+    for (uint32_t i = 0; i < n; ++i) r += keys[i] > key;
+    return r;
+}
+
+template <bool TOP>
+__global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
+    __shared__ typename std::conditional<TOP, TopLds, uint32_t>::type lds_top;
+    __shared__ float lds_stats[12];
+    const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, tid = threadIdx.x;
+    const float *x = p.logits + sg_row_offset(p.rows, row);
+    const Groups groups(x, p.C);
+    const uint32_t g0 = (uint32_t)((uint64_t)groups.count * split / p.splits), g1 = (uint32_t)((uint64_t)groups.count * (split + 1) / p.splits);
+    const float c = p.scale * LOG2E, nan = __builtin_nanf("");
+    Stats a = {nan, 0.0f, 0.0f};
+    f32x4 next[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) next[i] = g0 + i * THREADS + tid < g1 ? groups.load(g0 + i * THREADS + tid) : f32x4{nan, nan, nan, nan};
+    uint32_t bound = 0;
+    if constexpr (TOP) {
+        if (tid == 0) lds_top.count = 0;
+    }
+    for (uint32_t g = g0; g < g1; g += THREADS * VECS) {
+        f32x4 v[VECS];
+        float top = a.m;
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+            v[i] = next[i];
+            top = fmaxf(fmaxf(fmaxf(top, v[i].x), v[i].y), fmaxf(v[i].z, v[i].w));
+        }
+        // requested behind the wait for this round's logits, in flight during its arithmetic
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+            const uint32_t at = g + (VECS + i) * THREADS + tid;
+            if (at < g1) next[i] = groups.load(at);
+        }
+        if (top != a.m) a.move(top, c);
+        const float shift = a.shift();
+        const bool whole = groups.whole(g + tid) && g + (VECS - 1) * THREADS + tid < g1 && groups.whole(g + (VECS - 1) * THREADS + tid);
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < VECS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float y = finite((v[i][j] - shift) * c), e = __builtin_amdgcn_exp2f(y);
+                    a.s += e;
+                    a.t = __builtin_fmaf(e, y, a.t);
+                }
+        } else {
+            for (int i = 0; i < VECS; ++i)
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t at = g + i * THREADS + tid;
+                    if (at >= g1 || !groups.has(at, j)) continue;
+                    const float y = finite((v[i][j] - shift) * c), e = __builtin_amdgcn_exp2f(y);
+                    a.s += e;
+                    a.t = __builtin_fmaf(e, y, a.t);
+                }
+        }
+        if constexpr (TOP) {
+            const bool first = g == g0;
+            if (first) bound = bound_of(lds_top, a.m, p.k);
+            const float limit = number_of(bound);
+#pragma unroll
+            for (int i = 0; i < VECS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t at = g + i * THREADS + tid;
+                    // in the first round what equals the bound, later what is above it; NaN is sorted out below
+                    if (bound != 0 && (first ? v[i][j] < limit : v[i][j] <= limit)) continue;
+                    if (at < g1 && groups.has(at, j)) lds_top.keys[atomicAdd(&lds_top.count, 1u)] = top_key(v[i][j], groups.index(at, j));
+                }
+            __syncthreads();
+            if (lds_top.count > KEEP) {
+                bound = bound_of(lds_top, a.m, p.k);
+                tighten(lds_top, bound, p.k);
+            }
+            __syncthreads();
+        }
+    }
+    const Stats all = block_join(a, c, lds_stats);
+    const RowResult r(all, p.scale);
+    if (tid == 0) {
+        if (p.splits > 1) {
+            float *to = p.part_stats + (uint64_t)blockIdx.x * 3;
+            to[0] = all.m; to[1] = all.s; to[2] = all.t;
+        } else {
+            p.lse[row] = r.lse;
+            if (p.entropy) p.entropy[row] = r.entropy;
+            if (p.logprob) {
+                const uint32_t tok = p.tokens[sg_row_offset(p.token_rows, row)];
+                p.logprob[row] = tok < p.C ? r.logprob(x[tok], c) : 0.0f;
+            }
+        }
+    }
+    if constexpr (TOP) {
+        bound = bound_of(lds_top, a.m, p.k);
+        tighten(lds_top, bound, p.k);
+        const uint32_t n = lds_top.count;
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            const u64 key = lds_top.keys[i];
+            const uint32_t at = place_of(lds_top.keys, n, key);
+            if (at >= p.k) continue;
+            if (p.splits > 1) p.part_ids[(uint64_t)blockIdx.x * p.k + at] = index_of(key);
+            else {
+                p.top_ids[(uint64_t)row * p.k + at] = index_of(key);
+                p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(x[index_of(key)], c);
+            }
+        }
+        if (p.splits > 1)
+            for (uint32_t i = n + tid; i < p.k; i += THREADS) p.part_ids[(uint64_t)blockIdx.x * p.k + i] = ~0u;
+    }
+}
+
+// Joins the parts of a split row.
+__global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const LogpP p) {
+    __shared__ u64 keys[KEEP];
+    __shared__ float lds_stats[12];
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const float *x = p.logits + sg_row_offset(p.rows, row);
-    const float inf = __builtin_inff();
-    auto sum = [&](float v) {
-        __syncthreads();
-        red[tid] = v;
-        __syncthreads();
-        for (int o = 128; o > 0; o >>= 1) {
-            if ((int)tid < o) red[tid] += red[tid + o];
-            __syncthreads();
-        }
-        return red[0];
-    };
-    float m = -inf;
-    for (uint32_t j = tid; j < p.C; j += 256) m = fmaxf(m, x[j] * p.scale);
-    __syncthreads();
-    red[tid] = m;
-    __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-        if ((int)tid < o) red[tid] = fmaxf(red[tid], red[tid + o]);
-        __syncthreads();
+    const float c = p.scale * LOG2E;
+    Stats a = {__builtin_nanf(""), 0.0f, 0.0f};
+    if (tid < p.splits) {
+        const float *from = p.part_stats + ((uint64_t)row * p.splits + tid) * 3;
+        a = {from[0], from[1], from[2]};
     }
-    m = red[0];
-    const float shift = m == -inf ? 0.0f : m;
-    float s = 0.0f, t = 0.0f;
-    for (uint32_t j = tid; j < p.C; j += 256) {
-        const float d = x[j] * p.scale - shift;
-        const float e = expf(d);
-        s += e;
-        if (d != -inf) t += e * d;
-    }
-    s = sum(s);
-    t = sum(t);
-    const float logs = logf(s);
-    const bool empty = m == -inf && s == 0.0f;
+    const RowResult r(block_join(a, c, lds_stats), p.scale);
     if (tid == 0) {
-        p.lse[row] = empty ? -inf : shift + logs;
-        if (p.entropy) p.entropy[row] = empty ? 0.0f : logs - t / s;
+        p.lse[row] = r.lse;
+        if (p.entropy) p.entropy[row] = r.entropy;
         if (p.logprob) {
             const uint32_t tok = p.tokens[sg_row_offset(p.token_rows, row)];
-            float v = 0.0f;
-            if (tok < p.C) v = empty ? -inf : (x[tok] * p.scale - shift) - logs;
-            p.logprob[row] = v;
+            p.logprob[row] = tok < p.C ? r.logprob(x[tok], c) : 0.0f;
         }
     }
-    unsigned long long last = ~0ull;
-    for (uint32_t i = 0; i < p.k; ++i) {
-        unsigned long long b = 0;
-        for (uint32_t j = tid; j < p.C; j += 256) {
-            const unsigned long long key = top_key(x[j], j);
-            if (key < last && key > b) b = key;
-        }
-        __syncthreads();
-        best[tid] = b;
-        __syncthreads();
-        for (int o = 128; o > 0; o >>= 1) {
-            if ((int)tid < o && best[tid + o] > best[tid]) best[tid] = best[tid + o];
-            __syncthreads();
-        }
-        last = best[0];
-        if (tid == 0) {
-            const uint32_t j = ~(uint32_t)last;
-            p.top_ids[(uint64_t)row * p.k + i] = j;
-            p.top_logprobs[(uint64_t)row * p.k + i] = empty ? -inf : (x[j] * p.scale - shift) - logs;
-        }
+    const uint32_t n = p.splits * p.k;  // at most KEEP
+    for (uint32_t i = tid; i < n; i += THREADS) {
+        const uint32_t id = p.part_ids[(uint64_t)row * n + i];
+        keys[i] = id == ~0u ? 0 : top_key(x[id], id);
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += THREADS) {
+        if (!keys[i]) continue;
+        const uint32_t at = place_of(keys, n, keys[i]);
+        if (at >= p.k) continue;
+        p.top_ids[(uint64_t)row * p.k + at] = index_of(keys[i]);
+        p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(x[index_of(keys[i])], c);
     }
 }
 
@@ -104,29 +358,60 @@ struct LogpGradP {
     const float *lse, *entropy, *g_logprob, *g_entropy;
     float *glogits;
     sg_rows rows, token_rows, gl_rows, ge_rows;
-    uint32_t R, C;
+    uint32_t R, C, parts, part;  // workgroups of a row, 16-byte groups of each
     float scale;
 };
 
-__global__ void __launch_bounds__(256) logprobs_grad_kernel(const LogpGradP p) {
-    const uint32_t row = blockIdx.x;
+// lse carries half a step of its own size into every probability: beyond this it is not used (7.6e-6 there).
+constexpr float FAR = 128.0f;
+
+// glogits_j = scale (-p_j (gl + ge (log p_j + H)) + [j = token] gl)
+template <bool NT>
+__global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const LogpGradP p) {
+    __shared__ float lds_stats[12];
+    const uint32_t row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts, tid = threadIdx.x;
     const float *x = p.logits + sg_row_offset(p.rows, row);
     float *y = p.glogits + (uint64_t)row * p.C;
-    const float inf = __builtin_inff();
+    const float inf = __builtin_inff(), c = p.scale * LOG2E;
     const float lse = p.lse[row];
     const uint32_t tok = p.g_logprob ? p.tokens[sg_row_offset(p.token_rows, row)] : ~0u;
     const float gl = tok < p.C ? p.g_logprob[sg_row_offset(p.gl_rows, row)] : 0.0f;
     const float ge = p.g_entropy ? p.g_entropy[sg_row_offset(p.ge_rows, row)] : 0.0f;
     const float h = p.g_entropy ? p.entropy[row] : 0.0f;
-    for (uint32_t j = threadIdx.x; j < p.C; j += 256) {
-        const float z = x[j] * p.scale;
-        float g = 0.0f;
-        if (z != -inf) {
-            const float lp = z - lse, pr = expf(lp);
-            g = -pr * (gl + ge * (lp + h));
-            if (j == tok) g += gl;
+    // log2 p = (x - shift) c - log2s
+    float shift = 0.0f, log2s = lse * LOG2E;
+    if (fabsf(lse) > FAR) {  // the row's own maximum and sum again (each workgroup of the row does)
+        Stats a = {__builtin_nanf(""), 0.0f, 0.0f};
+        for (uint32_t j = tid; j < p.C; j += THREADS) {
+            const float v = x[j], top = fmaxf(a.m, v);
+            if (top != a.m) a.move(top, c);
+            a.s += __builtin_amdgcn_exp2f(finite((v - a.shift()) * c));
         }
-        y[j] = g * p.scale;
+        const RowResult r(block_join(a, c, lds_stats), p.scale);
+        shift = r.shift;
+        log2s = r.log2s;
+    }
+    auto grad = [&](float v, uint32_t j) {
+        const float lp2 = (v - shift) * c - log2s;
+        const float pr = __builtin_amdgcn_exp2f(lp2);
+        float g = -pr * (gl + ge * __builtin_fmaf(lp2, LN2, h));
+        if (j == tok) g += gl;
+        return v == -inf ? 0.0f : g * p.scale;
+    };
+    const Groups groups(y, p.C);  // whole groups of the output; the logits of one are at any element
+    const uint32_t last = min((part + 1) * p.part, groups.count);
+    for (uint32_t g = part * p.part + tid; g < last; g += THREADS) {
+        const uint32_t j = groups.index(g, 0);
+        if (groups.whole(g)) {
+            const f32x4 v = *reinterpret_cast<const f32x4_any *>(x + j);
+            const f32x4 o = {grad(v.x, j), grad(v.y, j + 1), grad(v.z, j + 2), grad(v.w, j + 3)};
+            if (NT) __builtin_nontemporal_store(o, reinterpret_cast<f32x4 *>(y + j));
+            else *reinterpret_cast<f32x4 *>(y + j) = o;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                if (groups.has(g, e)) y[j + e] = grad(x[j + e], j + e);
+        }
     }
 }
 
@@ -210,9 +495,29 @@ extern "C" int sg_token_logprobs(sg_ctx *ctx, const sg_tensor *logits, const sg_
     p.C = (uint32_t)C;
     p.k = (uint32_t)k;
     p.scale = scale;
+    // Few rows: a row over several workgroups, two for each compute unit in all, at least a round of logits each, and no
+    // more candidates than a workgroup joins.
+    const uint32_t want = 2u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+    p.splits = p.R >= want ? 1 : (want + p.R - 1) / p.R;
+    if (p.splits > p.C / ROUND) p.splits = p.C / ROUND;
+    if (p.splits > 64) p.splits = 64;
+    if (k && p.splits > KEEP / (uint32_t)k) p.splits = KEEP / (uint32_t)k;
+    if (p.splits < 1) p.splits = 1;
+    if ((uint64_t)p.R * p.splits >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs: too many rows for one launch");
     sg_device_guard guard(ctx);
-    hipLaunchKernelGGL(logprobs_kernel, dim3(p.R), dim3(256), 0, ctx->stream, p);
+    sg_workspace space(ctx);
+    if (p.splits > 1) {
+        if ((rc = space.take((uint64_t)p.R * p.splits * (3 + k) * 4)) != SG_OK) return rc;
+        p.part_stats = (float *)space.p;
+        p.part_ids = (uint32_t *)space.p + (uint64_t)p.R * p.splits * 3;
+    }
+    if (k) hipLaunchKernelGGL((logprobs_kernel<true>), dim3(p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((logprobs_kernel<false>), dim3(p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
     SG_CHECK_LAUNCH(ctx, "token_logprobs");
+    if (p.splits > 1) {
+        hipLaunchKernelGGL(logprobs_join_kernel, dim3(p.R), dim3(THREADS), 0, ctx->stream, p);
+        SG_CHECK_LAUNCH(ctx, "token_logprobs join");
+    }
     return SG_OK;
 }
 
@@ -255,8 +560,16 @@ extern "C" int sg_token_logprobs_grad(sg_ctx *ctx, const sg_tensor *logits, cons
     p.glogits = f32_ptr(glogits);
     p.C = (uint32_t)logits->extents[lead];
     p.scale = scale;
+    // 8192 logits a workgroup: rows of ordinary vocabularies are four or more, so that few rows fill the chip too
+    p.part = 2048;
+    // (in place: one workgroup a row, which has read the row when it first writes, if it reads the whole row at all)
+    if (p.glogits == p.logits) p.part = p.C / 4 + 2;
+    p.parts = (p.C + 3 + 4 * p.part - 1) / (4 * p.part);
+    if ((uint64_t)p.R * p.parts >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs_grad: too many elements for one launch");
     sg_device_guard guard(ctx);
-    hipLaunchKernelGGL(logprobs_grad_kernel, dim3(p.R), dim3(256), 0, ctx->stream, p);
+    const dim3 grid(p.R * p.parts);
+    if (sg_streaming((int64_t)p.R * p.C * 8)) hipLaunchKernelGGL((logprobs_grad_kernel<true>), grid, dim3(THREADS), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((logprobs_grad_kernel<false>), grid, dim3(THREADS), 0, ctx->stream, p);
     SG_CHECK_LAUNCH(ctx, "token_logprobs_grad");
     return SG_OK;
 }

@@ -267,6 +267,31 @@ def test_token_logprobs_gradient(ctx, rows, c):
     near(xd.numpy(), R.logprobs_grad(want, 0.8, all_same), R.logprobs_grad_tol(want, x, 0.8, all_same), "in place")
 
 
+@pytest.mark.parametrize("c", [300, 20001])
+def test_token_logprobs_of_rows_far_from_zero(ctx, c):
+    """A row moved by a constant has the same probabilities and gradients: multiples of 1/64 moved by 2^17 are exact, so the
+    tolerance is that of the row that was not moved.  A row of the type's lowest value throughout is uniform."""
+    rng = np.random.default_rng(c)
+    x = R.f32(np.round(rng.standard_normal((3, c)) * 128) / 64)
+    moved = x.copy()
+    moved[0] += 2.0 ** 17
+    moved[1] -= 2.0 ** 17
+    x[2], moved[2] = 0.0, np.finfo(np.float32).min
+    tokens = rng.integers(0, c, 3).astype(np.int32)
+    gl, ge = R.f32(rng.standard_normal(3)), R.f32(rng.standard_normal(3))
+    want, t_lp, t_h = R.logprobs(x, tokens, 1.0), *R.logprobs_tol(x, 1.0)
+    got = run_logprobs(ctx, moved, tokens, 1.0, 6)
+    near(got["logprob"], want["logprob"], t_lp, "logprob")
+    near(got["entropy"], want["entropy"], t_h, "entropy")
+    assert np.array_equal(got["top_ids"], R.logprobs(x, None, 1.0, 6)["top_ids"])
+    xd, tok, outs = got["dev"]
+    out = Tensor.uninit(ctx, [3, c])
+    for to in (out, xd):  # beside the logits and in their place
+        ctx.check(ctx._lib.sg_token_logprobs_grad(ctx.handle, ref(xd), ref(tok), C.c_float(1.0), ref(outs["lse"]), ref(outs["entropy"]), ref(dev(ctx, gl)), ref(dev(ctx, ge)),
+                                                  ref(to)))
+        near(to.numpy(), R.logprobs_grad(want, 1.0, gl, ge), R.logprobs_grad_tol(want, x, 1.0, gl, ge), "glogits")
+
+
 def test_token_logprobs_strided_operands(ctx):
     """[2, 3, C] logits with padded rows at every alignment and permuted leading axes; strided tokens; a rank-1 call."""
     rng = np.random.default_rng(9)
