@@ -5,9 +5,10 @@
 //
 // Forward: a workgroup a row, or a row over several workgroups where rows are few, whose parts a second launch joins.  A
 // thread takes 16 logits a round and keeps (m, s, t) of its own; (m1, s1, t1) moved to a maximum m is
-// (m, f s1, f (t1 + s1 d)) with d = (m1 - m) c, f = 2^d.  The k largest come out of the same pass: k threads' maxima
-// are a bound that k logits reach, so after a round only logits above the k-th largest of the 256 threads' maxima are
-// collected (a later one equal to the bound has a higher index than k that reach it), a few hundred of a row.
+// (m, f s1, f (t1 + s1 d)) with d = (m1 - m) c, f = 2^d.  The k largest come out of the same pass: k lanes' maxima are a
+// bound that k logits reach, so a wavefront collects only logits above the k-th largest of its 64 lanes' maxima (a later
+// one equal to the bound has a higher index than k that reach it), some ten to a hundred of its share, in a list of its own
+// in LDS and without a barrier; the k largest of the wavefronts' lists are ranked at the end.
 #include "rows.h"
 
 #include <type_traits>
@@ -19,7 +20,9 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 
 
 constexpr int TOP_MAX = 64;
 constexpr int THREADS = 256, VECS = 4, ROUND = THREADS * VECS * 4;  // logits a workgroup takes in a round
-constexpr int KEEP = 1024;                                          // candidates kept from round to round
+constexpr int KEEP = 192;                                           // candidates of a wavefront that wait for the next round
+constexpr int LIST = KEEP + 64 * VECS * 4;
+constexpr int JOIN = 1024;                                          // candidates of a split row, over all its parts
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 typedef unsigned long long u64;
 
@@ -29,7 +32,7 @@ struct LogpP {
     float *logprob, *entropy, *lse, *top_logprobs;
     uint32_t *top_ids;
     float *part_stats;    // of split rows: [row][split][3]
-    uint32_t *part_ids;   // [row][split][k], ~0 where a part has no k logits
+    unsigned long long *part_keys;  // [row][split][k], 0 where a part has no k logits
     sg_rows rows, token_rows;
     uint32_t R, C, k, splits;
     float scale;
@@ -44,6 +47,7 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 __device__ __forceinline__ float number_of(uint32_t order) { return __uint_as_float((order & 0x80000000u) ? (order & 0x7FFFFFFFu) : ~order); }
 __device__ __forceinline__ u64 top_key(float x, uint32_t j) { return ((u64)order_bits(x) << 32) | (uint32_t)~j; }
 __device__ __forceinline__ uint32_t index_of(u64 key) { return ~(uint32_t)key; }
+__device__ __forceinline__ float value_of(u64 key) { return (key >> 32) ? number_of((uint32_t)(key >> 32)) : __builtin_nanf(""); }
 
 // 0 * -inf is NaN: a distance whose exponential is 0 anyway becomes a finite one; NaN stays
 __device__ __forceinline__ float finite(float y) { return y < -1e4f ? -1e4f : y; }
@@ -119,94 +123,53 @@ __device__ __forceinline__ Stats block_join(Stats a, float c, float *lds) {  // 
     return a;
 }
 
-struct TopLds {
-    u64 keys[KEEP + ROUND];
-    u64 best[THREADS / 64];
-    __attribute__((aligned(16))) uint32_t maxima[THREADS];
-    uint32_t count, bound;
-};
-
-// The order of the k-th largest of the threads' maxima; 0 if fewer than k threads have seen a number.
-__device__ __forceinline__ uint32_t bound_of(TopLds &l, float thread_max, uint32_t k) {
-    const uint32_t mine = order_bits(thread_max);
-    __syncthreads();
-    l.maxima[threadIdx.x] = mine;
-    __syncthreads();
-    uint32_t rank = 0;
-    for (uint32_t i = 0; i < THREADS; i += 4) {
-        const uint4 o = *reinterpret_cast<const uint4 *>(&l.maxima[i]);
-        rank += (o.x > mine || (o.x == mine && i < threadIdx.x)) + (o.y > mine || (o.y == mine && i + 1 < threadIdx.x)) +
-                (o.z > mine || (o.z == mine && i + 2 < threadIdx.x)) + (o.w > mine || (o.w == mine && i + 3 < threadIdx.x));
+// A bound (as order_bits) that the k-th largest of the lanes' maxima reaches, its lowest byte cut off; 0 if fewer than k
+// lanes have seen a number.
+__device__ __forceinline__ uint32_t wave_bound(float lane_max, uint32_t k) {
+    const uint32_t mine = order_bits(lane_max), lowest = ~0xFF800000u;  // -inf: the lowest of the numbers
+    uint32_t bound = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 8; --bit) {
+        const uint32_t higher = bound | (1u << bit);
+        if (__popcll(__builtin_amdgcn_ballot_w64(mine >= higher)) >= (int)k) bound = higher;
     }
-    if (rank == k - 1) l.bound = mine;
-    __syncthreads();
-    return l.bound;
+    return bound == 0 || bound > lowest ? bound : lowest;
 }
 
-__device__ __forceinline__ u64 block_max(u64 x, u64 *lds) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const u64 y = __shfl_xor(x, o, 64);
-        x = x > y ? x : y;
+// Leaves the k largest of a wavefront's n > k keys in front of its list.  They are different, so some bound has exactly k.
+__device__ __forceinline__ void wave_select(u64 *list, uint32_t n, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 63;
+    u64 bound = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const u64 higher = bound | (1ull << bit);
+        uint32_t count = 0;
+        for (uint32_t i = 0; i < n; i += 64) count += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < n && list[i + lane] >= higher));
+        if (count >= k) bound = higher;
+        if (count == k) break;
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = lds[0];
-#pragma unroll
-    for (int w = 1; w < THREADS / 64; ++w) x = x > lds[w] ? x : lds[w];
-    return x;
+    uint32_t to = 0;
+    for (uint32_t i = 0; i < n; i += 64) {
+        const u64 key = i + lane < n ? list[i + lane] : 0;
+        const u64 stay = __builtin_amdgcn_ballot_w64(i + lane < n && key >= bound);
+        __builtin_amdgcn_wave_barrier();
+        if (stay >> lane & 1) list[to + __popcll(stay & ((1ull << lane) - 1))] = key;
+        __builtin_amdgcn_wave_barrier();
+        to += (uint32_t)__popcll(stay);
+    }
 }
 
-// Leaves the candidates that reach `bound`, and if that leaves more than KEEP of them (long runs of equal logits, or large
-// ones all in one thread's places), exactly the k largest.
-__device__ __forceinline__ void tighten(TopLds &l, uint32_t bound, uint32_t k) {
-    __syncthreads();
-    const uint32_t n = l.count;
-    // a thread's share is read before any is written back
-    u64 mine[(KEEP + ROUND) / THREADS];
-#pragma unroll
-    for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i) {
-        const uint32_t at = i * THREADS + threadIdx.x;
-        mine[i] = at < n ? l.keys[at] : 0;
-        if ((uint32_t)(mine[i] >> 32) < bound) mine[i] = 0;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) l.count = 0;
-    __syncthreads();
-    uint32_t left = 0;
-#pragma unroll
-    for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i) left += mine[i] != 0;
-    const uint32_t at = left ? atomicAdd(&l.count, left) : 0;
-    __syncthreads();
-    if (l.count <= KEEP) {
-        uint32_t to = at;
-#pragma unroll
-        for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i)
-            if (mine[i]) l.keys[to++] = mine[i];
-        __syncthreads();
-        return;
-    }
-    u64 last = ~0ull;
-    for (uint32_t r = 0; r < k; ++r) {
-        u64 b = 0;
-#pragma unroll
-        for (int i = 0; i < (KEEP + ROUND) / THREADS; ++i)
-            if (mine[i] < last && mine[i] > b) b = mine[i];
-        last = block_max(b, l.best);
-        if (threadIdx.x == 0) l.keys[r] = last;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) l.count = k;
-    __syncthreads();
-}
-
-// Place of a key among the n <= KEEP in LDS, largest first; keys are different.
+// Place of a key among n different ones, largest first.
 __device__ __forceinline__ uint32_t place_of(const u64 *keys, uint32_t n, u64 key) {
     uint32_t r = 0;
+#pragma unroll 4
     for (uint32_t i = 0; i < n; ++i) r += keys[i] > key;
     return r;
 }
+
+struct TopLds {
+    u64 list[THREADS / 64][LIST];
+    uint32_t count[THREADS / 64];
+};
 
 template <bool TOP>
 __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
@@ -221,10 +184,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
     f32x4 next[VECS];
 #pragma unroll
     for (int i = 0; i < VECS; ++i) next[i] = g0 + i * THREADS + tid < g1 ? groups.load(g0 + i * THREADS + tid) : f32x4{nan, nan, nan, nan};
-    uint32_t bound = 0;
-    if constexpr (TOP) {
-        if (tid == 0) lds_top.count = 0;
-    }
+    uint32_t bound = 0, n = 0, n_bound = 0;  // of this wavefront: collect above, candidates, candidates when bound was set
     for (uint32_t g = g0; g < g1; g += THREADS * VECS) {
         f32x4 v[VECS];
         float top = a.m;
@@ -263,23 +223,29 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
         }
         if constexpr (TOP) {
             const bool first = g == g0;
-            if (first) bound = bound_of(lds_top, a.m, p.k);
+            u64 *list = lds_top.list[tid >> 6];
+            if (first) bound = wave_bound(a.m, p.k);
             const float limit = number_of(bound);
 #pragma unroll
             for (int i = 0; i < VECS; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t at = g + i * THREADS + tid;
-                    // in the first round what equals the bound, later what is above it; NaN is sorted out below
-                    if (bound != 0 && (first ? v[i][j] < limit : v[i][j] <= limit)) continue;
-                    if (at < g1 && groups.has(at, j)) lds_top.keys[atomicAdd(&lds_top.count, 1u)] = top_key(v[i][j], groups.index(at, j));
+                    // in the first round also what equals the bound; NaN passes and is sorted out by its key
+                    const bool take = (bound == 0 || !(first ? v[i][j] < limit : v[i][j] <= limit)) && at < g1 && groups.has(at, j);
+                    const u64 taken = __builtin_amdgcn_ballot_w64(take);
+                    if (taken == 0) continue;
+                    if (take) list[n + __popcll(taken & ((1ull << (tid & 63)) - 1))] = top_key(v[i][j], groups.index(at, j));
+                    n += (uint32_t)__popcll(taken);
                 }
-            __syncthreads();
-            if (lds_top.count > KEEP) {
-                bound = bound_of(lds_top, a.m, p.k);
-                tighten(lds_top, bound, p.k);
+            if (n > KEEP) {
+                wave_select(list, n, p.k);
+                n = p.k;
             }
-            __syncthreads();
+            if (n >= n_bound + 16 || first) {
+                bound = wave_bound(a.m, p.k);
+                n_bound = n;
+            }
         }
     }
     const Stats all = block_join(a, c, lds_stats);
@@ -298,27 +264,34 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
         }
     }
     if constexpr (TOP) {
-        bound = bound_of(lds_top, a.m, p.k);
-        tighten(lds_top, bound, p.k);
-        const uint32_t n = lds_top.count;
-        for (uint32_t i = tid; i < n; i += THREADS) {
-            const u64 key = lds_top.keys[i];
-            const uint32_t at = place_of(lds_top.keys, n, key);
-            if (at >= p.k) continue;
-            if (p.splits > 1) p.part_ids[(uint64_t)blockIdx.x * p.k + at] = index_of(key);
-            else {
-                p.top_ids[(uint64_t)row * p.k + at] = index_of(key);
-                p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(x[index_of(key)], c);
+        const uint32_t lane = tid & 63, wave = tid >> 6;
+        if (n > p.k) wave_select(lds_top.list[wave], n, p.k);
+        n = n < p.k ? n : p.k;
+        if (lane == 0) lds_top.count[wave] = n;
+        __syncthreads();
+        if (lane < n) {
+            const u64 key = lds_top.list[wave][lane];
+            uint32_t at = 0;
+            for (int w = 0; w < THREADS / 64; ++w) at += place_of(lds_top.list[w], lds_top.count[w], key);
+            if (at < p.k) {
+                if (p.splits > 1) p.part_keys[(uint64_t)blockIdx.x * p.k + at] = key;
+                else {
+                    p.top_ids[(uint64_t)row * p.k + at] = index_of(key);
+                    p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(key), c);
+                }
             }
         }
-        if (p.splits > 1)
-            for (uint32_t i = n + tid; i < p.k; i += THREADS) p.part_ids[(uint64_t)blockIdx.x * p.k + i] = ~0u;
+        if (p.splits > 1) {
+            uint32_t all_n = 0;
+            for (int w = 0; w < THREADS / 64; ++w) all_n += lds_top.count[w];
+            for (uint32_t i = all_n + tid; i < p.k; i += THREADS) p.part_keys[(uint64_t)blockIdx.x * p.k + i] = 0;
+        }
     }
 }
 
 // Joins the parts of a split row.
 __global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const LogpP p) {
-    __shared__ u64 keys[KEEP];
+    __shared__ u64 keys[JOIN];
     __shared__ float lds_stats[12];
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const float *x = p.logits + sg_row_offset(p.rows, row);
@@ -337,18 +310,15 @@ __global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const LogpP p) {
             p.logprob[row] = tok < p.C ? r.logprob(x[tok], c) : 0.0f;
         }
     }
-    const uint32_t n = p.splits * p.k;  // at most KEEP
-    for (uint32_t i = tid; i < n; i += THREADS) {
-        const uint32_t id = p.part_ids[(uint64_t)row * n + i];
-        keys[i] = id == ~0u ? 0 : top_key(x[id], id);
-    }
+    const uint32_t n = p.splits * p.k;  // at most JOIN
+    for (uint32_t i = tid; i < n; i += THREADS) keys[i] = p.part_keys[(uint64_t)row * n + i];
     __syncthreads();
     for (uint32_t i = tid; i < n; i += THREADS) {
         if (!keys[i]) continue;
         const uint32_t at = place_of(keys, n, keys[i]);
         if (at >= p.k) continue;
         p.top_ids[(uint64_t)row * p.k + at] = index_of(keys[i]);
-        p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(x[index_of(keys[i])], c);
+        p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(keys[i]), c);
     }
 }
 
@@ -495,21 +465,21 @@ extern "C" int sg_token_logprobs(sg_ctx *ctx, const sg_tensor *logits, const sg_
     p.C = (uint32_t)C;
     p.k = (uint32_t)k;
     p.scale = scale;
-    // Few rows: a row over several workgroups, two for each compute unit in all, at least a round of logits each, and no
-    // more candidates than a workgroup joins.
-    const uint32_t want = 2u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+    // Few rows: a row over several workgroups, four for each compute unit in all (what it holds of them), a round of logits
+    // each at most, and no more candidates than a workgroup joins.
+    const uint32_t want = 4u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
     p.splits = p.R >= want ? 1 : (want + p.R - 1) / p.R;
-    if (p.splits > p.C / ROUND) p.splits = p.C / ROUND;
+    if (p.splits > (p.C + ROUND - 1) / ROUND) p.splits = (p.C + ROUND - 1) / ROUND;
     if (p.splits > 64) p.splits = 64;
-    if (k && p.splits > KEEP / (uint32_t)k) p.splits = KEEP / (uint32_t)k;
-    if (p.splits < 1) p.splits = 1;
+    if (k && p.splits > JOIN / (uint32_t)k) p.splits = JOIN / (uint32_t)k;
     if ((uint64_t)p.R * p.splits >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs: too many rows for one launch");
     sg_device_guard guard(ctx);
     sg_workspace space(ctx);
     if (p.splits > 1) {
-        if ((rc = space.take((uint64_t)p.R * p.splits * (3 + k) * 4)) != SG_OK) return rc;
-        p.part_stats = (float *)space.p;
-        p.part_ids = (uint32_t *)space.p + (uint64_t)p.R * p.splits * 3;
+        const uint64_t parts = (uint64_t)p.R * p.splits;
+        if ((rc = space.take(parts * (8 * k + 12))) != SG_OK) return rc;
+        p.part_keys = (unsigned long long *)space.p;
+        p.part_stats = (float *)(p.part_keys + parts * k);
     }
     if (k) hipLaunchKernelGGL((logprobs_kernel<true>), dim3(p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
     else hipLaunchKernelGGL((logprobs_kernel<false>), dim3(p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
