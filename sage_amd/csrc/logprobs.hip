@@ -64,6 +64,12 @@ struct Stats {
         s = s * f;
         m = m_new;
     }
+    // one more logit at distance y; where 2^y is 0 the distance is kept finite, and NaN comes in through the factor
+    __device__ void add(float y) {
+        const float e = __builtin_amdgcn_exp2f(y);
+        s += e;
+        t = __builtin_fmaf(e, fmaxf(y, -1e4f), t);
+    }
     __device__ void join(float mo, float so, float to, float c) {
         Stats o = {mo, so, to};
         const float top = fmaxf(m, mo);
@@ -110,9 +116,17 @@ struct Groups {
     __device__ uint32_t index(uint32_t g, uint32_t j) const { return 4 * g + j - lead; }
 };
 
+// The workgroup's Stats: the maximum first, then everyone moves to it once and plain sums are left.
 __device__ __forceinline__ Stats block_join(Stats a, float c, float *lds) {  // lds: 12 floats
+    float top = a.m;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) a.join(__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64), c);
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    a.move(top, c);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        a.s += __shfl_xor(a.s, o, 64);
+        a.t += __shfl_xor(a.t, o, 64);
+    }
     const int wave = threadIdx.x >> 6;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) { lds[3 * wave] = a.m; lds[3 * wave + 1] = a.s; lds[3 * wave + 2] = a.t; }
@@ -140,6 +154,20 @@ __device__ __forceinline__ uint32_t wave_bound(float lane_max, uint32_t k) {
 __device__ __forceinline__ void wave_select(u64 *list, uint32_t n, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63;
     u64 bound = 0;
+    if (n <= 64) {  // a key a lane
+        const u64 key = lane < n ? list[lane] : 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const u64 higher = bound | (1ull << bit);
+            const uint32_t count = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(key >= higher));
+            if (count >= k) bound = higher;
+            if (count == k) break;
+        }
+        const u64 stay = __builtin_amdgcn_ballot_w64(key >= bound && lane < n);
+        __builtin_amdgcn_wave_barrier();
+        if (stay >> lane & 1) list[__popcll(stay & ((1ull << lane) - 1))] = key;
+        __builtin_amdgcn_wave_barrier();
+        return;
+    }
     for (int bit = 63; bit >= 0; --bit) {
         const u64 higher = bound | (1ull << bit);
         uint32_t count = 0;
@@ -177,69 +205,51 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
     __shared__ float lds_stats[12];
     const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, tid = threadIdx.x;
     const float *x = p.logits + sg_row_offset(p.rows, row);
-    const Groups groups(x, p.C);
-    const uint32_t g0 = (uint32_t)((uint64_t)groups.count * split / p.splits), g1 = (uint32_t)((uint64_t)groups.count * (split + 1) / p.splits);
+    // 16-byte groups at whatever element the row starts; the C % 4 logits behind them are a round of their own
+    const uint32_t groups = p.C / 4;
+    const uint32_t g0 = (uint32_t)((uint64_t)groups * split / p.splits), g1 = (uint32_t)((uint64_t)groups * (split + 1) / p.splits);
     const float c = p.scale * LOG2E, nan = __builtin_nanf("");
     Stats a = {nan, 0.0f, 0.0f};
-    f32x4 next[VECS];
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) next[i] = g0 + i * THREADS + tid < g1 ? groups.load(g0 + i * THREADS + tid) : f32x4{nan, nan, nan, nan};
     uint32_t bound = 0, n = 0, n_bound = 0;  // of this wavefront: collect above, candidates, candidates when bound was set
-    for (uint32_t g = g0; g < g1; g += THREADS * VECS) {
-        f32x4 v[VECS];
-        float top = a.m;
-#pragma unroll
-        for (int i = 0; i < VECS; ++i) {
-            v[i] = next[i];
-            top = fmaxf(fmaxf(fmaxf(top, v[i].x), v[i].y), fmaxf(v[i].z, v[i].w));
+    auto collect = [&](float v, uint32_t j, bool take) {
+        if constexpr (TOP) {
+            const u64 taken = __builtin_amdgcn_ballot_w64(take);
+            if (taken == 0) return;
+            if (take) lds_top.list[tid >> 6][n + __popcll(taken & ((1ull << (tid & 63)) - 1))] = top_key(v, j);
+            n += (uint32_t)__popcll(taken);
         }
-        // requested behind the wait for this round's logits, in flight during its arithmetic
+    };
+    // One round: whole, or with lanes that have no logits left (theirs are NaN).
+    auto round = [&](const f32x4 *v, uint32_t g, auto whole) {
+        float high = nan;
 #pragma unroll
-        for (int i = 0; i < VECS; ++i) {
-            const uint32_t at = g + (VECS + i) * THREADS + tid;
-            if (at < g1) next[i] = groups.load(at);
-        }
+        for (int i = 0; i < VECS; ++i) high = fmaxf(fmaxf(fmaxf(high, v[i].x), v[i].y), fmaxf(v[i].z, v[i].w));
+        const float top = fmaxf(a.m, high);
         if (top != a.m) a.move(top, c);
         const float shift = a.shift();
-        const bool whole = groups.whole(g + tid) && g + (VECS - 1) * THREADS + tid < g1 && groups.whole(g + (VECS - 1) * THREADS + tid);
-        if (whole) {
 #pragma unroll
-            for (int i = 0; i < VECS; ++i)
+        for (int i = 0; i < VECS; ++i)
+            if (whole || g + i * THREADS + tid < g1) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float y = finite((v[i][j] - shift) * c), e = __builtin_amdgcn_exp2f(y);
-                    a.s += e;
-                    a.t = __builtin_fmaf(e, y, a.t);
-                }
-        } else {
-            for (int i = 0; i < VECS; ++i)
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t at = g + i * THREADS + tid;
-                    if (at >= g1 || !groups.has(at, j)) continue;
-                    const float y = finite((v[i][j] - shift) * c), e = __builtin_amdgcn_exp2f(y);
-                    a.s += e;
-                    a.t = __builtin_fmaf(e, y, a.t);
-                }
-        }
+                for (int j = 0; j < 4; ++j) a.add((v[i][j] - shift) * c);
+            }
         if constexpr (TOP) {
             const bool first = g == g0;
-            u64 *list = lds_top.list[tid >> 6];
             if (first) bound = wave_bound(a.m, p.k);
             const float limit = number_of(bound);
+            // many rounds behind the first have nothing above the bound (where NaN counts, bound is 0)
+            if (first || bound == 0 || __builtin_amdgcn_ballot_w64(high > limit) != 0) {
 #pragma unroll
-            for (int i = 0; i < VECS; ++i)
+                for (int i = 0; i < VECS; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t at = g + i * THREADS + tid;
-                    // in the first round also what equals the bound; NaN passes and is sorted out by its key
-                    const bool take = (bound == 0 || !(first ? v[i][j] < limit : v[i][j] <= limit)) && at < g1 && groups.has(at, j);
-                    const u64 taken = __builtin_amdgcn_ballot_w64(take);
-                    if (taken == 0) continue;
-                    if (take) list[n + __popcll(taken & ((1ull << (tid & 63)) - 1))] = top_key(v[i][j], groups.index(at, j));
-                    n += (uint32_t)__popcll(taken);
-                }
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t at = g + i * THREADS + tid;
+                        // in the first round also what equals the bound
+                        collect(v[i][j], 4 * at + j, (whole || at < g1) && (bound == 0 || (first ? v[i][j] >= limit : v[i][j] > limit)));
+                    }
+            }
             if (n > KEEP) {
-                wave_select(list, n, p.k);
+                wave_select(lds_top.list[tid >> 6], n, p.k);
                 n = p.k;
             }
             if (n >= n_bound + 16 || first) {
@@ -247,6 +257,37 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
                 n_bound = n;
             }
         }
+    };
+    auto load = [&](uint32_t at) { return *reinterpret_cast<const f32x4_any *>(x + 4 * (uint64_t)min(at, g1 - 1)); };
+    if (g0 < g1) {
+        f32x4 next[VECS];
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) next[i] = load(g0 + i * THREADS + tid);
+        uint32_t g = g0;
+        for (; g + VECS * THREADS <= g1; g += VECS * THREADS) {
+            f32x4 v[VECS];
+#pragma unroll
+            for (int i = 0; i < VECS; ++i) {
+                v[i] = next[i];
+                next[i] = load(g + (VECS + i) * THREADS + tid);  // in flight during this round's arithmetic
+            }
+            round(v, g, std::true_type());
+        }
+        if (g < g1) {
+#pragma unroll
+            for (int i = 0; i < VECS; ++i)
+                if (g + i * THREADS + tid >= g1) next[i] = f32x4{nan, nan, nan, nan};
+            round(next, g, std::false_type());
+        }
+    }
+    if (split == p.splits - 1 && p.C % 4 != 0) {
+        const bool there = tid < p.C % 4;
+        const float v = there ? x[4 * groups + tid] : nan, top = fmaxf(a.m, v);
+        if (there) {
+            if (top != a.m) a.move(top, c);
+            a.add((v - a.shift()) * c);
+        }
+        if constexpr (TOP) collect(v, 4 * groups + tid, there && (bound == 0 || v > number_of(bound)));
     }
     const Stats all = block_join(a, c, lds_stats);
     const RowResult r(all, p.scale);
@@ -355,7 +396,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const LogpGradP 
         for (uint32_t j = tid; j < p.C; j += THREADS) {
             const float v = x[j], top = fmaxf(a.m, v);
             if (top != a.m) a.move(top, c);
-            a.s += __builtin_amdgcn_exp2f(finite((v - a.shift()) * c));
+            a.s += __builtin_amdgcn_exp2f((v - a.shift()) * c);
         }
         const RowResult r(block_join(a, c, lds_stats), p.scale);
         shift = r.shift;
@@ -465,13 +506,14 @@ extern "C" int sg_token_logprobs(sg_ctx *ctx, const sg_tensor *logits, const sg_
     p.C = (uint32_t)C;
     p.k = (uint32_t)k;
     p.scale = scale;
-    // Few rows: a row over several workgroups, four for each compute unit in all (what it holds of them), a round of logits
-    // each at most, and no more candidates than a workgroup joins.
+    // Few rows: a row over several workgroups, at most four for each compute unit in all (what it holds of them), about a
+    // round of logits each at least, and no more candidates than a workgroup joins.
     const uint32_t want = 4u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
-    p.splits = p.R >= want ? 1 : (want + p.R - 1) / p.R;
+    p.splits = want / p.R;
     if (p.splits > (p.C + ROUND - 1) / ROUND) p.splits = (p.C + ROUND - 1) / ROUND;
     if (p.splits > 64) p.splits = 64;
     if (k && p.splits > JOIN / (uint32_t)k) p.splits = JOIN / (uint32_t)k;
+    if (p.splits < 1) p.splits = 1;
     if ((uint64_t)p.R * p.splits >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs: too many rows for one launch");
     sg_device_guard guard(ctx);
     sg_workspace space(ctx);

@@ -190,7 +190,7 @@ def check_logprobs(ctx, x, tokens, scale, top):
     return want, got
 
 
-@pytest.mark.parametrize("rows,c,top", [(1, 1, 1), (1, 2, 2), (3, 63, 5), (2, 64, 64), (5, 257, 20), (1, 30522, 5), (4, 50257, 32), (37, 4099, 64), (300, 1000, 1), (2, 131071, 64)])
+@pytest.mark.parametrize("rows,c,top", [(1, 1, 1), (1, 2, 2), (3, 63, 5), (2, 64, 64), (5, 257, 20), (1, 30522, 5), (4, 50257, 32), (37, 4099, 64), (300, 1000, 1), (2, 131071, 64), (1500, 203, 3)])
 @pytest.mark.parametrize("scale", [1.0, 1.7])
 def test_token_logprobs(ctx, rows, c, top, scale):
     say("logprobs", rows, c, top, scale)
