@@ -90,14 +90,17 @@ __device__ __forceinline__ uint32_t key_of(const SortP &p, uint32_t i) {
     return id < p.V ? id : p.V;
 }
 
-// rank[k]: tokens of the same digit in front of item k in this tile.  counts: [wave][digit], zeroed, in LDS; left as the
-// exclusive sums over the wavefronts.  Items that are not there have digit `digits`, which nothing counts.
+// rank[k]: tokens of the same digit in front of item k in this tile, for the first `items` of ITEMS registers.  counts:
+// [wave][digit], zeroed, in LDS; left as the exclusive sums over the wavefronts, with the tile's counts in totals.  Items
+// that are not there have digit `digits`, which nothing counts.
 template <uint32_t ITEMS>
-__device__ __forceinline__ void rank_items(const uint32_t *digit, uint32_t *rank, volatile uint32_t *counts, uint32_t digits) {
+__device__ __forceinline__ void rank_items(const uint32_t *digit, uint32_t *rank, uint16_t *counts, uint32_t *totals, uint32_t digits, uint32_t items) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint64_t below = (1ull << lane) - 1;
+    volatile uint16_t *mine = counts + wave * digits;
 #pragma unroll
     for (uint32_t k = 0; k < ITEMS; ++k) {
+        if (k >= items) break;
         uint64_t same = __builtin_amdgcn_ballot_w64(digit[k] < digits);
         for (uint32_t bit = 1; bit < digits; bit <<= 1) {
             const uint64_t set = __builtin_amdgcn_ballot_w64((digit[k] & bit) != 0);
@@ -105,27 +108,29 @@ __device__ __forceinline__ void rank_items(const uint32_t *digit, uint32_t *rank
         }
         rank[k] = 0;
         if (digit[k] < digits) {
-            volatile uint32_t *c = &counts[wave * digits + digit[k]];
-            const uint32_t before = *c;
+            const uint32_t before = mine[digit[k]];
             __builtin_amdgcn_wave_barrier();  // every lane has read before the first of its digit writes
             rank[k] = before + (uint32_t)__popcll(same & below);
-            if ((same & below) == 0) *c = before + (uint32_t)__popcll(same);
+            if ((same & below) == 0) mine[digit[k]] = (uint16_t)(before + (uint32_t)__popcll(same));
         }
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
     if (threadIdx.x < digits) {
-        uint32_t sum = 0;
+        uint32_t x[SORT_WAVES], sum = 0;
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) x[w] = counts[w * digits + threadIdx.x];
+#pragma unroll
         for (int w = 0; w < SORT_WAVES; ++w) {
-            const uint32_t x = counts[w * digits + threadIdx.x];
-            counts[w * digits + threadIdx.x] = sum;
-            sum += x;
+            counts[w * digits + threadIdx.x] = (uint16_t)sum;  // below the tile's 8192
+            sum += x[w];
         }
+        totals[threadIdx.x] = sum;
     }
     __syncthreads();
 #pragma unroll
     for (uint32_t k = 0; k < ITEMS; ++k)
-        if (digit[k] < digits) rank[k] += counts[wave * digits + digit[k]];
+        if (k < items && digit[k] < digits) rank[k] += counts[wave * digits + digit[k]];
 }
 
 // Exclusive prefix sums of totals[0..digits) in LDS, in place.  scratch: one word per wavefront.
@@ -140,15 +145,17 @@ __device__ __forceinline__ void prefix_digits(uint32_t *totals, uint32_t *scratc
     }
     if (lane == 63) scratch[wave] = sum;
     __syncthreads();
-    for (uint32_t w = 0; w < wave; ++w) sum += scratch[w];
+#pragma unroll
+    for (uint32_t w = 0; w < MAX_DIGITS / 64; ++w)
+        if (w < wave) sum += scratch[w];
     if (threadIdx.x < digits) totals[threadIdx.x] = sum - x;
     __syncthreads();
 }
 
 // Up to 8192 tokens: workgroup 0 sorts them, all passes in LDS; the others clear the table.
 __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const SortP p) {
-    __shared__ uint32_t keys[SINGLE], counts[SORT_WAVES * MAX_DIGITS], totals[MAX_DIGITS], scratch[SORT_WAVES];
-    __shared__ uint16_t places[SINGLE];
+    __shared__ uint32_t keys[SINGLE], totals[MAX_DIGITS], scratch[SORT_WAVES];
+    __shared__ uint16_t places[SINGLE], counts[SORT_WAVES * MAX_DIGITS];
     if (blockIdx.x > 0) {
         clear_part(p, blockIdx.x - 1);
         return;
@@ -164,15 +171,13 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const Sort
     for (uint32_t pass = 0; pass < p.passes; ++pass) {
         const uint32_t shift = pass * p.bits, digits = 1u << p.bits;
         for (uint32_t i = threadIdx.x; i < SORT_WAVES * digits; i += SORT_THREADS) counts[i] = 0;
-        if (threadIdx.x < digits) totals[threadIdx.x] = 0;
         __syncthreads();
 #pragma unroll
         for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
             const bool there = k < items && item_index(items, k) < p.n;
             digit[k] = there ? (key[k] >> shift) & (digits - 1) : digits;
-            if (there) atomicAdd(&totals[digit[k]], 1u);
         }
-        rank_items<SINGLE_ITEMS>(digit, rank, counts, digits);
+        rank_items<SINGLE_ITEMS>(digit, rank, counts, totals, digits, items);
         prefix_digits(totals, scratch, digits);
 #pragma unroll
         for (uint32_t k = 0; k < SINGLE_ITEMS; ++k)
@@ -215,7 +220,8 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_count_kernel(const Sor
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) embedding_move_kernel(const SortP p) {
-    __shared__ uint32_t counts[SORT_WAVES * MAX_DIGITS], totals[MAX_DIGITS], before[MAX_DIGITS], scratch[SORT_WAVES];
+    __shared__ uint32_t own[MAX_DIGITS], totals[MAX_DIGITS], before[MAX_DIGITS], scratch[SORT_WAVES];
+    __shared__ uint16_t counts[SORT_WAVES * MAX_DIGITS];
     if (blockIdx.x >= p.tiles) {
         clear_part(p, blockIdx.x - p.tiles);
         return;
@@ -244,7 +250,7 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_move_kernel(const Sort
         atomicAdd(&totals[d], all);
         atomicAdd(&before[d], front);
     }
-    rank_items<TILE_ITEMS>(digit, rank, counts, p.digits);
+    rank_items<TILE_ITEMS>(digit, rank, counts, own, p.digits, TILE_ITEMS);
     prefix_digits(totals, scratch, p.digits);
 #pragma unroll
     for (uint32_t k = 0; k < TILE_ITEMS; ++k)
@@ -288,8 +294,8 @@ __device__ __forceinline__ void store_cols(float *row, uint32_t c, uint32_t E, f
     }
 }
 
-// A wavefront sums 256 columns of one chunk of sorted tokens; 8 rows are in flight at a time.
-template <bool VEC>
+// A wavefront sums 256 columns of one chunk of sorted tokens; BATCH rows are in flight at a time.
+template <bool VEC, uint32_t BATCH>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
     const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (unit >= p.chunks * p.pieces) return;
@@ -301,19 +307,19 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
     const uint32_t prev = first > 0 ? p.key[first - 1] : ~0u, next = last < p.n ? p.key[last] : ~0u;  // no key is ~0
     bool from_before = prev == (uint32_t)__builtin_amdgcn_readfirstlane(key);
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t b = first; b < last; b += 8) {
-        f32x4 x[8];
-        uint32_t id[9];
+    for (uint32_t b = first; b < last; b += BATCH) {
+        f32x4 x[BATCH];
+        uint32_t id[BATCH + 1];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
+        for (uint32_t k = 0; k < BATCH; ++k) {
             const uint32_t at = min(b + k, last - 1) - first;
             id[k] = (uint32_t)__builtin_amdgcn_readlane((int)key, (int)at);
             if (b + k < last && id[k] < p.V)
                 x[k] = load_cols<VEC>(p.gout + sg_row_offset(p.g_rows, (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)at)), c, p.E);
         }
-        id[8] = b + 8 < last ? (uint32_t)__builtin_amdgcn_readlane((int)key, (int)(b + 8 - first)) : next;
+        id[BATCH] = b + BATCH < last ? (uint32_t)__builtin_amdgcn_readlane((int)key, (int)(b + BATCH - first)) : next;
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
+        for (uint32_t k = 0; k < BATCH; ++k) {
             if (b + k >= last || id[k] >= p.V) return;  // unknown tokens are the list's end
             acc += x[k];
             const bool end = b + k + 1 == last;
@@ -512,8 +518,8 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
     bool vec = E % 4 == 0 && aligned16(m.gout) && aligned16(table);
     for (int i = 0; i < m.g_rows.rank; ++i) vec = vec && m.g_rows.st[i] % 4 == 0;
     const dim3 sum_grid((m.chunks * m.pieces + 3) / 4), join_grid((m.chunks - 1) * m.pieces);
-    if (vec) hipLaunchKernelGGL((embedding_sum_kernel<true>), sum_grid, dim3(256), 0, ctx->stream, m);
-    else hipLaunchKernelGGL((embedding_sum_kernel<false>), sum_grid, dim3(256), 0, ctx->stream, m);
+    if (vec) hipLaunchKernelGGL((embedding_sum_kernel<true, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
+    else hipLaunchKernelGGL((embedding_sum_kernel<false, 4>), sum_grid, dim3(256), 0, ctx->stream, m);
     SG_CHECK_LAUNCH(ctx, "embedding_grad sums");
     if (m.chunks > 1) {
         if (vec) hipLaunchKernelGGL((embedding_join_kernel<true>), join_grid, dim3(256), 0, ctx->stream, m);
