@@ -13,11 +13,13 @@
 // kernel, where columns do not mix: they are left in and written as zeros.
 #include "rows.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes at any element
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
@@ -41,23 +43,28 @@ struct CrossP {
 
 __device__ __forceinline__ uint32_t fdiv(uint32_t n, sg_fastdiv d) { return (__umulhi(n, d.magic) + n) >> d.shift; }
 
-// Workgroup ids go round-robin over the 8 XCDs; consecutive work (tiles of one pair, which share keys or rows) goes to one.
-__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t total) {
-    const uint32_t per = total / 8, rest = total % 8, x = id % 8;
-    return x * per + (x < rest ? x : rest) + id / 8;
-}
-
 struct Work {
     uint32_t split, pair, tile;
     int b, g;
 };
+// Workgroup ids go round-robin over the 8 XCDs.  All tiles of a (split, pair), which share keys or rows, go to one of them,
+// and the pairs of a sequence, whose length they have in common, to different ones.
 __device__ __forceinline__ Work find_work(const CrossP &p) {
     Work w;
-    const uint32_t id = xcd_order(blockIdx.x, p.tiles * p.pairs * p.splits);
-    const uint32_t rest = fdiv(id, p.d_tiles);
-    w.tile = id - rest * p.tiles;
-    w.split = fdiv(rest, p.d_pairs);
-    w.pair = rest - w.split * p.pairs;
+    const uint32_t units = p.pairs * p.splits, even = units & ~7u;
+    uint32_t id = blockIdx.x, unit;
+    if (id < even * p.tiles) {
+        const uint32_t q = fdiv(id >> 3, p.d_tiles);
+        w.tile = (id >> 3) - q * p.tiles;
+        unit = q * 8 + (id & 7);
+    } else {
+        id -= even * p.tiles;
+        const uint32_t q = fdiv(id, p.d_tiles);
+        w.tile = id - q * p.tiles;
+        unit = even + q;
+    }
+    w.split = fdiv(unit, p.d_pairs);
+    w.pair = unit - w.split * p.pairs;
     w.b = (int)fdiv(w.pair, p.d_g);
     w.g = (int)w.pair - w.b * p.G;
     return w;
@@ -69,16 +76,8 @@ __device__ __forceinline__ int64_t row_at(const CrossP &p, const Rows &x, const 
     return w.b * x.b + (int64_t)(w.g * (p.H / p.G) + (int)hh) * x.h + (int64_t)(r - hh * p.Lq) * x.l;
 }
 
-__device__ __forceinline__ f32x4 load4(const float *p, bool vec) {
-    f32x4 v;
-    if (vec) v = *reinterpret_cast<const f32x4 *>(p);
-    else { v.x = p[0]; v.y = p[1]; v.z = p[2]; v.w = p[3]; }
-    return v;
-}
-__device__ __forceinline__ void store4(float *p, f32x4 v, bool vec) {
-    if (vec) *reinterpret_cast<f32x4 *>(p) = v;
-    else { p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w; }
-}
+__device__ __forceinline__ f32x4 load4(const float *p) { return *reinterpret_cast<const f32x4_any *>(p); }
+__device__ __forceinline__ void store4(float *p, f32x4 v) { *reinterpret_cast<f32x4_any *>(p) = v; }
 
 // One behind the last visible key of a sequence: a padded batch costs what its lengths cost.
 __device__ __forceinline__ int visible_end(const CrossP &p, int b, int *lds) {
@@ -208,7 +207,7 @@ __device__ __forceinline__ void accumulate(const float *tile, const floatx16 &w,
 
 // What accumulate() left of column c: consecutive head indices ND (8g + 4h) .. + 4 ND, times f.
 template <int D>
-__device__ __forceinline__ void write_column(float *row, const floatx16 *acc, float f, int h, bool vec) {
+__device__ __forceinline__ void write_column(float *row, const floatx16 *acc, float f, int h) {
     constexpr int ND = D / 32;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -218,20 +217,20 @@ __device__ __forceinline__ void write_column(float *row, const floatx16 *acc, fl
 #pragma unroll
             for (int j = 0; j < ND; ++j) t[ND * s + j] = acc[j][4 * g + s] * f;
 #pragma unroll
-        for (int c = 0; c < ND; ++c) store4(row + ND * (8 * g + 4 * h) + 4 * c, f32x4{t[4 * c], t[4 * c + 1], t[4 * c + 2], t[4 * c + 3]}, vec);
+        for (int c = 0; c < ND; ++c) store4(row + ND * (8 * g + 4 * h) + 4 * c, f32x4{t[4 * c], t[4 * c + 1], t[4 * c + 2], t[4 * c + 3]});
     }
 }
 
 // The 32 RW rows of a workgroup's tile, through the LDS of the key blocks, to the wavefronts that own them.
 template <int D, int RW, int KB>
-__device__ __forceinline__ void take_rows(const CrossP &p, const Rows &x, const Work &w, bool vec, float *lds_a, float *lds_b, int own_row, int h, Own<D> &own) {
+__device__ __forceinline__ void take_rows(const CrossP &p, const Rows &x, const Work &w, float *lds_a, float *lds_b, int own_row, int h, Own<D> &own) {
     constexpr int ROWV = D / 4, LD = D + 4;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 32 * RW * ROWV / 256; ++i) {
         const int f = threadIdx.x + i * 256, row = f / ROWV, c = (f % ROWV) * 4;
         const uint32_t r = min(w.tile * (32 * RW) + row, (uint32_t)p.R - 1);  // a row past the end repeats the last one; it is not written
-        *reinterpret_cast<f32x4 *>(&(row < KB ? lds_a : lds_b)[(row % KB) * LD + c]) = load4(x.p + row_at(p, x, w, r) + c, vec);
+        *reinterpret_cast<f32x4 *>(&(row < KB ? lds_a : lds_b)[(row % KB) * LD + c]) = load4(x.p + row_at(p, x, w, r) + c);
     }
     __syncthreads();
     own.take(&(own_row < KB ? lds_a : lds_b)[(own_row - own_row % 32) % KB * LD], own_row % 32, h);
@@ -239,7 +238,7 @@ __device__ __forceinline__ void take_rows(const CrossP &p, const Rows &x, const 
 
 // ---- forward.  RW wavefronts take the workgroup's 32 RW rows, the 4 / RW times as many share each block's keys and are
 // merged through LDS at the end.
-template <int D, int RW, bool VEC>
+template <int D, int RW>
 __global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = RW == 1 ? 128 : 64, NKB = KB / KW / 32, LD = D + 4, ND = D / 32;
     __shared__ __attribute__((aligned(16))) float lds_k[KB * LD], lds_v[KB * LD], lds_m[KB];
@@ -252,7 +251,7 @@ __global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
     const float inf = __builtin_inff();
 
     Own<D> q;
-    take_rows<D, RW, KB>(p, p.q, w, VEC, lds_k, lds_v, own_row, h, q);
+    take_rows<D, RW, KB>(p, p.q, w, lds_k, lds_v, own_row, h, q);
     floatx16 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = zero16();
@@ -265,8 +264,8 @@ __global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
 #pragma unroll
         for (int i = 0; i < ks.N; ++i) {
             const int64_t j = min(j0 + ks.row(i), p.Lk - 1);
-            ks.x[i] = load4(K + j * p.k.l + ks.col(), VEC);
-            vs.x[i] = load4(V + j * p.v.l + vs.col(), VEC);
+            ks.x[i] = load4(K + j * p.k.l + ks.col());
+            vs.x[i] = load4(V + j * p.v.l + vs.col());
         }
         seen.request(mask, j0, p.Lk);
     };
@@ -352,17 +351,143 @@ __global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
     const int64_t row = (int64_t)w.pair * p.R + r;
     if (p.splits > 1) {
         const int64_t at = (int64_t)w.split * p.pairs * p.R + row;
-        write_column<D>(p.part_o + at * D, acc, 1.0f, h, true);
+        write_column<D>(p.part_o + at * D, acc, 1.0f, h);
         if (h == 0) { p.part_ml[2 * at] = m_run; p.part_ml[2 * at + 1] = l_run; }
         return;
     }
-    write_column<D>(const_cast<float *>(p.o.p) + row_at(p, p.o, w, r), acc, l_run == 0.0f ? 0.0f : 1.0f / l_run, h, VEC);
+    write_column<D>(const_cast<float *>(p.o.p) + row_at(p, p.o, w, r), acc, l_run == 0.0f ? 0.0f : 1.0f / l_run, h);
     if (p.lse && h == 0) p.lse[row] = l_run == 0.0f ? -inf : (m_run + __builtin_amdgcn_logf(l_run)) * LN2;
+}
+
+// ---- forward with up to 8 rows a pair (a serving step).  Bound by memory: K and V are read once for few products, on
+// the vector unit.  D / 4 lanes hold a key's 16-byte pieces, so a wavefront takes 4 or 8 keys an instruction; every group of
+// lanes runs a softmax of its own over its keys, merged at the end.  UNROLL keys a group are in flight behind the UNROLL
+// that are worked on.
+template <int D>
+__device__ __forceinline__ float group_sum(float x) {  // over the D / 4 lanes of a key, in all of them
+    auto move = [](float v, auto ctrl) { return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xF, 0xF, true)); };
+    x += move(x, std::integral_constant<int, 0xB1>());   // quad_perm 1 0 3 2
+    x += move(x, std::integral_constant<int, 0x4E>());   // quad_perm 2 3 0 1
+    x += move(x, std::integral_constant<int, 0x141>());  // row_half_mirror
+    if (D == 64) x += move(x, std::integral_constant<int, 0x140>());  // row_mirror
+    return x;
+}
+
+template <int D, int ROWS, int UNROLL>
+__global__ void __launch_bounds__(256) cross_few_kernel(const CrossP p) {
+    constexpr int LPK = D / 4, KEYS = 64 / LPK, STEP = KEYS * UNROLL;  // lanes a key, keys an instruction, keys a step
+    __shared__ int lds_end[4];
+    __shared__ float lds_ml[4][ROWS][2];
+    __shared__ __attribute__((aligned(16))) float lds_o[4][ROWS][D];
+    const Work w = find_work(p);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPK, col = lane % LPK * 4;
+    const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h + col, *V = p.v.p + w.b * p.v.b + w.g * p.v.h + col;
+    const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
+    const float inf = __builtin_inff(), c2 = p.scale * LOG2E;
+    f32x4 q[ROWS], acc[ROWS];
+    float m[ROWS], l[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        q[r] = load4(p.q.p + row_at(p, p.q, w, min(r, p.R - 1)) + col) * c2;
+        acc[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[r] = -inf;
+        l[r] = 0.0f;
+    }
+    const int end = visible_end(p, w.b, lds_end);
+    uint32_t first, last;
+    split_range((end + STEP - 1) / STEP, w.split, p.splits, &first, &last);
+    f32x4 kn[UNROLL], vn[UNROLL];
+    float mn[UNROLL];
+    auto request = [&](uint32_t step) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int j = (int)step * STEP + u * KEYS + sub, at = min(j, p.Lk - 1);
+            kn[u] = load4(K + (int64_t)at * p.k.l);
+            vn[u] = load4(V + (int64_t)at * p.v.l);
+            mn[u] = j < end ? (mask ? mask[at] : 1.0f) : 0.0f;
+        }
+    };
+    if (first + wave < last) request(first + wave);
+    for (uint32_t step = first + wave; step < last; step += 4) {
+        f32x4 k[UNROLL], v[UNROLL];
+        bool seen[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            k[u] = kn[u];
+            seen[u] = mn[u] != 0.0f;
+            v[u] = seen[u] ? vn[u] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // 0 * NaN is NaN
+        }
+        if (step + 4 < last) request(step + 4);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            float s[UNROLL], top = m[r];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const float d = __builtin_fmaf(q[r].w, k[u].w, __builtin_fmaf(q[r].z, k[u].z, __builtin_fmaf(q[r].y, k[u].y, q[r].x * k[u].x)));
+                s[u] = seen[u] ? group_sum<D>(d) : -inf;
+                top = fmaxf(top, s[u]);
+            }
+            const float shift = top == -inf ? 0.0f : top;
+            if (__builtin_amdgcn_ballot_w64(top != m[r]) != 0) {
+                const float f = __builtin_amdgcn_exp2f(m[r] - shift);
+                l[r] *= f;
+                acc[r] *= f;
+                m[r] = top;
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const float e = __builtin_amdgcn_exp2f(s[u] - shift);
+                l[r] += e;
+                acc[r] += v[u] * e;
+            }
+        }
+    }
+    // the lane groups of a wavefront, then the wavefronts
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int o = LPK; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        const float f = __builtin_amdgcn_exp2f(m[r] - (top == -inf ? 0.0f : top));
+        l[r] *= f;
+        acc[r] *= f;
+#pragma unroll
+        for (int o = LPK; o < 64; o <<= 1) {
+            l[r] += __shfl_xor(l[r], o, 64);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[r][j] += __shfl_xor(acc[r][j], o, 64);
+        }
+        if (sub == 0) *reinterpret_cast<f32x4 *>(&lds_o[wave][r][col]) = acc[r];
+        if (lane == 0) { lds_ml[wave][r][0] = top; lds_ml[wave][r][1] = l[r]; }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x >= ROWS * LPK) return;
+    const int r = threadIdx.x / LPK, c = threadIdx.x % LPK * 4;
+    if (r >= p.R) return;
+    float top = -inf, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, lds_ml[i][r][0]);
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float f = __builtin_amdgcn_exp2f(lds_ml[i][r][0] - (top == -inf ? 0.0f : top));
+        sum += lds_ml[i][r][1] * f;
+        o += *reinterpret_cast<const f32x4 *>(&lds_o[i][r][c]) * f;
+    }
+    const int64_t row = (int64_t)w.pair * p.R + r;
+    if (p.splits > 1) {
+        const int64_t at = (int64_t)w.split * p.pairs * p.R + row;
+        *reinterpret_cast<f32x4 *>(p.part_o + at * D + c) = o;
+        if (c == 0) { p.part_ml[2 * at] = top; p.part_ml[2 * at + 1] = sum; }
+        return;
+    }
+    store4(const_cast<float *>(p.o.p) + row_at(p, p.o, w, r) + c, o * (sum == 0.0f ? 0.0f : 1.0f / sum));
+    if (p.lse && c == 0) p.lse[row] = sum == 0.0f ? -inf : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
 // Joins the splits of a row: D / 4 lanes a row.
 template <int D>
-__global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p, int vec) {
+__global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p) {
     constexpr int LPR = D / 4;
     const uint32_t total = p.pairs * p.R, row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
     if (row >= total) return;
@@ -381,12 +506,12 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p, int vec
     w.pair = row / p.R;
     w.b = (int)fdiv(w.pair, p.d_g);
     w.g = (int)w.pair - w.b * p.G;
-    store4(const_cast<float *>(p.o.p) + row_at(p, p.o, w, row - w.pair * p.R) + col, acc * (l == 0.0f ? 0.0f : 1.0f / l), vec);
+    store4(const_cast<float *>(p.o.p) + row_at(p, p.o, w, row - w.pair * p.R) + col, acc * (l == 0.0f ? 0.0f : 1.0f / l));
     if (p.lse && col == 0) p.lse[row] = l == 0.0f ? -inf : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // ---- gradient of the queries (and delta, for the other kernel)
-template <int D, int RW, bool VEC>
+template <int D, int RW>
 __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = RW == 1 ? 128 : 64, NKB = KB / KW / 32, LD = D + 4, ND = D / 32;
     __shared__ __attribute__((aligned(16))) float lds_k[KB * LD], lds_v[KB * LD], lds_m[KB];
@@ -401,15 +526,15 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
 
     Own<D> q, go;
     float delta = 0.0f;
-    take_rows<D, RW, KB>(p, p.o, w, VEC, lds_k, lds_v, own_row, h, q);
-    take_rows<D, RW, KB>(p, p.go, w, VEC, lds_k, lds_v, own_row, h, go);
+    take_rows<D, RW, KB>(p, p.o, w, lds_k, lds_v, own_row, h, q);
+    take_rows<D, RW, KB>(p, p.go, w, lds_k, lds_v, own_row, h, go);
 #pragma unroll
     for (int g = 0; g < D / 8; ++g)
 #pragma unroll
         for (int s = 0; s < 4; ++s) delta += q.x[g][s] * go.x[g][s];
     delta += __shfl_xor(delta, 32, 64);
     if (w.split == 0 && wave < RW && h == 0 && r < (uint32_t)p.R) p.delta[row] = delta;
-    take_rows<D, RW, KB>(p, p.q, w, VEC, lds_k, lds_v, own_row, h, q);
+    take_rows<D, RW, KB>(p, p.q, w, lds_k, lds_v, own_row, h, q);
     const float lse2 = p.lse[row] * LOG2E, c2 = p.scale * LOG2E;
     floatx16 acc[ND];
 #pragma unroll
@@ -421,8 +546,8 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
 #pragma unroll
         for (int i = 0; i < ks.N; ++i) {
             const int64_t j = min(j0 + ks.row(i), p.Lk - 1);
-            ks.x[i] = load4(K + j * p.k.l + ks.col(), VEC);
-            vs.x[i] = load4(V + j * p.v.l + vs.col(), VEC);
+            ks.x[i] = load4(K + j * p.k.l + ks.col());
+            vs.x[i] = load4(V + j * p.v.l + vs.col());
         }
         seen.request(mask, j0, p.Lk);
     };
@@ -477,12 +602,12 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
         }
     }
     if (r >= (uint32_t)p.R) return;
-    if (p.splits > 1) write_column<D>(p.part_o + ((int64_t)w.split * p.pairs * p.R + row) * D, acc, p.scale, h, true);
-    else write_column<D>(const_cast<float *>(p.gq.p) + row_at(p, p.gq, w, r), acc, p.scale, h, VEC);
+    if (p.splits > 1) write_column<D>(p.part_o + ((int64_t)w.split * p.pairs * p.R + row) * D, acc, p.scale, h);
+    else write_column<D>(const_cast<float *>(p.gq.p) + row_at(p, p.gq, w, r), acc, p.scale, h);
 }
 
 // ---- gradients of keys and values: a wavefront owns 32 keys and walks all rows of the pair.
-template <int D, bool VEC>
+template <int D>
 __global__ void __launch_bounds__(256) cross_gkv_kernel(const CrossP p) {
     constexpr int RB = 64, LD = D + 4, ND = D / 32, ROWV = D / 4;
     __shared__ __attribute__((aligned(16))) float lds_q[RB * LD], lds_go[RB * LD], lds_lse[RB], lds_delta[RB];
@@ -502,8 +627,8 @@ __global__ void __launch_bounds__(256) cross_gkv_kernel(const CrossP p) {
         for (int i = 0; i < RB * ROWV / 256; ++i) {
             const int f = tid + i * 256, row = f / ROWV, col = (f % ROWV) * 4;
             const int64_t jj = min((int)w.tile * 128 + half * 64 + row, p.Lk - 1);
-            *reinterpret_cast<f32x4 *>(&lds_q[row * LD + col]) = load4(K + jj * p.k.l + col, VEC);
-            *reinterpret_cast<f32x4 *>(&lds_go[row * LD + col]) = load4(V + jj * p.v.l + col, VEC);
+            *reinterpret_cast<f32x4 *>(&lds_q[row * LD + col]) = load4(K + jj * p.k.l + col);
+            *reinterpret_cast<f32x4 *>(&lds_go[row * LD + col]) = load4(V + jj * p.v.l + col);
         }
         __syncthreads();
         if (wave / 2 == half) {
@@ -523,8 +648,8 @@ __global__ void __launch_bounds__(256) cross_gkv_kernel(const CrossP p) {
 #pragma unroll
         for (int i = 0; i < qs.N; ++i) {
             const uint32_t r = min(r0 + qs.row(i), (uint32_t)p.R - 1);
-            qs.x[i] = load4(p.q.p + row_at(p, p.q, w, r) + qs.col(), VEC);
-            gs.x[i] = load4(p.go.p + row_at(p, p.go, w, r) + gs.col(), VEC);
+            qs.x[i] = load4(p.q.p + row_at(p, p.q, w, r) + qs.col());
+            gs.x[i] = load4(p.go.p + row_at(p, p.go, w, r) + gs.col());
         }
         if (tid < RB) {
             const uint32_t r = r0 + tid;
@@ -569,24 +694,24 @@ __global__ void __launch_bounds__(256) cross_gkv_kernel(const CrossP p) {
     }
     if (p.splits > 1) {
         const int64_t at = (((int64_t)w.split * p.pairs + w.pair) * p.Lk + j) * D;
-        write_column<D>(p.part_k + at, gk, p.scale, h, true);
-        write_column<D>(p.part_v + at, gv, 1.0f, h, true);
+        write_column<D>(p.part_k + at, gk, p.scale, h);
+        write_column<D>(p.part_v + at, gv, 1.0f, h);
     } else {
-        write_column<D>(const_cast<float *>(p.gk.p) + w.b * p.gk.b + w.g * p.gk.h + (int64_t)j * p.gk.l, gk, p.scale, h, VEC);
-        write_column<D>(const_cast<float *>(p.gv.p) + w.b * p.gv.b + w.g * p.gv.h + (int64_t)j * p.gv.l, gv, 1.0f, h, VEC);
+        write_column<D>(const_cast<float *>(p.gk.p) + w.b * p.gk.b + w.g * p.gk.h + (int64_t)j * p.gk.l, gk, p.scale, h);
+        write_column<D>(const_cast<float *>(p.gv.p) + w.b * p.gv.b + w.g * p.gv.h + (int64_t)j * p.gv.l, gv, 1.0f, h);
     }
 }
 
 // out[row] = sum of the splits' rows, in order: D / 4 lanes a row.  Rows of a pair are `heads` x `length`.
 template <int D>
-__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, Rows out, uint32_t total, uint32_t splits, uint32_t heads, uint32_t length, int vec) {
+__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, Rows out, uint32_t total, uint32_t splits, uint32_t heads, uint32_t length) {
     constexpr int LPR = D / 4;
     const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
     if (row >= total) return;
     f32x4 acc = *reinterpret_cast<const f32x4 *>(part + (int64_t)row * D + col);
     for (uint32_t i = 1; i < splits; ++i) acc += *reinterpret_cast<const f32x4 *>(part + ((int64_t)i * total + row) * D + col);
     const uint32_t bh = row / length;
-    store4(const_cast<float *>(out.p) + bh / heads * out.b + bh % heads * out.h + (int64_t)(row - bh * length) * out.l + col, acc, vec);
+    store4(const_cast<float *>(out.p) + bh / heads * out.b + bh % heads * out.h + (int64_t)(row - bh * length) * out.l + col, acc);
 }
 
 int check_operand(sg_ctx *ctx, const sg_tensor *t, int64_t n, int64_t heads, int64_t len, int64_t D, const char *who, Rows *r) {
@@ -653,8 +778,6 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
     return SG_OK;
 }
 
-bool vec_rows(const Rows &r) { return ((uintptr_t)r.p) % 16 == 0 && r.b % 4 == 0 && r.h % 4 == 0 && r.l % 4 == 0; }
-
 // Splits of a long axis of `blocks` blocks that bring `units` workgroups to two for each compute unit.
 uint32_t choose_splits(const sg_ctx *ctx, uint32_t units, uint32_t blocks) {
     const uint32_t want = 2u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
@@ -675,18 +798,14 @@ int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
 
 }  // namespace
 
-#define SG_CROSS_LAUNCH(KERNEL, RW, VEC, GRID)                                                                          \
+#define SG_CROSS_ROWS(KERNEL, RW, GRID)                                                                                 \
     do {                                                                                                                \
-        if (D == 64 && VEC) hipLaunchKernelGGL((KERNEL<64, RW, true>), GRID, dim3(256), 0, ctx->stream, p);             \
-        else if (D == 64) hipLaunchKernelGGL((KERNEL<64, RW, false>), GRID, dim3(256), 0, ctx->stream, p);              \
-        else if (VEC) hipLaunchKernelGGL((KERNEL<32, RW, true>), GRID, dim3(256), 0, ctx->stream, p);                   \
-        else hipLaunchKernelGGL((KERNEL<32, RW, false>), GRID, dim3(256), 0, ctx->stream, p);                           \
-    } while (0)
-#define SG_CROSS_ROWS(KERNEL, RW, VEC, GRID)                                                                            \
-    do {                                                                                                                \
-        if (RW == 4) SG_CROSS_LAUNCH(KERNEL, 4, VEC, GRID);                                                             \
-        else if (RW == 2) SG_CROSS_LAUNCH(KERNEL, 2, VEC, GRID);                                                        \
-        else SG_CROSS_LAUNCH(KERNEL, 1, VEC, GRID);                                                                     \
+        if (D == 64 && RW == 4) hipLaunchKernelGGL((KERNEL<64, 4>), GRID, dim3(256), 0, ctx->stream, p);                \
+        else if (D == 64 && RW == 2) hipLaunchKernelGGL((KERNEL<64, 2>), GRID, dim3(256), 0, ctx->stream, p);           \
+        else if (D == 64) hipLaunchKernelGGL((KERNEL<64, 1>), GRID, dim3(256), 0, ctx->stream, p);                      \
+        else if (RW == 4) hipLaunchKernelGGL((KERNEL<32, 4>), GRID, dim3(256), 0, ctx->stream, p);                      \
+        else if (RW == 2) hipLaunchKernelGGL((KERNEL<32, 2>), GRID, dim3(256), 0, ctx->stream, p);                      \
+        else hipLaunchKernelGGL((KERNEL<32, 1>), GRID, dim3(256), 0, ctx->stream, p);                                   \
     } while (0)
 
 extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask, float scale,
@@ -698,23 +817,38 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
     p.scale = scale;
     sg_device_guard guard(ctx);
     const int64_t D = q->extents[3];
+    const bool few = p.R <= 8;
     const int rw = row_waves(p.R), kb = rw == 1 ? 128 : 64;
-    const uint32_t tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), total = p.pairs * (uint32_t)p.R;
-    if ((rc = set_tiles(ctx, p, tiles, choose_splits(ctx, tiles * p.pairs, (uint32_t)((p.Lk + kb - 1) / kb)))) != SG_OK) return rc;
+    const uint32_t tiles = few ? 1 : (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), total = p.pairs * (uint32_t)p.R;
+    const uint32_t blocks = (uint32_t)((p.Lk + kb - 1) / kb), cus = (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+    // a serving step of at least as many pairs as compute units is not split: the join's launch costs more than it levels
+    if ((rc = set_tiles(ctx, p, tiles, few && p.pairs >= cus ? 1 : choose_splits(ctx, tiles * p.pairs, blocks))) != SG_OK) return rc;
     sg_workspace space(ctx);
     if (p.splits > 1) {
         if ((rc = space.take((uint64_t)p.splits * total * (D + 2) * 4)) != SG_OK) return rc;
         p.part_o = (float *)space.p;
         p.part_ml = p.part_o + (uint64_t)p.splits * total * D;
     }
-    const bool vec_o = vec_rows(p.o), vec = vec_rows(p.q) && vec_rows(p.k) && vec_rows(p.v) && vec_o;
     const dim3 grid(p.tiles * p.pairs * p.splits);
-    SG_CROSS_ROWS(cross_forward_kernel, rw, vec, grid);
+#define SG_CROSS_FEW(D_, ROWS, UNROLL) hipLaunchKernelGGL((cross_few_kernel<D_, ROWS, UNROLL>), grid, dim3(256), 0, ctx->stream, p)
+    if (!few) SG_CROSS_ROWS(cross_forward_kernel, rw, grid);
+    else if (D == 64) {
+        if (p.R == 1) SG_CROSS_FEW(64, 1, 8);
+        else if (p.R == 2) SG_CROSS_FEW(64, 2, 8);
+        else if (p.R <= 4) SG_CROSS_FEW(64, 4, 4);
+        else SG_CROSS_FEW(64, 8, 4);
+    } else {
+        if (p.R == 1) SG_CROSS_FEW(32, 1, 4);
+        else if (p.R == 2) SG_CROSS_FEW(32, 2, 4);
+        else if (p.R <= 4) SG_CROSS_FEW(32, 4, 4);
+        else SG_CROSS_FEW(32, 8, 4);
+    }
+#undef SG_CROSS_FEW
     SG_CHECK_LAUNCH(ctx, "cross_attention");
     if (p.splits > 1) {
         const dim3 rows((unsigned)((total + 1024 / D - 1) / (1024 / D)));
-        if (D == 64) hipLaunchKernelGGL((cross_join_kernel<64>), rows, dim3(256), 0, ctx->stream, p, (int)vec_o);
-        else hipLaunchKernelGGL((cross_join_kernel<32>), rows, dim3(256), 0, ctx->stream, p, (int)vec_o);
+        if (D == 64) hipLaunchKernelGGL((cross_join_kernel<64>), rows, dim3(256), 0, ctx->stream, p);
+        else hipLaunchKernelGGL((cross_join_kernel<32>), rows, dim3(256), 0, ctx->stream, p);
         SG_CHECK_LAUNCH(ctx, "cross_attention join");
     }
     return SG_OK;
@@ -751,30 +885,26 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     p.delta = (float *)space.p;
     p.part_o = p.part_k = p.delta + delta_floats;
     p.part_v = p.part_k + key_splits * keys * D;
-    const bool vec_gq = vec_rows(p.gq), vec_gk = vec_rows(p.gk), vec_gv = vec_rows(p.gv);
-    const bool vec = vec_rows(p.q) && vec_rows(p.k) && vec_rows(p.v) && vec_rows(p.o) && vec_rows(p.go) && vec_gq && vec_gk && vec_gv;
-    auto sum = [&](const float *part, const Rows &to, uint64_t n, uint32_t splits, int heads, int length, bool v4) {
+    auto sum = [&](const float *part, const Rows &to, uint64_t n, uint32_t splits, int heads, int length) {
         const dim3 grid((unsigned)((n + 1024 / D - 1) / (1024 / D)));
-        if (D == 64) hipLaunchKernelGGL((cross_sum_kernel<64>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length, (int)v4);
-        else hipLaunchKernelGGL((cross_sum_kernel<32>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length, (int)v4);
+        if (D == 64) hipLaunchKernelGGL((cross_sum_kernel<64>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
+        else hipLaunchKernelGGL((cross_sum_kernel<32>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
     };
     if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
-    SG_CROSS_ROWS(cross_gq_kernel, rw, vec, dim3(p.tiles * p.pairs * p.splits));
+    SG_CROSS_ROWS(cross_gq_kernel, rw, dim3(p.tiles * p.pairs * p.splits));
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
     if (row_splits > 1) {
-        sum(p.part_o, p.gq, total, row_splits, p.H, p.Lq, vec_gq);
+        sum(p.part_o, p.gq, total, row_splits, p.H, p.Lq);
         SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries' sums");
     }
     if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
     const dim3 grid(p.tiles * p.pairs * p.splits);
-    if (D == 64 && vec) hipLaunchKernelGGL((cross_gkv_kernel<64, true>), grid, dim3(256), 0, ctx->stream, p);
-    else if (D == 64) hipLaunchKernelGGL((cross_gkv_kernel<64, false>), grid, dim3(256), 0, ctx->stream, p);
-    else if (vec) hipLaunchKernelGGL((cross_gkv_kernel<32, true>), grid, dim3(256), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((cross_gkv_kernel<32, false>), grid, dim3(256), 0, ctx->stream, p);
+    if (D == 64) hipLaunchKernelGGL((cross_gkv_kernel<64>), grid, dim3(256), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((cross_gkv_kernel<32>), grid, dim3(256), 0, ctx->stream, p);
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys and values");
     if (key_splits > 1) {
-        sum(p.part_k, p.gk, keys, key_splits, p.G, p.Lk, vec_gk);
-        sum(p.part_v, p.gv, keys, key_splits, p.G, p.Lk, vec_gv);
+        sum(p.part_k, p.gk, keys, key_splits, p.G, p.Lk);
+        sum(p.part_v, p.gv, keys, key_splits, p.G, p.Lk);
         SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys' sums");
     }
     return SG_OK;
