@@ -102,67 +102,82 @@ __device__ __forceinline__ void split_range(uint32_t blocks, uint32_t split, uin
     *last = *first + per + (split < rest ? 1u : 0u);
 }
 
-// Rows of D floats from memory to registers to LDS, KB rows a block, 256 threads.  Piece i of a thread: row (tid + 256 i) / ROWV.
-template <int D, int KB>
-struct Stage {
-    static constexpr int LD = D + 4;  // LDS row stride (floats): 8 consecutive rows cover all banks
-    static constexpr int ROWV = D / 4, N = KB * ROWV / 256;
-    f32x4 x[N];
-    __device__ static int row(int i) { return ((int)threadIdx.x + i * 256) / ROWV; }
-    __device__ static int col() { return ((int)threadIdx.x % ROWV) * 4; }
-    __device__ void deposit(float *lds) const {
-#pragma unroll
-        for (int i = 0; i < N; ++i) *reinterpret_cast<f32x4 *>(&lds[row(i) * LD + col()]) = x[i];
-    }
-    // rows of hidden keys become zeros: 0 * NaN is NaN
-    __device__ void hide(const uint64_t *seen) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (!(seen[row(i) / 64] >> (row(i) % 64) & 1)) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+// Tiles of rows in LDS.  Rows lie behind one another without a gap, as loads straight into LDS write them; the 16-byte pieces
+// of a row change places with the row's number, so that the 32 rows that a read takes a piece of lie in different banks.
+template <int D>
+struct Tile {
+    static constexpr int PIECES = D / 4;
+    __device__ static int turn(int row) { return D == 64 ? row & 15 : (row >> 1) & 7; }
+    __device__ static int at(int row, int piece) { return row * D + ((piece ^ turn(row)) << 2); }
 };
 
-// Which keys of a block are visible: requested with the block, turned into bits (the same in every wavefront) and an
-// addend of the scores when it is deposited.
+// Requests ROWS rows of an LDS tile; row_at(r) is where row r begins.  DMA: straight into LDS, 16 bytes a lane, there after
+// arrived(); needs 16-byte aligned rows.
+template <int D, int ROWS, bool DMA, class F>
+__device__ __forceinline__ void stage(float *tile, F row_at) {
+    constexpr int PIECES = Tile<D>::PIECES;
+#pragma unroll
+    for (int i = 0; i < ROWS * PIECES / 256; ++i) {
+        const int f = i * 256 + (int)threadIdx.x, row = f / PIECES, piece = (f % PIECES) ^ Tile<D>::turn(row);
+        const float *src = row_at(row) + piece * 4;
+        if (DMA) {
+            float *dst = tile + (i * 256 + __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63)) * 4;  // of the wavefront's first lane
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+        } else {
+            *reinterpret_cast<f32x4 *>(tile + f * 4) = load4(src);
+        }
+    }
+}
+// What this wavefront requested is in LDS (and in registers).
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Zeros in place of the rows whose bit is not set, by the threads that staged them: 0 * NaN is NaN.
+template <int D, int ROWS>
+__device__ __forceinline__ void clear_rows(float *tile, const uint32_t *seen) {
+    constexpr int PIECES = Tile<D>::PIECES;
+#pragma unroll
+    for (int i = 0; i < ROWS * PIECES / 256; ++i) {
+        const int f = i * 256 + (int)threadIdx.x, row = f / PIECES;
+        uint32_t word = seen[0];
+#pragma unroll
+        for (int k = 1; k < ROWS / 32; ++k) word = row / 32 == k ? seen[k] : word;
+        if (!(word >> (row % 32) & 1)) *reinterpret_cast<f32x4 *>(tile + f * 4) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+}
+
+// Which keys of a block are visible, as bits: requested with the block, the same in every wavefront.
 template <int KB>
 struct Visible {
-    float x[KB / 64];
-    __device__ void request(const float *mask, int j0, int Lk) {
+    static constexpr int N = (KB + 63) / 64;
+    float x[N];  // as loaded: nothing looks at it, and waits for it, before bits()
+    __device__ static int key(int i) { return i * 64 + ((int)threadIdx.x & (KB < 64 ? KB - 1 : 63)); }
+    // mask: any 32 readable floats where there is none
+    __device__ void request(const float *mask, bool is_mask, int j0, int Lk) {
 #pragma unroll
-        for (int i = 0; i < KB / 64; ++i) {
-            const int j = j0 + i * 64 + ((int)threadIdx.x & 63);
-            x[i] = j < Lk ? (mask ? mask[j] : 1.0f) : 0.0f;
-        }
+        for (int i = 0; i < N; ++i) x[i] = mask[is_mask ? min(j0 + key(i), Lk - 1) : key(i) & 31];
     }
-    template <class S>
-    __device__ void hide(S &k, S &v) const {
-        uint64_t seen[KB / 64];
+    __device__ bool bits(bool is_mask, int j0, int Lk, uint32_t *words) const {  // whether all are
         bool all = true;
 #pragma unroll
-        for (int i = 0; i < KB / 64; ++i) {
-            seen[i] = __builtin_amdgcn_ballot_w64(x[i] != 0.0f);
-            all = all && seen[i] == ~0ull;
+        for (int i = 0; i < N; ++i) {
+            const uint64_t b = __builtin_amdgcn_ballot_w64((!is_mask || x[i] != 0.0f) && j0 + key(i) < Lk);
+            words[KB < 64 ? 0 : 2 * i] = (uint32_t)b;
+            if (KB >= 64) words[2 * i + 1] = (uint32_t)(b >> 32);
+            all = all && b == ~0ull;
         }
-        if (all) return;
-        k.hide(seen);
-        v.hide(seen);
-    }
-    __device__ void deposit(float *lds_m) const {
-#pragma unroll
-        for (int i = 0; i < KB / 64; ++i)
-            if (threadIdx.x < 64) lds_m[i * 64 + threadIdx.x] = x[i] != 0.0f ? 0.0f : -__builtin_inff();
+        return all;
     }
 };
 
-// A wavefront's own 32 columns as the right operand: register [g][s] of lane (c, h) = x[c][8g + 4h + s].
+// A wavefront's own 32 columns as the right operand: register [g][s] of lane (c, h) = x[c][8g + 4h + s] * f.
 template <int D>
 struct Own {
     float x[D / 8][4];
-    __device__ void take(const float *lds, int c, int h) {  // row c of an LDS tile
+    __device__ void take(const float *tile, int row, int h, float f) {
 #pragma unroll
         for (int g = 0; g < D / 8; ++g) {
-            const f32x4 t = *reinterpret_cast<const f32x4 *>(&lds[c * (D + 4) + 8 * g + 4 * h]);
-            x[g][0] = t.x; x[g][1] = t.y; x[g][2] = t.z; x[g][3] = t.w;
+            const f32x4 t = *reinterpret_cast<const f32x4 *>(&tile[Tile<D>::at(row, 2 * g + h)]);
+            x[g][0] = t.x * f; x[g][1] = t.y * f; x[g][2] = t.z * f; x[g][3] = t.w * f;
         }
     }
 };
@@ -180,7 +195,7 @@ __device__ __forceinline__ floatx16 scores(const float *tile, const Own<D> &own,
     floatx16 acc = zero16();
 #pragma unroll
     for (int g = 0; g < D / 8; ++g) {
-        const f32x4 a = *reinterpret_cast<const f32x4 *>(&tile[c * (D + 4) + 8 * g + 4 * h]);
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(&tile[Tile<D>::at(c, 2 * g + h)]);
 #pragma unroll
         for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], own.x[g][s], acc, 0, 0, 0);
     }
@@ -197,7 +212,7 @@ __device__ __forceinline__ void accumulate(const float *tile, const floatx16 &w,
     for (int g = 0; g < 4; ++g) {
         vecND a[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) a[s] = *reinterpret_cast<const vecND *>(&tile[(8 * g + 4 * h + s) * (D + 4) + ND * c]);
+        for (int s = 0; s < 4; ++s) a[s] = *reinterpret_cast<const vecND *>(&tile[Tile<D>::at(8 * g + 4 * h + s, ND * c / 4) + ND * c % 4]);
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -221,80 +236,104 @@ __device__ __forceinline__ void write_column(float *row, const floatx16 *acc, fl
     }
 }
 
-// The 32 RW rows of a workgroup's tile, through the LDS of the key blocks, to the wavefronts that own them.
-template <int D, int RW, int KB>
-__device__ __forceinline__ void take_rows(const CrossP &p, const Rows &x, const Work &w, float *lds_a, float *lds_b, int own_row, int h, Own<D> &own) {
-    constexpr int ROWV = D / 4, LD = D + 4;
+// The 32 RW rows of a workgroup's tile, through LDS, to the wavefronts that own them.  (The two buffers are arrays of their
+// own everywhere: the compiler waits for a load into LDS in front of any read that it cannot tell from the load's target.)
+template <int D, int RW, bool DMA, int N>
+__device__ __forceinline__ void take_rows(const CrossP &p, const Rows &x, const Work &w, float (&lds0)[N], float (&lds1)[N], int own_row, int h, float f, Own<D> &own) {
+    constexpr int HALF = N / D < 32 * RW ? N / D : 32 * RW;  // rows that go through the first buffer
     __syncthreads();
+    // a row past the end repeats the last one; it is not written
+    stage<D, HALF, DMA>(lds0, [&](int r) { return x.p + row_at(p, x, w, min(w.tile * (32 * RW) + r, (uint32_t)p.R - 1)); });
+    if (HALF < 32 * RW) stage<D, HALF, DMA>(lds1, [&](int r) { return x.p + row_at(p, x, w, min(w.tile * (32 * RW) + HALF + r, (uint32_t)p.R - 1)); });
+    arrived();
+    __syncthreads();
+    if (own_row < HALF) own.take(lds0, own_row, h, f);
+    else own.take(lds1, own_row - HALF, h, f);
+}
+
+// Walks the visible blocks of KB keys, two LDS buffers in turn: while one is worked on, the next block is on its way into
+// the other, and there is one barrier a block.  work(keys' tile, values' tile, bits of this wavefront's 32 keys).
+template <int D, int KB, bool DMA, class F>
+__device__ __forceinline__ void walk_keys(const CrossP &p, const Work &w, float (&lds0)[2 * KB * D], float (&lds1)[2 * KB * D], uint32_t first, uint32_t last, int kw,
+                                          F work) {
+    const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
+    const bool is_mask = p.mask != nullptr;
+    const float *mask = is_mask ? p.mask + w.b * p.mask_b : K;
+    Visible<KB> next;
+    auto request = [&](uint32_t blk, float *to) {
+        const int j0 = (int)blk * KB;
+        stage<D, KB, DMA>(to, [&](int r) { return K + (int64_t)min(j0 + r, p.Lk - 1) * p.k.l; });
+        stage<D, KB, DMA>(to + KB * D, [&](int r) { return V + (int64_t)min(j0 + r, p.Lk - 1) * p.v.l; });
+        next.request(mask, is_mask, j0, p.Lk);
+    };
+    auto step = [&](uint32_t blk, float *tile, float *other) {
+        arrived();
+        uint32_t seen[(KB + 31) / 32];
+        if (!next.bits(is_mask, (int)blk * KB, p.Lk, seen)) {
+            clear_rows<D, KB>(tile, seen);
+            clear_rows<D, KB>(tile + KB * D, seen);
+        }
+        __syncthreads();
+        if (blk + 1 < last) request(blk + 1, other);
+        uint32_t mine = seen[0];
 #pragma unroll
-    for (int i = 0; i < 32 * RW * ROWV / 256; ++i) {
-        const int f = threadIdx.x + i * 256, row = f / ROWV, c = (f % ROWV) * 4;
-        const uint32_t r = min(w.tile * (32 * RW) + row, (uint32_t)p.R - 1);  // a row past the end repeats the last one; it is not written
-        *reinterpret_cast<f32x4 *>(&(row < KB ? lds_a : lds_b)[(row % KB) * LD + c]) = load4(x.p + row_at(p, x, w, r) + c);
-    }
+        for (int k = 1; k < KB / 32; ++k) mine = kw == k * 32 ? seen[k] : mine;
+        work(tile + kw * D, tile + (KB + kw) * D, (uint32_t)__builtin_amdgcn_readfirstlane((int)mine));
+    };
     __syncthreads();
-    own.take(&(own_row < KB ? lds_a : lds_b)[(own_row - own_row % 32) % KB * LD], own_row % 32, h);
+    if (first < last) request(first, lds0);
+    for (uint32_t blk = first; blk < last; blk += 2) {
+        step(blk, lds0, lds1);
+        if (blk + 1 < last) step(blk + 1, lds1, lds0);
+    }
+}
+
+// Merges accumulators through LDS: wavefronts RW and up hand theirs over, the first RW call join(slot) for each.
+template <int RW, int SLOT, class G, class J>
+__device__ __forceinline__ bool merge_waves(float *lds, int wave, int lane, G give, J join) {
+    constexpr int KW = 4 / RW;
+    if (KW == 1) return true;
+    __syncthreads();
+    if (wave >= RW) give(&lds[((wave - RW) * 64 + lane) * SLOT]);
+    __syncthreads();
+    if (wave >= RW) return false;
+#pragma unroll
+    for (int o = 1; o < KW; ++o) join(&lds[((o - 1) * RW * 64 + wave * 64 + lane) * SLOT]);
+    return true;
 }
 
 // ---- forward.  RW wavefronts take the workgroup's 32 RW rows, the 4 / RW times as many share each block's keys and are
 // merged through LDS at the end.
-template <int D, int RW>
+template <int D, int RW, bool DMA>
 __global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
-    constexpr int KW = 4 / RW, KB = RW == 1 ? 128 : 64, NKB = KB / KW / 32, LD = D + 4, ND = D / 32;
-    __shared__ __attribute__((aligned(16))) float lds_k[KB * LD], lds_v[KB * LD], lds_m[KB];
+    constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND + 2;
+    __shared__ __attribute__((aligned(16))) float lds0[2 * KB * D], lds1[2 * KB * D];  // two buffers of keys and values
+    __shared__ int lds_end[4];
+    static_assert(32 * RW <= 4 * KB && (KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "rows and the merge fit in the buffers");
     const Work w = find_work(p);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int own_row = (wave % RW) * 32 + c, kw = wave / RW * (KB / KW);
-    const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
-    const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
-    const int end = visible_end(p, w.b, reinterpret_cast<int *>(lds_m));
+    const int own_row = (wave % RW) * 32 + c;
+    const int end = visible_end(p, w.b, lds_end);
     const float inf = __builtin_inff();
-
-    Own<D> q;
-    take_rows<D, RW, KB>(p, p.q, w, lds_k, lds_v, own_row, h, q);
+    Own<D> q;  // scaled: scores are logarithms to base 2
+    take_rows<D, RW, DMA>(p, p.q, w, lds0, lds1, own_row, h, p.scale * LOG2E, q);
     floatx16 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = zero16();
     float m_run = -inf, l_run = 0.0f;
-    const float c2 = p.scale * LOG2E;
-
-    Stage<D, KB> ks, vs;
-    Visible<KB> seen;
-    auto request = [&](int j0) {
-#pragma unroll
-        for (int i = 0; i < ks.N; ++i) {
-            const int64_t j = min(j0 + ks.row(i), p.Lk - 1);
-            ks.x[i] = load4(K + j * p.k.l + ks.col());
-            vs.x[i] = load4(V + j * p.v.l + vs.col());
-        }
-        seen.request(mask, j0, p.Lk);
-    };
     uint32_t first, last;
     split_range((end + KB - 1) / KB, w.split, p.splits, &first, &last);
-    if (first < last) request(first * KB);
-    for (uint32_t blk = first; blk < last; ++blk) {
-        seen.hide(ks, vs);
-        __syncthreads();
-        ks.deposit(lds_k);
-        vs.deposit(lds_v);
-        seen.deposit(lds_m);
-        __syncthreads();
-        if (blk + 1 < last) request((blk + 1) * KB);
-        floatx16 s[NKB];
+    walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&](const float *kt, const float *vt, uint32_t seen) {
+        floatx16 s = scores<D>(kt, q, c, h);
+        if (seen != ~0u) {
+            const uint32_t mine = seen >> (4 * h);
 #pragma unroll
-        for (int b = 0; b < NKB; ++b) s[b] = scores<D>(&lds_k[(kw + b * 32) * LD], q, c, h);
-        float top = -inf;
+            for (int r = 0; r < 16; ++r)
+                if (!(mine >> (8 * (r / 4) + r % 4) & 1)) s[r] = -inf;
+        }
+        float top = s[0];
 #pragma unroll
-        for (int b = 0; b < NKB; ++b)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 mk = *reinterpret_cast<const f32x4 *>(&lds_m[kw + b * 32 + 8 * g + 4 * h]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[b][4 * g + i] = __builtin_fmaf(s[b][4 * g + i], c2, mk[i]);
-                    top = fmaxf(top, s[b][4 * g + i]);
-                }
-            }
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float m_new = fmaxf(m_run, top);
         const float shift = m_new == -inf ? 0.0f : m_new;  // nothing visible so far: every exponential below is 0
@@ -308,46 +347,32 @@ __global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
         }
         m_run = m_new;
 #pragma unroll
-        for (int b = 0; b < NKB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - shift);
-                l_run += s[b][r];
-            }
-#pragma unroll
-        for (int b = 0; b < NKB; ++b) accumulate<D>(&lds_v[(kw + b * 32) * LD], s[b], acc, c, h);
-    }
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(s[r] - shift);
+            l_run += s[r];
+        }
+        accumulate<D>(vt, s, acc, c, h);
+    });
     l_run += __shfl_xor(l_run, 32, 64);
-    if (KW > 1) {
-        constexpr int SLOT = 16 * ND + 2;  // floats of a lane
-        static_assert((KW - 1) * RW * 64 * SLOT <= KB * LD, "the merge fits in the keys' LDS");
-        __syncthreads();
-        if (wave >= RW) {
-            float *to = &lds_k[((wave - RW) * 64 + lane) * SLOT];
+    const bool writes = merge_waves<RW, SLOT>(lds0, wave, lane, [&](float *to) {
 #pragma unroll
-            for (int j = 0; j < ND; ++j)
+        for (int j = 0; j < ND; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) to[16 * j + r] = acc[j][r];
-            to[16 * ND] = m_run;
-            to[16 * ND + 1] = l_run;
-        }
-        __syncthreads();
-        if (wave >= RW) return;
+            for (int r = 0; r < 16; ++r) to[16 * j + r] = acc[j][r];
+        to[16 * ND] = m_run;
+        to[16 * ND + 1] = l_run;
+    }, [&](const float *from) {
+        const float mo = from[16 * ND], m = fmaxf(m_run, mo), shift = m == -inf ? 0.0f : m;
+        const float fa = __builtin_amdgcn_exp2f(m_run - shift), fb = __builtin_amdgcn_exp2f(mo - shift);
+        l_run = l_run * fa + from[16 * ND + 1] * fb;
+        m_run = m;
 #pragma unroll
-        for (int o = 1; o < KW; ++o) {
-            const float *from = &lds_k[((o - 1) * RW * 64 + wave * 64 + lane) * SLOT];
-            const float mo = from[16 * ND], m = fmaxf(m_run, mo), shift = m == -inf ? 0.0f : m;
-            const float fa = __builtin_amdgcn_exp2f(m_run - shift), fb = __builtin_amdgcn_exp2f(mo - shift);
-            l_run = l_run * fa + from[16 * ND + 1] * fb;
-            m_run = m;
+        for (int j = 0; j < ND; ++j)
 #pragma unroll
-            for (int j = 0; j < ND; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[j][r] = acc[j][r] * fa + from[16 * j + r] * fb;
-        }
-    }
+            for (int r = 0; r < 16; ++r) acc[j][r] = acc[j][r] * fa + from[16 * j + r] * fb;
+    });
     const uint32_t r = w.tile * (32 * RW) + own_row;
-    if (r >= (uint32_t)p.R) return;
+    if (!writes || r >= (uint32_t)p.R) return;
     const int64_t row = (int64_t)w.pair * p.R + r;
     if (p.splits > 1) {
         const int64_t at = (int64_t)w.split * p.pairs * p.R + row;
@@ -511,180 +536,134 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p) {
 }
 
 // ---- gradient of the queries (and delta, for the other kernel)
-template <int D, int RW>
+template <int D, int RW, bool DMA>
 __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
-    constexpr int KW = 4 / RW, KB = RW == 1 ? 128 : 64, NKB = KB / KW / 32, LD = D + 4, ND = D / 32;
-    __shared__ __attribute__((aligned(16))) float lds_k[KB * LD], lds_v[KB * LD], lds_m[KB];
+    constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND;
+    __shared__ __attribute__((aligned(16))) float lds0[2 * KB * D], lds1[2 * KB * D];
+    __shared__ int lds_end[4];
+    static_assert(32 * RW <= 4 * KB && (KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "rows and the merge fit in the buffers");
     const Work w = find_work(p);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int own_row = (wave % RW) * 32 + c, kw = wave / RW * (KB / KW);
-    const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
-    const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
-    const int end = visible_end(p, w.b, reinterpret_cast<int *>(lds_m));
+    const int own_row = (wave % RW) * 32 + c;
+    const int end = visible_end(p, w.b, lds_end);
     const uint32_t r = w.tile * (32 * RW) + own_row;
     const int64_t row = (int64_t)w.pair * p.R + min(r, (uint32_t)p.R - 1);
-
     Own<D> q, go;
     float delta = 0.0f;
-    take_rows<D, RW, KB>(p, p.o, w, lds_k, lds_v, own_row, h, q);
-    take_rows<D, RW, KB>(p, p.go, w, lds_k, lds_v, own_row, h, go);
+    take_rows<D, RW, DMA>(p, p.o, w, lds0, lds1, own_row, h, 1.0f, q);
+    take_rows<D, RW, DMA>(p, p.go, w, lds0, lds1, own_row, h, 1.0f, go);
 #pragma unroll
     for (int g = 0; g < D / 8; ++g)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) delta += q.x[g][s] * go.x[g][s];
+        for (int i = 0; i < 4; ++i) delta += q.x[g][i] * go.x[g][i];
     delta += __shfl_xor(delta, 32, 64);
     if (w.split == 0 && wave < RW && h == 0 && r < (uint32_t)p.R) p.delta[row] = delta;
-    take_rows<D, RW, KB>(p, p.q, w, lds_k, lds_v, own_row, h, q);
-    const float lse2 = p.lse[row] * LOG2E, c2 = p.scale * LOG2E;
+    take_rows<D, RW, DMA>(p, p.q, w, lds0, lds1, own_row, h, p.scale * LOG2E, q);
+    const float lse2 = p.lse[row] * LOG2E;
     floatx16 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = zero16();
-
-    Stage<D, KB> ks, vs;
-    Visible<KB> seen;
-    auto request = [&](int j0) {
-#pragma unroll
-        for (int i = 0; i < ks.N; ++i) {
-            const int64_t j = min(j0 + ks.row(i), p.Lk - 1);
-            ks.x[i] = load4(K + j * p.k.l + ks.col());
-            vs.x[i] = load4(V + j * p.v.l + vs.col());
-        }
-        seen.request(mask, j0, p.Lk);
-    };
     uint32_t first, last;
     split_range((end + KB - 1) / KB, w.split, p.splits, &first, &last);
-    if (first < last) request(first * KB);
-    for (uint32_t blk = first; blk < last; ++blk) {
-        seen.hide(ks, vs);
-        __syncthreads();
-        ks.deposit(lds_k);
-        vs.deposit(lds_v);
-        seen.deposit(lds_m);
-        __syncthreads();
-        if (blk + 1 < last) request((blk + 1) * KB);
+    walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&](const float *kt, const float *vt, uint32_t seen) {
+        floatx16 s = scores<D>(kt, q, c, h);
+        const floatx16 dp = scores<D>(vt, go, c, h);
 #pragma unroll
-        for (int b = 0; b < NKB; ++b) {
-            const int at = kw + b * 32;
-            floatx16 s = scores<D>(&lds_k[at * LD], q, c, h);
-            const floatx16 dp = scores<D>(&lds_v[at * LD], go, c, h);
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - lse2) * (dp[i] - delta);
+        if (seen != ~0u) {
+            const uint32_t mine = seen >> (4 * h);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 mk = *reinterpret_cast<const f32x4 *>(&lds_m[at + 8 * g + 4 * h]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c2, mk[i]) - lse2);
-                    s[4 * g + i] = e * (dp[4 * g + i] - delta);
-                }
-            }
-            accumulate<D>(&lds_k[at * LD], s, acc, c, h);
+            for (int i = 0; i < 16; ++i)
+                if (!(mine >> (8 * (i / 4) + i % 4) & 1)) s[i] = 0.0f;
         }
-    }
-    if (KW > 1) {
-        constexpr int SLOT = 16 * ND + 2;
-        static_assert((KW - 1) * RW * 64 * SLOT <= KB * LD, "the merge fits in the keys' LDS");
-        __syncthreads();
-        if (wave >= RW) {
-            float *to = &lds_k[((wave - RW) * 64 + lane) * SLOT];
+        accumulate<D>(kt, s, acc, c, h);
+    });
+    const bool writes = merge_waves<RW, SLOT>(lds0, wave, lane, [&](float *to) {
 #pragma unroll
-            for (int j = 0; j < ND; ++j)
+        for (int j = 0; j < ND; ++j)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) to[16 * j + i] = acc[j][i];
-        }
-        __syncthreads();
-        if (wave >= RW) return;
+            for (int i = 0; i < 16; ++i) to[16 * j + i] = acc[j][i];
+    }, [&](const float *from) {
 #pragma unroll
-        for (int o = 1; o < KW; ++o) {
-            const float *from = &lds_k[((o - 1) * RW * 64 + wave * 64 + lane) * SLOT];
+        for (int j = 0; j < ND; ++j)
 #pragma unroll
-            for (int j = 0; j < ND; ++j)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[j][i] += from[16 * j + i];
-        }
-    }
-    if (r >= (uint32_t)p.R) return;
+            for (int i = 0; i < 16; ++i) acc[j][i] += from[16 * j + i];
+    });
+    if (!writes || r >= (uint32_t)p.R) return;
     if (p.splits > 1) write_column<D>(p.part_o + ((int64_t)w.split * p.pairs * p.R + row) * D, acc, p.scale, h);
     else write_column<D>(const_cast<float *>(p.gq.p) + row_at(p, p.gq, w, r), acc, p.scale, h);
 }
 
-// ---- gradients of keys and values: a wavefront owns 32 keys and walks all rows of the pair.
-template <int D>
-__global__ void __launch_bounds__(256) cross_gkv_kernel(const CrossP p) {
-    constexpr int RB = 64, LD = D + 4, ND = D / 32, ROWV = D / 4;
-    __shared__ __attribute__((aligned(16))) float lds_q[RB * LD], lds_go[RB * LD], lds_lse[RB], lds_delta[RB];
+// ---- gradients of keys and values: a wavefront owns 32 keys and walks all rows of the pair, 32 at a time.
+template <int D, bool DMA>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) cross_gkv_kernel(const CrossP p) {
+    constexpr int RB = 32, ND = D / 32;
+    __shared__ __attribute__((aligned(16))) float lds0[2 * RB * D], lds1[2 * RB * D];  // two buffers of rows of Q and dO
+    __shared__ __attribute__((aligned(16))) float rows0[2 * RB], rows1[2 * RB];        // their lse and delta
     const Work w = find_work(p);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int j = (int)w.tile * 128 + wave * 32 + c;
+    const int j0 = (int)w.tile * 128, j = j0 + wave * 32 + c;
     const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
-    const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
-    const bool seen = j < p.Lk && (!mask || mask[j] != 0.0f);
+    const bool seen = j < p.Lk && (!p.mask || p.mask[w.b * p.mask_b + j] != 0.0f);
     const float inf = __builtin_inff();
-
-    Own<D> k, v;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {  // two wavefronts' keys at a time go through the rows' LDS
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < RB * ROWV / 256; ++i) {
-            const int f = tid + i * 256, row = f / ROWV, col = (f % ROWV) * 4;
-            const int64_t jj = min((int)w.tile * 128 + half * 64 + row, p.Lk - 1);
-            *reinterpret_cast<f32x4 *>(&lds_q[row * LD + col]) = load4(K + jj * p.k.l + col);
-            *reinterpret_cast<f32x4 *>(&lds_go[row * LD + col]) = load4(V + jj * p.v.l + col);
-        }
-        __syncthreads();
-        if (wave / 2 == half) {
-            k.take(&lds_q[(wave & 1) * 32 * LD], c, h);
-            v.take(&lds_go[(wave & 1) * 32 * LD], c, h);
-        }
-    }
-    const bool any = __syncthreads_or(seen);
     floatx16 gk[ND], gv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) gk[d] = gv[d] = zero16();
-    const float c2 = p.scale * LOG2E;
-
-    Stage<D, RB> qs, gs;
-    float lreg = 0.0f, dreg = 0.0f;
-    auto request = [&](uint32_t r0) {
-#pragma unroll
-        for (int i = 0; i < qs.N; ++i) {
-            const uint32_t r = min(r0 + qs.row(i), (uint32_t)p.R - 1);
-            qs.x[i] = load4(p.q.p + row_at(p, p.q, w, r) + qs.col());
-            gs.x[i] = load4(p.go.p + row_at(p, p.go, w, r) + gs.col());
-        }
-        if (tid < RB) {
-            const uint32_t r = r0 + tid;
-            lreg = r < (uint32_t)p.R ? p.lse[(int64_t)w.pair * p.R + r] * LOG2E : inf;  // a row past the end: every exponential is 0
-            dreg = r < (uint32_t)p.R ? p.delta[(int64_t)w.pair * p.R + r] : 0.0f;
-        }
-    };
-    uint32_t first, last;
-    split_range((p.R + RB - 1) / RB, w.split, p.splits, &first, &last);
-    if (!any) last = first;
-    if (first < last) request(first * RB);
-    for (uint32_t blk = first; blk < last; ++blk) {
-        __syncthreads();
-        qs.deposit(lds_q);
-        gs.deposit(lds_go);
-        if (tid < RB) { lds_lse[tid] = lreg; lds_delta[tid] = dreg; }
-        __syncthreads();
-        if (blk + 1 < last) request((blk + 1) * RB);
-#pragma unroll
-        for (int b = 0; b < RB / 32; ++b) {
-            floatx16 s = scores<D>(&lds_q[b * 32 * LD], k, c, h);
-            floatx16 dp = scores<D>(&lds_go[b * 32 * LD], v, c, h);
+    if (__syncthreads_or(seen)) {
+        Own<D> k, v;  // k scaled: scores are logarithms to base 2
+        auto take = [&](const float *x, int64_t l, float f, Own<D> &own) {
+            __syncthreads();
+            stage<D, 64, DMA>(lds0, [&](int r) { return x + (int64_t)min(j0 + r, p.Lk - 1) * l; });
+            stage<D, 64, DMA>(lds1, [&](int r) { return x + (int64_t)min(j0 + 64 + r, p.Lk - 1) * l; });
+            arrived();
+            __syncthreads();
+            if (wave < 2) own.take(lds0, wave * 32 + c, h, f);
+            else own.take(lds1, (wave - 2) * 32 + c, h, f);
+        };
+        take(K, p.k.l, p.scale * LOG2E, k);
+        take(V, p.v.l, 1.0f, v);
+        float lreg = 0.0f, dreg = 0.0f;
+        auto request = [&](uint32_t blk, float *to) {
+            auto at = [&](int r) { return min(blk * RB + r, (uint32_t)p.R - 1); };
+            stage<D, RB, DMA>(to, [&](int r) { return p.q.p + row_at(p, p.q, w, at(r)); });
+            stage<D, RB, DMA>(to + RB * D, [&](int r) { return p.go.p + row_at(p, p.go, w, at(r)); });
+            if (tid < RB) {
+                const uint32_t r = blk * RB + tid;
+                lreg = r < (uint32_t)p.R ? p.lse[(int64_t)w.pair * p.R + r] : inf;  // a row past the end: every exponential is 0
+                dreg = r < (uint32_t)p.R ? p.delta[(int64_t)w.pair * p.R + r] : 0.0f;
+            }
+        };
+        uint32_t first, last;
+        split_range((p.R + RB - 1) / RB, w.split, p.splits, &first, &last);
+        // a wavefront none of whose keys is visible only helps to stage
+        const bool works = __builtin_amdgcn_ballot_w64(seen) != 0;
+        auto step = [&](uint32_t blk, float *tile, float *rows, float *other) {
+            if (tid < RB) { rows[tid] = lreg * LOG2E; rows[RB + tid] = dreg; }
+            arrived();
+            __syncthreads();
+            if (blk + 1 < last) request(blk + 1, other);
+            if (!works) return;
+            const float *qt = tile, *gt = tile + RB * D;
+            floatx16 s = scores<D>(qt, k, c, h);
+            floatx16 dp = scores<D>(gt, v, c, h);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 ls = *reinterpret_cast<const f32x4 *>(&lds_lse[b * 32 + 8 * g + 4 * h]);
-                const f32x4 dl = *reinterpret_cast<const f32x4 *>(&lds_delta[b * 32 + 8 * g + 4 * h]);
+                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&rows[8 * g + 4 * h]), d4 = *reinterpret_cast<const f32x4 *>(&rows[RB + 8 * g + 4 * h]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + i], c2, -ls[i]));
+                    const float e = __builtin_amdgcn_exp2f(s[4 * g + i] - l4[i]);
                     s[4 * g + i] = e;
-                    dp[4 * g + i] = e * (dp[4 * g + i] - dl[i]);
+                    dp[4 * g + i] = e * (dp[4 * g + i] - d4[i]);
                 }
             }
-            accumulate<D>(&lds_go[b * 32 * LD], s, gv, c, h);
-            accumulate<D>(&lds_q[b * 32 * LD], dp, gk, c, h);
+            accumulate<D>(gt, s, gv, c, h);
+            accumulate<D>(qt, dp, gk, c, h);
+        };
+        __syncthreads();
+        if (first < last) request(first, lds0);
+        for (uint32_t blk = first; blk < last; blk += 2) {
+            step(blk, lds0, rows0, lds1);
+            if (blk + 1 < last) step(blk + 1, lds1, rows1, lds0);
         }
     }
     if (j >= p.Lk) return;
@@ -778,6 +757,9 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
     return SG_OK;
 }
 
+// 16-byte aligned rows: loads straight into LDS take them.
+bool aligned_rows(const Rows &r) { return ((uintptr_t)r.p) % 16 == 0 && r.b % 4 == 0 && r.h % 4 == 0 && r.l % 4 == 0; }
+
 // Splits of a long axis of `blocks` blocks that bring `units` workgroups to two for each compute unit.
 uint32_t choose_splits(const sg_ctx *ctx, uint32_t units, uint32_t blocks) {
     const uint32_t want = 2u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
@@ -798,14 +780,18 @@ int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
 
 }  // namespace
 
-#define SG_CROSS_ROWS(KERNEL, RW, GRID)                                                                                 \
+#define SG_CROSS_ROWS_(KERNEL, D_, RW, DMA, GRID)                                                                       \
     do {                                                                                                                \
-        if (D == 64 && RW == 4) hipLaunchKernelGGL((KERNEL<64, 4>), GRID, dim3(256), 0, ctx->stream, p);                \
-        else if (D == 64 && RW == 2) hipLaunchKernelGGL((KERNEL<64, 2>), GRID, dim3(256), 0, ctx->stream, p);           \
-        else if (D == 64) hipLaunchKernelGGL((KERNEL<64, 1>), GRID, dim3(256), 0, ctx->stream, p);                      \
-        else if (RW == 4) hipLaunchKernelGGL((KERNEL<32, 4>), GRID, dim3(256), 0, ctx->stream, p);                      \
-        else if (RW == 2) hipLaunchKernelGGL((KERNEL<32, 2>), GRID, dim3(256), 0, ctx->stream, p);                      \
-        else hipLaunchKernelGGL((KERNEL<32, 1>), GRID, dim3(256), 0, ctx->stream, p);                                   \
+        if (RW == 4) hipLaunchKernelGGL((KERNEL<D_, 4, DMA>), GRID, dim3(256), 0, ctx->stream, p);                      \
+        else if (RW == 2) hipLaunchKernelGGL((KERNEL<D_, 2, DMA>), GRID, dim3(256), 0, ctx->stream, p);                 \
+        else hipLaunchKernelGGL((KERNEL<D_, 1, DMA>), GRID, dim3(256), 0, ctx->stream, p);                              \
+    } while (0)
+#define SG_CROSS_ROWS(KERNEL, RW, DMA, GRID)                                                                            \
+    do {                                                                                                                \
+        if (D == 64 && DMA) SG_CROSS_ROWS_(KERNEL, 64, RW, true, GRID);                                                 \
+        else if (D == 64) SG_CROSS_ROWS_(KERNEL, 64, RW, false, GRID);                                                  \
+        else if (DMA) SG_CROSS_ROWS_(KERNEL, 32, RW, true, GRID);                                                       \
+        else SG_CROSS_ROWS_(KERNEL, 32, RW, false, GRID);                                                               \
     } while (0)
 
 extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask, float scale,
@@ -818,7 +804,7 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
     sg_device_guard guard(ctx);
     const int64_t D = q->extents[3];
     const bool few = p.R <= 8;
-    const int rw = row_waves(p.R), kb = rw == 1 ? 128 : 64;
+    const int rw = row_waves(p.R), kb = 128 / rw;
     const uint32_t tiles = few ? 1 : (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), total = p.pairs * (uint32_t)p.R;
     const uint32_t blocks = (uint32_t)((p.Lk + kb - 1) / kb), cus = (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
     // a serving step of at least as many pairs as compute units is not split: the join's launch costs more than it levels
@@ -831,7 +817,8 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
     }
     const dim3 grid(p.tiles * p.pairs * p.splits);
 #define SG_CROSS_FEW(D_, ROWS, UNROLL) hipLaunchKernelGGL((cross_few_kernel<D_, ROWS, UNROLL>), grid, dim3(256), 0, ctx->stream, p)
-    if (!few) SG_CROSS_ROWS(cross_forward_kernel, rw, grid);
+    const bool dma = aligned_rows(p.q) && aligned_rows(p.k) && aligned_rows(p.v);
+    if (!few) SG_CROSS_ROWS(cross_forward_kernel, rw, dma, grid);
     else if (D == 64) {
         if (p.R == 1) SG_CROSS_FEW(64, 1, 8);
         else if (p.R == 2) SG_CROSS_FEW(64, 2, 8);
@@ -873,10 +860,10 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     p.scale = scale;
     sg_device_guard guard(ctx);
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
-    const int rw = row_waves(p.R), kb = rw == 1 ? 128 : 64;
+    const int rw = row_waves(p.R), kb = 128 / rw;
     const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 127) / 128);
     const uint32_t row_splits = choose_splits(ctx, row_tiles * p.pairs, (uint32_t)((p.Lk + kb - 1) / kb));
-    const uint32_t key_splits = choose_splits(ctx, key_tiles * p.pairs, (uint32_t)((p.R + 63) / 64));
+    const uint32_t key_splits = choose_splits(ctx, key_tiles * p.pairs, (uint32_t)((p.R + 31) / 32));
     // delta, and the larger of the two kernels' split sums: they run one after the other
     const uint64_t rows_part = row_splits > 1 ? row_splits * total * D : 0, keys_part = key_splits > 1 ? 2 * key_splits * keys * D : 0;
     const uint64_t delta_floats = (total + 3) / 4 * 4;
@@ -891,7 +878,8 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
         else hipLaunchKernelGGL((cross_sum_kernel<32>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
     };
     if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
-    SG_CROSS_ROWS(cross_gq_kernel, rw, dim3(p.tiles * p.pairs * p.splits));
+    const bool dma = aligned_rows(p.q) && aligned_rows(p.k) && aligned_rows(p.v) && aligned_rows(p.o) && aligned_rows(p.go);
+    SG_CROSS_ROWS(cross_gq_kernel, rw, dma, dim3(p.tiles * p.pairs * p.splits));
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
     if (row_splits > 1) {
         sum(p.part_o, p.gq, total, row_splits, p.H, p.Lq);
@@ -899,8 +887,10 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     }
     if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
     const dim3 grid(p.tiles * p.pairs * p.splits);
-    if (D == 64) hipLaunchKernelGGL((cross_gkv_kernel<64>), grid, dim3(256), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((cross_gkv_kernel<32>), grid, dim3(256), 0, ctx->stream, p);
+    if (D == 64 && dma) hipLaunchKernelGGL((cross_gkv_kernel<64, true>), grid, dim3(256), 0, ctx->stream, p);
+    else if (D == 64) hipLaunchKernelGGL((cross_gkv_kernel<64, false>), grid, dim3(256), 0, ctx->stream, p);
+    else if (dma) hipLaunchKernelGGL((cross_gkv_kernel<32, true>), grid, dim3(256), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((cross_gkv_kernel<32, false>), grid, dim3(256), 0, ctx->stream, p);
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys and values");
     if (key_splits > 1) {
         sum(p.part_k, p.gk, keys, key_splits, p.G, p.Lk);
