@@ -31,53 +31,19 @@ struct Rows {  // [N, heads, length, D] operand
 struct CrossP {
     Rows q, k, v, o, go, gq, gk, gv;  // o: written by the forward call, read by the gradient
     const float *mask;
+    int *ends;                // of each sequence, one behind its last visible key; NULL: the workgroups look for themselves
     float *lse, *delta;
     float *part_o, *part_ml;  // of split sums: [split][row][D], [split][row][2]
     float *part_k, *part_v;   // [split][key][D]
     int N, H, G, Lq, Lk, R;   // R = H / G * Lq: rows of a (batch, key head) pair
     int64_t mask_b;
+    int strided;  // a pair's rows of q and gout lie a stride apart
     float scale;
     uint32_t tiles, pairs, splits;
     sg_fastdiv d_lq, d_tiles, d_pairs, d_g;
 };
 
 __device__ __forceinline__ uint32_t fdiv(uint32_t n, sg_fastdiv d) { return (__umulhi(n, d.magic) + n) >> d.shift; }
-
-struct Work {
-    uint32_t split, pair, tile;
-    int b, g;
-};
-// Workgroup ids go round-robin over the 8 XCDs.  All tiles of a (split, pair), which share keys or rows, go to one of them,
-// and the pairs of a sequence, whose length they have in common, to different ones.
-__device__ __forceinline__ Work find_work(const CrossP &p) {
-    Work w;
-    const uint32_t units = p.pairs * p.splits, even = units & ~7u;
-    uint32_t id = blockIdx.x, unit;
-    if (id < even * p.tiles) {
-        const uint32_t q = fdiv(id >> 3, p.d_tiles);
-        w.tile = (id >> 3) - q * p.tiles;
-        unit = q * 8 + (id & 7);
-    } else {
-        id -= even * p.tiles;
-        const uint32_t q = fdiv(id, p.d_tiles);
-        w.tile = id - q * p.tiles;
-        unit = even + q;
-    }
-    w.split = fdiv(unit, p.d_pairs);
-    w.pair = unit - w.split * p.pairs;
-    w.b = (int)fdiv(w.pair, p.d_g);
-    w.g = (int)w.pair - w.b * p.G;
-    return w;
-}
-
-// Element offset of row r of a pair.
-__device__ __forceinline__ int64_t row_at(const CrossP &p, const Rows &x, const Work &w, uint32_t r) {
-    const uint32_t hh = fdiv(r, p.d_lq);
-    return w.b * x.b + (int64_t)(w.g * (p.H / p.G) + (int)hh) * x.h + (int64_t)(r - hh * p.Lq) * x.l;
-}
-
-__device__ __forceinline__ f32x4 load4(const float *p) { return *reinterpret_cast<const f32x4_any *>(p); }
-__device__ __forceinline__ void store4(float *p, f32x4 v) { *reinterpret_cast<f32x4_any *>(p) = v; }
 
 // One behind the last visible key of a sequence: a padded batch costs what its lengths cost.
 __device__ __forceinline__ int visible_end(const CrossP &p, int b, int *lds) {
@@ -95,6 +61,71 @@ __device__ __forceinline__ int visible_end(const CrossP &p, int b, int *lds) {
     return __builtin_amdgcn_readfirstlane(end);
 }
 
+__global__ void __launch_bounds__(256) cross_ends_kernel(const CrossP p) {
+    __shared__ int lds[4];
+    const int end = visible_end(p, blockIdx.x, lds);
+    if (threadIdx.x == 0) p.ends[blockIdx.x] = end;
+}
+
+struct Work {
+    uint32_t split, pair, tile;
+    int b, g, end;
+};
+// Workgroup ids go round-robin over the 8 XCDs.  All tiles of a (split, pair), which share keys or rows, go to one of them,
+// and the pairs of a sequence, whose length they have in common, to different ones.  Where the lengths are known in front
+// (ends), the longest sequences come first: a launch ends when its last workgroup does, and short ones fill the gaps
+// (32 x 12 heads of 512 x 512 with lengths 512 to 272: a tenth of the time).  lds: 4 words.
+__device__ __forceinline__ Work find_work(const CrossP &p, int *lds) {
+    Work w;
+    const uint32_t units = p.pairs * p.splits, even = units & ~7u;
+    uint32_t id = blockIdx.x, unit, q;
+    if (id < even * p.tiles) {
+        q = fdiv(id >> 3, p.d_tiles);
+        w.tile = (id >> 3) - q * p.tiles;
+        unit = q * 8 + (id & 7);
+    } else {
+        id -= even * p.tiles;
+        q = fdiv(id, p.d_tiles);
+        w.tile = id - q * p.tiles;
+        unit = even + q;
+    }
+    // every unit begins with another tile: the workgroups of an XCD go round its shader engines, and tiles behind the last
+    // visible key, which are done at once, would all go to the same ones
+    w.tile += q - fdiv(q, p.d_tiles) * p.tiles;
+    if (w.tile >= p.tiles) w.tile -= p.tiles;
+    w.split = fdiv(unit, p.d_pairs);
+    w.pair = unit - w.split * p.pairs;
+    w.b = (int)fdiv(w.pair, p.d_g);
+    w.g = (int)w.pair - w.b * p.G;
+    if (!p.ends) {
+        w.end = visible_end(p, w.b, lds);
+        return w;
+    }
+    // the w.b-th longest of the at most 256 sequences
+    const int t = threadIdx.x, mine = t < p.N ? p.ends[t] : -1;
+    int rank = 0;
+    for (int u = 0; u < p.N; ++u) {
+        const int e = p.ends[u];
+        rank += e > mine || (e == mine && u < t);
+    }
+    if (t < p.N && rank == w.b) { lds[0] = t; lds[1] = mine; }
+    __syncthreads();
+    w.b = __builtin_amdgcn_readfirstlane(lds[0]);
+    w.end = __builtin_amdgcn_readfirstlane(lds[1]);
+    w.pair = (uint32_t)(w.b * p.G + w.g);
+    __syncthreads();
+    return w;
+}
+
+// Element offset of row r of a pair.
+__device__ __forceinline__ int64_t row_at(const CrossP &p, const Rows &x, const Work &w, uint32_t r) {
+    const uint32_t hh = fdiv(r, p.d_lq);
+    return w.b * x.b + (int64_t)(w.g * (p.H / p.G) + (int)hh) * x.h + (int64_t)(r - hh * p.Lq) * x.l;
+}
+
+__device__ __forceinline__ f32x4 load4(const float *p) { return *reinterpret_cast<const f32x4_any *>(p); }
+__device__ __forceinline__ void store4(float *p, f32x4 v) { *reinterpret_cast<f32x4_any *>(p) = v; }
+
 // Blocks [first, last) of the `blocks` that this split takes.
 __device__ __forceinline__ void split_range(uint32_t blocks, uint32_t split, uint32_t splits, uint32_t *first, uint32_t *last) {
     const uint32_t per = blocks / splits, rest = blocks % splits;
@@ -111,23 +142,54 @@ struct Tile {
     __device__ static int at(int row, int piece) { return row * D + ((piece ^ turn(row)) << 2); }
 };
 
-// Requests ROWS rows of an LDS tile; row_at(r) is where row r begins.  DMA: straight into LDS, 16 bytes a lane, there after
-// arrived(); needs 16-byte aligned rows.
+// One 16-byte piece of a tile.  DMA: straight into LDS, from the wavefront's first lane's piece on, there after arrived();
+// needs 16-byte aligned rows.
+template <bool DMA>
+__device__ __forceinline__ void stage_piece(float *tile, int f, const float *src) {
+    if (DMA) {
+        float *dst = tile + __builtin_amdgcn_readfirstlane(f & ~63) * 4;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+    } else {
+        *reinterpret_cast<f32x4 *>(tile + f * 4) = load4(src);
+    }
+}
+
+// Requests ROWS rows of an LDS tile; row_at(r) is where row r begins.
 template <int D, int ROWS, bool DMA, class F>
 __device__ __forceinline__ void stage(float *tile, F row_at) {
     constexpr int PIECES = Tile<D>::PIECES;
 #pragma unroll
     for (int i = 0; i < ROWS * PIECES / 256; ++i) {
-        const int f = i * 256 + (int)threadIdx.x, row = f / PIECES, piece = (f % PIECES) ^ Tile<D>::turn(row);
-        const float *src = row_at(row) + piece * 4;
-        if (DMA) {
-            float *dst = tile + (i * 256 + __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63)) * 4;  // of the wavefront's first lane
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
-        } else {
-            *reinterpret_cast<f32x4 *>(tile + f * 4) = load4(src);
-        }
+        const int f = i * 256 + (int)threadIdx.x, row = f / PIECES;
+        stage_piece<DMA>(tile, f, row_at(row) + ((f % PIECES) ^ Tile<D>::turn(row)) * 4);
     }
 }
+
+// The same of rows that lie a stride apart.  A thread's pieces are 1024 / D rows apart and in the same place of each, so
+// where it starts is fixed for the kernel and the way from there is the same for all: address arithmetic of the scalar unit.
+template <int D>
+struct Strided {
+    const float *own;  // this thread's piece of the first row it takes of a tile at row 0
+    int64_t l;
+    int total;
+    __device__ Strided(const float *x, int64_t l_, int total_) : l(l_), total(total_) {
+        const int row = (int)threadIdx.x / Tile<D>::PIECES;
+        own = x + (int64_t)row * l + (((int)threadIdx.x % Tile<D>::PIECES) ^ Tile<D>::turn(row)) * 4;
+    }
+    template <int ROWS, bool DMA>
+    __device__ __forceinline__ void stage(float *tile, int first) const {
+        constexpr int STEP = 1024 / D;
+        if (first + ROWS <= total) {
+#pragma unroll
+            for (int i = 0; i < ROWS / STEP; ++i) stage_piece<DMA>(tile, i * 256 + (int)threadIdx.x, own + (int64_t)(first + i * STEP) * l);
+        } else {  // rows past the end repeat the last one
+            const int row = (int)threadIdx.x / Tile<D>::PIECES;
+#pragma unroll
+            for (int i = 0; i < ROWS / STEP; ++i)
+                stage_piece<DMA>(tile, i * 256 + (int)threadIdx.x, own + (int64_t)(min(first + i * STEP + row, total - 1) - row) * l);
+        }
+    }
+};
 // What this wavefront requested is in LDS (and in registers).
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -169,16 +231,19 @@ struct Visible {
     }
 };
 
-// A wavefront's own 32 columns as the right operand: register [g][s] of lane (c, h) = x[c][8g + 4h + s] * f.
+// A wavefront's own 32 columns as the right operand: register [g][s] of lane (c, h) = x[c][8g + 4h + s].  Loaded from memory
+// as they are needed, 32 bytes of 32 rows an instruction: a way through LDS would take whole lines, but one wait more in
+// front of the first block, and the buffers that this block is on its way into.
 template <int D>
 struct Own {
-    float x[D / 8][4];
-    __device__ void take(const float *tile, int row, int h, float f) {
+    f32x4 x[D / 8];
+    __device__ void load(const float *row, int h) {
 #pragma unroll
-        for (int g = 0; g < D / 8; ++g) {
-            const f32x4 t = *reinterpret_cast<const f32x4 *>(&tile[Tile<D>::at(row, 2 * g + h)]);
-            x[g][0] = t.x * f; x[g][1] = t.y * f; x[g][2] = t.z * f; x[g][3] = t.w * f;
-        }
+        for (int g = 0; g < D / 8; ++g) x[g] = load4(row + 8 * g + 4 * h);
+    }
+    __device__ void scale(float f) {
+#pragma unroll
+        for (int g = 0; g < D / 8; ++g) x[g] *= f;
     }
 };
 
@@ -236,34 +301,22 @@ __device__ __forceinline__ void write_column(float *row, const floatx16 *acc, fl
     }
 }
 
-// The 32 RW rows of a workgroup's tile, through LDS, to the wavefronts that own them.  (The two buffers are arrays of their
-// own everywhere: the compiler waits for a load into LDS in front of any read that it cannot tell from the load's target.)
-template <int D, int RW, bool DMA, int N>
-__device__ __forceinline__ void take_rows(const CrossP &p, const Rows &x, const Work &w, float (&lds0)[N], float (&lds1)[N], int own_row, int h, float f, Own<D> &own) {
-    constexpr int HALF = N / D < 32 * RW ? N / D : 32 * RW;  // rows that go through the first buffer
-    __syncthreads();
-    // a row past the end repeats the last one; it is not written
-    stage<D, HALF, DMA>(lds0, [&](int r) { return x.p + row_at(p, x, w, min(w.tile * (32 * RW) + r, (uint32_t)p.R - 1)); });
-    if (HALF < 32 * RW) stage<D, HALF, DMA>(lds1, [&](int r) { return x.p + row_at(p, x, w, min(w.tile * (32 * RW) + HALF + r, (uint32_t)p.R - 1)); });
-    arrived();
-    __syncthreads();
-    if (own_row < HALF) own.take(lds0, own_row, h, f);
-    else own.take(lds1, own_row - HALF, h, f);
-}
-
 // Walks the visible blocks of KB keys, two LDS buffers in turn: while one is worked on, the next block is on its way into
-// the other, and there is one barrier a block.  work(keys' tile, values' tile, bits of this wavefront's 32 keys).
-template <int D, int KB, bool DMA, class F>
+// the other, and there is one barrier a block.  (The buffers are arrays of their own: the compiler waits for a load into LDS
+// in front of any read that it cannot tell from the load's target.)  ready() is called when the first block is on its way;
+// work(keys' tile, values' tile, bits of this wavefront's 32 keys).
+template <int D, int KB, bool DMA, class G, class F>
 __device__ __forceinline__ void walk_keys(const CrossP &p, const Work &w, float (&lds0)[2 * KB * D], float (&lds1)[2 * KB * D], uint32_t first, uint32_t last, int kw,
-                                          F work) {
+                                          G ready, F work) {
     const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
     const bool is_mask = p.mask != nullptr;
     const float *mask = is_mask ? p.mask + w.b * p.mask_b : K;
     Visible<KB> next;
+    const Strided<D> keys(K, p.k.l, p.Lk), values(V, p.v.l, p.Lk);
     auto request = [&](uint32_t blk, float *to) {
         const int j0 = (int)blk * KB;
-        stage<D, KB, DMA>(to, [&](int r) { return K + (int64_t)min(j0 + r, p.Lk - 1) * p.k.l; });
-        stage<D, KB, DMA>(to + KB * D, [&](int r) { return V + (int64_t)min(j0 + r, p.Lk - 1) * p.v.l; });
+        keys.template stage<KB, DMA>(to, j0);
+        values.template stage<KB, DMA>(to + KB * D, j0);
         next.request(mask, is_mask, j0, p.Lk);
     };
     auto step = [&](uint32_t blk, float *tile, float *other) {
@@ -280,8 +333,8 @@ __device__ __forceinline__ void walk_keys(const CrossP &p, const Work &w, float 
         for (int k = 1; k < KB / 32; ++k) mine = kw == k * 32 ? seen[k] : mine;
         work(tile + kw * D, tile + (KB + kw) * D, (uint32_t)__builtin_amdgcn_readfirstlane((int)mine));
     };
-    __syncthreads();
     if (first < last) request(first, lds0);
+    ready();
     for (uint32_t blk = first; blk < last; blk += 2) {
         step(blk, lds0, lds1);
         if (blk + 1 < last) step(blk + 1, lds1, lds0);
@@ -305,25 +358,25 @@ __device__ __forceinline__ bool merge_waves(float *lds, int wave, int lane, G gi
 // ---- forward.  RW wavefronts take the workgroup's 32 RW rows, the 4 / RW times as many share each block's keys and are
 // merged through LDS at the end.
 template <int D, int RW, bool DMA>
-__global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 4 ? 3 : 1))) cross_forward_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND + 2;
     __shared__ __attribute__((aligned(16))) float lds0[2 * KB * D], lds1[2 * KB * D];  // two buffers of keys and values
     __shared__ int lds_end[4];
-    static_assert(32 * RW <= 4 * KB && (KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "rows and the merge fit in the buffers");
-    const Work w = find_work(p);
+    static_assert((KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "the merge fits in a buffer");
+    const Work w = find_work(p, lds_end);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int own_row = (wave % RW) * 32 + c;
-    const int end = visible_end(p, w.b, lds_end);
+    const uint32_t r = w.tile * (32 * RW) + (wave % RW) * 32 + c;
     const float inf = __builtin_inff();
-    Own<D> q;  // scaled: scores are logarithms to base 2
-    take_rows<D, RW, DMA>(p, p.q, w, lds0, lds1, own_row, h, p.scale * LOG2E, q);
+    Own<D> q;
+    q.load(p.q.p + row_at(p, p.q, w, min(r, (uint32_t)p.R - 1)), h);  // a row past the end repeats the last one; it is not written
     floatx16 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = zero16();
     float m_run = -inf, l_run = 0.0f;
     uint32_t first, last;
-    split_range((end + KB - 1) / KB, w.split, p.splits, &first, &last);
-    walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&](const float *kt, const float *vt, uint32_t seen) {
+    split_range((w.end + KB - 1) / KB, w.split, p.splits, &first, &last);
+    walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&] { q.scale(p.scale * LOG2E); /* scores are logarithms to base 2 */ },
+                          [&](const float *kt, const float *vt, uint32_t seen) {
         floatx16 s = scores<D>(kt, q, c, h);
         if (seen != ~0u) {
             const uint32_t mine = seen >> (4 * h);
@@ -371,7 +424,6 @@ __global__ void __launch_bounds__(256) cross_forward_kernel(const CrossP p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[j][r] = acc[j][r] * fa + from[16 * j + r] * fb;
     });
-    const uint32_t r = w.tile * (32 * RW) + own_row;
     if (!writes || r >= (uint32_t)p.R) return;
     const int64_t row = (int64_t)w.pair * p.R + r;
     if (p.splits > 1) {
@@ -404,7 +456,7 @@ __global__ void __launch_bounds__(256) cross_few_kernel(const CrossP p) {
     __shared__ int lds_end[4];
     __shared__ float lds_ml[4][ROWS][2];
     __shared__ __attribute__((aligned(16))) float lds_o[4][ROWS][D];
-    const Work w = find_work(p);
+    const Work w = find_work(p, lds_end);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPK, col = lane % LPK * 4;
     const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h + col, *V = p.v.p + w.b * p.v.b + w.g * p.v.h + col;
     const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
@@ -418,7 +470,7 @@ __global__ void __launch_bounds__(256) cross_few_kernel(const CrossP p) {
         m[r] = -inf;
         l[r] = 0.0f;
     }
-    const int end = visible_end(p, w.b, lds_end);
+    const int end = w.end;
     uint32_t first, last;
     split_range((end + STEP - 1) / STEP, w.split, p.splits, &first, &last);
     f32x4 kn[UNROLL], vn[UNROLL];
@@ -541,31 +593,31 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND;
     __shared__ __attribute__((aligned(16))) float lds0[2 * KB * D], lds1[2 * KB * D];
     __shared__ int lds_end[4];
-    static_assert(32 * RW <= 4 * KB && (KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "rows and the merge fit in the buffers");
-    const Work w = find_work(p);
+    static_assert((KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "the merge fits in a buffer");
+    const Work w = find_work(p, lds_end);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int own_row = (wave % RW) * 32 + c;
-    const int end = visible_end(p, w.b, lds_end);
-    const uint32_t r = w.tile * (32 * RW) + own_row;
-    const int64_t row = (int64_t)w.pair * p.R + min(r, (uint32_t)p.R - 1);
-    Own<D> q, go;
-    float delta = 0.0f;
-    take_rows<D, RW, DMA>(p, p.o, w, lds0, lds1, own_row, h, 1.0f, q);
-    take_rows<D, RW, DMA>(p, p.go, w, lds0, lds1, own_row, h, 1.0f, go);
-#pragma unroll
-    for (int g = 0; g < D / 8; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) delta += q.x[g][i] * go.x[g][i];
-    delta += __shfl_xor(delta, 32, 64);
-    if (w.split == 0 && wave < RW && h == 0 && r < (uint32_t)p.R) p.delta[row] = delta;
-    take_rows<D, RW, DMA>(p, p.q, w, lds0, lds1, own_row, h, p.scale * LOG2E, q);
-    const float lse2 = p.lse[row] * LOG2E;
+    const uint32_t r = w.tile * (32 * RW) + (wave % RW) * 32 + c, rr = min(r, (uint32_t)p.R - 1);
+    const int64_t row = (int64_t)w.pair * p.R + rr;
+    Own<D> q, go, o;
+    q.load(p.q.p + row_at(p, p.q, w, rr), h);
+    go.load(p.go.p + row_at(p, p.go, w, rr), h);
+    o.load(p.o.p + row_at(p, p.o, w, rr), h);
+    float lse2 = p.lse[row], delta = 0.0f;
     floatx16 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = zero16();
     uint32_t first, last;
-    split_range((end + KB - 1) / KB, w.split, p.splits, &first, &last);
-    walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&](const float *kt, const float *vt, uint32_t seen) {
+    split_range((w.end + KB - 1) / KB, w.split, p.splits, &first, &last);
+    walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&] {
+        q.scale(p.scale * LOG2E);
+        lse2 *= LOG2E;
+#pragma unroll
+        for (int g = 0; g < D / 8; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) delta += o.x[g][i] * go.x[g][i];
+        delta += __shfl_xor(delta, 32, 64);
+        if (w.split == 0 && wave < RW && h == 0 && r < (uint32_t)p.R) p.delta[row] = delta;
+    }, [&](const float *kt, const float *vt, uint32_t seen) {
         floatx16 s = scores<D>(kt, q, c, h);
         const floatx16 dp = scores<D>(vt, go, c, h);
 #pragma unroll
@@ -594,39 +646,39 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
     else write_column<D>(const_cast<float *>(p.gq.p) + row_at(p, p.gq, w, r), acc, p.scale, h);
 }
 
-// ---- gradients of keys and values: a wavefront owns 32 keys and walks all rows of the pair, 32 at a time.
-template <int D, bool DMA>
+// ---- gradients of keys and values: a wavefront owns 32 keys and walks the rows of the pair, 32 at a time.  CW wavefronts
+// take the workgroup's 32 CW keys, the 4 / CW times as many share each block's rows and are added up through LDS.
+template <int D, int CW, bool DMA>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) cross_gkv_kernel(const CrossP p) {
-    constexpr int RB = 32, ND = D / 32;
+    constexpr int GW = 4 / CW, RB = 32 * GW, ND = D / 32, KEYS = 32 * CW, SLOT = 32 * ND;
     __shared__ __attribute__((aligned(16))) float lds0[2 * RB * D], lds1[2 * RB * D];  // two buffers of rows of Q and dO
     __shared__ __attribute__((aligned(16))) float rows0[2 * RB], rows1[2 * RB];        // their lse and delta
-    const Work w = find_work(p);
+    __shared__ int lds_end[4];
+    static_assert((GW - 1) * CW * 64 * SLOT <= 2 * RB * D, "the merge fits in a buffer");
+    const Work w = find_work(p, lds_end);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
-    const int j0 = (int)w.tile * 128, j = j0 + wave * 32 + c;
+    const int j0 = (int)w.tile * KEYS, j = j0 + (wave % CW) * 32 + c, rw = wave / CW * 32;
     const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
-    const bool seen = j < p.Lk && (!p.mask || p.mask[w.b * p.mask_b + j] != 0.0f);
+    const bool seen = j < w.end && (!p.mask || p.mask[w.b * p.mask_b + j] != 0.0f);
     const float inf = __builtin_inff();
     floatx16 gk[ND], gv[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) gk[d] = gv[d] = zero16();
-    if (__syncthreads_or(seen)) {
-        Own<D> k, v;  // k scaled: scores are logarithms to base 2
-        auto take = [&](const float *x, int64_t l, float f, Own<D> &own) {
-            __syncthreads();
-            stage<D, 64, DMA>(lds0, [&](int r) { return x + (int64_t)min(j0 + r, p.Lk - 1) * l; });
-            stage<D, 64, DMA>(lds1, [&](int r) { return x + (int64_t)min(j0 + 64 + r, p.Lk - 1) * l; });
-            arrived();
-            __syncthreads();
-            if (wave < 2) own.take(lds0, wave * 32 + c, h, f);
-            else own.take(lds1, (wave - 2) * 32 + c, h, f);
-        };
-        take(K, p.k.l, p.scale * LOG2E, k);
-        take(V, p.v.l, 1.0f, v);
+    if (j0 < w.end) {
+        Own<D> k, v;  // k scaled in front of the walk: scores are logarithms to base 2
+        k.load(K + (int64_t)min(j, p.Lk - 1) * p.k.l, h);
+        v.load(V + (int64_t)min(j, p.Lk - 1) * p.v.l, h);
         float lreg = 0.0f, dreg = 0.0f;
+        const Strided<D> qs(p.q.p + row_at(p, p.q, w, 0), p.q.l, p.R), gs(p.go.p + row_at(p, p.go, w, 0), p.go.l, p.R);
         auto request = [&](uint32_t blk, float *to) {
-            auto at = [&](int r) { return min(blk * RB + r, (uint32_t)p.R - 1); };
-            stage<D, RB, DMA>(to, [&](int r) { return p.q.p + row_at(p, p.q, w, at(r)); });
-            stage<D, RB, DMA>(to + RB * D, [&](int r) { return p.go.p + row_at(p, p.go, w, at(r)); });
+            if (p.strided) {
+                qs.template stage<RB, DMA>(to, (int)blk * RB);
+                gs.template stage<RB, DMA>(to + RB * D, (int)blk * RB);
+            } else {
+                auto at = [&](int r) { return min(blk * RB + r, (uint32_t)p.R - 1); };
+                stage<D, RB, DMA>(to, [&](int r) { return p.q.p + row_at(p, p.q, w, at(r)); });
+                stage<D, RB, DMA>(to + RB * D, [&](int r) { return p.go.p + row_at(p, p.go, w, at(r)); });
+            }
             if (tid < RB) {
                 const uint32_t r = blk * RB + tid;
                 lreg = r < (uint32_t)p.R ? p.lse[(int64_t)w.pair * p.R + r] : inf;  // a row past the end: every exponential is 0
@@ -643,12 +695,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) c
             __syncthreads();
             if (blk + 1 < last) request(blk + 1, other);
             if (!works) return;
-            const float *qt = tile, *gt = tile + RB * D;
+            __builtin_amdgcn_sched_barrier(0);  // the parts one after the other: all operands at once do not fit the registers
+            const float *qt = tile + rw * D, *gt = tile + (RB + rw) * D, *ls = rows + rw, *dl = rows + RB + rw;
             floatx16 s = scores<D>(qt, k, c, h);
+            __builtin_amdgcn_sched_barrier(0);
             floatx16 dp = scores<D>(gt, v, c, h);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&rows[8 * g + 4 * h]), d4 = *reinterpret_cast<const f32x4 *>(&rows[RB + 8 * g + 4 * h]);
+                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&ls[8 * g + 4 * h]), d4 = *reinterpret_cast<const f32x4 *>(&dl[8 * g + 4 * h]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float e = __builtin_amdgcn_exp2f(s[4 * g + i] - l4[i]);
@@ -656,17 +711,30 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) c
                     dp[4 * g + i] = e * (dp[4 * g + i] - d4[i]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             accumulate<D>(gt, s, gv, c, h);
+            __builtin_amdgcn_sched_barrier(0);
             accumulate<D>(qt, dp, gk, c, h);
         };
-        __syncthreads();
         if (first < last) request(first, lds0);
+        k.scale(p.scale * LOG2E);
         for (uint32_t blk = first; blk < last; blk += 2) {
             step(blk, lds0, rows0, lds1);
             if (blk + 1 < last) step(blk + 1, lds1, rows1, lds0);
         }
     }
-    if (j >= p.Lk) return;
+    const bool writes = merge_waves<CW, SLOT>(lds0, wave, lane, [&](float *to) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { to[16 * d + i] = gk[d][i]; to[16 * (ND + d) + i] = gv[d][i]; }
+    }, [&](const float *from) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { gk[d][i] += from[16 * d + i]; gv[d][i] += from[16 * (ND + d) + i]; }
+    });
+    if (!writes || j >= p.Lk) return;
     if (!seen) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) gk[d] = gv[d] = zero16();
@@ -681,10 +749,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) c
     }
 }
 
-// out[row] = sum of the splits' rows, in order: D / 4 lanes a row.  Rows of a pair are `heads` x `length`.
+// out[row] = sum of the splits' rows, in order: D / 4 lanes a row.  Rows of a pair are `heads` x `length`.  blockIdx.y: which
+// of two such sums.
 template <int D>
-__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part, Rows out, uint32_t total, uint32_t splits, uint32_t heads, uint32_t length) {
+__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part0, const float *part1, Rows out0, Rows out1, uint32_t total, uint32_t splits,
+                                                        uint32_t heads, uint32_t length) {
     constexpr int LPR = D / 4;
+    const float *part = blockIdx.y ? part1 : part0;
+    const Rows out = blockIdx.y ? out1 : out0;
     const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
     if (row >= total) return;
     f32x4 acc = *reinterpret_cast<const f32x4 *>(part + (int64_t)row * D + col);
@@ -760,12 +832,21 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
 // 16-byte aligned rows: loads straight into LDS take them.
 bool aligned_rows(const Rows &r) { return ((uintptr_t)r.p) % 16 == 0 && r.b % 4 == 0 && r.h % 4 == 0 && r.l % 4 == 0; }
 
-// Splits of a long axis of `blocks` blocks that bring `units` workgroups to two for each compute unit.
-uint32_t choose_splits(const sg_ctx *ctx, uint32_t units, uint32_t blocks) {
-    const uint32_t want = 2u * (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
-    uint32_t s = units >= want ? 1 : (want + units - 1) / units;
-    if (s > blocks / 2) s = blocks / 2;
-    return s < 1 ? 1 : s > 64 ? 64 : s;
+// Splits of a long axis of `blocks` blocks, where there are fewer than two workgroups for each compute unit: the number that
+// leaves the busiest compute unit the least, which works at three quarters of its rate on a single workgroup, a join's
+// traffic counted as 3 % a split.  (154 tiles of 1332 rows, 8 + 32 keys:
+// 3 splits, 462 workgroups, at most 2 on a compute unit, against 4, 616 and 3.)
+uint32_t choose_splits(const sg_ctx *ctx, uint64_t units, uint32_t blocks) {
+    const uint64_t cus = (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+    if (units >= 2 * cus) return 1;
+    uint32_t best = 1;
+    double least = 1e30;
+    for (uint32_t s = 1; s <= 64 && (s == 1 || (s <= blocks / 2 && units * s <= 3 * cus)); ++s) {
+        const uint64_t most = (units * s + cus - 1) / cus;
+        const double cost = (most == 1 ? 1.33 : (double)most) / s * (1.0 + 0.03 * s);
+        if (cost < least) { least = cost; best = s; }
+    }
+    return best;
 }
 
 int row_waves(int R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
@@ -779,6 +860,11 @@ int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
 }
 
 }  // namespace
+
+// Lengths in front of the launches, where there are more workgroups than the chip holds and lengths to order them by.
+bool orders_lengths(const sg_ctx *ctx, const CrossP &p, uint64_t workgroups) {
+    return p.mask && p.N > 1 && p.N <= 256 && workgroups > 2u * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+}
 
 #define SG_CROSS_ROWS_(KERNEL, D_, RW, DMA, GRID)                                                                       \
     do {                                                                                                                \
@@ -814,6 +900,11 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
         if ((rc = space.take((uint64_t)p.splits * total * (D + 2) * 4)) != SG_OK) return rc;
         p.part_o = (float *)space.p;
         p.part_ml = p.part_o + (uint64_t)p.splits * total * D;
+    } else if (!few && orders_lengths(ctx, p, (uint64_t)tiles * p.pairs)) {
+        if ((rc = space.take((uint64_t)p.N * 4)) != SG_OK) return rc;
+        p.ends = (int *)space.p;
+        hipLaunchKernelGGL(cross_ends_kernel, dim3((unsigned)p.N), dim3(256), 0, ctx->stream, p);
+        SG_CHECK_LAUNCH(ctx, "cross_attention lengths");
     }
     const dim3 grid(p.tiles * p.pairs * p.splits);
 #define SG_CROSS_FEW(D_, ROWS, UNROLL) hipLaunchKernelGGL((cross_few_kernel<D_, ROWS, UNROLL>), grid, dim3(256), 0, ctx->stream, p)
@@ -858,43 +949,60 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     if ((rc = check_apart(ctx, gv, "sg_cross_attention_grad gv")) != SG_OK) return rc;
     if (!ctx) return SG_ERR_ARG;
     p.scale = scale;
+    p.strided = p.H == p.G || (p.q.h == p.Lq * p.q.l && p.go.h == p.Lq * p.go.l);
     sg_device_guard guard(ctx);
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
     const int rw = row_waves(p.R), kb = 128 / rw;
-    const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 127) / 128);
+    // Keys a workgroup: 128 where all are visible and workgroups are many (32 x 12 heads of 512 x 512: 441 us against 463 with
+    // 64), else 64, which waste less of a sequence's last tile and level better (lengths 512 to 272: 432 against 421 us; 7 x 2
+    // key heads of 1001 keys, size 32: 64 against 57 us).
+    const int cw = !p.mask && (uint64_t)((p.Lk + 127) / 128) * p.pairs >= 1024 ? 4 : 2, rb = 128 / cw;
+    const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 32 * cw - 1) / (32 * cw));
     const uint32_t row_splits = choose_splits(ctx, row_tiles * p.pairs, (uint32_t)((p.Lk + kb - 1) / kb));
-    const uint32_t key_splits = choose_splits(ctx, key_tiles * p.pairs, (uint32_t)((p.R + 31) / 32));
+    const uint32_t key_splits = choose_splits(ctx, key_tiles * p.pairs, (uint32_t)((p.R + rb - 1) / rb));
     // delta, and the larger of the two kernels' split sums: they run one after the other
     const uint64_t rows_part = row_splits > 1 ? row_splits * total * D : 0, keys_part = key_splits > 1 ? 2 * key_splits * keys * D : 0;
-    const uint64_t delta_floats = (total + 3) / 4 * 4;
+    const uint64_t delta_floats = (total + (uint64_t)p.N + 3) / 4 * 4;  // delta and the lengths
     sg_workspace space(ctx);
     if ((rc = space.take((delta_floats + (rows_part > keys_part ? rows_part : keys_part)) * 4)) != SG_OK) return rc;
     p.delta = (float *)space.p;
     p.part_o = p.part_k = p.delta + delta_floats;
     p.part_v = p.part_k + key_splits * keys * D;
-    auto sum = [&](const float *part, const Rows &to, uint64_t n, uint32_t splits, int heads, int length) {
-        const dim3 grid((unsigned)((n + 1024 / D - 1) / (1024 / D)));
-        if (D == 64) hipLaunchKernelGGL((cross_sum_kernel<64>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
-        else hipLaunchKernelGGL((cross_sum_kernel<32>), grid, dim3(256), 0, ctx->stream, part, to, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
+    if (orders_lengths(ctx, p, (uint64_t)key_tiles * p.pairs)) {
+        p.ends = (int *)(p.delta + total);
+        hipLaunchKernelGGL(cross_ends_kernel, dim3((unsigned)p.N), dim3(256), 0, ctx->stream, p);
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad lengths");
+    }
+    auto sum = [&](unsigned count, const float *part0, const float *part1, const Rows &to0, const Rows &to1, uint64_t n, uint32_t splits, int heads, int length) {
+        const dim3 grid((unsigned)((n + 1024 / D - 1) / (1024 / D)), count);
+        if (D == 64) hipLaunchKernelGGL((cross_sum_kernel<64>), grid, dim3(256), 0, ctx->stream, part0, part1, to0, to1, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
+        else hipLaunchKernelGGL((cross_sum_kernel<32>), grid, dim3(256), 0, ctx->stream, part0, part1, to0, to1, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
     };
     if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
     const bool dma = aligned_rows(p.q) && aligned_rows(p.k) && aligned_rows(p.v) && aligned_rows(p.o) && aligned_rows(p.go);
     SG_CROSS_ROWS(cross_gq_kernel, rw, dma, dim3(p.tiles * p.pairs * p.splits));
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
     if (row_splits > 1) {
-        sum(p.part_o, p.gq, total, row_splits, p.H, p.Lq);
+        sum(1, p.part_o, p.part_o, p.gq, p.gq, total, row_splits, p.H, p.Lq);
         SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries' sums");
     }
     if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
     const dim3 grid(p.tiles * p.pairs * p.splits);
-    if (D == 64 && dma) hipLaunchKernelGGL((cross_gkv_kernel<64, true>), grid, dim3(256), 0, ctx->stream, p);
-    else if (D == 64) hipLaunchKernelGGL((cross_gkv_kernel<64, false>), grid, dim3(256), 0, ctx->stream, p);
-    else if (dma) hipLaunchKernelGGL((cross_gkv_kernel<32, true>), grid, dim3(256), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((cross_gkv_kernel<32, false>), grid, dim3(256), 0, ctx->stream, p);
+#define SG_CROSS_KEYS(D_, CW, DMA) hipLaunchKernelGGL((cross_gkv_kernel<D_, CW, DMA>), grid, dim3(256), 0, ctx->stream, p)
+#define SG_CROSS_KEYS_(D_, CW)                 \
+    do {                                       \
+        if (dma) SG_CROSS_KEYS(D_, CW, true);  \
+        else SG_CROSS_KEYS(D_, CW, false);     \
+    } while (0)
+    if (D == 64 && cw == 4) SG_CROSS_KEYS_(64, 4);
+    else if (D == 64) SG_CROSS_KEYS_(64, 2);
+    else if (cw == 4) SG_CROSS_KEYS_(32, 4);
+    else SG_CROSS_KEYS_(32, 2);
+#undef SG_CROSS_KEYS_
+#undef SG_CROSS_KEYS
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys and values");
     if (key_splits > 1) {
-        sum(p.part_k, p.gk, keys, key_splits, p.G, p.Lk);
-        sum(p.part_v, p.gv, keys, key_splits, p.G, p.Lk);
+        sum(2, p.part_k, p.part_v, p.gk, p.gv, keys, key_splits, p.G, p.Lk);
         SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys' sums");
     }
     return SG_OK;
