@@ -54,15 +54,14 @@ constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 constexpr uint32_t MAX_DIGITS = 512;       // 9 bits a pass: two passes up to 262143 rows
 constexpr uint32_t TILE_ITEMS = 4;         // per thread, where tiles of 4096 tokens are sorted over several launches
 constexpr uint32_t TILE = SORT_THREADS * TILE_ITEMS;
-constexpr uint32_t SINGLE_ITEMS = 8;       // per thread, where one workgroup sorts everything in LDS in one launch:
-constexpr uint32_t SINGLE = SORT_THREADS * SINGLE_ITEMS;  // up to 8192 tokens
+constexpr uint32_t SINGLE = SORT_THREADS * 8;  // tokens that one workgroup sorts in LDS in one launch
 constexpr uint32_t FILL = 8;               // 16-byte pieces a thread of a clearing workgroup writes
 
 struct SortP {
     const uint32_t *ids;       // first pass: the ids themselves
     const uint32_t *key_in, *pos_in;
     uint32_t *key_out, *pos_out;
-    uint32_t *hist;            // [tile][digit]
+    uint32_t *hist, *next_hist;  // [tile][digit] of this pass; of the next one, if this one counts it
     sg_rows id_rows;
     uint32_t n, V, tiles, shift, digits, from_ids;
     uint32_t bits, passes;     // of the single-workgroup form
@@ -152,18 +151,20 @@ __device__ __forceinline__ void prefix_digits(uint32_t *totals, uint32_t *scratc
     __syncthreads();
 }
 
-// Up to 8192 tokens: workgroup 0 sorts them, all passes in LDS; the others clear the table.
+// Up to 8192 tokens: workgroup 0 sorts them, all passes in LDS; the others clear the table.  (Up to 4096 tokens in half the
+// registers and LDS, so that two clearing workgroups share a compute unit.)
+template <uint32_t ITEMS>
 __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const SortP p) {
-    __shared__ uint32_t keys[SINGLE], totals[MAX_DIGITS], scratch[SORT_WAVES];
-    __shared__ uint16_t places[SINGLE], counts[SORT_WAVES * MAX_DIGITS];
+    __shared__ uint32_t keys[SORT_THREADS * ITEMS], totals[MAX_DIGITS], scratch[SORT_WAVES];
+    __shared__ uint16_t places[SORT_THREADS * ITEMS], counts[SORT_WAVES * MAX_DIGITS];
     if (blockIdx.x > 0) {
         clear_part(p, blockIdx.x - 1);
         return;
     }
-    uint32_t key[SINGLE_ITEMS], pos[SINGLE_ITEMS], digit[SINGLE_ITEMS], rank[SINGLE_ITEMS];
+    uint32_t key[ITEMS], pos[ITEMS], digit[ITEMS], rank[ITEMS];
     const uint32_t items = (p.n + SORT_THREADS - 1) / SORT_THREADS;  // per thread; the rest of the registers stay empty
 #pragma unroll
-    for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+    for (uint32_t k = 0; k < ITEMS; ++k) {
         const uint32_t i = item_index(items, k);
         pos[k] = i;
         key[k] = k < items && i < p.n ? key_of(p, i) : 0;
@@ -173,14 +174,14 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const Sort
         for (uint32_t i = threadIdx.x; i < SORT_WAVES * digits; i += SORT_THREADS) counts[i] = 0;
         __syncthreads();
 #pragma unroll
-        for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+        for (uint32_t k = 0; k < ITEMS; ++k) {
             const bool there = k < items && item_index(items, k) < p.n;
             digit[k] = there ? (key[k] >> shift) & (digits - 1) : digits;
         }
-        rank_items<SINGLE_ITEMS>(digit, rank, counts, totals, digits, items);
+        rank_items<ITEMS>(digit, rank, counts, totals, digits, items);
         prefix_digits(totals, scratch, digits);
 #pragma unroll
-        for (uint32_t k = 0; k < SINGLE_ITEMS; ++k)
+        for (uint32_t k = 0; k < ITEMS; ++k)
             if (digit[k] < digits) {
                 const uint32_t to = totals[digit[k]] + rank[k];
                 keys[to] = key[k];
@@ -188,20 +189,22 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const Sort
             }
         __syncthreads();
 #pragma unroll
-        for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+        for (uint32_t k = 0; k < ITEMS; ++k) {
             const uint32_t i = item_index(items, k);
             if (k < items && i < p.n) { key[k] = keys[i]; pos[k] = places[i]; }
         }
         __syncthreads();
     }
 #pragma unroll
-    for (uint32_t k = 0; k < SINGLE_ITEMS; ++k) {
+    for (uint32_t k = 0; k < ITEMS; ++k) {
         const uint32_t i = item_index(items, k);
         if (k < items && i < p.n) { p.key_out[i] = key[k]; p.pos_out[i] = pos[k]; }
     }
 }
 
-// More tokens: a launch counts every tile's digits, the next moves every token to its place of this pass.
+// More tokens: a launch counts every tile's digits, the next moves every token to its place of this pass, and counts the
+// next pass's digits where the tokens land, in LDS first, if the tiles' counts fit there (else a launch of its own does).
+constexpr uint32_t NEXT_COUNTS = 8192;
 __global__ void __launch_bounds__(SORT_THREADS) embedding_count_kernel(const SortP p) {
     __shared__ uint32_t count[MAX_DIGITS];
     if (blockIdx.x >= p.tiles) {
@@ -216,16 +219,22 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_count_kernel(const Sor
         if (i < p.n) atomicAdd(&count[((p.from_ids ? key_of(p, i) : p.key_in[i]) >> p.shift) & (p.digits - 1)], 1u);
     }
     __syncthreads();
-    if (threadIdx.x < p.digits) p.hist[blockIdx.x * p.digits + threadIdx.x] = count[threadIdx.x];
+    if (threadIdx.x < p.digits) {
+        p.hist[blockIdx.x * p.digits + threadIdx.x] = count[threadIdx.x];
+        if (p.next_hist) p.next_hist[blockIdx.x * p.digits + threadIdx.x] = 0;
+    }
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) embedding_move_kernel(const SortP p) {
     __shared__ uint32_t own[MAX_DIGITS], totals[MAX_DIGITS], before[MAX_DIGITS], scratch[SORT_WAVES];
     __shared__ uint16_t counts[SORT_WAVES * MAX_DIGITS];
+    __shared__ uint32_t next[NEXT_COUNTS];
     if (blockIdx.x >= p.tiles) {
         clear_part(p, blockIdx.x - p.tiles);
         return;
     }
+    if (p.next_hist)
+        for (uint32_t i = threadIdx.x; i < p.tiles * p.digits; i += SORT_THREADS) next[i] = 0;
     const uint32_t tile = blockIdx.x;
     uint32_t key[TILE_ITEMS], pos[TILE_ITEMS], digit[TILE_ITEMS], rank[TILE_ITEMS];
 #pragma unroll
@@ -258,7 +267,12 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_move_kernel(const Sort
             const uint32_t to = totals[digit[k]] + before[digit[k]] + rank[k];
             p.key_out[to] = key[k];
             p.pos_out[to] = pos[k];
+            if (p.next_hist) atomicAdd(&next[to / TILE * p.digits + ((key[k] >> (p.shift + p.bits)) & (p.digits - 1))], 1u);
         }
+    if (!p.next_hist) return;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < p.tiles * p.digits; i += SORT_THREADS)
+        if (next[i]) atomicAdd(&p.next_hist[i], next[i]);
 }
 
 struct SumP {
@@ -291,6 +305,71 @@ __device__ __forceinline__ void store_cols(float *row, uint32_t c, uint32_t E, f
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (c + 64 * j < E) row[c + 64 * j] = v[j];
+    }
+}
+
+// Up to 128 tokens, in one launch: a workgroup owns some rows of the table, clears them, finds its tokens among all and sums
+// the rows that have some in the tokens' order.  (Sort, sums and join are three launches of 4 us at the least.)  At most 32
+// rows a workgroup: where the table is small all tokens are on a few workgroups, each wavefront a row at a time.
+constexpr uint32_t FEW = 128, FEW_ROWS = 32, FEW_THREADS = 512;
+struct FewP {
+    const float *gout;
+    const uint32_t *ids;
+    float *gtable;
+    sg_rows id_rows, g_rows;
+    uint32_t n, E, V, rows;  // rows: what a workgroup owns
+    float scale;
+};
+
+template <bool VEC>
+__global__ void __launch_bounds__(FEW_THREADS) embedding_few_kernel(const FewP p) {
+    __shared__ __attribute__((aligned(16))) uint32_t row_of[FEW];  // of each token, ~0: not here
+    __shared__ uint32_t firsts[FEW], distinct;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t v0 = blockIdx.x * p.rows, rows = min(p.rows, p.V - v0);
+    const uint32_t id = tid < p.n ? p.ids[sg_row_offset(p.id_rows, tid)] : ~0u;
+    float *table = p.gtable + (uint64_t)v0 * p.E;
+    const uint64_t total = (uint64_t)rows * p.E;
+    for (uint64_t i = tid * (VEC ? 4u : 1u); i < total; i += FEW_THREADS * (VEC ? 4 : 1)) {
+        if (VEC) *reinterpret_cast<f32x4 *>(table + i) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        else table[i] = 0.0f;
+    }
+    const bool here = id >= v0 && id - v0 < rows;
+    const uint32_t row = here ? id - v0 : ~0u;
+    if (tid < FEW) row_of[tid] = row;
+    if (tid == 0) distinct = 0;
+    if (!__syncthreads_or(here)) return;
+    if (here) {
+        bool first = true;
+        for (uint32_t i = 0; i < tid; i += 4) {
+            const uint4 o = *reinterpret_cast<const uint4 *>(&row_of[i]);
+            first = first && o.x != row && (i + 1 >= tid || o.y != row) && (i + 2 >= tid || o.z != row) && (i + 3 >= tid || o.w != row);
+        }
+        if (first) firsts[atomicAdd(&distinct, 1u)] = row;  // in any order: the rows are summed each on its own
+    }
+    __syncthreads();  // the zeros, too, are written before the sums
+    const uint32_t pieces = (p.E + 255) / 256, units = distinct * pieces;
+    for (uint32_t u = wave; u < units; u += FEW_THREADS / 64) {  // a wavefront sums 256 columns of a row, 8 tokens in flight
+        const uint32_t r = firsts[u / pieces], c = u % pieces * 256 + (VEC ? lane * 4 : lane);
+        uint64_t a = __builtin_amdgcn_ballot_w64(row_of[lane] == r), b = __builtin_amdgcn_ballot_w64(row_of[64 + lane] == r);
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        while (a | b) {
+            f32x4 x[8];
+            uint32_t got = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                if (!(a | b)) continue;
+                const uint32_t token = a ? (uint32_t)__builtin_ctzll(a) : 64 + (uint32_t)__builtin_ctzll(b);
+                if (a) a &= a - 1;
+                else b &= b - 1;
+                x[k] = load_cols<VEC>(p.gout + sg_row_offset(p.g_rows, token), c, p.E);
+                got = k + 1;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (k < got) acc += x[k];
+        }
+        store_cols<VEC>(table + (uint64_t)r * p.E, c, p.E, acc * p.scale);
     }
 }
 
@@ -446,6 +525,29 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
     m.V = s.V;
     m.scale = scale;
     m.pieces = (m.E + 255) / 256;
+    if (s.n <= FEW) {
+        FewP f{};
+        f.gout = m.gout;
+        f.ids = s.ids;
+        f.gtable = table;
+        f.id_rows = s.id_rows;
+        f.g_rows = m.g_rows;
+        f.n = s.n;
+        f.E = m.E;
+        f.V = s.V;
+        f.scale = scale;
+        // 64 KB of the table a workgroup, so that clearing fills the chip
+        const uint32_t rows = 16384 / f.E;
+        f.rows = rows < 1 ? 1 : rows > FEW_ROWS ? FEW_ROWS : rows;
+        sg_device_guard guard(ctx);
+        bool vec = E % 4 == 0 && aligned16(f.gout) && aligned16(table);
+        for (int i = 0; i < f.g_rows.rank; ++i) vec = vec && f.g_rows.st[i] % 4 == 0;
+        const dim3 grid((s.V + f.rows - 1) / f.rows);
+        if (vec) hipLaunchKernelGGL((embedding_few_kernel<true>), grid, dim3(FEW_THREADS), 0, ctx->stream, f);
+        else hipLaunchKernelGGL((embedding_few_kernel<false>), grid, dim3(FEW_THREADS), 0, ctx->stream, f);
+        SG_CHECK_LAUNCH(ctx, "embedding_grad");
+        return SG_OK;
+    }
     // Chunks short enough that their wavefronts fill the chip (4096 tokens of 768: 768 wavefronts of 16 tokens), long enough
     // that a run over all tokens leaves few partial sums.
     m.chunk = s.n <= 16384 ? 16 : s.n <= 65536 ? 32 : 64;
@@ -460,7 +562,7 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
     const bool single = s.n <= SINGLE;
     s.tiles = single ? 1 : (s.n + TILE - 1) / TILE;
     // the sorted list, a second one to move between where there are several launches, the tiles' counts, the partial sums
-    const uint64_t list = (uint64_t)(s.n + 3) / 4 * 4, counts = single ? 0 : (uint64_t)s.tiles * s.digits;
+    const uint64_t list = (uint64_t)(s.n + 3) / 4 * 4, counts = single ? 0 : 2 * (uint64_t)s.tiles * s.digits;
     const uint64_t words = list * (single ? 2 : 4) + (counts + 3) / 4 * 4 + (uint64_t)m.chunks * 2 * E;
     sg_device_guard guard(ctx);
     sg_workspace space(ctx);
@@ -481,15 +583,19 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
         s.pos_out = pos[0];
         s.fill = table;
         s.fill_floats = table_floats;
-        hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)(1 + fill_blocks)), dim3(SORT_THREADS), 0, ctx->stream, s);
+        const dim3 grid((unsigned)(1 + fill_blocks));
+        if (s.n <= SORT_THREADS * 4) hipLaunchKernelGGL((embedding_sort_kernel<4>), grid, dim3(SORT_THREADS), 0, ctx->stream, s);
+        else hipLaunchKernelGGL((embedding_sort_kernel<8>), grid, dim3(SORT_THREADS), 0, ctx->stream, s);
         SG_CHECK_LAUNCH(ctx, "embedding_grad sort");
         m.key = key[0];
         m.pos = pos[0];
     } else {
         // every launch clears its share of the table
-        const uint32_t launches = 2 * s.passes;
+        const bool fused = (uint64_t)s.tiles * s.digits <= NEXT_COUNTS && s.passes == 2;
+        const uint32_t launches = fused ? 3 : 2 * s.passes;
         const uint64_t share = (fill_blocks + launches - 1) / launches;
         uint64_t cleared = 0;
+        uint32_t *const hist[2] = {s.hist, s.hist + (uint64_t)s.tiles * s.digits};
         auto take_share = [&]() {
             const uint64_t at = cleared * per_block;
             const uint64_t blocks = cleared + share <= fill_blocks ? share : fill_blocks - cleared;
@@ -505,9 +611,13 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
             s.pos_in = pos[(pass + 1) & 1];
             s.key_out = key[pass & 1];
             s.pos_out = pos[pass & 1];
-            const dim3 count_grid = take_share();
-            hipLaunchKernelGGL(embedding_count_kernel, count_grid, dim3(SORT_THREADS), 0, ctx->stream, s);
-            SG_CHECK_LAUNCH(ctx, "embedding_grad count");
+            s.hist = hist[fused ? pass : 0];
+            s.next_hist = fused && pass == 0 ? hist[1] : nullptr;
+            if (!fused || pass == 0) {
+                const dim3 count_grid = take_share();
+                hipLaunchKernelGGL(embedding_count_kernel, count_grid, dim3(SORT_THREADS), 0, ctx->stream, s);
+                SG_CHECK_LAUNCH(ctx, "embedding_grad count");
+            }
             const dim3 move_grid = take_share();
             hipLaunchKernelGGL(embedding_move_kernel, move_grid, dim3(SORT_THREADS), 0, ctx->stream, s);
             SG_CHECK_LAUNCH(ctx, "embedding_grad move");

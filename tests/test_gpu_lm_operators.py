@@ -81,7 +81,8 @@ def zipf_ids(rng, n, v):
     return np.minimum(np.exp(rng.random(n) * np.log(v + 1)).astype(np.int64) - 1, v - 1)
 
 
-@pytest.mark.parametrize("n,v,e", [(1, 1, 1), (1, 5, 768), (7, 3, 64), (64, 1000, 33), (257, 10, 260), (300, 70000, 4), (4096, 500, 96), (5, 100, 2050)])
+@pytest.mark.parametrize("n,v,e", [(1, 1, 1), (1, 5, 768), (7, 3, 64), (64, 1000, 33), (257, 10, 260), (300, 70000, 4), (4096, 500, 96), (5, 100, 2050),
+                                   (128, 3, 768), (128, 1000, 24), (127, 40000, 8), (129, 20, 70), (100, 700, 13), (8000, 4000, 12)])
 def test_embedding_and_gradient(ctx, n, v, e):
     say("embedding", n, v, e)
     rng = np.random.default_rng(n + v + e)
@@ -104,7 +105,7 @@ def test_embedding_and_gradient(ctx, n, v, e):
         first = got
 
 
-@pytest.mark.parametrize("n,distinct", [(2048, 1), (5000, 1), (20000, 3), (8193, 2), (70000, 5), (16384, 16384)])
+@pytest.mark.parametrize("n,distinct", [(2048, 1), (5000, 1), (20000, 3), (8193, 2), (70000, 5), (16384, 16384), (140000, 7), (128, 1)])
 def test_embedding_gradient_of_long_runs_and_many_tokens(ctx, n, distinct):
     """All tokens on a few rows of a large table, and every token on a row of its own."""
     say("runs", n, distinct)
