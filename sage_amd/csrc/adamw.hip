@@ -58,6 +58,15 @@ __device__ __forceinline__ int find_entry(const Entry *t, int count, uint32_t ch
     return lo;
 }
 
+// Large steps go past the caches: nothing of them is read again soon.
+template <bool NT, class T>
+__device__ __forceinline__ T load(const T *p) { return NT ? __builtin_nontemporal_load(p) : *p; }
+template <bool NT, class T>
+__device__ __forceinline__ void store(T *p, T x) {
+    if (NT) __builtin_nontemporal_store(x, p);
+    else *p = x;
+}
+
 struct Correction {
     float first, second;  // 1 / (1 - beta1^t), 1 / (1 - beta2^t)
 };
@@ -74,6 +83,7 @@ __device__ __forceinline__ void step_element(float &value, float g, float &m, fl
     value = value - a.lr * (m * c.first / (sqrtf(v * c.second) + a.eps) + a.decay * value);
 }
 
+template <bool NT>
 __global__ void __launch_bounds__(256) adamw_kernel(const StepArgs a) {
     const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
     const Correction c = correction(a);
@@ -84,8 +94,9 @@ __global__ void __launch_bounds__(256) adamw_kernel(const StepArgs a) {
         const uint32_t i = base + k * 1024 + threadIdx.x * 4;
         if (i >= t.n) return;
         if (t.vec && i + 4 <= t.n) {
-            f32x4 x = *reinterpret_cast<const f32x4 *>(t.value + i), m = *reinterpret_cast<const f32x4 *>(mp + i), v = *reinterpret_cast<const f32x4 *>(vp + i);
-            const f32x4 g = *reinterpret_cast<const f32x4 *>(t.grad + i);
+            f32x4 *xp = reinterpret_cast<f32x4 *>(t.value + i), *m4 = reinterpret_cast<f32x4 *>(mp + i), *v4 = reinterpret_cast<f32x4 *>(vp + i);
+            f32x4 x = load<NT>(xp), m = load<NT>(m4), v = load<NT>(v4);
+            const f32x4 g = load<NT>(reinterpret_cast<const f32x4 *>(t.grad + i));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float xj = x[j], mj = m[j], vj = v[j];
@@ -94,9 +105,9 @@ __global__ void __launch_bounds__(256) adamw_kernel(const StepArgs a) {
                 m[j] = mj;
                 v[j] = vj;
             }
-            *reinterpret_cast<f32x4 *>(t.value + i) = x;
-            *reinterpret_cast<f32x4 *>(mp + i) = m;
-            *reinterpret_cast<f32x4 *>(vp + i) = v;
+            store<NT>(xp, x);
+            store<NT>(m4, m);
+            store<NT>(v4, v);
         } else {
             for (uint32_t j = i; j < i + 4 && j < t.n; ++j) {
                 float x = t.value[j], m = mp[j], v = vp[j];
@@ -147,6 +158,7 @@ __device__ __forceinline__ uint32_t scale_exponent(uint32_t largest) {
 }
 
 // A wavefront takes a block of 256 elements, a lane 4 of them and one word of either state.
+template <bool NT>
 __global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
     const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
     const Correction c = correction(a);
@@ -162,7 +174,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
         float x[4] = {}, g[4] = {}, m[4], v[4];
         uint32_t mw = 0, vw = 0;
         if (left == 4 && t.vec) {
-            const f32x4 x4 = *reinterpret_cast<const f32x4 *>(t.value + i), g4 = *reinterpret_cast<const f32x4 *>(t.grad + i);
+            const f32x4 x4 = load<NT>(reinterpret_cast<const f32x4 *>(t.value + i)), g4 = load<NT>(reinterpret_cast<const f32x4 *>(t.grad + i));
 #pragma unroll
             for (int j = 0; j < 4; ++j) { x[j] = x4[j]; g[j] = g4[j]; }
         } else {
@@ -170,7 +182,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
             for (uint32_t j = 0; j < 4; ++j)
                 if (j < left) { x[j] = t.value[i + j]; g[j] = t.grad[i + j]; }
         }
-        if (left) { mw = mp[i / 4]; vw = vp[i / 4]; }
+        if (left) { mw = load<NT>(mp + i / 4); vw = load<NT>(vp + i / 4); }
         const uint32_t me = __float_as_uint(t.m_scale[block]) >> 23 & 255u, ve = __float_as_uint(t.v_scale[block]) >> 23 & 255u;
         uint32_t mtop = 0, vtop = 0;
 #pragma unroll
@@ -198,13 +210,13 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
             mw |= mc << (8 * j);
             vw |= vc << (8 * j);
         }
-        if (left == 4 && t.vec) *reinterpret_cast<f32x4 *>(t.value + i) = f32x4{x[0], x[1], x[2], x[3]};
+        if (left == 4 && t.vec) store<NT>(reinterpret_cast<f32x4 *>(t.value + i), f32x4{x[0], x[1], x[2], x[3]});
         else {
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
                 if (j < left) t.value[i + j] = x[j];
         }
-        if (left) { mp[i / 4] = mw; vp[i / 4] = vw; }
+        if (left) { store<NT>(mp + i / 4, mw); store<NT>(vp + i / 4, vw); }
         if (lane == 0) {
             t.m_scale[block] = __uint_as_float(me2 == 255 ? 0x7FC00000u : me2 << 23);
             t.v_scale[block] = __uint_as_float(ve2 == 255 ? 0x7FC00000u : ve2 << 23);
@@ -212,6 +224,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
     }
 }
 
+template <bool NT>
 __global__ void __launch_bounds__(256) adamw_state_read_kernel(const ReadArgs a) {
     const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
     const uint32_t base = (blockIdx.x - t.first_chunk) * CHUNK;
@@ -221,7 +234,7 @@ __global__ void __launch_bounds__(256) adamw_state_read_kernel(const ReadArgs a)
     for (uint32_t k = 0; k < CHUNK / 1024; ++k) {
         const uint32_t i = base + k * 1024 + threadIdx.x * 4;
         if (i >= t.n) return;
-        const uint32_t mw = mp[i / 4], vw = vp[i / 4];
+        const uint32_t mw = load<NT>(mp + i / 4), vw = load<NT>(vp + i / 4);
         const uint32_t me = __float_as_uint(t.m_scale[i / BLOCK]) >> 23 & 255u, ve = __float_as_uint(t.v_scale[i / BLOCK]) >> 23 & 255u;
         f32x4 m, v;
 #pragma unroll
@@ -230,8 +243,8 @@ __global__ void __launch_bounds__(256) adamw_state_read_kernel(const ReadArgs a)
             v[j] = decode(vw >> (8 * j) & 255u, ve, V_TOP);
         }
         if (t.vec && i + 4 <= t.n) {
-            *reinterpret_cast<f32x4 *>(mo + i) = m;
-            *reinterpret_cast<f32x4 *>(vo + i) = v;
+            store<NT>(reinterpret_cast<f32x4 *>(mo + i), m);
+            store<NT>(reinterpret_cast<f32x4 *>(vo + i), v);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
@@ -324,8 +337,11 @@ extern "C" int sg_adamw_update(sg_ctx *ctx, int n_tensors, const sg_tensor *valu
                 e.v_scale = f32_ptr(&v_scale[i]);
             }
         });
-        if (eight) hipLaunchKernelGGL(adamw8_kernel, dim3(chunks), dim3(256), 0, ctx->stream, a);
-        else hipLaunchKernelGGL(adamw_kernel, dim3(chunks), dim3(256), 0, ctx->stream, a);
+        const bool nt = sg_streaming((int64_t)chunks * CHUNK * (eight ? 16 : 28));
+        if (eight && nt) hipLaunchKernelGGL((adamw8_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, a);
+        else if (eight) hipLaunchKernelGGL((adamw8_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, a);
+        else if (nt) hipLaunchKernelGGL((adamw_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((adamw_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, a);
         SG_CHECK_LAUNCH(ctx, "adamw");
     }
     return SG_OK;
@@ -356,7 +372,8 @@ extern "C" int sg_adamw_state_read(sg_ctx *ctx, int n_tensors, const sg_tensor *
             e.v_scale = f32_ptr(&v_scale[i]);
             e.vec = aligned16(e.value) && aligned16(e.grad);
         });
-        hipLaunchKernelGGL(adamw_state_read_kernel, dim3(chunks), dim3(256), 0, ctx->stream, a);
+        if (sg_streaming((int64_t)chunks * CHUNK * 10)) hipLaunchKernelGGL((adamw_state_read_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((adamw_state_read_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, a);
         SG_CHECK_LAUNCH(ctx, "adamw_state_read");
     }
     return SG_OK;
