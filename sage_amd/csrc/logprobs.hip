@@ -380,7 +380,8 @@ constexpr float FAR = 128.0f;
 template <bool NT>
 __global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const LogpGradP p) {
     __shared__ float lds_stats[12];
-    const uint32_t row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts, tid = threadIdx.x;
+    // from the last row to the first: the forward call's last rows are still in the last-level cache
+    const uint32_t block = gridDim.x - 1 - blockIdx.x, row = block / p.parts, part = block - row * p.parts, tid = threadIdx.x;
     const float *x = p.logits + sg_row_offset(p.rows, row);
     float *y = p.glogits + (uint64_t)row * p.C;
     const float inf = __builtin_inff(), c = p.scale * LOG2E;
@@ -414,7 +415,8 @@ __global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const LogpGradP 
     for (uint32_t g = part * p.part + tid; g < last; g += THREADS) {
         const uint32_t j = groups.index(g, 0);
         if (groups.whole(g)) {
-            const f32x4 v = *reinterpret_cast<const f32x4_any *>(x + j);
+            const f32x4_any *xp = reinterpret_cast<const f32x4_any *>(x + j);
+            const f32x4 v = NT ? __builtin_nontemporal_load(xp) : *xp;
             const f32x4 o = {grad(v.x, j), grad(v.y, j + 1), grad(v.z, j + 2), grad(v.w, j + 3)};
             if (NT) __builtin_nontemporal_store(o, reinterpret_cast<f32x4 *>(y + j));
             else *reinterpret_cast<f32x4 *>(y + j) = o;
