@@ -284,12 +284,13 @@ struct SumP {
     float scale;
 };
 
-// 4 columns of a lane: consecutive (VEC) or 64 apart.
-template <bool VEC>
+// 4 columns of a lane: consecutive (VEC) or 64 apart.  NT: past the caches.
+template <bool VEC, bool NT = false>
 __device__ __forceinline__ f32x4 load_cols(const float *row, uint32_t c, uint32_t E) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (VEC) {
-        if (c < E) v = *reinterpret_cast<const f32x4 *>(row + c);
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(row + c);
+        if (c < E) v = NT ? __builtin_nontemporal_load(p) : *p;
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -373,8 +374,9 @@ __global__ void __launch_bounds__(FEW_THREADS) embedding_few_kernel(const FewP p
     }
 }
 
-// A wavefront sums 256 columns of one chunk of sorted tokens; BATCH rows are in flight at a time.
-template <bool VEC, uint32_t BATCH>
+// A wavefront sums 256 columns of one chunk of sorted tokens; BATCH rows are in flight at a time.  A large gout goes past
+// the caches and leaves them to the table, which the next lookup reads (32768 tokens: that lookup 32 -> 20 us).
+template <bool VEC, bool NT, uint32_t BATCH>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
     const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (unit >= p.chunks * p.pieces) return;
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
             const uint32_t at = min(b + k, last - 1) - first;
             id[k] = (uint32_t)__builtin_amdgcn_readlane((int)key, (int)at);
             if (b + k < last && id[k] < p.V)
-                x[k] = load_cols<VEC>(p.gout + sg_row_offset(p.g_rows, (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)at)), c, p.E);
+                x[k] = load_cols<VEC, NT>(p.gout + sg_row_offset(p.g_rows, (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)at)), c, p.E);
         }
         id[BATCH] = b + BATCH < last ? (uint32_t)__builtin_amdgcn_readlane((int)key, (int)(b + BATCH - first)) : next;
 #pragma unroll
@@ -628,8 +630,9 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
     bool vec = E % 4 == 0 && aligned16(m.gout) && aligned16(table);
     for (int i = 0; i < m.g_rows.rank; ++i) vec = vec && m.g_rows.st[i] % 4 == 0;
     const dim3 sum_grid((m.chunks * m.pieces + 3) / 4), join_grid((m.chunks - 1) * m.pieces);
-    if (vec) hipLaunchKernelGGL((embedding_sum_kernel<true, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
-    else hipLaunchKernelGGL((embedding_sum_kernel<false, 4>), sum_grid, dim3(256), 0, ctx->stream, m);
+    if (vec && sg_streaming((int64_t)m.n * E * 4)) hipLaunchKernelGGL((embedding_sum_kernel<true, true, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
+    else if (vec) hipLaunchKernelGGL((embedding_sum_kernel<true, false, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
+    else hipLaunchKernelGGL((embedding_sum_kernel<false, false, 4>), sum_grid, dim3(256), 0, ctx->stream, m);
     SG_CHECK_LAUNCH(ctx, "embedding_grad sums");
     if (m.chunks > 1) {
         if (vec) hipLaunchKernelGGL((embedding_join_kernel<true>), join_grid, dim3(256), 0, ctx->stream, m);
