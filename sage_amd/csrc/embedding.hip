@@ -437,12 +437,12 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const SumP p) {
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     if (wave == 0) acc = load_cols<VEC>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E);
     uint32_t i = from;
-    for (; i + 8 <= to; i += 8) {
-        f32x4 x[8];
+    for (; i + 16 <= to; i += 16) {
+        f32x4 x[16];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) x[k] = load_cols<VEC>(p.part + (uint64_t)(i + k) * 2 * p.E, c, p.E);
+        for (uint32_t k = 0; k < 16; ++k) x[k] = load_cols<VEC>(p.part + (uint64_t)(i + k) * 2 * p.E, c, p.E);
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) acc += x[k];
+        for (uint32_t k = 0; k < 16; ++k) acc += x[k];
     }
     for (; i < to; ++i) acc += load_cols<VEC>(p.part + (uint64_t)i * 2 * p.E, c, p.E);
     sums[wave][lane] = acc;
@@ -550,9 +550,10 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
         SG_CHECK_LAUNCH(ctx, "embedding_grad");
         return SG_OK;
     }
-    // Chunks short enough that their wavefronts fill the chip (4096 tokens of 768: 768 wavefronts of 16 tokens), long enough
-    // that a run over all tokens leaves few partial sums.
-    m.chunk = s.n <= 16384 ? 16 : s.n <= 65536 ? 32 : 64;
+    // Chunks short enough that their wavefronts fill the chip and none waits for rows twice (4096 tokens of 768: 8 a chunk 7.4 us,
+    // 16 10.4 us; 32768 tokens: 16 a chunk 18.9 us and a join of 6.6, 32 28.8 and 6.4, 8 21.6 and 8.6), long enough that a run over
+    // all tokens leaves few partial sums.
+    m.chunk = s.n <= 16384 ? 8 : s.n <= 65536 ? 16 : s.n <= 262144 ? 32 : 64;
     m.chunks = (s.n + m.chunk - 1) / m.chunk;
     if ((uint64_t)m.chunks * m.pieces >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_embedding_grad: too many elements for one launch");
 
