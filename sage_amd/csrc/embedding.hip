@@ -437,12 +437,12 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const SumP p) {
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     if (wave == 0) acc = load_cols<VEC>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E);
     uint32_t i = from;
-    for (; i + 16 <= to; i += 16) {
-        f32x4 x[16];
+    for (; i + 8 <= to; i += 8) {
+        f32x4 x[8];
 #pragma unroll
-        for (uint32_t k = 0; k < 16; ++k) x[k] = load_cols<VEC>(p.part + (uint64_t)(i + k) * 2 * p.E, c, p.E);
+        for (uint32_t k = 0; k < 8; ++k) x[k] = load_cols<VEC>(p.part + (uint64_t)(i + k) * 2 * p.E, c, p.E);
 #pragma unroll
-        for (uint32_t k = 0; k < 16; ++k) acc += x[k];
+        for (uint32_t k = 0; k < 8; ++k) acc += x[k];
     }
     for (; i < to; ++i) acc += load_cols<VEC>(p.part + (uint64_t)i * 2 * p.E, c, p.E);
     sums[wave][lane] = acc;
