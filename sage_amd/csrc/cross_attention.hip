@@ -832,24 +832,34 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
 // 16-byte aligned rows: loads straight into LDS take them.
 bool aligned_rows(const Rows &r) { return ((uintptr_t)r.p) % 16 == 0 && r.b % 4 == 0 && r.h % 4 == 0 && r.l % 4 == 0; }
 
-// Splits of a long axis of `blocks` blocks, where there are fewer than two workgroups for each compute unit: the number that
-// leaves the busiest compute unit the least, which works at three quarters of its rate on a single workgroup, a join's
-// traffic counted as 3 % a split.  (154 tiles of 1332 rows, 8 + 32 keys:
-// 3 splits, 462 workgroups, at most 2 on a compute unit, against 4, 616 and 3.)
-uint32_t choose_splits(const sg_ctx *ctx, uint64_t units, uint32_t blocks) {
+// How a kernel takes an axis of `own` rows (or keys) that walk `other` of the other side: wavefronts of a workgroup side by
+// side on it (the 4 / waves others share the blocks of the walk), and workgroups a walk is split over.
+struct Plan {
+    int waves;
+    uint32_t splits;
+};
+
+// The plan of the least estimated time: what the busiest compute unit has of 32 x 32 steps of `step_us`, at three quarters of
+// the rate where only one workgroup is there to work, 5 us for a join, a few per cent for the blocks that smaller tiles load
+// more often.  (1332 rows of 14 pairs, 1001 keys of size 32, forward: 4 waves in 3 splits 33 us and a join of 5, 1 wave 29 us and
+// none.  512 rows of 384 pairs, 512 keys of size 64: 4 waves 206 us, 2 waves 220 us.)
+Plan plan(const sg_ctx *ctx, int64_t D, uint32_t own, uint32_t other, uint32_t pairs, int least_waves, int most_waves, double step_us) {
     const uint64_t cus = (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
-    if (units >= 2 * cus) return 1;
-    uint32_t best = 1;
+    Plan best = {most_waves, 1};
     double least = 1e30;
-    for (uint32_t s = 1; s <= 64 && (s == 1 || (s <= blocks / 2 && units * s <= 3 * cus)); ++s) {
-        const uint64_t most = (units * s + cus - 1) / cus;
-        const double cost = (most == 1 ? 1.33 : (double)most) / s * (1.0 + 0.03 * s);
-        if (cost < least) { least = cost; best = s; }
+    for (int w = most_waves; w >= least_waves; w /= 2) {
+        const uint64_t units = (uint64_t)((own + 32 * w - 1) / (32 * w)) * pairs;
+        const uint32_t blocks = (other + 128 / w - 1) / (128 / w);
+        for (uint32_t s = 1; s <= 64 && (s == 1 || (s <= blocks / 2 && units * s <= 3 * cus)); ++s) {
+            const uint64_t most = (units * s + cus - 1) / cus;
+            const bool alone = most == 1 || (D == 64 && w == 1);  // 128 KB of LDS
+            const double cost = (double)most * ((blocks + s - 1) / s) * step_us * (alone ? 1.33 : 1.0) * (w == 4 ? 1.0 : w == 2 ? 1.05 : 1.08) +
+                                (s > 1 ? 5.0 + 0.2 * s : 0.0);
+            if (cost < least) { least = cost; best = {w, s}; }
+        }
     }
     return best;
 }
-
-int row_waves(int R) { return R <= 32 ? 1 : R <= 64 ? 2 : 4; }
 
 int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
     p.tiles = (uint32_t)tiles;
@@ -890,11 +900,22 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
     sg_device_guard guard(ctx);
     const int64_t D = q->extents[3];
     const bool few = p.R <= 8;
-    const int rw = row_waves(p.R), kb = 128 / rw;
-    const uint32_t tiles = few ? 1 : (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), total = p.pairs * (uint32_t)p.R;
-    const uint32_t blocks = (uint32_t)((p.Lk + kb - 1) / kb), cus = (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
-    // a serving step of at least as many pairs as compute units is not split: the join's launch costs more than it levels
-    if ((rc = set_tiles(ctx, p, tiles, few && p.pairs >= cus ? 1 : choose_splits(ctx, tiles * p.pairs, blocks))) != SG_OK) return rc;
+    const uint32_t total = p.pairs * (uint32_t)p.R;
+    Plan how;
+    if (few) {
+        // Bound by memory: two workgroups for each compute unit, of 128 keys at least.  From as many pairs as compute units on
+        // nothing is split: the join's launch costs more than it levels.
+        const uint32_t cus = (uint32_t)(ctx->num_cus > 0 ? ctx->num_cus : 256), most = (uint32_t)p.Lk / 128;
+        how.splits = p.pairs >= cus ? 1 : (2 * cus + p.pairs - 1) / p.pairs;
+        how.splits = how.splits > most ? most : how.splits;
+        how.splits = how.splits < 1 ? 1 : how.splits > 64 ? 64 : how.splits;
+        how.waves = 1;
+    } else {
+        how = plan(ctx, D, (uint32_t)p.R, (uint32_t)p.Lk, p.pairs, 1, 4, D == 64 ? 1.7 : 1.1);
+    }
+    const int rw = how.waves;
+    const uint32_t tiles = few ? 1 : (uint32_t)((p.R + 32 * rw - 1) / (32 * rw));
+    if ((rc = set_tiles(ctx, p, tiles, how.splits)) != SG_OK) return rc;
     sg_workspace space(ctx);
     if (p.splits > 1) {
         if ((rc = space.take((uint64_t)p.splits * total * (D + 2) * 4)) != SG_OK) return rc;
@@ -952,14 +973,13 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     p.strided = p.H == p.G || (p.q.h == p.Lq * p.q.l && p.go.h == p.Lq * p.go.l);
     sg_device_guard guard(ctx);
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
-    const int rw = row_waves(p.R), kb = 128 / rw;
-    // Keys a workgroup: 128 where all are visible and workgroups are many (32 x 12 heads of 512 x 512: 441 us against 463 with
-    // 64), else 64, which waste less of a sequence's last tile and level better (lengths 512 to 272: 432 against 421 us; 7 x 2
-    // key heads of 1001 keys, size 32: 64 against 57 us).
-    const int cw = !p.mask && (uint64_t)((p.Lk + 127) / 128) * p.pairs >= 1024 ? 4 : 2, rb = 128 / cw;
+    const Plan by_rows = plan(ctx, D, (uint32_t)p.R, (uint32_t)p.Lk, p.pairs, 1, 4, D == 64 ? 2.6 : 1.6);
+    // 128 keys a workgroup only where all are visible: smaller tiles waste less of a sequence's last one and level better
+    // (32 x 12 heads of 512 x 512: 441 us against 463 with 64 keys; with lengths 512 to 272: 432 against 421 us)
+    const Plan by_keys = plan(ctx, D, (uint32_t)p.Lk, (uint32_t)p.R, p.pairs, 2, p.mask ? 2 : 4, D == 64 ? 3.4 : 2.0);
+    const int rw = by_rows.waves, cw = by_keys.waves;
     const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 32 * cw - 1) / (32 * cw));
-    const uint32_t row_splits = choose_splits(ctx, row_tiles * p.pairs, (uint32_t)((p.Lk + kb - 1) / kb));
-    const uint32_t key_splits = choose_splits(ctx, key_tiles * p.pairs, (uint32_t)((p.R + rb - 1) / rb));
+    const uint32_t row_splits = by_rows.splits, key_splits = by_keys.splits;
     // delta, and the larger of the two kernels' split sums: they run one after the other
     const uint64_t rows_part = row_splits > 1 ? row_splits * total * D : 0, keys_part = key_splits > 1 ? 2 * key_splits * keys * D : 0;
     const uint64_t delta_floats = (total + (uint64_t)p.N + 3) / 4 * 4;  // delta and the lengths
