@@ -869,12 +869,12 @@ int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
     return SG_OK;
 }
 
-}  // namespace
-
 // Lengths in front of the launches, where there are more workgroups than the chip holds and lengths to order them by.
 bool orders_lengths(const sg_ctx *ctx, const CrossP &p, uint64_t workgroups) {
     return p.mask && p.N > 1 && p.N <= 256 && workgroups > 2u * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
 }
+
+}  // namespace
 
 #define SG_CROSS_ROWS_(KERNEL, D_, RW, DMA, GRID)                                                                       \
     do {                                                                                                                \

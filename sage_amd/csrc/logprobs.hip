@@ -554,6 +554,8 @@ extern "C" int sg_token_logprobs_grad(sg_ctx *ctx, const sg_tensor *logits, cons
     for (int i = 0; i < logits->rank; ++i)
         if (glogits->extents[i] != logits->extents[i]) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs_grad: glogits' extent[%d] differs from the logits'", i);
     if (!sg_is_dense(glogits)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs_grad: glogits must be dense row-major");
+    if (f32_ptr(glogits) == f32_ptr(logits) && !sg_is_dense(logits))
+        return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs_grad: in place of logits that are not dense row-major");
     if (!ctx) return SG_ERR_ARG;
     const int lead = logits->rank - 1;
     LogpGradP p{};

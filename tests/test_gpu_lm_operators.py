@@ -121,6 +121,25 @@ def test_embedding_gradient_of_long_runs_and_many_tokens(ctx, n, distinct):
     near(out.numpy(), want, tol, "gtable")
 
 
+@pytest.mark.parametrize("n,v", [(9000, 500), (8193, 511), (20000, 512), (70000, 60000), (30000, 262143), (9000, 262144), (140000, 60000)])
+def test_embedding_gradient_of_sorts_over_several_launches(ctx, n, v):
+    """One, two and three passes; the second pass counted by the first, or (many tiles) by a launch of its own; a gradient
+    with padded rows and permuted axes; the largest ids of their tables, and unknown ones."""
+    say("sort", n, v)
+    rng = np.random.default_rng(n + v)
+    ids = zipf_ids(rng, n, v).astype(np.uint32).reshape(2, n // 2) if n % 2 == 0 else zipf_ids(rng, n, v).astype(np.uint32).reshape(1, n)
+    ids[:, ::7] = v - 1
+    ids[:, ::11] = rng.integers(0, v, ids[:, ::11].shape)
+    ids[:, ::13] = v
+    ids[:, ::17] = 0xFFFFFFFF
+    g = R.f32(rng.standard_normal((*ids.shape, 8)))
+    want, tol = R.embedding_grad(g, ids, v, 1.0)
+    for gd in (dev(ctx, g), strided(ctx, g, pad=1, order=[1, 0, 2])):
+        out = dev(ctx, np.full((v, 8), np.nan, np.float32))
+        ctx.check(ctx._lib.sg_embedding_grad(ctx.handle, ref(gd), ref(dev(ctx, ids)), C.c_float(1.0), ref(out)))
+        near(out.numpy(), want, tol, "gtable")
+
+
 def test_embedding_strided_operands(ctx):
     """Ids of a wider batch (its last position dropped), a broadcast batch, a table and a gradient with padded or permuted rows."""
     rng = np.random.default_rng(3)
@@ -375,6 +394,30 @@ def test_cross_attention_masks(ctx, n, h, g, lq, lk, d):
     assert not got["out"][2].any() and np.isneginf(got["lse"][2]).all() and not got["gq"][2].any() and not got["gk"][2].any() and not got["gv"][2].any()
     again = run_cross(ctx, *[dev(ctx, a) for a in (q, k, v)], dev(ctx, mask), 0.2, dev(ctx, go))
     assert all(same_bits(got[x], again[x]) for x in got)
+
+
+# More workgroups than the chip holds (the longest sequences first; more than 256 sequences), walks split over workgroups, every
+# number of wavefronts side by side, few rows over many keys.
+@pytest.mark.parametrize("n,h,g,lq,lk,d,masked", [
+    (24, 12, 12, 70, 96, 32, True), (24, 12, 12, 70, 96, 64, True), (300, 2, 1, 40, 50, 32, True), (40, 8, 4, 200, 130, 64, True), (24, 12, 12, 96, 128, 64, False),
+    (5, 4, 4, 9, 2000, 64, True), (8, 16, 4, 100, 200, 32, False), (9, 12, 12, 512, 33, 64, True), (1, 1, 1, 2000, 2000, 64, False), (1, 1, 1, 2000, 2000, 32, True),
+    (22, 12, 12, 250, 40, 32, True), (4, 2, 2, 200, 31, 32, True), (40, 12, 12, 97, 100, 32, True), (3, 2, 2, 700, 300, 32, False), (2, 2, 2, 1, 7000, 32, False), (2, 4, 2, 2, 5000, 64, True), (2, 8, 1, 1, 3000, 64, True),
+    (300, 1, 1, 8, 70, 32, True), (1, 2, 1, 1, 4000, 32, True), (2, 3, 1, 1, 900, 32, True), (1, 4, 2, 1, 600, 64, True)])
+def test_cross_attention_of_many_and_of_long_sequences(ctx, n, h, g, lq, lk, d, masked):
+    """Against the formula; rows that begin at any element give the bits that aligned ones give."""
+    say("paths", n, h, g, lq, lk, d, masked)
+    rng = np.random.default_rng(n * lq + lk)
+    q, k, v, go = cross_case(rng, n, h, g, lq, lk, d)
+    mask = None
+    if masked:
+        lengths = rng.integers(0, lk + 1, n)
+        lengths[:1] = lk
+        mask = R.f32((np.arange(lk)[None] < lengths[:, None]) & (rng.random((n, lk)) < 0.9))
+    got = check_cross(ctx, q, k, v, mask, 1 / np.sqrt(d), go)
+    m = None if mask is None else strided(ctx, mask, pad=1, offset=1)
+    again = run_cross(ctx, *[strided(ctx, a, pad=1, offset=1) for a in (q, k, v)], m, 1 / np.sqrt(d), strided(ctx, go, pad=3, offset=2))
+    for name in got:
+        assert same_bits(got[name], again[name]), name
 
 
 def test_cross_attention_large_scores_do_not_overflow(ctx):

@@ -97,6 +97,9 @@ def test_token_logprobs_refusals():
     assert lp_grad(ge=desc([2, 4])) == abi.ERR_SHAPE
     assert lp_grad(out=desc([2, 3, 50], strides=[160, 50, 1])) == abi.ERR_SHAPE
     assert lp_grad(out=desc([6, 50])) == abi.ERR_SHAPE
+    # in place of logits with padded rows or of one row for all: other places than the gradient's
+    assert lp_grad(logits=desc([2, 3, 50], strides=[160, 50, 1])) == lp_grad(logits=desc([2, 3, 50], strides=[0, 0, 1])) == abi.ERR_SHAPE
+    assert lp_grad(logits=desc([2, 3, 50], strides=[160, 50, 1]), out=desc([2, 3, 50], base=8192)) == OK_BUT_NO_CONTEXT
 
 
 Q, K, M, L = [2, 4, 5, 32], [2, 2, 7, 32], [2, 7], [2, 4, 5]
