@@ -354,9 +354,9 @@ int sg_adam_update(sg_ctx *ctx, int n_tensors, const sg_tensor *values, const sg
  * A new state is cut to a byte after 16 bits of noise are added below the bits that are kept (so it is rounded up or down
  * with the chance that keeps its mean; a step moves v by less than half a code), and a v that is not zero does not become
  * zero.  The noise of element i is a hash of i + seed + t, low half for m, high half for v: h = i 0x9E3779B9 + seed +
- * t 0xAC502949; h = (h ^ h >> 16) 0x82D3099F; h = (h ^ h >> 15) 0x2ACAE79F; h ^= h >> 16.  A value or gradient that is
- * not finite makes its value and state not finite (an 8-bit state: its whole block, NaN).  Two tensors of a call must not
- * share memory. */
+ * t 0xAC502949; h = (h ^ h >> 16) 0x82D3099F; h = (h ^ h >> 15) 0x2ACAE79F; h ^= h >> 16.  A gradient that is not finite makes
+ * its value and state not finite; a value that is not finite stays so.  In 8 bits a state that is not finite, or is beyond
+ * 1.875 * 2^127, makes its whole block NaN from there on.  Two tensors of a call must not share memory. */
 int sg_adamw_update(sg_ctx *ctx, int n_tensors, const sg_tensor *values, const sg_tensor *grads, const sg_tensor *m,
                     const sg_tensor *v, const sg_tensor *m_scale, const sg_tensor *v_scale, const sg_tensor *step,
                     const sg_adam_hyper *h, uint32_t seed);

@@ -1,7 +1,7 @@
 """Optimizers: host-side mirror of optim.rs.
 
 As in the reference an update is a handful of map expressions per parameter, evaluated eagerly
-(optim.rs:128-131 "eager-execution like mode"); nothing here has a kernel of its own.  `grads` is the
+(optim.rs:128-131 "eager-execution like mode"); AdamW alone is one call for all parameters.  `grads` is the
 {parameter: gradient Var} mapping of `grad_param`; every gradient must already hold its value (the
 reference warns and evaluates it inside the optimizer otherwise, optim.rs:55-58, 144-147; so do we).
 
@@ -19,6 +19,7 @@ Reference behaviour that is kept because results would differ otherwise:
 """
 import ctypes as C
 
+from .shape import Shape
 from .tensor import Tensor
 from .var import Var, evaluate, params_changed, scalar
 
@@ -304,11 +305,11 @@ class AdamW(Optimizer):
         return prog
 
     def state(self, param, ctx):
-        """(m, v) of a parameter as fp32 tensors, whatever the bits they are held in."""
+        """(m, v) of a parameter as fp32 tensors of its extents: with 32 bits the states themselves, with 8 what they stand for."""
         from . import abi
         s = self.states[param]
         if self.state_bits == 32:
-            return s
+            return tuple(x.with_shape(Shape(param.extents)) for x in s)
         out = tuple(Tensor.uninit(ctx, param.extents) for _ in range(2))
         arrays = [(abi.sg_tensor * 1)(x.c()) for x in s + out]
         ctx.check(ctx._lib.sg_adamw_state_read(ctx.handle, 1, *arrays))
