@@ -117,6 +117,54 @@ __device__ __forceinline__ Work find_work(const CrossP &p, int *lds) {
     return w;
 }
 
+// The same for tiles of KEYS keys, whose work does not depend on the length but is nothing behind it.  Where the lengths are
+// known, the tiles that hold visible keys come first, an eighth of them for each XCD, a pair's behind one another, and the
+// others, which only write zeros, last: every compute unit gets as many of the former (7 x 2 key heads, 1001 keys, lengths
+// 1001 to 501: 57 -> 44 us).  b is -1 for what rounds the grid up to the 8 XCDs.  lds: 8 words.
+template <int KEYS>
+__device__ __forceinline__ Work find_key_work(const CrossP &p, int *lds) {
+    if (!p.ends) return find_work(p, lds);
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, units = p.G * p.splits, all = units * p.tiles;
+    const int mine = t < (uint32_t)p.N ? p.ends[t] : 0;
+    const uint32_t count = (uint32_t)((mine + KEYS - 1) / KEYS) * units;
+    uint32_t sum = count;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = (uint32_t)__shfl_up((int)sum, o, 64);
+        if ((int)lane >= o) sum += y;
+    }
+    if (lane == 63) lds[wave] = (int)sum;
+    if (t == 0) lds[4] = -1;
+    __syncthreads();
+    uint32_t total = 0, before = sum - count;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        if (i < wave) before += (uint32_t)lds[i];
+        total += (uint32_t)lds[i];
+    }
+    const uint32_t id = blockIdx.x, per = (total + 7) / 8, slot = id >> 3, at = (id & 7) * per + slot;
+    const bool first = slot < per && at < total;                   // one with visible keys
+    const uint32_t place = first ? at : slot < per ? at - total : id - total;
+    const uint32_t from = first ? before : t * all - before, n = first ? count : all - count;
+    if (t < (uint32_t)p.N && place >= from && place - from < n) {
+        lds[4] = (int)t;
+        lds[5] = mine;
+        lds[6] = (int)(place - from);
+    }
+    __syncthreads();
+    Work w;
+    w.b = __builtin_amdgcn_readfirstlane(lds[4]);
+    w.end = __builtin_amdgcn_readfirstlane(lds[5]);
+    const uint32_t rest = (uint32_t)__builtin_amdgcn_readfirstlane(lds[6]);
+    if (w.b < 0) return w;
+    const uint32_t seen = (uint32_t)((w.end + KEYS - 1) / KEYS), tiles = first ? seen : p.tiles - seen, unit = rest / tiles;
+    w.tile = rest - unit * tiles + (first ? 0 : seen);
+    w.split = unit / (uint32_t)p.G;
+    w.g = (int)(unit - w.split * (uint32_t)p.G);
+    w.pair = (uint32_t)(w.b * p.G + w.g);
+    return w;
+}
+
 // Element offset of row r of a pair.
 __device__ __forceinline__ int64_t row_at(const CrossP &p, const Rows &x, const Work &w, uint32_t r) {
     const uint32_t hh = fdiv(r, p.d_lq);
@@ -653,9 +701,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) c
     constexpr int GW = 4 / CW, RB = 32 * GW, ND = D / 32, KEYS = 32 * CW, SLOT = 32 * ND;
     __shared__ __attribute__((aligned(16))) float lds0[2 * RB * D], lds1[2 * RB * D];  // two buffers of rows of Q and dO
     __shared__ __attribute__((aligned(16))) float rows0[2 * RB], rows1[2 * RB];        // their lse and delta
-    __shared__ int lds_end[4];
+    __shared__ int lds_end[8];
     static_assert((GW - 1) * CW * 64 * SLOT <= 2 * RB * D, "the merge fits in a buffer");
-    const Work w = find_work(p, lds_end);
+    const Work w = find_key_work<KEYS>(p, lds_end);
+    if (w.b < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
     const int j0 = (int)w.tile * KEYS, j = j0 + (wave % CW) * 32 + c, rw = wave / CW * 32;
     const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h, *V = p.v.p + w.b * p.v.b + w.g * p.v.h;
@@ -749,20 +798,30 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) c
     }
 }
 
-// out[row] = sum of the splits' rows, in order: D / 4 lanes a row.  Rows of a pair are `heads` x `length`.  blockIdx.y: which
-// of two such sums.
+// out[row] = sum of the splits' rows, in order: D / 4 lanes a row.  Rows are [batch][heads][length].  The gradients that were
+// split, one after the other in one launch.
+struct SumJob {
+    const float *part;
+    Rows out;
+    uint32_t total, splits, heads, length;
+    uint32_t first_block;
+};
+struct SumJobs {
+    SumJob job[3];
+    int count;
+};
 template <int D>
-__global__ void __launch_bounds__(256) cross_sum_kernel(const float *part0, const float *part1, Rows out0, Rows out1, uint32_t total, uint32_t splits,
-                                                        uint32_t heads, uint32_t length) {
+__global__ void __launch_bounds__(256) cross_sum_kernel(const SumJobs jobs) {
     constexpr int LPR = D / 4;
-    const float *part = blockIdx.y ? part1 : part0;
-    const Rows out = blockIdx.y ? out1 : out0;
-    const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
-    if (row >= total) return;
-    f32x4 acc = *reinterpret_cast<const f32x4 *>(part + (int64_t)row * D + col);
-    for (uint32_t i = 1; i < splits; ++i) acc += *reinterpret_cast<const f32x4 *>(part + ((int64_t)i * total + row) * D + col);
-    const uint32_t bh = row / length;
-    store4(const_cast<float *>(out.p) + bh / heads * out.b + bh % heads * out.h + (int64_t)(row - bh * length) * out.l + col, acc);
+    int which = 0;
+    while (which + 1 < jobs.count && blockIdx.x >= jobs.job[which + 1].first_block) ++which;
+    const SumJob &j = jobs.job[which];
+    const uint32_t row = (blockIdx.x - j.first_block) * (256 / LPR) + threadIdx.x / LPR, col = threadIdx.x % LPR * 4;
+    if (row >= j.total) return;
+    f32x4 acc = *reinterpret_cast<const f32x4 *>(j.part + (int64_t)row * D + col);
+    for (uint32_t i = 1; i < j.splits; ++i) acc += *reinterpret_cast<const f32x4 *>(j.part + ((int64_t)i * j.total + row) * D + col);
+    const uint32_t bh = row / j.length;
+    store4(const_cast<float *>(j.out.p) + bh / j.heads * j.out.b + bh % j.heads * j.out.h + (int64_t)(row - bh * j.length) * j.out.l + col, acc);
 }
 
 int check_operand(sg_ctx *ctx, const sg_tensor *t, int64_t n, int64_t heads, int64_t len, int64_t D, const char *who, Rows *r) {
@@ -839,22 +898,25 @@ struct Plan {
     uint32_t splits;
 };
 
-// The plan of the least estimated time: what the busiest compute unit has of 32 x 32 steps of `step_us`, at three quarters of
-// the rate where only one workgroup is there to work, 5 us for a join, a few per cent for the blocks that smaller tiles load
-// more often.  (1332 rows of 14 pairs, 1001 keys of size 32, forward: 4 waves in 3 splits 33 us and a join of 5, 1 wave 29 us and
-// none.  512 rows of 384 pairs, 512 keys of size 64: 4 waves 206 us, 2 waves 220 us.)
-Plan plan(const sg_ctx *ctx, int64_t D, uint32_t own, uint32_t other, uint32_t pairs, int least_waves, int most_waves, double step_us) {
+// The plan of the least estimated time: what the busiest compute unit has of workgroups, each so many blocks of `step_us` and
+// 1.5 us to begin and end, at three quarters of the rate where only one is there to work; a join of 4 us and 0.4 a split; a
+// fifth more for the blocks that smaller tiles load more often.  With a mask, of which only the device knows the lengths,
+// three quarters of the keys are taken to be visible: finer workgroups then level what the lengths leave uneven.
+// (1332 rows of 14 pairs, 1001 keys of size 32, lengths 1001 to 501: forward 4 wavefronts side by side in 3 splits 33 us and a
+// join of 5, 1 wavefront 29 and none; gradient of the queries 43 and a sum, 39 and none.  512 rows of 384 pairs, 512 keys of
+// size 64: 4 wavefronts 186 and 266 us, 2 wavefronts 220 and 300.)
+Plan plan(const sg_ctx *ctx, const CrossP &p, int64_t D, int own, int other, int least_waves, int most_waves, double step_us) {
     const uint64_t cus = (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
     Plan best = {most_waves, 1};
     double least = 1e30;
     for (int w = most_waves; w >= least_waves; w /= 2) {
-        const uint64_t units = (uint64_t)((own + 32 * w - 1) / (32 * w)) * pairs;
-        const uint32_t blocks = (other + 128 / w - 1) / (128 / w);
+        const uint64_t units = (uint64_t)((own + 32 * w - 1) / (32 * w)) * p.pairs;
+        const uint32_t blocks = (uint32_t)((other + 128 / w - 1) / (128 / w));
         for (uint32_t s = 1; s <= 64 && (s == 1 || (s <= blocks / 2 && units * s <= 3 * cus)); ++s) {
-            const uint64_t most = (units * s + cus - 1) / cus;
+            const uint64_t most = ((p.mask ? units * s * 3 / 4 : units * s) + cus - 1) / cus;
             const bool alone = most == 1 || (D == 64 && w == 1);  // 128 KB of LDS
-            const double cost = (double)most * ((blocks + s - 1) / s) * step_us * (alone ? 1.33 : 1.0) * (w == 4 ? 1.0 : w == 2 ? 1.05 : 1.08) +
-                                (s > 1 ? 5.0 + 0.2 * s : 0.0);
+            const double block_us = step_us * (alone ? 1.33 : 1.0) * (w == 4 ? 1.0 : w == 2 ? 1.15 : 1.2);
+            const double cost = (double)most * ((blocks + s - 1) / s * block_us + 1.5) + (s > 1 ? 4.0 + 0.4 * s : 0.0);
             if (cost < least) { least = cost; best = {w, s}; }
         }
     }
@@ -869,9 +931,9 @@ int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
     return SG_OK;
 }
 
-// Lengths in front of the launches, where there are more workgroups than the chip holds and lengths to order them by.
-bool orders_lengths(const sg_ctx *ctx, const CrossP &p, uint64_t workgroups) {
-    return p.mask && p.N > 1 && p.N <= 256 && workgroups > 2u * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+// Lengths in front of the launches, where there are more workgroups than `each` for a compute unit and lengths to order them by.
+bool orders_lengths(const sg_ctx *ctx, const CrossP &p, uint64_t workgroups, uint32_t each) {
+    return p.mask && p.N > 1 && p.N <= 256 && workgroups > each * (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
 }
 
 }  // namespace
@@ -911,7 +973,7 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
         how.splits = how.splits < 1 ? 1 : how.splits > 64 ? 64 : how.splits;
         how.waves = 1;
     } else {
-        how = plan(ctx, D, (uint32_t)p.R, (uint32_t)p.Lk, p.pairs, 1, 4, D == 64 ? 1.7 : 1.1);
+        how = plan(ctx, p, D, p.R, p.Lk, 1, 4, D == 64 ? 1.7 : 1.1);
     }
     const int rw = how.waves;
     const uint32_t tiles = few ? 1 : (uint32_t)((p.R + 32 * rw - 1) / (32 * rw));
@@ -921,7 +983,7 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
         if ((rc = space.take((uint64_t)p.splits * total * (D + 2) * 4)) != SG_OK) return rc;
         p.part_o = (float *)space.p;
         p.part_ml = p.part_o + (uint64_t)p.splits * total * D;
-    } else if (!few && orders_lengths(ctx, p, (uint64_t)tiles * p.pairs)) {
+    } else if (!few && orders_lengths(ctx, p, (uint64_t)tiles * p.pairs, 2)) {
         if ((rc = space.take((uint64_t)p.N * 4)) != SG_OK) return rc;
         p.ends = (int *)space.p;
         hipLaunchKernelGGL(cross_ends_kernel, dim3((unsigned)p.N), dim3(256), 0, ctx->stream, p);
@@ -973,41 +1035,35 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     p.strided = p.H == p.G || (p.q.h == p.Lq * p.q.l && p.go.h == p.Lq * p.go.l);
     sg_device_guard guard(ctx);
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
-    const Plan by_rows = plan(ctx, D, (uint32_t)p.R, (uint32_t)p.Lk, p.pairs, 1, 4, D == 64 ? 2.6 : 1.6);
+    const Plan by_rows = plan(ctx, p, D, p.R, p.Lk, 1, 4, D == 64 ? 2.6 : 1.6);
     // 128 keys a workgroup only where all are visible: smaller tiles waste less of a sequence's last one and level better
     // (32 x 12 heads of 512 x 512: 441 us against 463 with 64 keys; with lengths 512 to 272: 432 against 421 us)
-    const Plan by_keys = plan(ctx, D, (uint32_t)p.Lk, (uint32_t)p.R, p.pairs, 2, p.mask ? 2 : 4, D == 64 ? 3.4 : 2.0);
+    const Plan by_keys = plan(ctx, p, D, p.Lk, p.R, 2, p.mask ? 2 : 4, D == 64 ? 3.4 : 2.0);
     const int rw = by_rows.waves, cw = by_keys.waves;
     const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 32 * cw - 1) / (32 * cw));
     const uint32_t row_splits = by_rows.splits, key_splits = by_keys.splits;
-    // delta, and the larger of the two kernels' split sums: they run one after the other
+    // delta and the lengths, the split sums of both kernels
     const uint64_t rows_part = row_splits > 1 ? row_splits * total * D : 0, keys_part = key_splits > 1 ? 2 * key_splits * keys * D : 0;
-    const uint64_t delta_floats = (total + (uint64_t)p.N + 3) / 4 * 4;  // delta and the lengths
+    const uint64_t delta_floats = (total + (uint64_t)p.N + 3) / 4 * 4;
     sg_workspace space(ctx);
-    if ((rc = space.take((delta_floats + (rows_part > keys_part ? rows_part : keys_part)) * 4)) != SG_OK) return rc;
+    if ((rc = space.take((delta_floats + rows_part + keys_part) * 4)) != SG_OK) return rc;
     p.delta = (float *)space.p;
-    p.part_o = p.part_k = p.delta + delta_floats;
+    p.part_o = p.delta + delta_floats;
+    p.part_k = p.part_o + rows_part;
     p.part_v = p.part_k + key_splits * keys * D;
-    if (orders_lengths(ctx, p, (uint64_t)key_tiles * p.pairs)) {
+    if (orders_lengths(ctx, p, (uint64_t)key_tiles * key_splits * p.pairs, 1)) {
         p.ends = (int *)(p.delta + total);
         hipLaunchKernelGGL(cross_ends_kernel, dim3((unsigned)p.N), dim3(256), 0, ctx->stream, p);
         SG_CHECK_LAUNCH(ctx, "cross_attention_grad lengths");
     }
-    auto sum = [&](unsigned count, const float *part0, const float *part1, const Rows &to0, const Rows &to1, uint64_t n, uint32_t splits, int heads, int length) {
-        const dim3 grid((unsigned)((n + 1024 / D - 1) / (1024 / D)), count);
-        if (D == 64) hipLaunchKernelGGL((cross_sum_kernel<64>), grid, dim3(256), 0, ctx->stream, part0, part1, to0, to1, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
-        else hipLaunchKernelGGL((cross_sum_kernel<32>), grid, dim3(256), 0, ctx->stream, part0, part1, to0, to1, (uint32_t)n, splits, (uint32_t)heads, (uint32_t)length);
-    };
     if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
     const bool dma = aligned_rows(p.q) && aligned_rows(p.k) && aligned_rows(p.v) && aligned_rows(p.o) && aligned_rows(p.go);
     SG_CROSS_ROWS(cross_gq_kernel, rw, dma, dim3(p.tiles * p.pairs * p.splits));
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
-    if (row_splits > 1) {
-        sum(1, p.part_o, p.part_o, p.gq, p.gq, total, row_splits, p.H, p.Lq);
-        SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries' sums");
-    }
     if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
-    const dim3 grid(p.tiles * p.pairs * p.splits);
+    uint32_t workgroups = p.tiles * p.pairs * p.splits;
+    if (p.ends) workgroups = (workgroups + 7) / 8 * 8;
+    const dim3 grid(workgroups);
 #define SG_CROSS_KEYS(D_, CW, DMA) hipLaunchKernelGGL((cross_gkv_kernel<D_, CW, DMA>), grid, dim3(256), 0, ctx->stream, p)
 #define SG_CROSS_KEYS_(D_, CW)                 \
     do {                                       \
@@ -1021,9 +1077,20 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
 #undef SG_CROSS_KEYS_
 #undef SG_CROSS_KEYS
     SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys and values");
-    if (key_splits > 1) {
-        sum(2, p.part_k, p.part_v, p.gk, p.gv, keys, key_splits, p.G, p.Lk);
-        SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys' sums");
+    SumJobs sums{};
+    uint32_t blocks = 0;
+    auto add = [&](const float *part, const Rows &out, uint64_t rows, uint32_t splits, int heads, int length) {
+        if (splits == 1) return;
+        sums.job[sums.count++] = {part, out, (uint32_t)rows, splits, (uint32_t)heads, (uint32_t)length, blocks};
+        blocks += (uint32_t)((rows + 1024 / D - 1) / (1024 / D));
+    };
+    add(p.part_o, p.gq, total, row_splits, p.H, p.Lq);
+    add(p.part_k, p.gk, keys, key_splits, p.G, p.Lk);
+    add(p.part_v, p.gv, keys, key_splits, p.G, p.Lk);
+    if (blocks) {
+        if (D == 64) hipLaunchKernelGGL((cross_sum_kernel<64>), dim3(blocks), dim3(256), 0, ctx->stream, sums);
+        else hipLaunchKernelGGL((cross_sum_kernel<32>), dim3(blocks), dim3(256), 0, ctx->stream, sums);
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad sums");
     }
     return SG_OK;
 }
