@@ -11,7 +11,7 @@ from sage_amd import var as V
 from sage_amd.grad import grad, grad_param
 from sage_amd.layers import Dense, Embedding, Layer
 from sage_amd.shape import Shape, default_strides
-from sage_amd.tensor import FLOAT, INT, UINT, Tensor
+from sage_amd.tensor import FLOAT, INT, UINT, Buffer, Tensor
 from sage_amd.var import Program, Var
 from tests import lm_reference as R
 
@@ -761,4 +761,91 @@ def test_out_of_memory_is_reported_and_harmless(ctx):
     want, tol = R.embedding_grad(g.numpy(), ids.numpy(), 50, 1.0)
     near(out.numpy(), want, tol, "gtable")
     del ids, g, out
+    c.close()
+
+
+def test_rows_beyond_two_to_the_31_elements(ctx):
+    """Rows 2^24 + 4 elements apart in one buffer of 8.7 GB: the last ones begin behind element 2^31."""
+    rows, stride = 130, (1 << 24) + 4
+    assert (rows - 1) * stride > 1 << 31
+    buf = Buffer(ctx, ((rows - 1) * stride + 4096) * 4)
+
+    def view(offset, extents):
+        return Tensor(buf, FLOAT, Shape(extents, [0] * (len(extents) - 2) + [stride, 1], offset))
+
+    def far(a, offset, extents=None):
+        for i, row in enumerate(a):
+            ctx.check(ctx._lib.sg_memcpy_h2d(ctx.handle, C.c_void_p(buf.ptr + (i * stride + offset) * 4), row.ctypes.data_as(C.c_void_p), row.nbytes))
+        return view(offset, extents or list(a.shape))
+
+    def back(offset, cols):
+        out = np.empty((rows, cols), np.float32)
+        for i in range(rows):
+            ctx.check(ctx._lib.sg_memcpy_d2h(ctx.handle, out[i].ctypes.data_as(C.c_void_p), C.c_void_p(buf.ptr + (i * stride + offset) * 4), cols * 4))
+        return out
+
+    rng = np.random.default_rng(21)
+    for lq, d in ((40, 64), (1, 64), (50, 32)):
+        say("far cross", lq, d)
+        q, k, v, go = cross_case(rng, 1, 1, 1, lq, rows, d)
+        kf, vf = (far(x[0, 0], o, [1, 1, rows, d]) for x, o in ((k, 0), (v, 64)))
+        out, lse, gq = Tensor.uninit(ctx, [1, 1, lq, d]), Tensor.uninit(ctx, [1, 1, lq]), Tensor.uninit(ctx, [1, 1, lq, d])
+        qd, god = dev(ctx, q), dev(ctx, go)
+        ctx.check(ctx._lib.sg_cross_attention(ctx.handle, ref(qd), ref(kf), ref(vf), None, C.c_float(0.1), ref(out), ref(lse)))
+        near(out.numpy(), R.cross(q, k, v, None, 0.1)[0], R.cross_tol(q, k, v, None, 0.1)[0], "out")
+        ctx.check(ctx._lib.sg_cross_attention_grad(ctx.handle, ref(qd), ref(kf), ref(vf), None, C.c_float(0.1), ref(out), ref(lse), ref(god), ref(gq),
+                                                   ref(view(128, [1, 1, rows, d])), ref(view(192, [1, 1, rows, d]))))
+        want, tol = R.cross_grad(q, k, v, None, 0.1, go), R.cross_grad_tol(q, k, v, None, 0.1, go)
+        for got, w, t, name in zip((gq.numpy()[0, 0], back(128, d), back(192, d)), want, tol, ("gq", "gk", "gv")):
+            near(got, w[0, 0], np.broadcast_to(t, w.shape)[0, 0], name)
+    say("far embedding")
+    table, ids = R.f32(rng.standard_normal((rows, 60))), rng.permutation(rows).astype(np.uint32)
+    out = Tensor.uninit(ctx, [rows, 60])
+    ctx.check(ctx._lib.sg_embedding(ctx.handle, ref(far(table, 256)), ref(dev(ctx, ids)), C.c_float(2.0), ref(out)))
+    assert same_bits(out.numpy(), R.embedding(table, ids, 2.0))
+    ctx.check(ctx._lib.sg_embedding_grad(ctx.handle, ref(view(256, [rows, 60])), ref(dev(ctx, ids)), C.c_float(2.0), ref(out)))
+    want, tol = R.embedding_grad(table, ids, rows, 2.0)
+    near(out.numpy(), want, tol, "gtable")
+    say("far logprobs")
+    x, tokens = R.f32(rng.standard_normal((rows, 1001))), rng.integers(0, 1001, rows).astype(np.int32)
+    got = run_logprobs(ctx, far(x, 512), tokens, 1.0, 3)
+    want = R.logprobs(x, tokens, 1.0, 3)
+    near(got["logprob"], want["logprob"], R.logprobs_tol(x, 1.0)[0], "logprob")
+    assert np.array_equal(got["top_ids"], want["top_ids"])
+
+
+def test_captured_in_a_caching_context_beside_another_context(ctx):
+    """A graph whose workspaces come from the chunks of a caching allocator keeps them while eager calls of this context and of
+    another one, on a stream of its own, take and give back workspaces."""
+    c = S.Context(use_cache=True)
+    rng = np.random.default_rng(31)
+
+    def calls(where, n, lk):
+        ids, g = zipf_ids(rng, n, 400).astype(np.uint32), R.f32(rng.standard_normal((n, 24)))
+        q, k, v, go = cross_case(rng, 2, 2, 1, 20, lk, 32)
+        mask = R.f32(np.arange(lk)[None] < np.array([[lk], [lk // 3]]))
+        x = R.f32(rng.standard_normal((3, 30000)))
+        new = lambda a: Var.new(dev(where, a))  # noqa: E731
+        vs = [new(a) for a in (q, k, v)]
+        at = nn.cross_attention(*vs, new(mask))
+        lp = nn.token_logprobs(new(x), top=5)
+        return Program(where, [Var(Shape([400, 24]), FLOAT, "embedding_grad", [new(g), new(ids)], {"scale": 1.0}), at,
+                               *grad(at, vs, seed=new(go)), lp.top_ids, lp.entropy])
+    prog = calls(c, 9000, 1500)
+    want = [o.numpy() for o in prog.outputs]
+    other = calls(ctx, 3000, 700)
+    other_want = [o.numpy() for o in other.outputs]
+    prog.capture()
+    for i in range(3):
+        prog.run()
+        other.run()
+        again = calls(c, 1000 + 3000 * i, 200 + 600 * i)
+        del again
+        c.sync()
+        ctx.sync()
+        for p, w in ((prog, want), (other, other_want)):
+            for o, a in zip(p.outputs, w):
+                assert same_bits(o.numpy(), a)
+    prog.release_graph()
+    del prog
     c.close()
