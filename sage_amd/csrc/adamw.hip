@@ -1,7 +1,8 @@
 // One AdamW step over many parameters, in place, with states in 32 or in 8 bits, for gfx950.
 //   m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g g
 //   value' = value - lr ((m' / (1 - beta1^t)) / (sqrt(v' / (1 - beta2^t)) + eps) + decay value)
-// Bound by memory: 28 bytes an element with states in 32 bits, 16 with states in 8.
+// Bound by memory: 28 bytes an element with states in 32 bits, 16 with states in 8, 10 to read the latter.  78.6 M values in 193
+// tensors: 390 us (5.6 TB/s), 238 us (5.3 TB/s) and 147 us; a copy of 1 GiB reaches 5.0 TB/s.
 //
 // 8-bit states.  256 elements share a power of two, so scaling is an addition to exponent fields and exact, and a byte is
 // the top of a number's fp32 pattern: no division, no table.  v is never negative and gets the sign's bit for a fifth
@@ -17,45 +18,44 @@
 
 namespace {
 
-constexpr int MAX_TENSORS = 56;       // table entries per launch: the arguments stay below 4 KB
-constexpr uint32_t CHUNK = 4096;      // elements per workgroup: 4 wavefronts x 4 blocks of 256
+// Elements per workgroup: 4 wavefronts x 4 blocks of 256, or one block where the step is small and what counts is how long
+// one workgroup takes (65 tensors of 210 thousand values: 5.5 us with 4096, 3.7 us with 1024).
+constexpr uint32_t chunk_of(bool large) { return large ? 4096 : 1024; }
 constexpr uint32_t BLOCK = 256;       // elements that share a scale: 4 for each lane of a wavefront
 constexpr int MIN_EXPONENT = 33;      // the smallest number of a block, 31 octaves below its largest, stays normal
 constexpr uint32_t V_TOP = 255, M_TOP = 127;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-struct Entry {
-    float *value;
-    const float *grad;
-    void *m, *v;
-    float *m_scale, *v_scale;
-    uint32_t n, first_chunk;
-    uint32_t vec;  // all pointers of 4 elements 16-byte aligned
+// The tensors of a launch, in its arguments, which may be 4 KB: 100 tensors of 4 pointers, 72 of 6.
+template <int POINTERS>
+struct Table {
+    static constexpr int MAX = POINTERS == 4 ? 100 : 72;
+    void *p[MAX][POINTERS];
+    uint32_t first_chunk[MAX], n[MAX];  // ~0 and 0 behind the last
 };
+constexpr int VALUE = 0, GRAD = 1, M = 2, V = 3, M_SCALE = 4, V_SCALE = 5;
 
-struct StepArgs {
-    Entry t[MAX_TENSORS];
-    int count;
+struct StepScalars {
     const float *step;
     float lr, beta1, beta2, c1, c2, eps, decay, ln1, ln2;
     uint32_t seed;
 };
-
-struct ReadArgs {
-    Entry t[MAX_TENSORS];  // value: m_out, grad: v_out
-    int count;
+template <int POINTERS>
+struct StepArgs {
+    Table<POINTERS> t;
+    StepScalars s;
 };
+static_assert(sizeof(StepArgs<4>) <= 4096 && sizeof(StepArgs<6>) <= 4096, "arguments of a launch");
 
-// The entry a workgroup belongs to: the last one that starts at or before it.
-__device__ __forceinline__ int find_entry(const Entry *t, int count, uint32_t chunk) {
-    int lo = 0, hi = count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t[mid].first_chunk <= chunk) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
+// The entry a workgroup belongs to: the last one that starts at or before it.  Every lane looks at its own, so the search
+// waits once for the arguments, which lie in host memory, and not at every step (65 tensors of 210
+// thousand values: two launches of 6.0 us each with a binary search in tables of 56, one of 5.5 us).
+template <class T>
+__device__ __forceinline__ int find_entry(const T &t, uint32_t chunk) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t low = t.first_chunk[lane], high = lane < T::MAX - 64 ? t.first_chunk[64 + lane] : ~0u;
+    return (int)__popcll(__builtin_amdgcn_ballot_w64(low <= chunk)) + (int)__popcll(__builtin_amdgcn_ballot_w64(high <= chunk)) - 1;
 }
 
 // Large steps go past the caches: nothing of them is read again soon.
@@ -67,36 +67,42 @@ __device__ __forceinline__ void store(T *p, T x) {
     else *p = x;
 }
 
+__device__ __forceinline__ bool aligned16(const void *a, const void *b) { return (((uintptr_t)a | (uintptr_t)b) & 15) == 0; }
+
 struct Correction {
     float first, second;  // 1 / (1 - beta1^t), 1 / (1 - beta2^t)
 };
 
 // 1 - beta^t as -expm1(t ln beta): for small t the difference would lose what it is made of
-__device__ __forceinline__ Correction correction(const StepArgs &a) {
+__device__ __forceinline__ Correction correction(const StepScalars &a) {
     const float t = *a.step;
     return {-1.0f / expm1f(t * a.ln1), -1.0f / expm1f(t * a.ln2)};
 }
 
-__device__ __forceinline__ void step_element(float &value, float g, float &m, float &v, const StepArgs &a, const Correction &c) {
+__device__ __forceinline__ void step_element(float &value, float g, float &m, float &v, const StepScalars &a, const Correction &c) {
     m = m * a.beta1 + g * a.c1;
     v = v * a.beta2 + g * g * a.c2;
     value = value - a.lr * (m * c.first / (sqrtf(v * c.second) + a.eps) + a.decay * value);
 }
 
 template <bool NT>
-__global__ void __launch_bounds__(256) adamw_kernel(const StepArgs a) {
-    const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
+__global__ void __launch_bounds__(256) adamw_kernel(const StepArgs<4> args) {
+    const StepScalars &a = args.s;
+    const int entry = find_entry(args.t, blockIdx.x);
     const Correction c = correction(a);
-    const uint32_t base = (blockIdx.x - t.first_chunk) * CHUNK;
-    float *mp = (float *)t.m, *vp = (float *)t.v;
+    void *const *p = args.t.p[entry];
+    const uint32_t n = args.t.n[entry], base = (blockIdx.x - args.t.first_chunk[entry]) * chunk_of(NT);
+    float *xp = (float *)p[VALUE], *mp = (float *)p[M], *vp = (float *)p[V];
+    const float *gp = (const float *)p[GRAD];
+    const bool vec = aligned16(xp, gp) && aligned16(mp, vp);
 #pragma unroll
-    for (uint32_t k = 0; k < CHUNK / 1024; ++k) {
+    for (uint32_t k = 0; k < chunk_of(NT) / 1024; ++k) {
         const uint32_t i = base + k * 1024 + threadIdx.x * 4;
-        if (i >= t.n) return;
-        if (t.vec && i + 4 <= t.n) {
-            f32x4 *xp = reinterpret_cast<f32x4 *>(t.value + i), *m4 = reinterpret_cast<f32x4 *>(mp + i), *v4 = reinterpret_cast<f32x4 *>(vp + i);
-            f32x4 x = load<NT>(xp), m = load<NT>(m4), v = load<NT>(v4);
-            const f32x4 g = load<NT>(reinterpret_cast<const f32x4 *>(t.grad + i));
+        if (i >= n) return;
+        if (vec && i + 4 <= n) {
+            f32x4 *x4 = reinterpret_cast<f32x4 *>(xp + i), *m4 = reinterpret_cast<f32x4 *>(mp + i), *v4 = reinterpret_cast<f32x4 *>(vp + i);
+            f32x4 x = load<NT>(x4), m = load<NT>(m4), v = load<NT>(v4);
+            const f32x4 g = load<NT>(reinterpret_cast<const f32x4 *>(gp + i));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float xj = x[j], mj = m[j], vj = v[j];
@@ -105,14 +111,14 @@ __global__ void __launch_bounds__(256) adamw_kernel(const StepArgs a) {
                 m[j] = mj;
                 v[j] = vj;
             }
-            store<NT>(xp, x);
+            store<NT>(x4, x);
             store<NT>(m4, m);
             store<NT>(v4, v);
         } else {
-            for (uint32_t j = i; j < i + 4 && j < t.n; ++j) {
-                float x = t.value[j], m = mp[j], v = vp[j];
-                step_element(x, t.grad[j], m, v, a, c);
-                t.value[j] = x;
+            for (uint32_t j = i; j < i + 4 && j < n; ++j) {
+                float x = xp[j], m = mp[j], v = vp[j];
+                step_element(x, gp[j], m, v, a, c);
+                xp[j] = x;
                 mp[j] = m;
                 vp[j] = v;
             }
@@ -159,31 +165,37 @@ __device__ __forceinline__ uint32_t scale_exponent(uint32_t largest) {
 
 // A wavefront takes a block of 256 elements, a lane 4 of them and one word of either state.
 template <bool NT>
-__global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
-    const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
+__global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs<6> args) {
+    const StepScalars &a = args.s;
+    const int entry = find_entry(args.t, blockIdx.x);
     const Correction c = correction(a);
+    void *const *p = args.t.p[entry];
+    const uint32_t n = args.t.n[entry], chunk = blockIdx.x - args.t.first_chunk[entry];
+    float *xp = (float *)p[VALUE], *m_scale = (float *)p[M_SCALE], *v_scale = (float *)p[V_SCALE];
+    const float *gp = (const float *)p[GRAD];
+    const bool vec = aligned16(xp, gp);
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t salt = a.seed + (uint32_t)*a.step * 0xAC502949u;
-    uint32_t *mp = (uint32_t *)t.m, *vp = (uint32_t *)t.v;
+    uint32_t *mp = (uint32_t *)p[M], *vp = (uint32_t *)p[V];
 #pragma unroll
-    for (uint32_t k = 0; k < CHUNK / (4 * BLOCK); ++k) {
-        const uint32_t block = (blockIdx.x - t.first_chunk) * (CHUNK / BLOCK) + k * 4 + wave;
-        if (block * BLOCK >= t.n) return;  // the whole wavefront
+    for (uint32_t k = 0; k < chunk_of(NT) / (4 * BLOCK); ++k) {
+        const uint32_t block = chunk * (chunk_of(NT) / BLOCK) + k * 4 + wave;
+        if (block * BLOCK >= n) return;  // the whole wavefront
         const uint32_t i = block * BLOCK + lane * 4;
-        const uint32_t left = i < t.n ? (t.n - i < 4 ? t.n - i : 4) : 0;
+        const uint32_t left = i < n ? (n - i < 4 ? n - i : 4) : 0;
         float x[4] = {}, g[4] = {}, m[4], v[4];
         uint32_t mw = 0, vw = 0;
-        if (left == 4 && t.vec) {
-            const f32x4 x4 = load<NT>(reinterpret_cast<const f32x4 *>(t.value + i)), g4 = load<NT>(reinterpret_cast<const f32x4 *>(t.grad + i));
+        if (left == 4 && vec) {
+            const f32x4 x4 = load<NT>(reinterpret_cast<const f32x4 *>(xp + i)), g4 = load<NT>(reinterpret_cast<const f32x4 *>(gp + i));
 #pragma unroll
             for (int j = 0; j < 4; ++j) { x[j] = x4[j]; g[j] = g4[j]; }
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
-                if (j < left) { x[j] = t.value[i + j]; g[j] = t.grad[i + j]; }
+                if (j < left) { x[j] = xp[i + j]; g[j] = gp[i + j]; }
         }
         if (left) { mw = load<NT>(mp + i / 4); vw = load<NT>(vp + i / 4); }
-        const uint32_t me = __float_as_uint(t.m_scale[block]) >> 23 & 255u, ve = __float_as_uint(t.v_scale[block]) >> 23 & 255u;
+        const uint32_t me = __float_as_uint(m_scale[block]) >> 23 & 255u, ve = __float_as_uint(v_scale[block]) >> 23 & 255u;
         uint32_t mtop = 0, vtop = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
@@ -210,50 +222,52 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const StepArgs a) {
             mw |= mc << (8 * j);
             vw |= vc << (8 * j);
         }
-        if (left == 4 && t.vec) store<NT>(reinterpret_cast<f32x4 *>(t.value + i), f32x4{x[0], x[1], x[2], x[3]});
+        if (left == 4 && vec) store<NT>(reinterpret_cast<f32x4 *>(xp + i), f32x4{x[0], x[1], x[2], x[3]});
         else {
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
-                if (j < left) t.value[i + j] = x[j];
+                if (j < left) xp[i + j] = x[j];
         }
         if (left) { store<NT>(mp + i / 4, mw); store<NT>(vp + i / 4, vw); }
         if (lane == 0) {
-            t.m_scale[block] = __uint_as_float(me2 == 255 ? 0x7FC00000u : me2 << 23);
-            t.v_scale[block] = __uint_as_float(ve2 == 255 ? 0x7FC00000u : ve2 << 23);
+            m_scale[block] = __uint_as_float(me2 == 255 ? 0x7FC00000u : me2 << 23);
+            v_scale[block] = __uint_as_float(ve2 == 255 ? 0x7FC00000u : ve2 << 23);
         }
     }
 }
 
 template <bool NT>
-__global__ void __launch_bounds__(256) adamw_state_read_kernel(const ReadArgs a) {
-    const Entry t = a.t[find_entry(a.t, a.count, blockIdx.x)];
-    const uint32_t base = (blockIdx.x - t.first_chunk) * CHUNK;
-    const uint32_t *mp = (const uint32_t *)t.m, *vp = (const uint32_t *)t.v;
-    float *mo = t.value, *vo = const_cast<float *>(t.grad);
+__global__ void __launch_bounds__(256) adamw_state_read_kernel(const Table<6> t) {  // m_out in VALUE's place, v_out in GRAD's
+    const int entry = find_entry(t, blockIdx.x);
+    void *const *p = t.p[entry];
+    const uint32_t n = t.n[entry], base = (blockIdx.x - t.first_chunk[entry]) * chunk_of(NT);
+    const uint32_t *mp = (const uint32_t *)p[M], *vp = (const uint32_t *)p[V];
+    const float *m_scale = (const float *)p[M_SCALE], *v_scale = (const float *)p[V_SCALE];
+    float *mo = (float *)p[VALUE], *vo = (float *)p[GRAD];
+    const bool vec = aligned16(mo, vo);
 #pragma unroll
-    for (uint32_t k = 0; k < CHUNK / 1024; ++k) {
+    for (uint32_t k = 0; k < chunk_of(NT) / 1024; ++k) {
         const uint32_t i = base + k * 1024 + threadIdx.x * 4;
-        if (i >= t.n) return;
+        if (i >= n) return;
         const uint32_t mw = load<NT>(mp + i / 4), vw = load<NT>(vp + i / 4);
-        const uint32_t me = __float_as_uint(t.m_scale[i / BLOCK]) >> 23 & 255u, ve = __float_as_uint(t.v_scale[i / BLOCK]) >> 23 & 255u;
+        const uint32_t me = __float_as_uint(m_scale[i / BLOCK]) >> 23 & 255u, ve = __float_as_uint(v_scale[i / BLOCK]) >> 23 & 255u;
         f32x4 m, v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             m[j] = decode_m(mw >> (8 * j) & 255u, me);
             v[j] = decode(vw >> (8 * j) & 255u, ve, V_TOP);
         }
-        if (t.vec && i + 4 <= t.n) {
+        if (vec && i + 4 <= n) {
             store<NT>(reinterpret_cast<f32x4 *>(mo + i), m);
             store<NT>(reinterpret_cast<f32x4 *>(vo + i), v);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j)
-                if (i + j < t.n) { mo[i + j] = m[j]; vo[i + j] = v[j]; }
+                if (i + j < n) { mo[i + j] = m[j]; vo[i + j] = v[j]; }
         }
     }
 }
 
-bool aligned16(const void *p) { return ((uintptr_t)p) % 16 == 0; }
 float *f32_ptr(const sg_tensor *t) { return (float *)t->base + t->offset; }
 
 int check_dense(sg_ctx *ctx, const sg_tensor *t, int dtype, int64_t n, const char *who) {
@@ -274,22 +288,42 @@ int check_state8(sg_ctx *ctx, const sg_tensor *m, const sg_tensor *v, const sg_t
 }
 
 // Fills one launch's table from tensor `first` on; returns the index behind the last one taken, the workgroups in *chunks.
-template <class Fill>
-int fill_table(Entry *table, int *count, uint32_t *chunks, int first, int n_tensors, const sg_tensor *sizes, Fill fill) {
+template <int POINTERS>
+int fill_table(Table<POINTERS> &t, uint32_t *chunks, int first, int n_tensors, const sg_tensor *const (&arrays)[6], uint32_t chunk) {
     uint64_t at = 0;
-    int i = first;
-    for (*count = 0; i < n_tensors && *count < MAX_TENSORS; ++i) {
-        const int64_t n = sg_numel(&sizes[i]);
-        const uint64_t need = (uint64_t)(n + CHUNK - 1) / CHUNK;
+    int i = first, count = 0;
+    for (; i < n_tensors && count < Table<POINTERS>::MAX; ++i) {
+        const int64_t n = sg_numel(&arrays[VALUE][i]);
+        const uint64_t need = ((uint64_t)n + chunk - 1) / chunk;
         if (at + need >= (1ull << 31)) break;  // the rest in a launch of its own
-        Entry &e = table[(*count)++];
-        fill(e, i);
-        e.n = (uint32_t)n;
-        e.first_chunk = (uint32_t)at;
+        for (int k = 0; k < POINTERS; ++k) t.p[count][k] = f32_ptr(&arrays[k][i]);
+        t.n[count] = (uint32_t)n;
+        t.first_chunk[count++] = (uint32_t)at;
         at += need;
+    }
+    for (; count < Table<POINTERS>::MAX; ++count) {
+        for (int k = 0; k < POINTERS; ++k) t.p[count][k] = nullptr;
+        t.first_chunk[count] = ~0u;
+        t.n[count] = 0;
     }
     *chunks = (uint32_t)at;
     return i;
+}
+
+// The launches of a step over all tensors, `bytes` an element.
+template <int POINTERS, class Launch>
+int for_tables(sg_ctx *ctx, int n_tensors, const sg_tensor *const (&arrays)[6], int bytes, Launch launch) {
+    int64_t elements = 0;
+    for (int i = 0; i < n_tensors; ++i) elements += sg_numel(&arrays[VALUE][i]);
+    const bool large = sg_streaming(elements * bytes);
+    for (int first = 0; first < n_tensors;) {
+        Table<POINTERS> t;
+        uint32_t chunks = 0;
+        first = fill_table(t, &chunks, first, n_tensors, arrays, chunk_of(large));
+        launch(t, chunks, large);
+        SG_CHECK_LAUNCH(ctx, "adamw");
+    }
+    return SG_OK;
 }
 
 }  // namespace
@@ -317,34 +351,23 @@ extern "C" int sg_adamw_update(sg_ctx *ctx, int n_tensors, const sg_tensor *valu
     }
     if (!ctx) return SG_ERR_ARG;
     sg_device_guard guard(ctx);
-    for (int first = 0; first < n_tensors;) {
-        StepArgs a{};
-        a.step = f32_ptr(step);
-        a.lr = h->lr; a.beta1 = h->beta1; a.beta2 = h->beta2; a.c1 = h->one_minus_beta1; a.c2 = h->one_minus_beta2;
-        a.eps = h->eps; a.decay = h->weight_decay;
-        a.ln1 = (float)std::log((double)h->beta1);
-        a.ln2 = (float)std::log((double)h->beta2);
-        a.seed = seed;
-        uint32_t chunks = 0;
-        first = fill_table(a.t, &a.count, &chunks, first, n_tensors, values, [&](Entry &e, int i) {
-            e.value = f32_ptr(&values[i]);
-            e.grad = f32_ptr(&grads[i]);
-            e.m = f32_ptr(&m[i]);
-            e.v = f32_ptr(&v[i]);
-            e.vec = aligned16(e.value) && aligned16(e.grad) && (eight || (aligned16(e.m) && aligned16(e.v)));
-            if (eight) {
-                e.m_scale = f32_ptr(&m_scale[i]);
-                e.v_scale = f32_ptr(&v_scale[i]);
-            }
+    StepScalars a{};
+    a.step = f32_ptr(step);
+    a.lr = h->lr; a.beta1 = h->beta1; a.beta2 = h->beta2; a.c1 = h->one_minus_beta1; a.c2 = h->one_minus_beta2;
+    a.eps = h->eps; a.decay = h->weight_decay;
+    a.ln1 = (float)std::log((double)h->beta1);
+    a.ln2 = (float)std::log((double)h->beta2);
+    a.seed = seed;
+    const sg_tensor *const arrays[6] = {values, grads, m, v, m_scale, v_scale};
+    if (eight)
+        return for_tables<6>(ctx, n_tensors, arrays, 16, [&](const Table<6> &t, uint32_t chunks, bool large) {
+            if (large) hipLaunchKernelGGL((adamw8_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, StepArgs<6>{t, a});
+            else hipLaunchKernelGGL((adamw8_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, StepArgs<6>{t, a});
         });
-        const bool nt = sg_streaming((int64_t)chunks * CHUNK * (eight ? 16 : 28));
-        if (eight && nt) hipLaunchKernelGGL((adamw8_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, a);
-        else if (eight) hipLaunchKernelGGL((adamw8_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, a);
-        else if (nt) hipLaunchKernelGGL((adamw_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((adamw_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, a);
-        SG_CHECK_LAUNCH(ctx, "adamw");
-    }
-    return SG_OK;
+    return for_tables<4>(ctx, n_tensors, arrays, 28, [&](const Table<4> &t, uint32_t chunks, bool large) {
+        if (large) hipLaunchKernelGGL((adamw_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, StepArgs<4>{t, a});
+        else hipLaunchKernelGGL((adamw_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, StepArgs<4>{t, a});
+    });
 }
 
 extern "C" int sg_adamw_state_read(sg_ctx *ctx, int n_tensors, const sg_tensor *m, const sg_tensor *v, const sg_tensor *m_scale, const sg_tensor *v_scale,
@@ -360,21 +383,9 @@ extern "C" int sg_adamw_state_read(sg_ctx *ctx, int n_tensors, const sg_tensor *
     }
     if (!ctx) return SG_ERR_ARG;
     sg_device_guard guard(ctx);
-    for (int first = 0; first < n_tensors;) {
-        ReadArgs a{};
-        uint32_t chunks = 0;
-        first = fill_table(a.t, &a.count, &chunks, first, n_tensors, m_out, [&](Entry &e, int i) {
-            e.value = f32_ptr(&m_out[i]);
-            e.grad = f32_ptr(&v_out[i]);
-            e.m = f32_ptr(&m[i]);
-            e.v = f32_ptr(&v[i]);
-            e.m_scale = f32_ptr(&m_scale[i]);
-            e.v_scale = f32_ptr(&v_scale[i]);
-            e.vec = aligned16(e.value) && aligned16(e.grad);
-        });
-        if (sg_streaming((int64_t)chunks * CHUNK * 10)) hipLaunchKernelGGL((adamw_state_read_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((adamw_state_read_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, a);
-        SG_CHECK_LAUNCH(ctx, "adamw_state_read");
-    }
-    return SG_OK;
+    const sg_tensor *const arrays[6] = {m_out, v_out, m, v, m_scale, v_scale};
+    return for_tables<6>(ctx, n_tensors, arrays, 10, [&](const Table<6> &t, uint32_t chunks, bool large) {
+        if (large) hipLaunchKernelGGL((adamw_state_read_kernel<true>), dim3(chunks), dim3(256), 0, ctx->stream, t);
+        else hipLaunchKernelGGL((adamw_state_read_kernel<false>), dim3(chunks), dim3(256), 0, ctx->stream, t);
+    });
 }

@@ -578,6 +578,29 @@ def test_adamw_optimizer_eager_compiled_and_captured(ctx, bits):
     prog.release_graph()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("count", [63, 64, 65, 72, 73, 100, 101, 230])
+def test_adamw_of_many_tensors(ctx, bits, count):
+    """As many as a launch's table holds, one more, several launches: each tensor gets the step it gets alone, whatever its place
+    (the noise of 8-bit states depends on the element, not on the tensor)."""
+    say("adamw tensors", bits, count)
+    rng = np.random.default_rng(count)
+    sizes = [int(n) for n in rng.choice([1, 5, 64, 300, 4096, 4097, 9000], count)]
+    one = {}
+    for n in set(sizes):
+        a, g = R.f32(np.cos(np.arange(n))), R.f32(np.sin(np.arange(n)))
+        p, opt = Var.new(dev(ctx, a)), optim.AdamW(1e-2, state_bits=bits)
+        opt.update({p: Var.new(dev(ctx, g))}, ctx)
+        one[n] = a, g, p.value.numpy(), [x.numpy() for x in opt.state(p, ctx)]
+    params = [Var.new(dev(ctx, one[n][0])) for n in sizes]
+    opt = optim.AdamW(1e-2, state_bits=bits)
+    opt.update({p: Var.new(dev(ctx, one[n][1])) for p, n in zip(params, sizes)}, ctx)
+    for p, n in zip(params, sizes):
+        assert same_bits(p.value.numpy(), one[n][2])
+        for x, y in zip(opt.state(p, ctx), one[n][3]):
+            assert same_bits(x.numpy(), y)
+
+
 def test_adamw_takes_strided_gradients_and_a_broadcast_one(ctx):
     rng = np.random.default_rng(4)
     a, g = R.f32(rng.standard_normal((6, 10))), R.f32(rng.standard_normal((10, 6)))
