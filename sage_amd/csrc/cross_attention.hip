@@ -74,7 +74,8 @@ struct Work {
 // Workgroup ids go round-robin over the 8 XCDs.  All tiles of a (split, pair), which share keys or rows, go to one of them,
 // and the pairs of a sequence, whose length they have in common, to different ones.  Where the lengths are known in front
 // (ends), the longest sequences come first: a launch ends when its last workgroup does, and short ones fill the gaps
-// (32 x 12 heads of 512 x 512 with lengths 512 to 272: a tenth of the time).  lds: 4 words.
+// (32 x 12 heads of 512 x 512 with lengths 512 to 272: a tenth of the time; 7 x 2 pairs of 1332 rows, 1001 to 501 keys: forward 39
+// -> 30 us).  lds: 4 words.
 __device__ __forceinline__ Work find_work(const CrossP &p, int *lds) {
     Work w;
     const uint32_t units = p.pairs * p.splits, even = units & ~7u;
@@ -404,7 +405,9 @@ __device__ __forceinline__ bool merge_waves(float *lds, int wave, int lane, G gi
 }
 
 // ---- forward.  RW wavefronts take the workgroup's 32 RW rows, the 4 / RW times as many share each block's keys and are
-// merged through LDS at the end.
+// merged through LDS at the end.  Bound by the matrix pipes, which fp32 vector instructions share: counters show them busy for
+// 80 % (D = 64) and 74 % (D = 32) of the time a compute unit has work, the vector instructions of the softmax are the rest.
+// 32 x 12 heads, 512 x 512, D = 64: 238 us (108 TFLOP/s); lengths 512 to 272: 188 us; D = 32: 133 us (97 TFLOP/s).
 template <int D, int RW, bool DMA>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 4 ? 3 : 1))) cross_forward_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND + 2;
@@ -487,7 +490,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 
 // ---- forward with up to 8 rows a pair (a serving step).  Bound by memory: K and V are read once for few products, on
 // the vector unit.  D / 4 lanes hold a key's 16-byte pieces, so a wavefront takes 4 or 8 keys an instruction; every group of
 // lanes runs a softmax of its own over its keys, merged at the end.  UNROLL keys a group are in flight behind the UNROLL
-// that are worked on.
+// that are worked on.  One query of 32 x 12 heads over 512 to 272 keys of size 64: 17.4 us (75 MB, 4.3 TB/s).
 template <int D>
 __device__ __forceinline__ float group_sum(float x) {  // over the D / 4 lanes of a key, in all of them
     auto move = [](float v, auto ctrl) { return __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xF, 0xF, true)); };
@@ -610,7 +613,7 @@ __global__ void __launch_bounds__(256) cross_few_kernel(const CrossP p) {
     if (p.lse && c == 0) p.lse[row] = sum == 0.0f ? -inf : (top + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// Joins the splits of a row: D / 4 lanes a row.
+// Joins the splits of a row: D / 4 lanes a row (bound by its launch: 4 to 8 us).
 template <int D>
 __global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p) {
     constexpr int LPR = D / 4;
@@ -635,7 +638,8 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p) {
     if (p.lse && col == 0) p.lse[row] = l == 0.0f ? -inf : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// ---- gradient of the queries (and delta, for the other kernel)
+// ---- gradient of the queries (and delta, for the other kernel).  Three products a block, the matrix pipes busy for 84 % of the
+// time there is work.  32 x 12 heads, 512 x 512, D = 64: 337 us (115 TFLOP/s); lengths 512 to 272: 267 us.
 template <int D, int RW, bool DMA>
 __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND;
@@ -695,7 +699,9 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
 }
 
 // ---- gradients of keys and values: a wavefront owns 32 keys and walks the rows of the pair, 32 at a time.  CW wavefronts
-// take the workgroup's 32 CW keys, the 4 / CW times as many share each block's rows and are added up through LDS.
+// take the workgroup's 32 CW keys, the 4 / CW times as many share each block's rows and are added up through LDS.  Four
+// products a block, the matrix pipes busy for 85 %.  32 x 12 heads, 512 x 512, D = 64: 440 us (117 TFLOP/s); lengths 512 to 272:
+// 390 us.  (dQ from here too would save two of the seven products of a gradient, and cost sums over workgroups.)
 template <int D, int CW, bool DMA>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) cross_gkv_kernel(const CrossP p) {
     constexpr int GW = 4 / CW, RB = 32 * GW, ND = D / 32, KEYS = 32 * CW, SLOT = 32 * ND;
