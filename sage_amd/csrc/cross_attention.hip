@@ -1043,7 +1043,7 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
     const Plan by_rows = plan(ctx, p, D, p.R, p.Lk, 1, 4, D == 64 ? 2.6 : 1.6);
     // 128 keys a workgroup only where all are visible: smaller tiles waste less of a sequence's last one and level better
-    // (32 x 12 heads of 512 x 512: 441 us against 463 with 64 keys; with lengths 512 to 272: 432 against 421 us)
+    // (32 x 12 heads of 512 x 512: 446 us against 473 with 64 keys; with lengths 512 to 272: 423 against 404 us)
     const Plan by_keys = plan(ctx, p, D, p.Lk, p.R, 2, p.mask ? 2 : 4, D == 64 ? 3.4 : 2.0);
     const int rw = by_rows.waves, cw = by_keys.waves;
     const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 32 * cw - 1) / (32 * cw));
