@@ -214,28 +214,38 @@ __device__ __forceinline__ void stage(float *tile, F row_at) {
     }
 }
 
-// The same of rows that lie a stride apart.  A thread's pieces are 1024 / D rows apart and in the same place of each, so
-// where it starts is fixed for the kernel and the way from there is the same for all: address arithmetic of the scalar unit.
+// The same of rows that lie a stride apart.  A thread's pieces are 1024 / D rows apart and in the same place of each, so what
+// is its own of their addresses is fixed for the kernel; in 32 bits (DMA: strides below 2^22 elements) beside a base in scalar
+// registers, the loads need no vector instruction, which would be taken from the matrix pipes' time.
 template <int D>
 struct Strided {
-    const float *own;  // this thread's piece of the first row it takes of a tile at row 0
+    static constexpr int STEP = 1024 / D;
+    const float *x;
     int64_t l;
-    int total;
-    __device__ Strided(const float *x, int64_t l_, int total_) : l(l_), total(total_) {
-        const int row = (int)threadIdx.x / Tile<D>::PIECES;
-        own = x + (int64_t)row * l + (((int)threadIdx.x % Tile<D>::PIECES) ^ Tile<D>::turn(row)) * 4;
+    int total, row, wave_piece;
+    uint32_t own;  // bytes from a tile's first row to this thread's first piece
+    __device__ Strided(const float *x_, int64_t l_, int total_) : x(x_), l(l_), total(total_) {
+        row = (int)threadIdx.x / Tile<D>::PIECES;
+        own = ((uint32_t)row * (uint32_t)l + (((int)threadIdx.x % Tile<D>::PIECES) ^ Tile<D>::turn(row)) * 4) * 4;
+        wave_piece = __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63);
     }
     template <int ROWS, bool DMA>
     __device__ __forceinline__ void stage(float *tile, int first) const {
-        constexpr int STEP = 1024 / D;
-        if (first + ROWS <= total) {
+        const bool whole = first + ROWS <= total;
 #pragma unroll
-            for (int i = 0; i < ROWS / STEP; ++i) stage_piece<DMA>(tile, i * 256 + (int)threadIdx.x, own + (int64_t)(first + i * STEP) * l);
-        } else {  // rows past the end repeat the last one
-            const int row = (int)threadIdx.x / Tile<D>::PIECES;
-#pragma unroll
-            for (int i = 0; i < ROWS / STEP; ++i)
-                stage_piece<DMA>(tile, i * 256 + (int)threadIdx.x, own + (int64_t)(min(first + i * STEP + row, total - 1) - row) * l);
+        for (int i = 0; i < ROWS / STEP; ++i) {
+            if (DMA) {
+                const char *base = reinterpret_cast<const char *>(x + (int64_t)(whole ? first + i * STEP : first) * l);
+                uint32_t at = own;
+                // rows past the end repeat the last one
+                if (!whole) at += (uint32_t)(min(row + i * STEP, total - 1 - first) - row) * (uint32_t)l * 4;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(base + at),
+                                                 (__attribute__((address_space(3))) void *)(tile + (i * 256 + wave_piece) * 4), 16, 0, 0);
+            } else {
+                const int64_t r = min(first + i * STEP + row, total - 1);
+                const float *src = x + r * l + (((int)threadIdx.x % Tile<D>::PIECES) ^ Tile<D>::turn(row)) * 4;
+                *reinterpret_cast<f32x4 *>(tile + (i * 256 + (int)threadIdx.x) * 4) = load4(src);
+            }
         }
     }
 };
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 
     floatx16 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = zero16();
-    float m_run = -inf, l_run = 0.0f;
+    float m_run = -inf, l_run = 0.0f, shift = 0.0f;
     uint32_t first, last;
     split_range((w.end + KB - 1) / KB, w.split, p.splits, &first, &last);
     walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&] { q.scale(p.scale * LOG2E); /* scores are logarithms to base 2 */ },
@@ -438,18 +448,20 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 
         float top = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float m_new = fmaxf(m_run, top);
-        const float shift = m_new == -inf ? 0.0f : m_new;  // nothing visible so far: every exponential below is 0
-        if (__builtin_amdgcn_ballot_w64(m_new != m_run) != 0) {
+        // The largest so far and 8 (octaves) more is what exponentials are taken relative to: later blocks rarely pass it and
+        // have everything moved to a new one.
+        if (__builtin_amdgcn_ballot_w64(top > m_run) != 0) {
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float m_new = top > m_run ? top + 8.0f : m_run;
+            shift = m_new == -inf ? 0.0f : m_new;  // nothing visible so far: every exponential below is 0
             const float f = __builtin_amdgcn_exp2f(m_run - shift);
             l_run *= f;
 #pragma unroll
             for (int j = 0; j < ND; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[j][r] *= f;
+            m_run = m_new;
         }
-        m_run = m_new;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s[r] = __builtin_amdgcn_exp2f(s[r] - shift);
@@ -703,7 +715,7 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
 // products a block, the matrix pipes busy for 85 %.  32 x 12 heads, 512 x 512, D = 64: 440 us (117 TFLOP/s); lengths 512 to 272:
 // 390 us.  (dQ from here too would save two of the seven products of a gradient, and cost sums over workgroups.)
 template <int D, int CW, bool DMA>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) cross_gkv_kernel(const CrossP p) {
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 32 ? 3 : 2))) cross_gkv_kernel(const CrossP p) {
     constexpr int GW = 4 / CW, RB = 32 * GW, ND = D / 32, KEYS = 32 * CW, SLOT = 32 * ND;
     __shared__ __attribute__((aligned(16))) float lds0[2 * RB * D], lds1[2 * RB * D];  // two buffers of rows of Q and dO
     __shared__ __attribute__((aligned(16))) float rows0[2 * RB], rows1[2 * RB];        // their lse and delta
@@ -894,8 +906,8 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
     return SG_OK;
 }
 
-// 16-byte aligned rows: loads straight into LDS take them.
-bool aligned_rows(const Rows &r) { return ((uintptr_t)r.p) % 16 == 0 && r.b % 4 == 0 && r.h % 4 == 0 && r.l % 4 == 0; }
+// 16-byte aligned rows less than 16 MB apart: loads straight into LDS take them.
+bool aligned_rows(const Rows &r) { return ((uintptr_t)r.p) % 16 == 0 && r.b % 4 == 0 && r.h % 4 == 0 && r.l % 4 == 0 && r.l < (1 << 22); }
 
 // How a kernel takes an axis of `own` rows (or keys) that walk `other` of the other side: wavefronts of a workgroup side by
 // side on it (the 4 / waves others share the blocks of the walk), and workgroups a walk is split over.
