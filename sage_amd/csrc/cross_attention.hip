@@ -50,8 +50,14 @@ __device__ __forceinline__ int visible_end(const CrossP &p, int b, int *lds) {
     if (!p.mask) return p.Lk;
     const float *m = p.mask + b * p.mask_b;
     int end = 0;
-    for (int j = threadIdx.x; j < p.Lk; j += 256)
-        if (m[j] != 0.0f) end = j + 1;
+    for (int j = threadIdx.x; j < p.Lk; j += 256 * 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = m[min(j + 256 * i, p.Lk - 1)];  // in flight together
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (x[i] != 0.0f) end = max(end, min(j + 256 * i, p.Lk - 1) + 1);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) end = max(end, __shfl_xor(end, o, 64));
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = end;
@@ -417,7 +423,7 @@ __device__ __forceinline__ bool merge_waves(float *lds, int wave, int lane, G gi
 // ---- forward.  RW wavefronts take the workgroup's 32 RW rows, the 4 / RW times as many share each block's keys and are
 // merged through LDS at the end.  Bound by the matrix pipes, which fp32 vector instructions share: counters show them busy for
 // 80 % (D = 64) and 74 % (D = 32) of the time a compute unit has work, the vector instructions of the softmax are the rest.
-// 32 x 12 heads, 512 x 512, D = 64: 238 us (108 TFLOP/s); lengths 512 to 272: 188 us; D = 32: 133 us (97 TFLOP/s).
+// 32 x 12 heads, 512 x 512, D = 64: 233 us (111 TFLOP/s); lengths 512 to 272: 188 us; D = 32: 129 us (100 TFLOP/s).
 template <int D, int RW, bool DMA>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 4 ? 3 : 1))) cross_forward_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND + 2;
@@ -1055,8 +1061,9 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
     const Plan by_rows = plan(ctx, p, D, p.R, p.Lk, 1, 4, D == 64 ? 2.6 : 1.6);
     // 128 keys a workgroup only where all are visible: smaller tiles waste less of a sequence's last one and level better
-    // (32 x 12 heads of 512 x 512: 446 us against 473 with 64 keys; with lengths 512 to 272: 423 against 404 us)
-    const Plan by_keys = plan(ctx, p, D, p.Lk, p.R, 2, p.mask ? 2 : 4, D == 64 ? 3.4 : 2.0);
+    // (32 x 12 heads of 512 x 512: 446 us against 473 with 64 keys; with lengths 512 to 272: 423 against 404 us); and up to 32
+    // rows, all of which a wavefront takes (15 rows, 14 x 8 heads, 4048 keys of size 32: 99 us with 64 keys, 53 us).
+    const Plan by_keys = plan(ctx, p, D, p.Lk, p.R, p.R <= 32 ? 4 : 2, p.mask && p.R > 32 ? 2 : 4, D == 64 ? 3.4 : 2.0);
     const int rw = by_rows.waves, cw = by_keys.waves;
     const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 32 * cw - 1) / (32 * cw));
     const uint32_t row_splits = by_rows.splits, key_splits = by_keys.splits;

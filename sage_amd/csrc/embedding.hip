@@ -316,16 +316,17 @@ __device__ __forceinline__ void store_cols(float *row, uint32_t c, uint32_t E, f
 }
 
 // Up to 128 tokens, in one launch: a workgroup owns some rows of the table, clears them, finds its tokens among all and sums
-// the rows that have some in the tokens' order (23 tokens, table of 230 x 243: 6.6 us with the lookup; sort, sums and join are three
-// launches: 13 us).  At most 32
-// rows a workgroup: where the table is small all tokens are on a few workgroups, each wavefront a row at a time.
+// the rows that have some in the tokens' order (23 tokens, table of 230 x 243: 5.4 us; 90 tokens, 2633 x 538: 10.8 us, with 30
+// rows a workgroup instead of 4 15.6 us; 120 tokens, 30522 x 768: 20 us, 14 of them a fill's.  Sort, sums and join are three
+// launches of 3.4 to 6.5 us at the least).
 constexpr uint32_t FEW = 128, FEW_ROWS = 32, FEW_THREADS = 512;
 struct FewP {
     const float *gout;
     const uint32_t *ids;
     float *gtable;
     sg_rows id_rows, g_rows;
-    uint32_t n, E, V, rows;  // rows: what a workgroup owns
+    uint32_t n, E, V, rows;  // rows: what a workgroup owns, a multiple of 4
+    uint32_t fill_vec;
     float scale;
 };
 
@@ -338,9 +339,9 @@ __global__ void __launch_bounds__(FEW_THREADS) embedding_few_kernel(const FewP p
     const uint32_t id = tid < p.n ? p.ids[sg_row_offset(p.id_rows, tid)] : ~0u;
     float *table = p.gtable + (uint64_t)v0 * p.E;
     const uint64_t total = (uint64_t)rows * p.E;
-    for (uint64_t i = tid * (VEC ? 4u : 1u); i < total; i += FEW_THREADS * (VEC ? 4 : 1)) {
-        if (VEC) *reinterpret_cast<f32x4 *>(table + i) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        else table[i] = 0.0f;
+    for (uint64_t i = tid * 4u; i < total; i += FEW_THREADS * 4) {  // (whole tables of any E: a workgroup's rows begin at 16 bytes)
+        if (p.fill_vec && i + 4 <= total) *reinterpret_cast<f32x4 *>(table + i) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        else for (uint64_t j = i; j < i + 4 && j < total; ++j) table[j] = 0.0f;
     }
     const bool here = id >= v0 && id - v0 < rows;
     const uint32_t row = here ? id - v0 : ~0u;
@@ -545,9 +546,12 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
         f.E = m.E;
         f.V = s.V;
         f.scale = scale;
-        // 64 KB of the table a workgroup, so that clearing fills the chip
-        const uint32_t rows = 16384 / f.E;
-        f.rows = rows < 1 ? 1 : rows > FEW_ROWS ? FEW_ROWS : rows;
+        // 512 workgroups or 64 KB of the table each, whichever is less, so that clearing fills the chip
+        uint32_t rows = 16384 / f.E;
+        rows = rows > FEW_ROWS ? FEW_ROWS : rows;
+        rows = rows > (f.V + 511) / 512 ? (f.V + 511) / 512 : rows;
+        f.rows = rows < 4 ? 4 : rows / 4 * 4;
+        f.fill_vec = aligned16(table);
         sg_device_guard guard(ctx);
         bool vec = E % 4 == 0 && aligned16(f.gout) && aligned16(table);
         for (int i = 0; i < f.g_rows.rank; ++i) vec = vec && f.g_rows.st[i] % 4 == 0;

@@ -10,7 +10,7 @@
 // one equal to the bound has a higher index than k that reach it), some ten to a hundred of its share, in a list of its own
 // in LDS and without a barrier; the k largest of the wavefronts' lists are ranked at the end.
 // 4096 x 30522 without alternatives: 88 us (500 MB, 5.7 TB/s).  1021 x 50257 with 20: 60 us (205 MB, 3.4 TB/s: all rows are
-// on the chip at once, and choosing does not overlap another row's loads).  4 x 50257 with 5: 8.6 us and a join of 4.5.
+// on the chip at once, and choosing does not overlap another row's loads).  4 x 30522 with 5: 8.6 us and a join of 4.5.
 #include "rows.h"
 
 #include <type_traits>

@@ -82,7 +82,7 @@ def zipf_ids(rng, n, v):
 
 
 @pytest.mark.parametrize("n,v,e", [(1, 1, 1), (1, 5, 768), (7, 3, 64), (64, 1000, 33), (257, 10, 260), (300, 70000, 4), (4096, 500, 96), (5, 100, 2050),
-                                   (128, 3, 768), (128, 1000, 24), (127, 40000, 8), (129, 20, 70), (100, 700, 13), (8000, 4000, 12)])
+                                   (128, 3, 768), (128, 1000, 24), (127, 40000, 8), (129, 20, 70), (100, 700, 13), (8000, 4000, 12), (3, 6, 17001), (90, 2633, 538)])
 def test_embedding_and_gradient(ctx, n, v, e):
     say("embedding", n, v, e)
     rng = np.random.default_rng(n + v + e)
