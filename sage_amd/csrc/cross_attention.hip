@@ -37,6 +37,7 @@ struct CrossP {
     float *part_k, *part_v;   // [split][key][D]
     int N, H, G, Lq, Lk, R;   // R = H / G * Lq: rows of a (batch, key head) pair
     int64_t mask_b;
+    int spread;   // tiles of a pair on all XCDs
     int strided;  // a pair's rows of q and gout lie a stride apart
     float scale;
     uint32_t tiles, pairs, splits;
@@ -78,14 +79,15 @@ struct Work {
     int b, g, end;
 };
 // Workgroup ids go round-robin over the 8 XCDs.  All tiles of a (split, pair), which share keys or rows, go to one of them,
-// and the pairs of a sequence, whose length they have in common, to different ones.  Where the lengths are known in front
+// and the pairs of a sequence, whose length they have in common, to different ones; where there are few pairs, the tiles go to
+// all XCDs (7 x 2 pairs of 1332 rows: both gradients 78 -> 70 us).  Where the lengths are known in front
 // (ends), the longest sequences come first: a launch ends when its last workgroup does, and short ones fill the gaps
 // (32 x 12 heads of 512 x 512 with lengths 512 to 272: a tenth of the time; 7 x 2 pairs of 1332 rows, 1001 to 501 keys: forward 39
 // -> 30 us).  lds: 4 words.
-__device__ __forceinline__ Work find_work(const CrossP &p, int *lds) {
+__device__ __forceinline__ Work find_work(const CrossP &p, uint32_t id, int *lds) {
     Work w;
-    const uint32_t units = p.pairs * p.splits, even = units & ~7u;
-    uint32_t id = blockIdx.x, unit, q;
+    const uint32_t units = p.pairs * p.splits, even = p.spread ? 0 : units & ~7u;
+    uint32_t unit, q;
     if (id < even * p.tiles) {
         q = fdiv(id >> 3, p.d_tiles);
         w.tile = (id >> 3) - q * p.tiles;
@@ -100,8 +102,13 @@ __device__ __forceinline__ Work find_work(const CrossP &p, int *lds) {
     // visible key, which are done at once, would all go to the same ones
     w.tile += q - fdiv(q, p.d_tiles) * p.tiles;
     if (w.tile >= p.tiles) w.tile -= p.tiles;
-    w.split = fdiv(unit, p.d_pairs);
-    w.pair = unit - w.split * p.pairs;
+    if (p.spread) {
+        w.pair = unit / p.splits;
+        w.split = unit - w.pair * p.splits;
+    } else {
+        w.split = fdiv(unit, p.d_pairs);
+        w.pair = unit - w.split * p.pairs;
+    }
     w.b = (int)fdiv(w.pair, p.d_g);
     w.g = (int)w.pair - w.b * p.G;
     if (!p.ends) {
@@ -129,8 +136,8 @@ __device__ __forceinline__ Work find_work(const CrossP &p, int *lds) {
 // others, which only write zeros, last: every compute unit gets as many of the former (7 x 2 key heads, 1001 keys, lengths
 // 1001 to 501: 57 -> 44 us).  b is -1 for what rounds the grid up to the 8 XCDs.  lds: 8 words.
 template <int KEYS>
-__device__ __forceinline__ Work find_key_work(const CrossP &p, int *lds) {
-    if (!p.ends) return find_work(p, lds);
+__device__ __forceinline__ Work find_key_work(const CrossP &p, uint32_t id, int *lds) {
+    if (!p.ends) return find_work(p, id, lds);
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, units = p.G * p.splits, all = units * p.tiles;
     const int mine = t < (uint32_t)p.N ? p.ends[t] : 0;
     const uint32_t count = (uint32_t)((mine + KEYS - 1) / KEYS) * units;
@@ -149,7 +156,7 @@ __device__ __forceinline__ Work find_key_work(const CrossP &p, int *lds) {
         if (i < wave) before += (uint32_t)lds[i];
         total += (uint32_t)lds[i];
     }
-    const uint32_t id = blockIdx.x, per = (total + 7) / 8, slot = id >> 3, at = (id & 7) * per + slot;
+    const uint32_t per = (total + 7) / 8, slot = id >> 3, at = (id & 7) * per + slot;
     const bool first = slot < per && at < total;                   // one with visible keys
     const uint32_t place = first ? at : slot < per ? at - total : id - total;
     const uint32_t from = first ? before : t * all - before, n = first ? count : all - count;
@@ -430,7 +437,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 
     __shared__ __attribute__((aligned(16))) float lds0[2 * KB * D], lds1[2 * KB * D];  // two buffers of keys and values
     __shared__ int lds_end[4];
     static_assert((KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "the merge fits in a buffer");
-    const Work w = find_work(p, lds_end);
+    const Work w = find_work(p, blockIdx.x, lds_end);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
     const uint32_t r = w.tile * (32 * RW) + (wave % RW) * 32 + c;
     const float inf = __builtin_inff();
@@ -525,7 +532,7 @@ __global__ void __launch_bounds__(256) cross_few_kernel(const CrossP p) {
     __shared__ int lds_end[4];
     __shared__ float lds_ml[4][ROWS][2];
     __shared__ __attribute__((aligned(16))) float lds_o[4][ROWS][D];
-    const Work w = find_work(p, lds_end);
+    const Work w = find_work(p, blockIdx.x, lds_end);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / LPK, col = lane % LPK * 4;
     const float *K = p.k.p + w.b * p.k.b + w.g * p.k.h + col, *V = p.v.p + w.b * p.v.b + w.g * p.v.h + col;
     const float *mask = p.mask ? p.mask + w.b * p.mask_b : nullptr;
@@ -658,21 +665,20 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p) {
 
 // ---- gradient of the queries (and delta, for the other kernel).  Three products a block, the matrix pipes busy for 84 % of the
 // time there is work.  32 x 12 heads, 512 x 512, D = 64: 336 us (115 TFLOP/s); lengths 512 to 272: 264 us.
-template <int D, int RW, bool DMA>
-__global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
+// GIVEN: delta is there already.
+template <int D, int RW, bool DMA, bool GIVEN>
+__device__ __forceinline__ void gq_work(const CrossP &p, uint32_t id, float (&lds0)[256 / RW * D], float (&lds1)[256 / RW * D], int *lds_end) {
     constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND;
-    __shared__ __attribute__((aligned(16))) float lds0[2 * KB * D], lds1[2 * KB * D];
-    __shared__ int lds_end[4];
     static_assert((KW - 1) * RW * 64 * SLOT <= 2 * KB * D, "the merge fits in a buffer");
-    const Work w = find_work(p, lds_end);
+    const Work w = find_work(p, id, lds_end);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
     const uint32_t r = w.tile * (32 * RW) + (wave % RW) * 32 + c, rr = min(r, (uint32_t)p.R - 1);
     const int64_t row = (int64_t)w.pair * p.R + rr;
     Own<D> q, go, o;
     q.load(p.q.p + row_at(p, p.q, w, rr), h);
     go.load(p.go.p + row_at(p, p.go, w, rr), h);
-    o.load(p.o.p + row_at(p, p.o, w, rr), h);
-    float lse2 = p.lse[row], delta = 0.0f;
+    if (!GIVEN) o.load(p.o.p + row_at(p, p.o, w, rr), h);
+    float lse2 = p.lse[row], delta = GIVEN ? p.delta[row] : 0.0f;
     floatx16 acc[ND];
 #pragma unroll
     for (int j = 0; j < ND; ++j) acc[j] = zero16();
@@ -681,6 +687,7 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
     walk_keys<D, KB, DMA>(p, w, lds0, lds1, first, last, wave / RW * 32, [&] {
         q.scale(p.scale * LOG2E);
         lse2 *= LOG2E;
+        if (GIVEN) return;
 #pragma unroll
         for (int g = 0; g < D / 8; ++g)
 #pragma unroll
@@ -716,18 +723,23 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
     else write_column<D>(const_cast<float *>(p.gq.p) + row_at(p, p.gq, w, r), acc, p.scale, h);
 }
 
+template <int D, int RW, bool DMA>
+__global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
+    __shared__ __attribute__((aligned(16))) float lds0[256 / RW * D], lds1[256 / RW * D];
+    __shared__ int lds_end[4];
+    gq_work<D, RW, DMA, false>(p, blockIdx.x, lds0, lds1, lds_end);
+}
+
 // ---- gradients of keys and values: a wavefront owns 32 keys and walks the rows of the pair, 32 at a time.  CW wavefronts
 // take the workgroup's 32 CW keys, the 4 / CW times as many share each block's rows and are added up through LDS.  Four
 // products a block, the matrix pipes busy for 86 %.  32 x 12 heads, 512 x 512, D = 64: 440 us (117 TFLOP/s); lengths 512 to 272:
 // 378 us.  (dQ from here too would save two of the seven products of a gradient, and cost sums over workgroups.)
 template <int D, int CW, bool DMA>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 32 ? 3 : 2))) cross_gkv_kernel(const CrossP p) {
+__device__ __forceinline__ void gkv_work(const CrossP &p, uint32_t id, float (&lds0)[256 / CW * D], float (&lds1)[256 / CW * D], float (&rows0)[256 / CW],
+                                         float (&rows1)[256 / CW], int *lds_end) {  // rows: their lse and delta
     constexpr int GW = 4 / CW, RB = 32 * GW, ND = D / 32, KEYS = 32 * CW, SLOT = 32 * ND;
-    __shared__ __attribute__((aligned(16))) float lds0[2 * RB * D], lds1[2 * RB * D];  // two buffers of rows of Q and dO
-    __shared__ __attribute__((aligned(16))) float rows0[2 * RB], rows1[2 * RB];        // their lse and delta
-    __shared__ int lds_end[8];
     static_assert((GW - 1) * CW * 64 * SLOT <= 2 * RB * D, "the merge fits in a buffer");
-    const Work w = find_key_work<KEYS>(p, lds_end);
+    const Work w = find_key_work<KEYS>(p, id, lds_end);
     if (w.b < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 31, h = lane >> 5;
     const int j0 = (int)w.tile * KEYS, j = j0 + (wave % CW) * 32 + c, rw = wave / CW * 32;
@@ -820,6 +832,48 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 3
         write_column<D>(const_cast<float *>(p.gk.p) + w.b * p.gk.b + w.g * p.gk.h + (int64_t)j * p.gk.l, gk, p.scale, h);
         write_column<D>(const_cast<float *>(p.gv.p) + w.b * p.gv.b + w.g * p.gv.h + (int64_t)j * p.gv.l, gv, 1.0f, h);
     }
+}
+
+template <int D, int CW, bool DMA>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 32 ? 3 : 2))) cross_gkv_kernel(const CrossP p) {
+    __shared__ __attribute__((aligned(16))) float lds0[256 / CW * D], lds1[256 / CW * D];  // two buffers of rows of Q and dO
+    __shared__ __attribute__((aligned(16))) float rows0[256 / CW], rows1[256 / CW];
+    __shared__ int lds_end[8];
+    gkv_work<D, CW, DMA>(p, blockIdx.x, lds0, lds1, rows0, rows1, lds_end);
+}
+
+// ---- both gradients in one launch, where each on its own leaves compute units idle at its end: the first key_ids workgroups
+// (a multiple of 8) take keys, the others rows.  All launches of a gradient, apart and together: 7 x 2 key heads of 1332 rows, 1001
+// keys of size 32 91 and 80 us; 12 heads of 512 x 512, size 64, 8 sequences 217 and 185 us, 16 (50 MB of O and dO) 364 and 351 us,
+// 32 (101 MB) 661 and 676 us.
+template <int D, bool DMA>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 32 ? 3 : 2))) cross_both_kernel(const CrossP keys, const CrossP rows, uint32_t key_ids) {
+    __shared__ __attribute__((aligned(16))) float lds0[128 * D], lds1[128 * D];
+    __shared__ __attribute__((aligned(16))) float rows0[128], rows1[128];
+    __shared__ int lds_end[8];
+    if (blockIdx.x >= key_ids) gq_work<D, 2, DMA, true>(rows, blockIdx.x - key_ids, lds0, lds1, lds_end);
+    else if (keys.ends || blockIdx.x < keys.tiles * keys.pairs * keys.splits) gkv_work<D, 2, DMA>(keys, blockIdx.x, lds0, lds1, rows0, rows1, lds_end);
+}
+
+// In front of it: the lengths (the first `ends` workgroups), and delta by D / 4 lanes a row.
+template <int D>
+__global__ void __launch_bounds__(256) cross_front_kernel(const CrossP p, uint32_t ends) {
+    __shared__ int lds[4];
+    if (blockIdx.x < ends) {
+        const int end = visible_end(p, blockIdx.x, lds);
+        if (threadIdx.x == 0) p.ends[blockIdx.x] = end;
+        return;
+    }
+    constexpr int LPR = D / 4;
+    const uint32_t total = p.pairs * p.R, row = (blockIdx.x - ends) * (256 / LPR) + threadIdx.x / LPR, at = min(row, total - 1);
+    Work w;
+    w.pair = at / p.R;
+    w.b = (int)fdiv(w.pair, p.d_g);
+    w.g = (int)w.pair - w.b * p.G;
+    const uint32_t r = at - w.pair * p.R, col = threadIdx.x % LPR * 4;
+    const f32x4 o = load4(p.o.p + row_at(p, p.o, w, r) + col), g = load4(p.go.p + row_at(p, p.go, w, r) + col);
+    const float sum = group_sum<D>(__builtin_fmaf(o.w, g.w, __builtin_fmaf(o.z, g.z, __builtin_fmaf(o.y, g.y, o.x * g.x))));
+    if (row < total && col == 0) p.delta[row] = sum;
 }
 
 // out[row] = sum of the splits' rows, in order: D / 4 lanes a row.  Rows are [batch][heads][length].  The gradients that were
@@ -950,6 +1004,7 @@ Plan plan(const sg_ctx *ctx, const CrossP &p, int64_t D, int own, int other, int
 int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
     p.tiles = (uint32_t)tiles;
     p.splits = splits;
+    p.spread = (uint64_t)p.pairs * splits < 64;  // an XCD would have fewer than 8 units, of different lengths
     if (tiles * p.pairs * splits >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: too many rows for one launch");
     p.d_tiles = sg_make_fastdiv(p.tiles);
     return SG_OK;
@@ -1059,11 +1114,14 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     p.strided = p.H == p.G || (p.q.h == p.Lq * p.q.l && p.go.h == p.Lq * p.go.l);
     sg_device_guard guard(ctx);
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
-    const Plan by_rows = plan(ctx, p, D, p.R, p.Lk, 1, 4, D == 64 ? 2.6 : 1.6);
+    const bool dma = aligned_rows(p.q) && aligned_rows(p.k) && aligned_rows(p.v) && aligned_rows(p.o) && aligned_rows(p.go);
+    // One launch for both gradients up to 64 MB of O and dO, which delta has to be made of in front then
+    const bool both = p.R > 32 && total * D * 8 <= (64u << 20);
+    const Plan by_rows = plan(ctx, p, D, p.R, p.Lk, both ? 2 : 1, both ? 2 : 4, D == 64 ? 2.6 : 1.6);
     // 128 keys a workgroup only where all are visible: smaller tiles waste less of a sequence's last one and level better
     // (32 x 12 heads of 512 x 512: 446 us against 473 with 64 keys; with lengths 512 to 272: 423 against 404 us); and up to 32
     // rows, all of which a wavefront takes (15 rows, 14 x 8 heads, 4048 keys of size 32: 99 us with 64 keys, 53 us).
-    const Plan by_keys = plan(ctx, p, D, p.Lk, p.R, p.R <= 32 ? 4 : 2, p.mask && p.R > 32 ? 2 : 4, D == 64 ? 3.4 : 2.0);
+    const Plan by_keys = plan(ctx, p, D, p.Lk, p.R, p.R <= 32 ? 4 : 2, both || (p.mask && p.R > 32) ? 2 : 4, D == 64 ? 3.4 : 2.0);
     const int rw = by_rows.waves, cw = by_keys.waves;
     const uint32_t row_tiles = (uint32_t)((p.R + 32 * rw - 1) / (32 * rw)), key_tiles = (uint32_t)((p.Lk + 32 * cw - 1) / (32 * cw));
     const uint32_t row_splits = by_rows.splits, key_splits = by_keys.splits;
@@ -1076,32 +1134,50 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     p.part_o = p.delta + delta_floats;
     p.part_k = p.part_o + rows_part;
     p.part_v = p.part_k + key_splits * keys * D;
-    if (orders_lengths(ctx, p, (uint64_t)key_tiles * key_splits * p.pairs, 1)) {
-        p.ends = (int *)(p.delta + total);
-        hipLaunchKernelGGL(cross_ends_kernel, dim3((unsigned)p.N), dim3(256), 0, ctx->stream, p);
-        SG_CHECK_LAUNCH(ctx, "cross_attention_grad lengths");
-    }
-    if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
-    const bool dma = aligned_rows(p.q) && aligned_rows(p.k) && aligned_rows(p.v) && aligned_rows(p.o) && aligned_rows(p.go);
-    SG_CROSS_ROWS(cross_gq_kernel, rw, dma, dim3(p.tiles * p.pairs * p.splits));
-    SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
-    if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
-    uint32_t workgroups = p.tiles * p.pairs * p.splits;
-    if (p.ends) workgroups = (workgroups + 7) / 8 * 8;
-    const dim3 grid(workgroups);
+    if (both) {
+        const uint32_t ends = p.mask && p.N <= 256 ? (uint32_t)p.N : 0;
+        if (ends) p.ends = (int *)(p.delta + total);
+        const dim3 front(ends + (unsigned)((total + 1024 / D - 1) / (1024 / D)));
+        if (D == 64) hipLaunchKernelGGL((cross_front_kernel<64>), front, dim3(256), 0, ctx->stream, p, ends);
+        else hipLaunchKernelGGL((cross_front_kernel<32>), front, dim3(256), 0, ctx->stream, p, ends);
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad delta");
+        CrossP rows = p;
+        if ((rc = set_tiles(ctx, rows, row_tiles, row_splits)) != SG_OK) return rc;
+        if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
+        const uint32_t key_ids = (p.tiles * p.pairs * p.splits + 7) / 8 * 8;
+        const dim3 grid(key_ids + rows.tiles * rows.pairs * rows.splits);
+        if (D == 64 && dma) hipLaunchKernelGGL((cross_both_kernel<64, true>), grid, dim3(256), 0, ctx->stream, p, rows, key_ids);
+        else if (D == 64) hipLaunchKernelGGL((cross_both_kernel<64, false>), grid, dim3(256), 0, ctx->stream, p, rows, key_ids);
+        else if (dma) hipLaunchKernelGGL((cross_both_kernel<32, true>), grid, dim3(256), 0, ctx->stream, p, rows, key_ids);
+        else hipLaunchKernelGGL((cross_both_kernel<32, false>), grid, dim3(256), 0, ctx->stream, p, rows, key_ids);
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad");
+    } else {
+        if (orders_lengths(ctx, p, (uint64_t)key_tiles * key_splits * p.pairs, 1)) {
+            p.ends = (int *)(p.delta + total);
+            hipLaunchKernelGGL(cross_ends_kernel, dim3((unsigned)p.N), dim3(256), 0, ctx->stream, p);
+            SG_CHECK_LAUNCH(ctx, "cross_attention_grad lengths");
+        }
+        if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
+        SG_CROSS_ROWS(cross_gq_kernel, rw, dma, dim3(p.tiles * p.pairs * p.splits));
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
+        if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
+        uint32_t workgroups = p.tiles * p.pairs * p.splits;
+        if (p.ends) workgroups = (workgroups + 7) / 8 * 8;
+        const dim3 grid(workgroups);
 #define SG_CROSS_KEYS(D_, CW, DMA) hipLaunchKernelGGL((cross_gkv_kernel<D_, CW, DMA>), grid, dim3(256), 0, ctx->stream, p)
 #define SG_CROSS_KEYS_(D_, CW)                 \
-    do {                                       \
-        if (dma) SG_CROSS_KEYS(D_, CW, true);  \
-        else SG_CROSS_KEYS(D_, CW, false);     \
-    } while (0)
-    if (D == 64 && cw == 4) SG_CROSS_KEYS_(64, 4);
-    else if (D == 64) SG_CROSS_KEYS_(64, 2);
-    else if (cw == 4) SG_CROSS_KEYS_(32, 4);
-    else SG_CROSS_KEYS_(32, 2);
+        do {                                       \
+            if (dma) SG_CROSS_KEYS(D_, CW, true);  \
+            else SG_CROSS_KEYS(D_, CW, false);     \
+        } while (0)
+        if (D == 64 && cw == 4) SG_CROSS_KEYS_(64, 4);
+        else if (D == 64) SG_CROSS_KEYS_(64, 2);
+        else if (cw == 4) SG_CROSS_KEYS_(32, 4);
+        else SG_CROSS_KEYS_(32, 2);
 #undef SG_CROSS_KEYS_
 #undef SG_CROSS_KEYS
-    SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys and values");
+        SG_CHECK_LAUNCH(ctx, "cross_attention_grad keys and values");
+    }
     SumJobs sums{};
     uint32_t blocks = 0;
     auto add = [&](const float *part, const Rows &out, uint64_t rows, uint32_t splits, int heads, int length) {

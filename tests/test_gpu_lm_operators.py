@@ -402,7 +402,8 @@ def test_cross_attention_masks(ctx, n, h, g, lq, lk, d):
     (24, 12, 12, 70, 96, 32, True), (24, 12, 12, 70, 96, 64, True), (300, 2, 1, 40, 50, 32, True), (40, 8, 4, 200, 130, 64, True), (24, 12, 12, 96, 128, 64, False),
     (5, 4, 4, 9, 2000, 64, True), (8, 16, 4, 100, 200, 32, False), (9, 12, 12, 512, 33, 64, True), (1, 1, 1, 2000, 2000, 64, False), (1, 1, 1, 2000, 2000, 32, True),
     (22, 12, 12, 250, 40, 32, True), (4, 2, 2, 200, 31, 32, True), (40, 12, 12, 97, 100, 32, True), (3, 2, 2, 700, 300, 32, False), (2, 2, 2, 1, 7000, 32, False), (2, 4, 2, 2, 5000, 64, True), (2, 8, 1, 1, 3000, 64, True),
-    (300, 1, 1, 8, 70, 32, True), (1, 2, 1, 1, 4000, 32, True), (2, 3, 1, 1, 900, 32, True), (1, 4, 2, 1, 600, 64, True)])
+    (300, 1, 1, 8, 70, 32, True), (1, 2, 1, 1, 4000, 32, True), (2, 3, 1, 1, 900, 32, True), (1, 4, 2, 1, 600, 64, True),
+    (32, 12, 12, 352, 70, 64, True), (32, 12, 12, 352, 140, 64, False), (44, 12, 12, 520, 40, 32, True), (6, 4, 2, 30, 700, 64, True), (7, 8, 2, 60, 300, 32, True)])
 def test_cross_attention_of_many_and_of_long_sequences(ctx, n, h, g, lq, lk, d, masked):
     """Against the formula; rows that begin at any element give the bits that aligned ones give."""
     say("paths", n, h, g, lq, lk, d, masked)
