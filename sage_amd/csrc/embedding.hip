@@ -7,6 +7,37 @@
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes at any element
+
+// Columns c .. c + 3 of a row of E.  Where fewer than 4 are left the row's last 4 are taken instead: two lanes then do the
+// same for some columns and store the same values there, but no load waits behind a branch (a row of any width begins
+// anywhere; 21969 tokens of 145: lookup 7.5, sums of the gradient 10.9, join 7.8 us, with 4 bytes a load 9.8, 13.5 and 9.6).
+// NARROW: E below 4.  NT: past the caches.
+template <bool NARROW, bool NT = false>
+__device__ __forceinline__ f32x4 load_cols(const float *row, uint32_t c, uint32_t E) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (NARROW) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (c + j < E) v[j] = row[c + j];
+    } else if (c < E) {
+        const f32x4_any *p = reinterpret_cast<const f32x4_any *>(row + min(c, E - 4));
+        v = NT ? __builtin_nontemporal_load(p) : *p;
+    }
+    return v;
+}
+template <bool NARROW, bool NT = false>
+__device__ __forceinline__ void store_cols(float *row, uint32_t c, uint32_t E, f32x4 v) {
+    if (NARROW) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (c + j < E) row[c + j] = v[j];
+    } else if (c < E) {
+        f32x4_any *p = reinterpret_cast<f32x4_any *>(row + min(c, E - 4));
+        if (NT) __builtin_nontemporal_store(v, p);
+        else *p = v;
+    }
+}
 
 struct EmbP {
     const float *table;
@@ -14,14 +45,14 @@ struct EmbP {
     float *out;
     sg_rows id_rows;
     uint32_t n, E, V, pieces;
-    int64_t table_stride, E_stride;
+    int64_t table_stride;
     float scale;
 };
 
-// A wavefront writes 256 columns of one token's row (VEC: 16 bytes a lane): every piece of every row is a wavefront of its
+// A wavefront writes 256 columns of one token's row, 16 bytes a lane: every piece of every row is a wavefront of its
 // own, so that the few rows of a serving batch are in flight together too.  Rows of 768: 8 tokens 2.6 us, the time of a launch;
 // 4096 tokens 6.4 us (25 MB, 3.9 TB/s); 32768 tokens, three tenths of them none, 20 us (101 MB written past the caches, 5 TB/s).
-template <bool VEC, bool NT>
+template <bool NARROW, bool NT>
 __global__ void __launch_bounds__(256) embedding_kernel(const EmbP p) {
     const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (unit >= (uint64_t)p.n * p.pieces) return;
@@ -31,17 +62,10 @@ __global__ void __launch_bounds__(256) embedding_kernel(const EmbP p) {
     const bool known = id < p.V;
     const float *src = p.table + (known ? (int64_t)id * p.table_stride : 0);
     float *dst = p.out + (int64_t)token * p.E;
-    if (VEC) {
-        const uint32_t c = piece * 256 + lane * 4;
-        if (c >= p.E) return;
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (known) v = *reinterpret_cast<const f32x4 *>(src + c) * p.scale;
-        if (NT) __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(dst + c));
-        else *reinterpret_cast<f32x4 *>(dst + c) = v;
-    } else {
-        for (uint32_t c = piece * 256 + lane; c < p.E && c < piece * 256 + 256; c += 64)
-            dst[c] = known ? src[(int64_t)c * p.E_stride] * p.scale : 0.0f;
-    }
+    const uint32_t c = piece * 256 + lane * 4;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (known) v = load_cols<NARROW>(src, c, p.E) * p.scale;
+    store_cols<NARROW, NT>(dst, c, p.E, v);
 }
 
 // ---- gradient.  The tokens are sorted by id (stable, so a row's tokens stay in order), unknown ones behind the last row;
@@ -290,31 +314,6 @@ struct SumP {
     float scale;
 };
 
-// 4 columns of a lane: consecutive (VEC) or 64 apart.  NT: past the caches.
-template <bool VEC, bool NT = false>
-__device__ __forceinline__ f32x4 load_cols(const float *row, uint32_t c, uint32_t E) {
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (VEC) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(row + c);
-        if (c < E) v = NT ? __builtin_nontemporal_load(p) : *p;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + 64 * j < E) v[j] = row[c + 64 * j];
-    }
-    return v;
-}
-template <bool VEC>
-__device__ __forceinline__ void store_cols(float *row, uint32_t c, uint32_t E, f32x4 v) {
-    if (VEC) {
-        if (c < E) *reinterpret_cast<f32x4 *>(row + c) = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + 64 * j < E) row[c + 64 * j] = v[j];
-    }
-}
-
 // Up to 128 tokens, in one launch: a workgroup owns some rows of the table, clears them, finds its tokens among all and sums
 // the rows that have some in the tokens' order (23 tokens, table of 230 x 243: 5.4 us; 90 tokens, 2633 x 538: 10.8 us, with 30
 // rows a workgroup instead of 4 15.6 us; 120 tokens, 30522 x 768: 20 us, 14 of them a fill's.  Sort, sums and join are three
@@ -330,7 +329,7 @@ struct FewP {
     float scale;
 };
 
-template <bool VEC>
+template <bool NARROW>
 __global__ void __launch_bounds__(FEW_THREADS) embedding_few_kernel(const FewP p) {
     __shared__ __attribute__((aligned(16))) uint32_t row_of[FEW];  // of each token, ~0: not here
     __shared__ uint32_t firsts[FEW], distinct;
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(FEW_THREADS) embedding_few_kernel(const FewP p
     __syncthreads();  // the zeros, too, are written before the sums
     const uint32_t pieces = (p.E + 255) / 256, units = distinct * pieces;
     for (uint32_t u = wave; u < units; u += FEW_THREADS / 64) {  // a wavefront sums 256 columns of a row, 8 tokens in flight
-        const uint32_t r = firsts[u / pieces], c = u % pieces * 256 + (VEC ? lane * 4 : lane);
+        const uint32_t r = firsts[u / pieces], c = u % pieces * 256 + lane * 4;
         uint64_t a = __builtin_amdgcn_ballot_w64(row_of[lane] == r), b = __builtin_amdgcn_ballot_w64(row_of[64 + lane] == r);
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         while (a | b) {
@@ -371,25 +370,25 @@ __global__ void __launch_bounds__(FEW_THREADS) embedding_few_kernel(const FewP p
                 const uint32_t token = a ? (uint32_t)__builtin_ctzll(a) : 64 + (uint32_t)__builtin_ctzll(b);
                 if (a) a &= a - 1;
                 else b &= b - 1;
-                x[k] = load_cols<VEC>(p.gout + sg_row_offset(p.g_rows, token), c, p.E);
+                x[k] = load_cols<NARROW>(p.gout + sg_row_offset(p.g_rows, token), c, p.E);
                 got = k + 1;
             }
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k)
                 if (k < got) acc += x[k];
         }
-        store_cols<VEC>(table + (uint64_t)r * p.E, c, p.E, acc * p.scale);
+        store_cols<NARROW>(table + (uint64_t)r * p.E, c, p.E, acc * p.scale);
     }
 }
 
 // A wavefront sums 256 columns of one chunk of sorted tokens; BATCH rows are in flight at a time.  A large gout goes past
 // the caches and leaves them to the table, which the next lookup reads (32768 tokens: that lookup 32 -> 20 us).
-template <bool VEC, bool NT, uint32_t BATCH>
+template <bool NARROW, bool NT, uint32_t BATCH>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
     const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (unit >= p.chunks * p.pieces) return;
     const uint32_t chunk = unit / p.pieces, piece = unit - chunk * p.pieces;
-    const uint32_t c = piece * 256 + (VEC ? lane * 4 : lane);
+    const uint32_t c = piece * 256 + lane * 4;
     const uint32_t first = chunk * p.chunk, last = min(first + p.chunk, p.n);
     const uint32_t own = min(first + lane, p.n - 1);
     const uint32_t key = p.key[own], pos = p.pos[own];
@@ -404,7 +403,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
             const uint32_t at = min(b + k, last - 1) - first;
             id[k] = (uint32_t)__builtin_amdgcn_readlane((int)key, (int)at);
             if (b + k < last && id[k] < p.V)
-                x[k] = load_cols<VEC, NT>(p.gout + sg_row_offset(p.g_rows, (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)at)), c, p.E);
+                x[k] = load_cols<NARROW, NT>(p.gout + sg_row_offset(p.g_rows, (uint32_t)__builtin_amdgcn_readlane((int)pos, (int)at)), c, p.E);
         }
         id[BATCH] = b + BATCH < last ? (uint32_t)__builtin_amdgcn_readlane((int)key, (int)(b + BATCH - first)) : next;
 #pragma unroll
@@ -414,9 +413,9 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
             const bool end = b + k + 1 == last;
             const uint32_t follow = end ? next : id[k + 1];
             if (follow == id[k] && !end) continue;
-            if (from_before) store_cols<VEC>(p.part + (uint64_t)chunk * 2 * p.E, c, p.E, acc);
-            else if (follow == id[k]) store_cols<VEC>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E, acc);
-            else store_cols<VEC>(p.gtable + (uint64_t)id[k] * p.E, c, p.E, acc * p.scale);
+            if (from_before) store_cols<NARROW>(p.part + (uint64_t)chunk * 2 * p.E, c, p.E, acc);
+            else if (follow == id[k]) store_cols<NARROW>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E, acc);
+            else store_cols<NARROW>(p.gtable + (uint64_t)id[k] * p.E, c, p.E, acc * p.scale);
             acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             from_before = false;
         }
@@ -425,12 +424,12 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
 
 // A workgroup for 256 columns of the run that begins in a chunk and goes on behind it: the partial sums of the chunks it
 // covers, shared out over the wavefronts in order and joined in order.
-template <bool VEC>
+template <bool NARROW>
 __global__ void __launch_bounds__(256) embedding_join_kernel(const SumP p) {
     __shared__ f32x4 sums[4][64];
     const uint32_t chunk = blockIdx.x / p.pieces, piece = blockIdx.x - chunk * p.pieces;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t c = piece * 256 + (VEC ? lane * 4 : lane);
+    const uint32_t c = piece * 256 + lane * 4;
     const uint32_t behind = (chunk + 1) * p.chunk;  // this kernel has a workgroup for every chunk but the last
     const uint32_t id = p.key[behind];
     if (id >= p.V || p.key[behind - 1] != id) return;                            // nothing goes on
@@ -443,22 +442,22 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const SumP p) {
     }
     const uint32_t count = lo - chunk, from = chunk + 1 + count * wave / 4, to = chunk + 1 + count * (wave + 1) / 4;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (wave == 0) acc = load_cols<VEC>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E);
+    if (wave == 0) acc = load_cols<NARROW>(p.part + ((uint64_t)chunk * 2 + 1) * p.E, c, p.E);
     uint32_t i = from;
     for (; i + 8 <= to; i += 8) {
         f32x4 x[8];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) x[k] = load_cols<VEC>(p.part + (uint64_t)(i + k) * 2 * p.E, c, p.E);
+        for (uint32_t k = 0; k < 8; ++k) x[k] = load_cols<NARROW>(p.part + (uint64_t)(i + k) * 2 * p.E, c, p.E);
 #pragma unroll
         for (uint32_t k = 0; k < 8; ++k) acc += x[k];
     }
-    for (; i < to; ++i) acc += load_cols<VEC>(p.part + (uint64_t)i * 2 * p.E, c, p.E);
+    for (; i < to; ++i) acc += load_cols<NARROW>(p.part + (uint64_t)i * 2 * p.E, c, p.E);
     sums[wave][lane] = acc;
     __syncthreads();
     if (wave) return;
 #pragma unroll
     for (int w = 1; w < 4; ++w) acc += sums[w][lane];
-    store_cols<VEC>(p.gtable + (uint64_t)id * p.E, c, p.E, acc * p.scale);
+    store_cols<NARROW>(p.gtable + (uint64_t)id * p.E, c, p.E, acc * p.scale);
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p) % 16 == 0; }
@@ -494,15 +493,13 @@ extern "C" int sg_embedding(sg_ctx *ctx, const sg_tensor *table, const sg_tensor
     p.V = (uint32_t)table->extents[0];
     p.pieces = (p.E + 255) / 256;
     p.table_stride = table->strides[0];
-    p.E_stride = 1;
     p.scale = scale;
-    const bool vec = E % 4 == 0 && p.table_stride % 4 == 0 && aligned16(p.table) && aligned16(p.out);
     const bool nt = sg_streaming((int64_t)p.n * E * 4);
     const uint64_t units = (uint64_t)p.n * p.pieces;
     sg_device_guard guard(ctx);
     const dim3 grid((unsigned)((units + 3) / 4));
-    if (vec && nt) hipLaunchKernelGGL((embedding_kernel<true, true>), grid, dim3(256), 0, ctx->stream, p);
-    else if (vec) hipLaunchKernelGGL((embedding_kernel<true, false>), grid, dim3(256), 0, ctx->stream, p);
+    if (E < 4) hipLaunchKernelGGL((embedding_kernel<true, false>), grid, dim3(256), 0, ctx->stream, p);
+    else if (nt) hipLaunchKernelGGL((embedding_kernel<false, true>), grid, dim3(256), 0, ctx->stream, p);
     else hipLaunchKernelGGL((embedding_kernel<false, false>), grid, dim3(256), 0, ctx->stream, p);
     SG_CHECK_LAUNCH(ctx, "embedding");
     return SG_OK;
@@ -553,10 +550,8 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
         f.rows = rows < 4 ? 4 : rows / 4 * 4;
         f.fill_vec = aligned16(table);
         sg_device_guard guard(ctx);
-        bool vec = E % 4 == 0 && aligned16(f.gout) && aligned16(table);
-        for (int i = 0; i < f.g_rows.rank; ++i) vec = vec && f.g_rows.st[i] % 4 == 0;
         const dim3 grid((s.V + f.rows - 1) / f.rows);
-        if (vec) hipLaunchKernelGGL((embedding_few_kernel<true>), grid, dim3(FEW_THREADS), 0, ctx->stream, f);
+        if (E < 4) hipLaunchKernelGGL((embedding_few_kernel<true>), grid, dim3(FEW_THREADS), 0, ctx->stream, f);
         else hipLaunchKernelGGL((embedding_few_kernel<false>), grid, dim3(FEW_THREADS), 0, ctx->stream, f);
         SG_CHECK_LAUNCH(ctx, "embedding_grad");
         return SG_OK;
@@ -642,15 +637,14 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
         m.key = s.key_out;
         m.pos = s.pos_out;
     }
-    bool vec = E % 4 == 0 && aligned16(m.gout) && aligned16(table);
-    for (int i = 0; i < m.g_rows.rank; ++i) vec = vec && m.g_rows.st[i] % 4 == 0;
+    const bool narrow = E < 4, nt = sg_streaming((int64_t)m.n * E * 4);
     const dim3 sum_grid((m.chunks * m.pieces + 3) / 4), join_grid((m.chunks - 1) * m.pieces);
-    if (vec && sg_streaming((int64_t)m.n * E * 4)) hipLaunchKernelGGL((embedding_sum_kernel<true, true, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
-    else if (vec) hipLaunchKernelGGL((embedding_sum_kernel<true, false, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
-    else hipLaunchKernelGGL((embedding_sum_kernel<false, false, 4>), sum_grid, dim3(256), 0, ctx->stream, m);
+    if (narrow) hipLaunchKernelGGL((embedding_sum_kernel<true, false, 4>), sum_grid, dim3(256), 0, ctx->stream, m);
+    else if (nt) hipLaunchKernelGGL((embedding_sum_kernel<false, true, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
+    else hipLaunchKernelGGL((embedding_sum_kernel<false, false, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
     SG_CHECK_LAUNCH(ctx, "embedding_grad sums");
     if (m.chunks > 1) {
-        if (vec) hipLaunchKernelGGL((embedding_join_kernel<true>), join_grid, dim3(256), 0, ctx->stream, m);
+        if (narrow) hipLaunchKernelGGL((embedding_join_kernel<true>), join_grid, dim3(256), 0, ctx->stream, m);
         else hipLaunchKernelGGL((embedding_join_kernel<false>), join_grid, dim3(256), 0, ctx->stream, m);
         SG_CHECK_LAUNCH(ctx, "embedding_grad join");
     }
