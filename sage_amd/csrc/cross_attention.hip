@@ -844,8 +844,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 3
 
 // ---- both gradients in one launch, where each on its own leaves compute units idle at its end: the first key_ids workgroups
 // (a multiple of 8) take keys, the others rows.  All launches of a gradient, apart and together: 7 x 2 key heads of 1332 rows, 1001
-// keys of size 32 91 and 80 us; 12 heads of 512 x 512, size 64, 8 sequences 217 and 185 us, 16 (50 MB of O and dO) 364 and 351 us,
-// 32 (101 MB) 661 and 676 us.
+// to 501 keys of size 32 91 and 80 us; 12 heads of 512 x 512, size 64, 8 sequences 247 and 223 us, 16 408 and 432 us, with lengths
+// 512 to 272 8 sequences 217 and 185 us, 16 364 and 351 us, 32 661 and 676 us.
 template <int D, bool DMA>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 32 ? 3 : 2))) cross_both_kernel(const CrossP keys, const CrossP rows, uint32_t key_ids) {
     __shared__ __attribute__((aligned(16))) float lds0[128 * D], lds1[128 * D];
@@ -1115,8 +1115,10 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
     sg_device_guard guard(ctx);
     const uint64_t total = (uint64_t)p.pairs * p.R, keys = (uint64_t)p.pairs * p.Lk;
     const bool dma = aligned_rows(p.q) && aligned_rows(p.k) && aligned_rows(p.v) && aligned_rows(p.o) && aligned_rows(p.go);
-    // One launch for both gradients up to 64 MB of O and dO, which delta has to be made of in front then
-    const bool both = p.R > 32 && total * D * 8 <= (64u << 20);
+    // One launch for both gradients, while their workgroups of 64 rows or keys are few enough for a launch's end to count (8 for a
+    // compute unit, 12 where lengths differ), and O and dO, of which delta has to be made in front then, are 64 MB at most.
+    const uint64_t tiles64 = (uint64_t)((p.R + 63) / 64 + (p.Lk + 63) / 64) * p.pairs, cus = (uint64_t)(ctx->num_cus > 0 ? ctx->num_cus : 256);
+    const bool both = p.R > 32 && total * D * 8 <= (64u << 20) && tiles64 <= (p.mask ? 12 : 8) * cus;
     const Plan by_rows = plan(ctx, p, D, p.R, p.Lk, both ? 2 : 1, both ? 2 : 4, D == 64 ? 2.6 : 1.6);
     // 128 keys a workgroup only where all are visible: smaller tiles waste less of a sequence's last one and level better
     // (32 x 12 heads of 512 x 512: 446 us against 473 with 64 keys; with lengths 512 to 272: 423 against 404 us); and up to 32
