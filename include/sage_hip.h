@@ -420,9 +420,9 @@ int sg_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_t
  * h / (H/G); unit stride on D, any strides elsewhere (separate_heads views, merged-heads outputs); D = 32 or 64.
  * mask: NULL or fp32 [N, Lk], unit stride on Lk, any batch stride: key j of sequence b is visible unless mask[b, j] is 0.
  * What a hidden key's k and v hold is not used, NaN or not.  A query without a visible key gives zeros and lse = -inf.
- * The softmax shift is the row's largest visible score.  lse: NULL or dense [N, H, Lq], log of the row's sum, for the
- * gradient.  A call with few query rows splits the keys over workgroups and joins the parts through a workspace of the
- * context allocator (SG_ERR_OOM). */
+ * The softmax shift follows the row's largest visible score, whatever its size.  lse: NULL or dense [N, H, Lq], log of the
+ * row's sum, for the gradient.  Keys may be split over workgroups and the lengths of masked sequences are found in front:
+ * both take a workspace from the context allocator (SG_ERR_OOM). */
 int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask,
                        float scale, const sg_tensor *out, const sg_tensor *lse);
 /* Its gradient: with P = e^(scale q.k - lse), dP = gout . v^T and dS = P (dP - rowsum(gout out)):
