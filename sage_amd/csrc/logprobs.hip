@@ -10,7 +10,8 @@
 // one equal to the bound has a higher index than k that reach it), some ten to a hundred of its share, in a list of its own
 // in LDS and without a barrier; the k largest of the wavefronts' lists are ranked at the end.
 // 4096 x 30522 without alternatives: 88 us (500 MB, 5.7 TB/s).  1021 x 50257 with 20: 60 us (205 MB, 3.4 TB/s: all rows are
-// on the chip at once, and choosing does not overlap another row's loads).  4 x 30522 with 5: 8.6 us and a join of 4.5.
+// on the chip at once, and choosing does not overlap another row's loads).  4 x 30522 with 5: 8.9 us and a join of 4.8;
+// 4 x 50257 with 64: 23 us and a join of 8.
 #include "rows.h"
 
 #include <type_traits>
@@ -170,22 +171,30 @@ __device__ __forceinline__ void wave_select(u64 *list, uint32_t n, uint32_t k) {
         __builtin_amdgcn_wave_barrier();
         return;
     }
+    constexpr uint32_t EACH = LIST / 64;
+    const uint32_t blocks = (n + 63) / 64;
+    u64 mine[EACH];  // read once, not for every bit (200 x 50257 with 64 alternatives: 62 us, 78 from LDS)
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) mine[i] = i < blocks && 64 * i + lane < n ? list[64 * i + lane] : 0;
     for (int bit = 63; bit >= 0; --bit) {
         const u64 higher = bound | (1ull << bit);
         uint32_t count = 0;
-        for (uint32_t i = 0; i < n; i += 64) count += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < n && list[i + lane] >= higher));
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i)
+            if (i < blocks) count += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(mine[i] >= higher));
         if (count >= k) bound = higher;
         if (count == k) break;
     }
     uint32_t to = 0;
-    for (uint32_t i = 0; i < n; i += 64) {
-        const u64 key = i + lane < n ? list[i + lane] : 0;
-        const u64 stay = __builtin_amdgcn_ballot_w64(i + lane < n && key >= bound);
-        __builtin_amdgcn_wave_barrier();
-        if (stay >> lane & 1) list[to + __popcll(stay & ((1ull << lane) - 1))] = key;
-        __builtin_amdgcn_wave_barrier();
-        to += (uint32_t)__popcll(stay);
-    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i)
+        if (i < blocks) {
+            const u64 stay = __builtin_amdgcn_ballot_w64(64 * i + lane < n && mine[i] >= bound);
+            if (stay >> lane & 1) list[to + __popcll(stay & ((1ull << lane) - 1))] = mine[i];
+            to += (uint32_t)__popcll(stay);
+        }
+    __builtin_amdgcn_wave_barrier();
 }
 
 // Place of a key among n different ones, largest first.
@@ -332,9 +341,10 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
     }
 }
 
-// Joins the parts of a split row.
+// Joins the parts of a split row.  (13 parts of 64 candidates: 8 us, 61 us where every candidate is compared with all.)
 __global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const LogpP p) {
-    __shared__ u64 keys[JOIN];
+    __shared__ u64 keys[JOIN], bound;
+    __shared__ uint32_t count;
     __shared__ float lds_stats[12];
     const uint32_t row = blockIdx.x, tid = threadIdx.x;
     const float *x = p.logits + sg_row_offset(p.rows, row);
@@ -353,12 +363,33 @@ __global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const LogpP p) {
             p.logprob[row] = tok < p.C ? r.logprob(x[tok], c) : 0.0f;
         }
     }
+    if (p.k == 0) return;
     const uint32_t n = p.splits * p.k;  // at most JOIN
-    for (uint32_t i = tid; i < n; i += THREADS) keys[i] = p.part_keys[(uint64_t)row * n + i];
+    const u64 *parts = p.part_keys + (uint64_t)row * n;
+    if (n <= 128) {
+        if (tid < n) keys[tid] = parts[tid];
+        if (tid == 0) count = n;
+    } else {
+        // A part's keys are in order: the lowest of the parts' ceil(k / splits)-th keys is a bound that k keys reach, and few more do.
+        if (tid < 64) {
+            u64 low = tid < p.splits ? parts[tid * p.k + (p.k + p.splits - 1) / p.splits - 1] : ~0ull;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const u64 other = __shfl_xor(low, o, 64);
+                low = low < other ? low : other;
+            }
+            if (tid == 0) { bound = low; count = 0; }
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            const u64 key = parts[i];
+            if (key >= bound) keys[atomicAdd(&count, 1u)] = key;  // in any order: each finds its place among all
+        }
+    }
     __syncthreads();
-    for (uint32_t i = tid; i < n; i += THREADS) {
-        if (!keys[i]) continue;
-        const uint32_t at = place_of(keys, n, keys[i]);
+    for (uint32_t i = tid; i < count; i += THREADS) {
+        if (!keys[i]) continue;  // a part with fewer than k logits
+        const uint32_t at = place_of(keys, count, keys[i]);
         if (at >= p.k) continue;
         p.top_ids[(uint64_t)row * p.k + at] = index_of(keys[i]);
         p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(keys[i]), c);
