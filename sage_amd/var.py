@@ -1740,13 +1740,24 @@ class _Evaluator:
         return None, None
 
     def try_merged_heads(self, v):
-        """copy(permute(x)) where cross attention or its gradient left x in the permuted layout already."""
+        """copy(permute(x)) where cross attention or its gradient left x in the permuted layout already: the copy takes x's
+        memory over.  Only while nothing else that is handed out can view that memory: x is of this evaluation, neither x
+        nor the permuted node is asked for or viewed by another node (the gradient only reads x)."""
         p = v.inputs[0]
-        if p.op != "permute" or self.done(p) or p.inputs[0].op not in ("cross_attention", "cross_attention_grad", "part"):
+        if p.op != "permute" or not self._private(p):
             return None
-        x = self.get(p.inputs[0])
-        x = x.with_shape(x.shape.permute(p.attrs["axes"]))
-        return x if x.is_dense() else None
+        x = p.inputs[0]
+        if x.op not in ("cross_attention", "cross_attention_grad", "part") or x.value is not None or id(x) in self.targets:
+            return None
+        if any(u is not p and u.op not in ("cross_attention_grad", "part") for u in self.users[id(x)]):
+            return None
+        if x.op == "part":  # it belongs to the tensor of its operator
+            y = x.inputs[0]
+            if y.value is not None or id(y) in self.targets or any(u is not x and u.attrs == x.attrs for u in self.users[id(y)]):
+                return None
+        t = self.get(x)
+        t = t.with_shape(t.shape.permute(p.attrs["axes"]))
+        return t if t.is_dense() else None
 
     def try_permuted_matmul(self, v):
         """copy(permute(G)) with the last axis kept in place: let G write the permuted layout."""

@@ -873,3 +873,28 @@ def test_captured_in_a_caching_context_beside_another_context(ctx):
     prog.release_graph()
     del prog
     c.close()
+
+
+def test_a_copy_of_bound_outputs_is_a_snapshot(ctx):
+    """The transposed output and gradients of a bound program, copied: later runs of the program, and writes into one of two
+    targets, leave the copies alone."""
+    rng = np.random.default_rng(41)
+    q, k, v, go = cross_case(rng, 2, 4, 2, 6, 30, 32)
+    vs = [Var.new(dev(ctx, a)) for a in (q, k, v)]
+    y = nn.cross_attention(*vs)
+    nodes = [y, *grad(y, vs, seed=Var.new(dev(ctx, go)))]
+    prog = Program(ctx, nodes).bind()
+    copies = [x.transpose(2, 1).copy().eval(ctx) for x in nodes]
+    first = [c.numpy() for c in copies]
+    for c, x in zip(first, nodes):
+        assert same_bits(c, x.value.numpy().transpose(0, 2, 1, 3))
+    for t, a in zip(vs, (q, k, v)):
+        t.value.copy_from_numpy(a * np.float32(0.5))
+    prog.run()
+    for c, a, x in zip(copies, first, nodes):
+        assert same_bits(c.numpy(), a) and not same_bits(a, x.value.numpy().transpose(0, 2, 1, 3))
+    out = nn.cross_attention(*vs)
+    one, two = V.evaluate(ctx, [out, out.transpose(2, 1).copy()])
+    kept = one.numpy()
+    two.copy_from_numpy(np.zeros(two.extents, np.float32))
+    assert same_bits(one.numpy(), kept) and kept.any()

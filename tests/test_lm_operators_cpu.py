@@ -290,3 +290,73 @@ def test_eight_bit_states_at_the_borders():
     assert np.all(np.abs(R.decode(c, s, True)[:2]) == 2.0)  # rounded up past the mantissa: the scale has room
     c, s = R.encode(R.f32([np.inf, 1.0]), True, np.zeros(2, np.int64))
     assert np.isnan(s[0]) and np.isnan(R.decode(c, s, True)).all()
+
+
+# ----------------------------------------------------------------------------- copies own their memory
+def evaluated(targets):
+    """The targets' tensors, and how many copies (maps) were launched, on a context without a device."""
+    from sage_amd.var import _Evaluator
+    from tests.test_host_cpu import _DryCtx
+
+    class Log:
+        def __init__(self, lib):
+            self.lib, self.maps = lib, 0
+
+        def __getattr__(self, name):
+            self.maps += name == "sg_map"
+            return getattr(self.lib, name)
+    ctx = _DryCtx()
+    ctx._lib = Log(ctx._lib)
+    ev = _Evaluator(ctx, targets)
+    return [ev.get(t) for t in targets], ctx._lib.maps
+
+
+def cross_nodes():
+    from tests.test_host_cpu import _DryCtx, _data
+    ctx = _DryCtx()
+    q, k, v = (_data(ctx, *e) for e in (Q, K, K))
+    y = nn.cross_attention(q, k, v)
+    return y, *grad(y, [q, k, v], seed=_data(ctx, *Q))
+
+
+def bound(*nodes):
+    for n, t in zip(nodes, evaluated(list(nodes))[0]):
+        n.value = t
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+def test_copies_of_cross_attentions_tensors_have_memory_of_their_own(which):
+    """The operator leaves heads side by side, so the copy of its transposed output or gradients finds the layout it asks for;
+    it may take that memory over only where nobody else can see it."""
+    y = cross_nodes()[which]
+    (a, b), maps = evaluated([y, y.transpose(2, 1).copy()])  # both asked for
+    assert a.buf is not b.buf and maps == 1
+    y = cross_nodes()[which]
+    (a, b), maps = evaluated([y.transpose(2, 1), y.transpose(2, 1).copy()])  # the permuted view asked for
+    assert a.buf is not b.buf and maps == 1
+    y = cross_nodes()[which]
+    (a, b), maps = evaluated([y.transpose(2, 1).copy(), y.transpose(2, 1).copy()])  # two copies
+    assert a.buf is not b.buf
+    y = cross_nodes()[which]
+    (a, b), maps = evaluated([y.transpose(2, 1).copy(), y.slice(0, 0, 1)])  # another view
+    assert a.buf is not b.buf and maps == 1
+    nodes = cross_nodes()
+    bound(*nodes)  # as Program.bind leaves them
+    (a,), maps = evaluated([nodes[which].transpose(2, 1).copy()])
+    assert a.buf is not nodes[which].value.buf and maps == 1
+    if which >= 2:  # the same output of a bound operator, or asked for beside the copy
+        y, gq, gk, gv = cross_nodes()
+        bound(gq)
+        (a,), maps = evaluated([(gk, gv)[which - 2].transpose(2, 1).copy()])
+        assert a.buf is not gq.value.parts[("gk", "gv")[which - 2]].buf and maps == 1
+        y, gq, gk, gv = cross_nodes()
+        again = Var(gk.shape, FLOAT, "part", [gq], dict((gk, gv)[which - 2].attrs))
+        (a, b), maps = evaluated([again, (gk, gv)[which - 2].transpose(2, 1).copy()])
+        assert a.buf is not b.buf and maps == 1
+
+
+def test_merged_heads_inside_a_step_take_no_copy():
+    y, gq, gk, gv = cross_nodes()
+    merged = [x.transpose(2, 1).view([2, -1, x.extents[1] * 32]) for x in (y, gq, gk, gv)]
+    outs, maps = evaluated(merged)
+    assert maps == 0 and len({id(t.buf) for t in outs}) == 4
