@@ -438,7 +438,8 @@ __global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const LogpGradP 
         log2s = r.log2s;
     }
     auto grad = [&](float v, uint32_t j) {
-        const float lp2 = (v - shift) * c - log2s;
+        // a finite logit may be so low that its distance is not (the type's lowest value hides a token): 0 * -inf is NaN
+        const float lp2 = finite((v - shift) * c - log2s);
         const float pr = __builtin_amdgcn_exp2f(lp2);
         float g = -pr * (gl + ge * __builtin_fmaf(lp2, LN2, h));
         if (j == tok) g += gl;

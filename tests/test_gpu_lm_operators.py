@@ -898,3 +898,38 @@ def test_a_copy_of_bound_outputs_is_a_snapshot(ctx):
     kept = one.numpy()
     two.copy_from_numpy(np.zeros(two.extents, np.float32))
     assert same_bits(one.numpy(), kept) and kept.any()
+
+
+@pytest.mark.parametrize("c", [50, 9001, 30522])
+@pytest.mark.parametrize("scale", [1.0, 1.4])
+def test_token_logprobs_gradient_of_tokens_hidden_by_the_lowest_value(ctx, c, scale):
+    """Vocabularies masked with the type's lowest number: what -inf in its place gives, so 0 at hidden tokens (a hidden
+    target keeps its own gradient, which is exact); near 0 and far from it, beside the logits and in their place."""
+    say("hidden", c, scale)
+    rng = np.random.default_rng(c)
+    x = R.f32(rng.standard_normal((4, c)) * 2)
+    x[2] += 700.0
+    hidden = rng.random((4, c)) < 0.5
+    tokens = np.array([7, 3, 11, -100], np.int32)
+    hidden[np.arange(3), tokens[:3]] = [False, True, False]
+    hidden[:, 20] = False
+    clean = np.where(hidden, np.float32(-np.inf), x)
+    x[hidden] = np.finfo(np.float32).min
+    want = R.logprobs(clean, tokens, scale)
+    gl, ge = R.f32(rng.standard_normal(4)), R.f32(rng.standard_normal(4))
+    for a, b in ((gl, ge), (gl, None), (None, ge)):
+        xd = dev(ctx, x)
+        got = run_logprobs(ctx, xd, tokens, scale)
+        _, tok, outs = got["dev"]
+        ref_g, tol = R.logprobs_grad(want, scale, a, b), R.logprobs_grad_tol(want, clean, scale, a, b)
+        if a is not None:
+            ref_g[1, 3] = np.float32(scale) * gl[1]
+        for out in (Tensor.uninit(ctx, [4, c]), xd):
+            ctx.check(ctx._lib.sg_token_logprobs_grad(ctx.handle, ref(xd), ref(tok) if a is not None else None, C.c_float(scale), ref(outs["lse"]),
+                                                      ref(outs["entropy"]) if b is not None else None, ref(dev(ctx, a)) if a is not None else None,
+                                                      ref(dev(ctx, b)) if b is not None else None, ref(out)))
+            g = out.numpy()
+            near(g, ref_g, tol, "glogits")
+            hit = hidden.copy()
+            hit[1, 3] = False
+            assert not g[hit].any()
