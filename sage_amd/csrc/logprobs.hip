@@ -94,7 +94,8 @@ struct RowResult {
         lse = empty ? -inf : __builtin_fmaf(shift, scale, log2s * LN2);
         entropy = empty ? 0.0f : (log2s - a.t / a.s) * LN2;
     }
-    __device__ float logprob(float x, float c) const { return empty ? -__builtin_inff() : ((x - shift) * c - log2s) * LN2; }
+    // (not by way of base 2, where the distance of the type's lowest value is -inf)
+    __device__ float logprob(float x, float scale) const { return empty ? -__builtin_inff() : __builtin_fmaf(x - shift, scale, -(log2s * LN2)); }
 };
 
 // The row as 16-byte groups: group g holds logits 4g - lead .. 4g - lead + 3, those that exist.
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
             if (p.entropy) p.entropy[row] = r.entropy;
             if (p.logprob) {
                 const uint32_t tok = p.tokens[sg_row_offset(p.token_rows, row)];
-                p.logprob[row] = tok < p.C ? r.logprob(x[tok], c) : 0.0f;
+                p.logprob[row] = tok < p.C ? r.logprob(x[tok], p.scale) : 0.0f;
             }
         }
     }
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
                 if (p.splits > 1) p.part_keys[(uint64_t)blockIdx.x * p.k + at] = key;
                 else {
                     p.top_ids[(uint64_t)row * p.k + at] = index_of(key);
-                    p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(key), c);
+                    p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(key), p.scale);
                 }
             }
         }
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const LogpP p) {
         if (p.entropy) p.entropy[row] = r.entropy;
         if (p.logprob) {
             const uint32_t tok = p.tokens[sg_row_offset(p.token_rows, row)];
-            p.logprob[row] = tok < p.C ? r.logprob(x[tok], c) : 0.0f;
+            p.logprob[row] = tok < p.C ? r.logprob(x[tok], p.scale) : 0.0f;
         }
     }
     if (p.k == 0) return;
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_join_kernel(const LogpP p) {
         const uint32_t at = place_of(keys, count, keys[i]);
         if (at >= p.k) continue;
         p.top_ids[(uint64_t)row * p.k + at] = index_of(keys[i]);
-        p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(keys[i]), c);
+        p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(keys[i]), p.scale);
     }
 }
 

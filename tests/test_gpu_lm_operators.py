@@ -933,3 +933,32 @@ def test_token_logprobs_gradient_of_tokens_hidden_by_the_lowest_value(ctx, c, sc
             hit = hidden.copy()
             hit[1, 3] = False
             assert not g[hit].any()
+
+
+@pytest.mark.parametrize("c", [40, 20000])
+@pytest.mark.parametrize("scale", [0.5, 1.0, 1.4])
+def test_token_logprobs_of_hidden_tokens_are_as_low_as_their_logits(ctx, c, scale):
+    """Logits near the type's lowest value beside ordinary ones: their log probabilities are finite where the number is (three
+    roundings: the distance, its scaling, the sum), as given tokens and among the alternatives."""
+    say("low", c, scale)
+    rng = np.random.default_rng(c)
+    x = R.f32(rng.standard_normal((6, c)) * 2)
+    x[4:] += 500.0
+    low = np.array([np.finfo(np.float32).min, -2.5e38, -1e38], np.float32)
+    hidden = np.ones((6, c), bool)
+    hidden[:, 5:9] = False
+    clean = np.where(hidden, np.float32(-np.inf), x)
+    x[hidden] = low[rng.integers(0, 3, hidden.sum())]
+    tokens = np.array([0, 6, c - 1, 30, 12, 7], np.int32)
+    want, t_lp = R.logprobs(clean, None, scale), R.logprobs_tol(clean, scale)[0]
+    lp = x.astype(np.float64) * float(np.float32(scale)) - want["lse"][:, None]
+    lp[np.abs(lp) > np.finfo(np.float32).max * (1 + R.U)] = -np.inf
+    tol = t_lp[:, None] + 4 * R.U * np.where(np.isfinite(lp), np.abs(lp), 0.0)
+    got = run_logprobs(ctx, x, tokens, scale, 16)
+    at = np.arange(6)
+    near(got["logprob"], lp[at, tokens], tol[at, tokens], "logprob")
+    order = np.argsort(-x.astype(np.float64), axis=1, kind="stable")[:, :16]
+    assert np.array_equal(got["top_ids"], order)
+    near(got["top_logprobs"], np.take_along_axis(lp, order, 1), np.take_along_axis(tol, order, 1), "alternatives")
+    near(got["lse"], want["lse"], t_lp + 2 * R.U * np.abs(want["lse"]), "lse")
+    near(got["entropy"], want["entropy"], R.logprobs_tol(clean, scale)[1], "entropy")
