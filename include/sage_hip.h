@@ -380,7 +380,7 @@ int sg_softmax_cross_entropy(sg_ctx *ctx, const sg_tensor *logits, const sg_tens
 int sg_layer_norm_lastaxis(sg_ctx *ctx, const sg_tensor *x, const sg_tensor *gamma,
                            const sg_tensor *beta, float eps, const sg_tensor *out);
 
-/* Log probabilities of given tokens under z = scale * logits (scale > 0: one over a temperature), with
+/* Log probabilities of given tokens under z = scale * logits (0 < scale <= 2^127: one over a temperature), with
  * lse = log sum_j e^(z_j): logprob = z_token - lse, entropy = lse - sum_j p_j z_j, and the k largest logits' indexes with
  * their log probabilities, largest first, equal ones by index.  Beside sg_softmax_cross_entropy, whose loss is -logprob.
  * logits [.., C], unit stride on C; tokens, logprob, entropy, lse: the leading extents (a rank-1 logits: one element),

@@ -490,7 +490,8 @@ int check_logits(sg_ctx *ctx, const sg_tensor *logits, float scale, const char *
     if ((rc = sg_check_f32(ctx, logits, who)) != SG_OK) return rc;
     if (logits->extents[logits->rank - 1] > 1 && logits->strides[logits->rank - 1] != 1)
         return sg_fail(ctx, SG_ERR_SHAPE, "%s: the last axis must have unit stride", who);
-    if (!(scale > 0.0f) || scale > 3.4028234e38f) return sg_fail(ctx, SG_ERR_ARG, "%s: scale must be positive and finite", who);
+    // the kernels' scale log2(e) is finite up to here
+    if (!(scale > 0.0f && scale <= 0x1p127f)) return sg_fail(ctx, SG_ERR_ARG, "%s: scale must be positive and at most 2^127", who);
     return SG_OK;
 }
 

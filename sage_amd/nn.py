@@ -134,8 +134,8 @@ def token_logprobs(logits, tokens=None, top=0, scale=1.0):
             raise abi.ShapeError(abi.ERR_SHAPE, f"token_logprobs: tokens {tokens.extents} for logits {logits.extents}")
         ins.append(tokens)
     scale = float(np.float32(scale))
-    if not 0.0 < scale < float("inf"):
-        raise abi.SageError(abi.ERR_ARG, "token_logprobs: scale must be positive and finite")
+    if not 0.0 < scale <= 2.0 ** 127:
+        raise abi.SageError(abi.ERR_ARG, "token_logprobs: scale must be positive and at most 2^127")
     if not 0 <= top <= min(abi.MAX_TOP, logits.extents[-1]):
         raise abi.ShapeError(abi.ERR_SHAPE, f"token_logprobs: {top} alternatives of {logits.extents[-1]} (at most {abi.MAX_TOP})")
     lse = Var(Shape(lead), FLOAT, "token_lse", ins, {"scale": scale, "top": int(top)})

@@ -360,3 +360,13 @@ def test_merged_heads_inside_a_step_take_no_copy():
     merged = [x.transpose(2, 1).view([2, -1, x.extents[1] * 32]) for x in (y, gq, gk, gv)]
     outs, maps = evaluated(merged)
     assert maps == 0 and len({id(t.buf) for t in outs}) == 4
+
+
+def test_token_logprobs_refuse_a_scale_whose_logarithm_to_base_2_overflows():
+    """scale * log2(e) is what the kernels multiply by: beyond 2^127 it may be infinite, and 0 times it NaN."""
+    for scale in (2.0 ** 127 * (1 + 2.0 ** -23), 3.4e38):
+        assert lp(scale=scale) == lp_grad(scale=scale) == abi.ERR_ARG
+        with pytest.raises(abi.SageError):
+            nn.token_logprobs(Var.empty([2, 3, 50]), scale=scale)
+    assert lp(scale=2.0 ** 127) == lp_grad(scale=2.0 ** 127) == OK_BUT_NO_CONTEXT
+    assert np.isfinite(np.float32(2.0 ** 127) * np.float32(1.44269504088896340736))
