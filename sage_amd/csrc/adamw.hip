@@ -7,9 +7,11 @@
 // 8-bit states.  256 elements share a power of two, so scaling is an addition to exponent fields and exact, and a byte is
 // the top of a number's fp32 pattern: no division, no table.  v is never negative and gets the sign's bit for a fifth
 // exponent bit: it is a square, and 32 octaves of v are the 16 octaves of g that the 4 exponent bits of m cover.
-// Bytes keep 3 mantissa bits (steps of 6 to 12 %), while a step moves v by 1 - beta2 = 0.1 %: rounded to nearest it would
-// stay where it is for good.  So 16 bits of noise, a hash of element, step and seed, are added below the kept bits before
-// the rest is cut off, which rounds up or down with the chances that keep the mean.
+// Bytes keep 3 mantissa bits (steps of 6 to 12 %), while a step moves v by 1 - beta2 = 0.1 % of what g g is off from it: rounded
+// to nearest it would stay where it is for good, unless g g is dozens of times v.  So 16 bits of noise, a hash of element, step
+// and seed, are added below the kept bits before the rest is cut off, which rounds up or down with the chances that keep the
+// mean.  That holds from the smallest code on: a smaller m is on its way to zero, a smaller v is held at that code (zero would
+// make the element's steps as large as eps lets them be).
 // The moments are formed without contraction (this file is compiled with -ffp-contract=off): which byte a moment becomes
 // hangs on its last bit.
 #include "rows.h"

@@ -228,7 +228,8 @@ class AdamW(Optimizer):
         value -= lr ((m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay value)
     with both moments zero in front of the first update and t = 1 in it.  state_bits=8 keeps each moment in a byte (blocks of 256
     elements share a power of two, rounding up or down by a hash of element, step and `seed`): 2 bytes a parameter
-    instead of 8.  Parameters and gradients are fp32."""
+    instead of 8.  The mean is kept down to about 2^-15 (m) and 2^-31 (v) of a block's largest; what is smaller becomes zero (m) or is
+    held there (v), so such elements take smaller steps.  Parameters and gradients are fp32."""
 
     def __init__(self, lr, beta1=0.9, beta2=0.999, eps=1e-08, weight_decay=0.01, state_bits=32, seed=0):
         if state_bits not in (8, 32):

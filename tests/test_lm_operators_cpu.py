@@ -370,3 +370,24 @@ def test_token_logprobs_refuse_a_scale_whose_logarithm_to_base_2_overflows():
             nn.token_logprobs(Var.empty([2, 3, 50]), scale=scale)
     assert lp(scale=2.0 ** 127) == lp_grad(scale=2.0 ** 127) == OK_BUT_NO_CONTEXT
     assert np.isfinite(np.float32(2.0 ** 127) * np.float32(1.44269504088896340736))
+
+
+@pytest.mark.parametrize("signed,bottom", [(True, -15), (False, -31)])
+def test_eight_bit_states_at_the_bottom_of_a_block(signed, bottom):
+    """Beside a largest of 1, whose power of two is 1: the mean is kept from 1.125 * 2^bottom on; below, a first moment loses it
+    and becomes zero under 2^bottom, a second moment is held at 1.125 * 2^bottom."""
+    lowest = 1.125 * 2.0 ** bottom
+    x = R.f32([1.0] + [lowest * f for f in (1.0, 1.05, 1.3, 1.77, 3.1, 7.7)] + [2.0 ** bottom * f for f in (1.06, 1.0, 0.999, 0.5, 0.25, 2.0 ** -20)])
+    assert np.all(x > 0)
+    n = 999
+    draws = np.array([R.decode(*R.encode(x, signed, R.noise(x.size, t, 3)[0 if signed else 1]), signed) for t in range(1, n + 1)])
+    # a draw is off by at most a step of 1/8 with variance at most its square / 4: the mean by 6 deviations
+    assert np.all(np.abs(draws.mean(0) - x)[:7] <= 6 * 2.0 ** -4 / np.sqrt(n) * x[:7])
+    if signed:
+        # 1.06 is 0.06 / 0.125 of the way from 2^bottom, which is no number of the block, to the smallest: else 0
+        part = 0.06 / 0.125
+        assert set(np.unique(draws[:, 7])) == {np.float32(0), np.float32(lowest)}
+        assert abs((draws[:, 7] > 0).mean() - part) <= 6 * 0.5 / np.sqrt(n)
+        assert not draws[:, 8:].any()
+    else:
+        assert np.all(draws[:, 7:] == np.float32(lowest))
