@@ -215,7 +215,8 @@ template <bool TOP>
 __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
     __shared__ typename std::conditional<TOP, TopLds, uint32_t>::type lds_top;
     __shared__ float lds_stats[12];
-    const uint32_t row = blockIdx.x / p.splits, split = blockIdx.x - row * p.splits, tid = threadIdx.x;
+    const uint32_t block = sg_workgroup(), row = block / p.splits, split = block - row * p.splits, tid = threadIdx.x;
+    if (row >= p.R) return;
     const float *x = p.logits + sg_row_offset(p.rows, row);
     // 16-byte groups at whatever element the row starts; the C % 4 logits behind them are a round of their own
     const uint32_t groups = p.C / 4;
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
     const RowResult r(all, p.scale);
     if (tid == 0) {
         if (p.splits > 1) {
-            float *to = p.part_stats + (uint64_t)blockIdx.x * 3;
+            float *to = p.part_stats + (uint64_t)block * 3;
             to[0] = all.m; to[1] = all.s; to[2] = all.t;
         } else {
             p.lse[row] = r.lse;
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
             uint32_t at = 0;
             for (int w = 0; w < THREADS / 64; ++w) at += place_of(lds_top.list[w], lds_top.count[w], key);
             if (at < p.k) {
-                if (p.splits > 1) p.part_keys[(uint64_t)blockIdx.x * p.k + at] = key;
+                if (p.splits > 1) p.part_keys[(uint64_t)block * p.k + at] = key;
                 else {
                     p.top_ids[(uint64_t)row * p.k + at] = index_of(key);
                     p.top_logprobs[(uint64_t)row * p.k + at] = r.logprob(value_of(key), p.scale);
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_kernel(const LogpP p) {
         if (p.splits > 1) {
             uint32_t all_n = 0;
             for (int w = 0; w < THREADS / 64; ++w) all_n += lds_top.count[w];
-            for (uint32_t i = all_n + tid; i < p.k; i += THREADS) p.part_keys[(uint64_t)blockIdx.x * p.k + i] = 0;
+            for (uint32_t i = all_n + tid; i < p.k; i += THREADS) p.part_keys[(uint64_t)block * p.k + i] = 0;
         }
     }
 }
@@ -416,7 +417,9 @@ template <bool NT>
 __global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const LogpGradP p) {
     __shared__ float lds_stats[12];
     // from the last row to the first: the forward call's last rows are still in the last-level cache
-    const uint32_t block = gridDim.x - 1 - blockIdx.x, row = block / p.parts, part = block - row * p.parts, tid = threadIdx.x;
+    const uint32_t blocks = p.R * p.parts, from_end = sg_workgroup(), tid = threadIdx.x;
+    if (from_end >= blocks) return;
+    const uint32_t block = blocks - 1 - from_end, row = block / p.parts, part = block - row * p.parts;
     const float *x = p.logits + sg_row_offset(p.rows, row);
     float *y = p.glogits + (uint64_t)row * p.C;
     const float inf = __builtin_inff(), c = p.scale * LOG2E;
@@ -553,7 +556,6 @@ extern "C" int sg_token_logprobs(sg_ctx *ctx, const sg_tensor *logits, const sg_
     if (p.splits > 64) p.splits = 64;
     if (k && p.splits > JOIN / (uint32_t)k) p.splits = JOIN / (uint32_t)k;
     if (p.splits < 1) p.splits = 1;
-    if ((uint64_t)p.R * p.splits >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs: too many rows for one launch");
     sg_device_guard guard(ctx);
     sg_workspace space(ctx);
     if (p.splits > 1) {
@@ -562,8 +564,8 @@ extern "C" int sg_token_logprobs(sg_ctx *ctx, const sg_tensor *logits, const sg_
         p.part_keys = (unsigned long long *)space.p;
         p.part_stats = (float *)(p.part_keys + parts * k);
     }
-    if (k) hipLaunchKernelGGL((logprobs_kernel<true>), dim3(p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((logprobs_kernel<false>), dim3(p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
+    if (k) hipLaunchKernelGGL((logprobs_kernel<true>), sg_grid((uint64_t)p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((logprobs_kernel<false>), sg_grid((uint64_t)p.R * p.splits), dim3(THREADS), 0, ctx->stream, p);
     SG_CHECK_LAUNCH(ctx, "token_logprobs");
     if (p.splits > 1) {
         hipLaunchKernelGGL(logprobs_join_kernel, dim3(p.R), dim3(THREADS), 0, ctx->stream, p);
@@ -618,9 +620,8 @@ extern "C" int sg_token_logprobs_grad(sg_ctx *ctx, const sg_tensor *logits, cons
     // (in place: one workgroup a row, which has read the row when it first writes, if it reads the whole row at all)
     if (p.glogits == p.logits) p.part = p.C / 4 + 2;
     p.parts = (p.C + 3 + 4 * p.part - 1) / (4 * p.part);
-    if ((uint64_t)p.R * p.parts >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_token_logprobs_grad: too many elements for one launch");
     sg_device_guard guard(ctx);
-    const dim3 grid(p.R * p.parts);
+    const dim3 grid = sg_grid((uint64_t)p.R * p.parts);
     if (sg_streaming((int64_t)p.R * p.C * 8)) hipLaunchKernelGGL((logprobs_grad_kernel<true>), grid, dim3(THREADS), 0, ctx->stream, p);
     else hipLaunchKernelGGL((logprobs_grad_kernel<false>), grid, dim3(THREADS), 0, ctx->stream, p);
     SG_CHECK_LAUNCH(ctx, "token_logprobs_grad");

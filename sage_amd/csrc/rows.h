@@ -46,6 +46,15 @@ __device__ __forceinline__ int64_t sg_row_offset(const sg_rows &r, uint32_t i) {
     return off + (int64_t)i * r.st[0];
 }
 
+// A launch has fewer than 2^32 threads in a dimension.  Grids of more workgroups (of at most 1024 threads) go on in y, and their
+// last ones may lie behind the end.
+constexpr uint32_t SG_GRID_X = 1u << 21;
+static inline dim3 sg_grid(uint64_t workgroups) {
+    if (workgroups <= SG_GRID_X) return dim3((unsigned)workgroups);
+    return dim3(SG_GRID_X, (unsigned)((workgroups + SG_GRID_X - 1) / SG_GRID_X));
+}
+__device__ __forceinline__ uint32_t sg_workgroup() { return blockIdx.y * SG_GRID_X + blockIdx.x; }
+
 // Launches go to the device of the context, whichever is current in the calling thread.
 struct sg_device_guard {
     int back = -1;

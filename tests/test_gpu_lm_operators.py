@@ -962,3 +962,28 @@ def test_token_logprobs_of_hidden_tokens_are_as_low_as_their_logits(ctx, c, scal
     near(got["top_logprobs"], np.take_along_axis(lp, order, 1), np.take_along_axis(tol, order, 1), "alternatives")
     near(got["lse"], want["lse"], t_lp + 2 * R.U * np.abs(want["lse"]), "lse")
     near(got["entropy"], want["entropy"], R.logprobs_tol(clean, scale)[1], "entropy")
+
+
+def test_token_logprobs_of_more_rows_than_a_launch_has_in_x(ctx):
+    """2^24 + 77 rows of 6 logits, each one logit behind the one above: a workgroup a row is more than 2^32 threads."""
+    rows, c, top = (1 << 24) + 77, 6, 2
+    rng = np.random.default_rng(51)
+    base = R.f32(rng.standard_normal(rows + c - 1))
+    tokens = rng.integers(-1, c, rows).astype(np.int32)
+    x = Tensor(dev(ctx, base).buf, FLOAT, Shape([rows, c], [1, 1], 0))
+    got = run_logprobs(ctx, x, tokens, 1.0, top)
+    gl = R.f32(rng.standard_normal(rows))
+    _, tok, outs = got["dev"]
+    out = Tensor.uninit(ctx, [rows, c])
+    ctx.check(ctx._lib.sg_token_logprobs_grad(ctx.handle, ref(x), ref(tok), C.c_float(1.0), ref(outs["lse"]), None, ref(dev(ctx, gl)), None, ref(out)))
+    g = out.numpy()
+    for k in ("logprob", "entropy", "lse"):
+        assert np.isfinite(got[k]).all(), k
+    at = np.concatenate([np.arange(2000), np.arange((1 << 21) - 500, (1 << 21) + 500), np.arange(rows - 3000, rows), rng.integers(0, rows, 50000)])
+    part = base[at[:, None] + np.arange(c)]
+    want = R.logprobs(part, tokens[at], 1.0, top)
+    t_lp, t_h = R.logprobs_tol(part, 1.0)
+    near(got["logprob"][at], want["logprob"], t_lp, "logprob")
+    near(got["entropy"][at], want["entropy"], t_h, "entropy")
+    assert np.array_equal(got["top_ids"][at], want["top_ids"])
+    near(g[at], R.logprobs_grad(want, 1.0, gl[at]), R.logprobs_grad_tol(want, part, 1.0, gl[at]), "glogits")
