@@ -54,7 +54,7 @@ struct EmbP {
 // 4096 tokens 6.4 us (25 MB, 3.9 TB/s); 32768 tokens, three tenths of them none, 20 us (101 MB written past the caches, 5 TB/s).
 template <bool NARROW, bool NT>
 __global__ void __launch_bounds__(256) embedding_kernel(const EmbP p) {
-    const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint64_t unit = (uint64_t)sg_workgroup() * 4 + (threadIdx.x >> 6);
     if (unit >= (uint64_t)p.n * p.pieces) return;
     const uint32_t token = (uint32_t)(unit / p.pieces), piece = (uint32_t)(unit - (uint64_t)token * p.pieces);
     const uint32_t lane = threadIdx.x & 63;
@@ -343,7 +343,9 @@ __global__ void __launch_bounds__(FEW_THREADS) embedding_few_kernel(const FewP p
     __shared__ __attribute__((aligned(16))) uint32_t row_of[FEW];  // of each token, ~0: not here
     __shared__ uint32_t firsts[FEW], distinct;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t v0 = blockIdx.x * p.rows, rows = min(p.rows, p.V - v0);
+    const uint32_t v0 = sg_workgroup() * p.rows;
+    if (v0 >= p.V) return;
+    const uint32_t rows = min(p.rows, p.V - v0);
     const uint32_t id = tid < p.n ? p.ids[sg_row_offset(p.id_rows, tid)] : ~0u;
     float *table = p.gtable + (uint64_t)v0 * p.E;
     const uint64_t total = (uint64_t)rows * p.E;
@@ -436,10 +438,11 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const SumP p) {
 template <bool NARROW>
 __global__ void __launch_bounds__(256) embedding_join_kernel(const SumP p) {
     __shared__ f32x4 sums[4][64];
-    const uint32_t chunk = blockIdx.x / p.pieces, piece = blockIdx.x - chunk * p.pieces;
+    const uint32_t block = sg_workgroup(), chunk = block / p.pieces, piece = block - chunk * p.pieces;
+    if (chunk + 1 >= p.chunks) return;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t c = piece * 256 + lane * 4;
-    const uint32_t behind = (chunk + 1) * p.chunk;  // this kernel has a workgroup for every chunk but the last
+    const uint32_t behind = (chunk + 1) * p.chunk;  // there is no work for the last chunk
     const uint32_t id = p.key[behind];
     if (id >= p.V || p.key[behind - 1] != id) return;                            // nothing goes on
     if (chunk > 0 && p.key[chunk * p.chunk - 1] == id) return;                   // it began further in front
@@ -506,7 +509,7 @@ extern "C" int sg_embedding(sg_ctx *ctx, const sg_tensor *table, const sg_tensor
     const bool nt = sg_streaming((int64_t)p.n * E * 4);
     const uint64_t units = (uint64_t)p.n * p.pieces;
     sg_device_guard guard(ctx);
-    const dim3 grid((unsigned)((units + 3) / 4));
+    const dim3 grid = sg_grid((units + 3) / 4);
     if (E < 4) hipLaunchKernelGGL((embedding_kernel<true, false>), grid, dim3(256), 0, ctx->stream, p);
     else if (nt) hipLaunchKernelGGL((embedding_kernel<false, true>), grid, dim3(256), 0, ctx->stream, p);
     else hipLaunchKernelGGL((embedding_kernel<false, false>), grid, dim3(256), 0, ctx->stream, p);
@@ -559,7 +562,7 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
         f.rows = rows < 4 ? 4 : rows / 4 * 4;
         f.fill_vec = aligned16(table);
         sg_device_guard guard(ctx);
-        const dim3 grid((s.V + f.rows - 1) / f.rows);
+        const dim3 grid = sg_grid((s.V + f.rows - 1) / f.rows);
         if (E < 4) hipLaunchKernelGGL((embedding_few_kernel<true>), grid, dim3(FEW_THREADS), 0, ctx->stream, f);
         else hipLaunchKernelGGL((embedding_few_kernel<false>), grid, dim3(FEW_THREADS), 0, ctx->stream, f);
         SG_CHECK_LAUNCH(ctx, "embedding_grad");
@@ -570,7 +573,6 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
     // all tokens leaves few partial sums.
     m.chunk = s.n <= 16384 ? 8 : s.n <= 65536 ? 16 : s.n <= 262144 ? 32 : 64;
     m.chunks = (s.n + m.chunk - 1) / m.chunk;
-    if ((uint64_t)m.chunks * m.pieces >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "sg_embedding_grad: too many elements for one launch");
 
     uint32_t bits = 1;
     while ((s.V >> bits) != 0) ++bits;  // keys are 0..V
@@ -648,7 +650,7 @@ extern "C" int sg_embedding_grad(sg_ctx *ctx, const sg_tensor *gout, const sg_te
         m.pos = s.pos_out;
     }
     const bool narrow = E < 4, nt = sg_streaming((int64_t)m.n * E * 4);
-    const dim3 sum_grid((m.chunks * m.pieces + 3) / 4), join_grid((m.chunks - 1) * m.pieces);
+    const dim3 sum_grid((m.chunks * m.pieces + 3) / 4), join_grid = sg_grid((uint64_t)(m.chunks - 1) * m.pieces);
     if (narrow) hipLaunchKernelGGL((embedding_sum_kernel<true, false, 4>), sum_grid, dim3(256), 0, ctx->stream, m);
     else if (nt) hipLaunchKernelGGL((embedding_sum_kernel<false, true, 16>), sum_grid, dim3(256), 0, ctx->stream, m);
     else hipLaunchKernelGGL((embedding_sum_kernel<false, false, 16>), sum_grid, dim3(256), 0, ctx->stream, m);

@@ -987,3 +987,28 @@ def test_token_logprobs_of_more_rows_than_a_launch_has_in_x(ctx):
     near(got["entropy"][at], want["entropy"], t_h, "entropy")
     assert np.array_equal(got["top_ids"][at], want["top_ids"])
     near(g[at], R.logprobs_grad(want, 1.0, gl[at]), R.logprobs_grad_tol(want, part, 1.0, gl[at]), "glogits")
+
+
+def test_embedding_of_more_tokens_and_rows_than_a_launch_has_in_x(ctx):
+    """2^26 tokens of one value (ids of each sequence one behind those above), and the gradient of a few tokens in a table of
+    2^28 rows: more than 2^32 threads either way."""
+    rng = np.random.default_rng(52)
+    n, l, v = 8193, 8192, 1000
+    base, table = rng.integers(0, v + 1, n + l - 1).astype(np.uint32), R.f32(rng.standard_normal((v, 1)))
+    ids = Tensor(dev(ctx, base).buf, UINT, Shape([n, l], [1, 1], 0))
+    out = dev(ctx, np.full((n, l, 1), np.nan, np.float32))
+    ctx.check(ctx._lib.sg_embedding(ctx.handle, ref(dev(ctx, table)), ref(ids), C.c_float(0.3), ref(out)))
+    got, once = out.numpy(), R.embedding(table, base, 0.3)[:, 0]
+    assert same_bits(got, np.lib.stride_tricks.sliding_window_view(once, l)[..., None])
+    del out
+    v = (1 << 28) + 100
+    at = np.array([3, v - 1, 1 << 26, 3, v - 1, 0xFFFFFFFF, (1 << 28) - 1], np.uint32)
+    g = R.f32(rng.standard_normal((at.size, 1)))
+    out = Tensor.uninit(ctx, [v, 1])
+    ctx.check(ctx._lib.sg_embedding_grad(ctx.handle, ref(dev(ctx, g)), ref(dev(ctx, at)), C.c_float(1.5), ref(out)))
+    got = out.numpy()[:, 0]
+    for row in set(at.tolist()) - {0xFFFFFFFF}:
+        mine = g[at == row, 0].astype(np.float64)
+        near(got[row], mine.sum() * 1.5, (mine.size + 2) * R.U * np.abs(mine).sum() * 1.5, f"row {row}")
+        got[row] = 0.0
+    assert not got.any()
