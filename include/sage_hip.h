@@ -419,7 +419,8 @@ int sg_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_t
 
 /* out = softmax(scale * (q . k^T)) . v over the visible keys, the shape of MultiHeadAttention::pass (bert.rs:262-271) with
  * keys and values of an encoder: q, out [N, H, Lq, D]; k, v [N, G, Lk, D], G a divisor of H, query head h reading key head
- * h / (H/G); unit stride on D, any strides elsewhere (separate_heads views, merged-heads outputs); D = 32 or 64.
+ * h / (H/G); unit stride on D, any strides elsewhere (separate_heads views, merged-heads outputs); D = 32 or 64; N G at most
+ * 2^24 - 8.
  * mask: NULL or fp32 [N, Lk], unit stride on Lk, any batch stride: key j of sequence b is visible unless mask[b, j] is 0.
  * What a hidden key's k and v hold is not used, NaN or not.  A query without a visible key gives zeros and lse = -inf.
  * The softmax shift follows the row's largest visible score, whatever its size.  lse: NULL or dense [N, H, Lq], log of the

@@ -939,6 +939,9 @@ int check_call(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_ten
     const int64_t N = q->extents[0], H = q->extents[1], Lq = q->extents[2], D = q->extents[3], G = k->extents[1], Lk = k->extents[2];
     if (D != 32 && D != 64) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: head size %lld (32 and 64 are built)", (long long)D);
     if (H % G != 0) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: %lld query heads over %lld key heads", (long long)H, (long long)G);
+    // A launch has fewer than 2^32 threads, in workgroups of 256, rounded up to the 8 XCDs.  (More than one tile of rows or keys a
+    // pair leaves room: 2^31 elements are the most of an operand.)
+    if (N * G > (1 << 24) - 8) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: %lld sequences of %lld key heads (2^24 - 8 together at most)", (long long)N, (long long)G);
     if ((rc = check_operand(ctx, q, N, H, Lq, D, "cross attention q", &p.q)) != SG_OK) return rc;
     if ((rc = check_operand(ctx, k, N, G, Lk, D, "cross attention k", &p.k)) != SG_OK) return rc;
     if ((rc = check_operand(ctx, v, N, G, Lk, D, "cross attention v", &p.v)) != SG_OK) return rc;
@@ -1001,13 +1004,11 @@ Plan plan(const sg_ctx *ctx, const CrossP &p, int64_t D, int own, int other, int
     return best;
 }
 
-int set_tiles(sg_ctx *ctx, CrossP &p, uint64_t tiles, uint32_t splits) {
-    p.tiles = (uint32_t)tiles;
+void set_tiles(CrossP &p, uint32_t tiles, uint32_t splits) {
+    p.tiles = tiles;
     p.splits = splits;
     p.spread = (uint64_t)p.pairs * splits < 64;  // an XCD would have fewer than 8 units, of different lengths
-    if (tiles * p.pairs * splits >= (1ull << 31)) return sg_fail(ctx, SG_ERR_SHAPE, "cross attention: too many rows for one launch");
     p.d_tiles = sg_make_fastdiv(p.tiles);
-    return SG_OK;
 }
 
 // Lengths in front of the launches, where there are more workgroups than `each` for a compute unit and lengths to order them by.
@@ -1056,7 +1057,7 @@ extern "C" int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tens
     }
     const int rw = how.waves;
     const uint32_t tiles = few ? 1 : (uint32_t)((p.R + 32 * rw - 1) / (32 * rw));
-    if ((rc = set_tiles(ctx, p, tiles, how.splits)) != SG_OK) return rc;
+    set_tiles(p, tiles, how.splits);
     sg_workspace space(ctx);
     if (p.splits > 1) {
         if ((rc = space.take((uint64_t)p.splits * total * (D + 2) * 4)) != SG_OK) return rc;
@@ -1144,8 +1145,8 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
         else hipLaunchKernelGGL((cross_front_kernel<32>), front, dim3(256), 0, ctx->stream, p, ends);
         SG_CHECK_LAUNCH(ctx, "cross_attention_grad delta");
         CrossP rows = p;
-        if ((rc = set_tiles(ctx, rows, row_tiles, row_splits)) != SG_OK) return rc;
-        if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
+        set_tiles(rows, row_tiles, row_splits);
+        set_tiles(p, key_tiles, key_splits);
         const uint32_t key_ids = (p.tiles * p.pairs * p.splits + 7) / 8 * 8;
         const dim3 grid(key_ids + rows.tiles * rows.pairs * rows.splits);
         if (D == 64 && dma) hipLaunchKernelGGL((cross_both_kernel<64, true>), grid, dim3(256), 0, ctx->stream, p, rows, key_ids);
@@ -1159,10 +1160,10 @@ extern "C" int sg_cross_attention_grad(sg_ctx *ctx, const sg_tensor *q, const sg
             hipLaunchKernelGGL(cross_ends_kernel, dim3((unsigned)p.N), dim3(256), 0, ctx->stream, p);
             SG_CHECK_LAUNCH(ctx, "cross_attention_grad lengths");
         }
-        if ((rc = set_tiles(ctx, p, row_tiles, row_splits)) != SG_OK) return rc;
+        set_tiles(p, row_tiles, row_splits);
         SG_CROSS_ROWS(cross_gq_kernel, rw, dma, dim3(p.tiles * p.pairs * p.splits));
         SG_CHECK_LAUNCH(ctx, "cross_attention_grad queries");
-        if ((rc = set_tiles(ctx, p, key_tiles, key_splits)) != SG_OK) return rc;
+        set_tiles(p, key_tiles, key_splits);
         uint32_t workgroups = p.tiles * p.pairs * p.splits;
         if (p.ends) workgroups = (workgroups + 7) / 8 * 8;
         const dim3 grid(workgroups);

@@ -391,3 +391,13 @@ def test_eight_bit_states_at_the_bottom_of_a_block(signed, bottom):
         assert not draws[:, 8:].any()
     else:
         assert np.all(draws[:, 7:] == np.float32(lowest))
+
+
+def test_cross_attention_refuses_more_pairs_than_a_launch_has_workgroups():
+    """2^24 workgroups of 256 threads are more than a launch takes; refused in front of the context, like any argument."""
+    def both(n, heads):
+        q, k, m, lse = [n, heads, 1, 32], [n, heads, 2, 32], [n, 2], [n, heads, 1]
+        return (call("sg_cross_attention", desc(q), desc(k), desc(k), desc(m), C.c_float(1.0), desc(q), desc(lse)),
+                call("sg_cross_attention_grad", desc(q), desc(k), desc(k), desc(m), C.c_float(1.0), desc(q), desc(lse), desc(q), desc(q), desc(k), desc(k)))
+    assert both(1 << 24, 1) == both(1 << 12, 1 << 12) == both((1 << 24) - 7, 1) == (abi.ERR_SHAPE, abi.ERR_SHAPE)
+    assert both((1 << 24) - 8, 1) == (OK_BUT_NO_CONTEXT, OK_BUT_NO_CONTEXT)
