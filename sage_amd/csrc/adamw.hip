@@ -297,7 +297,7 @@ int fill_table(Table<POINTERS> &t, uint32_t *chunks, int first, int n_tensors, c
     for (; i < n_tensors && count < Table<POINTERS>::MAX; ++i) {
         const int64_t n = sg_numel(&arrays[VALUE][i]);
         const uint64_t need = ((uint64_t)n + chunk - 1) / chunk;
-        if (at + need >= (1ull << 31)) break;  // the rest in a launch of its own
+        if (at + need >= (1ull << 24)) break;  // a launch has fewer than 2^32 threads: the rest in one of its own
         for (int k = 0; k < POINTERS; ++k) t.p[count][k] = f32_ptr(&arrays[k][i]);
         t.n[count] = (uint32_t)n;
         t.first_chunk[count++] = (uint32_t)at;
