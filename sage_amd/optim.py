@@ -17,6 +17,7 @@ Reference behaviour that is kept because results would differ otherwise:
 * `Sgd` with momentum != 0 indexes a missing entry on first use (optim.rs:67-69: the `contains_key`
   test is inverted) and panics; here that is a KeyError.  Plain SGD (momentum 0) works.
 """
+import bisect
 import ctypes as C
 
 from .shape import Shape
@@ -255,17 +256,38 @@ class AdamW(Optimizer):
             self.states[param] = tuple(Tensor.from_numpy(ctx, z) for z in zeros)
         return self.states[param]
 
+    def _gradients(self, grads, ctx):
+        """The gradients' tensors, and which of them have to be copied first: those that are not dense, and those that lie in a
+        parameter's memory, which is rewritten while they are read.  Two parameters in one memory are refused."""
+        from . import abi
+
+        def span(t):
+            start = t.buf.ptr + t.offset * 4
+            return start, start + t.size() * 4
+        values = [_value(g, ctx) for g in grads.values()]
+        for param in grads:
+            if not param.is_data():
+                raise TypeError("param is not data tensor")
+            if not param.value.is_dense():
+                param.set(_dense(param.value, ctx))
+        spans = sorted(span(param.value) for param in grads)
+        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+            raise abi.SageError(abi.ERR_ARG, "AdamW: two parameters share memory")
+        starts = [a for a, _ in spans]
+
+        def apart(t):
+            first, last = span(t)
+            i = bisect.bisect_left(starts, last)  # the spans in front of it begin before t ends
+            return i == 0 or spans[i - 1][1] <= first
+        return values, [not (t.is_dense() and apart(t)) for t in values]
+
     def _call(self, grads, grad_tensors, ctx):
         """The arguments of sg_adamw_update behind the context, and what has to live as long as they are used."""
         from . import abi
         cols = [[] for _ in range(2 + (2 if self.state_bits == 32 else 4))]
         for param, g in zip(grads, grad_tensors):
-            if not param.is_data():
-                raise TypeError("param is not data tensor")
             if g.extents != param.extents:
                 raise abi.ShapeError(abi.ERR_SHAPE, f"AdamW: gradient {g.extents} for a parameter {param.extents}")
-            if not param.value.is_dense():
-                param.set(_dense(param.value, ctx))
             for col, x in zip(cols, (param.value, g) + self._state(param, ctx)):
                 col.append(x)
         n = len(grads)
@@ -278,7 +300,8 @@ class AdamW(Optimizer):
     def update(self, grads, ctx):
         if self.t is None:
             self.init(ctx)
-        args, _ = self._call(grads, [_dense(_value(g, ctx), ctx) for g in grads.values()], ctx)
+        values, copied = self._gradients(grads, ctx)
+        args, _ = self._call(grads, [Var.new(t).copy().eval(ctx) if c else t for t, c in zip(values, copied)], ctx)
         ctx.launches += 1
         ctx.check(ctx._lib.sg_adamw_update(ctx.handle, *args))
         params_changed()
@@ -290,11 +313,10 @@ class AdamW(Optimizer):
         from .var import Program
         if self.t is None:
             self.init(ctx)
-        values = [_value(g, ctx) for g in grads.values()]
-        strided = [Var.new(t).copy() for t in values if not t.is_dense()]
-        prog = Program(ctx, strided)  # their copies, made again on every run
+        values, copied = self._gradients(grads, ctx)
+        prog = Program(ctx, [Var.new(t).copy() for t, c in zip(values, copied) if c])  # made again on every run
         copies = iter(prog.outputs)
-        args, keep = self._call(grads, [t if t.is_dense() else next(copies) for t in values], ctx)
+        args, keep = self._call(grads, [next(copies) if c else t for t, c in zip(values, copied)], ctx)
         lib = ctx._lib
         ctx.check(lib.sg_adamw_update(ctx.handle, *args))
         prog.calls.append((lib.sg_adamw_update, args, keep))

@@ -1012,3 +1012,42 @@ def test_embedding_of_more_tokens_and_rows_than_a_launch_has_in_x(ctx):
         near(got[row], mine.sum() * 1.5, (mine.size + 2) * R.U * np.abs(mine).sum() * 1.5, f"row {row}")
         got[row] = 0.0
     assert not got.any()
+
+
+def test_adamw_of_gradients_in_the_parameters_memory(ctx):
+    """Gradients that are other parameters' values (of a product of two parameters, say), views of them or the parameter itself:
+    read as they are in front of the step, eager and compiled.  Two parameters in one memory are refused."""
+    rng = np.random.default_rng(61)
+    a, b, c = (R.f32(rng.standard_normal((300, 400))) for _ in range(3))
+
+    def params():
+        return [Var.new(dev(ctx, x)) for x in (a, b, c)]
+
+    def crossed(p):
+        flat = p[0].value
+        return {p[0]: Var.new(p[1].value), p[1]: Var.new(flat.with_shape(Shape([300, 400]))), p[2]: Var.new(p[2].value)}
+    for bits in (32, 8):
+        want = params()
+        opt = optim.AdamW(1e-2, state_bits=bits)
+        eager, compiled = params(), params()
+        o1, o2 = optim.AdamW(1e-2, state_bits=bits), optim.AdamW(1e-2, state_bits=bits)
+        prog = None
+        for _ in range(3):
+            x, y, z = (dev(ctx, p.value.numpy()) for p in want)
+            opt.update({want[0]: Var.new(y), want[1]: Var.new(x), want[2]: Var.new(z)}, ctx)
+            o1.update(crossed(eager), ctx)
+            if prog is None:
+                prog = o2.compile(crossed(compiled), ctx)
+            else:
+                prog.run()
+            for w, e, p in zip(want, eager, compiled):
+                assert same_bits(w.value.numpy(), e.value.numpy()) and same_bits(w.value.numpy(), p.value.numpy())
+    whole = dev(ctx, a)
+    half = lambda o, n: Var.new(Tensor(whole.buf, FLOAT, Shape([n], [1], o)))  # noqa: E731
+    gh = Var.new(dev(ctx, b[0, :100].copy()))
+    optim.AdamW(1e-2).update({half(0, 100): gh, half(100, 100): gh}, ctx)  # beside one another in one buffer
+    for two in ([half(0, 100), half(99, 100)], [half(5, 100), half(5, 100)]):
+        with pytest.raises(abi.SageError):
+            optim.AdamW(1e-2).update({p: gh for p in two}, ctx)
+        with pytest.raises(abi.SageError):
+            optim.AdamW(1e-2).compile({p: gh for p in two}, ctx)
