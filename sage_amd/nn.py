@@ -149,7 +149,15 @@ def token_logprobs(logits, tokens=None, top=0, scale=1.0):
 
 
 def token_logprobs_grad(logits, lse, tokens=None, g_logprob=None, g_entropy=None):
-    """The gradient of token_logprobs: the logits', from those of its log probabilities and entropies."""
+    """The gradient of token_logprobs: the logits', from those of its log probabilities (which need the tokens) and entropies, one
+    of them at least.  lse: the node that token_logprobs gave for these logits, which holds the scale and the entropy too.  It
+    has no gradient of its own."""
+    if lse.op != "token_lse":
+        raise abi.SageError(abi.ERR_ARG, "token_logprobs_grad: the lse of token_logprobs expected")
+    if g_logprob is None and g_entropy is None:
+        raise abi.SageError(abi.ERR_ARG, "token_logprobs_grad: no gradient given")
+    if g_logprob is not None and tokens is None:
+        raise abi.SageError(abi.ERR_ARG, "token_logprobs_grad: g_logprob needs tokens")
     ins = [logits, lse] + [v for v in (tokens, g_logprob, g_entropy) if v is not None]
     return Var(Shape(logits.extents), FLOAT, "token_logprobs_grad", ins, {"logprob": g_logprob is not None, "entropy": g_entropy is not None})
 
@@ -158,7 +166,7 @@ def cross_attention(q, k, v, mask=None, scale=None):
     """softmax(scale * q . k^T) . v over the keys that `mask` ([N, Lk], 0 = hidden) leaves visible: q [N, H, Lq, D], k and v
     [N, G, Lk, D] with G dividing H (query head h reads key head h / (H/G)), D = 32 or 64, scale 1/sqrt(D) by default.
     A query without a visible key gives zeros; what hidden keys hold is not used.  MultiHeadAttention::pass
-    (bert.rs:262-271) with the keys and values of another sequence, and a gradient of its own."""
+    (bert.rs:262-271) with the keys and values of another sequence, and a gradient of its own, which has none in turn."""
     q, k, v = into_var(q), into_var(k), into_var(v)
     ins = [q, k, v]
     if mask is not None:

@@ -401,3 +401,17 @@ def test_cross_attention_refuses_more_pairs_than_a_launch_has_workgroups():
                 call("sg_cross_attention_grad", desc(q), desc(k), desc(k), desc(m), C.c_float(1.0), desc(q), desc(lse), desc(q), desc(q), desc(k), desc(k)))
     assert both(1 << 24, 1) == both(1 << 12, 1 << 12) == both((1 << 24) - 7, 1) == (abi.ERR_SHAPE, abi.ERR_SHAPE)
     assert both((1 << 24) - 8, 1) == (OK_BUT_NO_CONTEXT, OK_BUT_NO_CONTEXT)
+
+
+def test_token_logprobs_grad_refuses_what_it_cannot_compute():
+    logits, tokens, g = Var.empty([6, 50]), Var.empty([6], INT), Var.empty([6])
+    lse = nn.token_logprobs(logits, tokens).lse
+    assert nn.token_logprobs_grad(logits, lse, tokens, g).extents == nn.token_logprobs_grad(logits, lse, g_entropy=g).extents == [6, 50]
+    for bad in (lambda: nn.token_logprobs_grad(logits, lse, None, g), lambda: nn.token_logprobs_grad(logits, lse, tokens),
+                lambda: nn.token_logprobs_grad(logits, Var.empty([6]), tokens, g)):
+        with pytest.raises(abi.SageError):
+            bad()
+    q, k = Var.empty(Q), Var.empty(K)  # gradients of these gradients are refused, not wrong
+    for first in (grad(nn.cross_attention(q, k, k), [q])[0], nn.token_logprobs_grad(logits, lse, tokens, g)):
+        with pytest.raises(ValueError):
+            grad(first, [q if first.op == "cross_attention_grad" else logits])
