@@ -430,7 +430,7 @@ __device__ __forceinline__ bool merge_waves(float *lds, int wave, int lane, G gi
 // ---- forward.  RW wavefronts take the workgroup's 32 RW rows, the 4 / RW times as many share each block's keys and are
 // merged through LDS at the end.  Bound by the matrix pipes, which fp32 vector instructions share: counters show them busy for
 // 84 % (D = 64) and 77 % (D = 32) of the time a compute unit has work, the vector instructions of the softmax are the rest.
-// 32 x 12 heads, 512 x 512, D = 64: 228 us (113 TFLOP/s); lengths 512 to 272: 177 us; D = 32: 126 us (102 TFLOP/s).
+// 32 x 12 heads, 512 x 512, D = 64: 224 us (115 TFLOP/s); lengths 512 to 272: 181 us; D = 32: 126 us (102 TFLOP/s).
 template <int D, int RW, bool DMA>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RW == 4 ? 3 : 1))) cross_forward_kernel(const CrossP p) {
     constexpr int KW = 4 / RW, KB = 32 * KW, ND = D / 32, SLOT = 16 * ND + 2;
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossP p) {
 }
 
 // ---- gradient of the queries (and delta, for the other kernel).  Three products a block, the matrix pipes busy for 84 % of the
-// time there is work.  32 x 12 heads, 512 x 512, D = 64: 336 us (115 TFLOP/s); lengths 512 to 272: 264 us.
+// time there is work.  32 x 12 heads, 512 x 512, D = 64: 329 us (117 TFLOP/s); lengths 512 to 272: 265 us.
 // GIVEN: delta is there already.
 template <int D, int RW, bool DMA, bool GIVEN>
 __device__ __forceinline__ void gq_work(const CrossP &p, uint32_t id, float (&lds0)[256 / RW * D], float (&lds1)[256 / RW * D], int *lds_end) {
@@ -732,8 +732,8 @@ __global__ void __launch_bounds__(256) cross_gq_kernel(const CrossP p) {
 
 // ---- gradients of keys and values: a wavefront owns 32 keys and walks the rows of the pair, 32 at a time.  CW wavefronts
 // take the workgroup's 32 CW keys, the 4 / CW times as many share each block's rows and are added up through LDS.  Four
-// products a block, the matrix pipes busy for 86 %.  32 x 12 heads, 512 x 512, D = 64: 440 us (117 TFLOP/s); lengths 512 to 272:
-// 378 us.  (dQ from here too would save two of the seven products of a gradient, and cost sums over workgroups.)
+// products a block, the matrix pipes busy for 86 %.  32 x 12 heads, 512 x 512, D = 64: 431 us (119 TFLOP/s); lengths 512 to 272:
+// 379 us.  (dQ from here too would save two of the seven products of a gradient, and cost sums over workgroups.)
 template <int D, int CW, bool DMA>
 __device__ __forceinline__ void gkv_work(const CrossP &p, uint32_t id, float (&lds0)[256 / CW * D], float (&lds1)[256 / CW * D], float (&rows0)[256 / CW],
                                          float (&rows1)[256 / CW], int *lds_end) {  // rows: their lse and delta

@@ -9,9 +9,9 @@
 // bound that k logits reach, so a wavefront collects only logits above the k-th largest of its 64 lanes' maxima (a later
 // one equal to the bound has a higher index than k that reach it), some ten to a hundred of its share, in a list of its own
 // in LDS and without a barrier; the k largest of the wavefronts' lists are ranked at the end.
-// 4096 x 30522 without alternatives: 88 us (500 MB, 5.7 TB/s).  1021 x 50257 with 20: 60 us (205 MB, 3.4 TB/s: all rows are
-// on the chip at once, and choosing does not overlap another row's loads).  4 x 30522 with 5: 8.9 us and a join of 4.8;
-// 4 x 50257 with 64: 23 us and a join of 8.
+// 4096 x 30522 without alternatives: 88 us (500 MB, 5.7 TB/s).  1021 x 50257: 39 us without (205 MB, 5.3 TB/s), 48 with 5, 59 with
+// 20 (the lists leave room for 4 workgroups a compute unit, which are all rows; what choosing adds no other row's loads hide).
+// 4 x 30522 with 5: 9.1 us and a join of 4.6; 4 x 50257 with 64: 23 us and a join of 8.
 #include "rows.h"
 
 #include <type_traits>
@@ -411,8 +411,8 @@ struct LogpGradP {
 // lse carries half a step of its own size into every probability: beyond this it is not used (7.6e-6 there).
 constexpr float FAR = 128.0f;
 
-// glogits_j = scale (-p_j (gl + ge (log p_j + H)) + [j = token] gl).  4096 x 30522: 182 us (1 GB, 5.5 TB/s; a copy of 1 GiB
-// reaches 5.0).  NT: large ones past the caches, 182 us against 207.
+// glogits_j = scale (-p_j (gl + ge (log p_j + H)) + [j = token] gl).  4096 x 30522: 182 us (1 GB, 5.5 TB/s; a copy of
+// 512 MiB reaches 6.5).  NT: large ones past the caches, 182 us against 207.
 template <bool NT>
 __global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const LogpGradP p) {
     __shared__ float lds_stats[12];

@@ -1,7 +1,7 @@
 """Optimizers: host-side mirror of optim.rs.
 
 As in the reference an update is a handful of map expressions per parameter, evaluated eagerly
-(optim.rs:128-131 "eager-execution like mode"); AdamW alone is one call for all parameters.  `grads` is the
+(optim.rs:128-131 "eager-execution like mode"); AdamW alone is one call for all parameters, and the step count two launches.  `grads` is the
 {parameter: gradient Var} mapping of `grad_param`; every gradient must already hold its value (the
 reference warns and evaluates it inside the optimizer otherwise, optim.rs:55-58, 144-147; so do we).
 
