@@ -423,7 +423,7 @@ int sg_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_t
  * 2^24 - 8.
  * mask: NULL or fp32 [N, Lk], unit stride on Lk, any batch stride: key j of sequence b is visible unless mask[b, j] is 0.
  * What a hidden key's k and v hold is not used, NaN or not.  A query without a visible key gives zeros and lse = -inf.
- * The softmax shift follows the row's largest visible score, whatever its size.  lse: NULL or dense [N, H, Lq], log of the
+ * The softmax shift follows the row's largest visible score, whatever its size up to 2^127.  lse: NULL or dense [N, H, Lq], log of the
  * row's sum, for the gradient.  Keys may be split over workgroups and the lengths of masked sequences are found in front:
  * both take a workspace from the context allocator (SG_ERR_OOM). */
 int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask,
