@@ -352,12 +352,13 @@ int sg_adam_update(sg_ctx *ctx, int n_tensors, const sg_tensor *values, const sg
  * to 3 bits).  A byte of v holds 5 exponent and 3 mantissa bits, 0 standing for zero, else the number with the bits
  * (byte + 8e + 7 - 255) << 20; a byte of m a sign (bit 7) and 4 + 3 bits, 127 in the place of 255.  All zeros are zero states.
  * A new state is cut to a byte after 16 bits of noise are added below the bits that are kept, which rounds it up or down
- * with the chances that keep its mean, from the smallest number a block holds on: 1.125 * 2^-15 times the block's power of
- * two for m, 1.125 * 2^-31 times it for v.  A smaller m loses its mean, up to 2^-15 times the power of two it becomes zero (the
- * step then sees one_minus_beta1 g alone); a smaller v that is not zero becomes that smallest number.  Elements whose
- * gradients are that far below the largest of their block therefore take smaller steps than with 32 bits.  The noise of element i is a hash of i + seed + t, low half for m, high half for v: h = i 0x9E3779B9 + seed +
- * t 0xAC502949; h = (h ^ h >> 16) 0x82D3099F; h = (h ^ h >> 15) 0x2ACAE79F; h ^= h >> 16.  A gradient that is not finite makes
- * its value and state not finite; a value that is not finite stays so.  In 8 bits a state that is not finite, or is beyond
+ * with the chances that keep its mean, from the smallest number a block holds on: 1.125 * 2^-15 times the block's power
+ * of two for m, 1.125 * 2^-31 times it for v.  A smaller m loses its mean, up to 2^-15 times the power of two it becomes
+ * zero (the step then sees one_minus_beta1 g alone); a smaller v that is not zero becomes that smallest number.  Elements
+ * whose gradients are that far below the largest of their block therefore take smaller steps than with 32 bits.  The
+ * noise of element i is a hash of i + seed + t, low half for m, high half for v: h = i 0x9E3779B9 + seed + t 0xAC502949;
+ * h = (h ^ h >> 16) 0x82D3099F; h = (h ^ h >> 15) 0x2ACAE79F; h ^= h >> 16.  A gradient that is not finite makes its
+ * value and state not finite; a value that is not finite stays so.  In 8 bits a state that is not finite, or is beyond
  * 1.875 * 2^127, makes its whole block NaN from there on.  Two tensors of a call must not share memory. */
 int sg_adamw_update(sg_ctx *ctx, int n_tensors, const sg_tensor *values, const sg_tensor *grads, const sg_tensor *m,
                     const sg_tensor *v, const sg_tensor *m_scale, const sg_tensor *v_scale, const sg_tensor *step,
@@ -423,9 +424,9 @@ int sg_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_t
  * 2^24 - 8.
  * mask: NULL or fp32 [N, Lk], unit stride on Lk, any batch stride: key j of sequence b is visible unless mask[b, j] is 0.
  * What a hidden key's k and v hold is not used, NaN or not.  A query without a visible key gives zeros and lse = -inf.
- * The softmax shift follows the row's largest visible score, whatever its size up to 2^127.  lse: NULL or dense [N, H, Lq], log of the
- * row's sum, for the gradient.  Keys may be split over workgroups and the lengths of masked sequences are found in front:
- * both take a workspace from the context allocator (SG_ERR_OOM). */
+ * The softmax shift follows the row's largest visible score, whatever its size up to 2^127.  lse: NULL or dense [N, H,
+ * Lq], log of the row's sum, for the gradient.  Keys may be split over workgroups and the lengths of masked sequences are
+ * found in front: both take a workspace from the context allocator (SG_ERR_OOM). */
 int sg_cross_attention(sg_ctx *ctx, const sg_tensor *q, const sg_tensor *k, const sg_tensor *v, const sg_tensor *mask,
                        float scale, const sg_tensor *out, const sg_tensor *lse);
 /* Its gradient: with P = e^(scale q.k - lse), dP = gout . v^T and dS = P (dP - rowsum(gout out)):
